@@ -14,7 +14,11 @@ Modules mirror the reference repository's files (KiritoHugh/attention_kernel_tri
   kept_index                                    select_kept (device kept-index selection)
   merge_states                                  merge_states (LSE merge of partial results)
   sparse_csr                                    sparse decodes over CSR kept indices (inds + ptr)
-  paged_kv                                      append_paged_kv, PagedKVCache (paged KV write side)
+  paged_kv                                      append_paged_kv, append_paged_kv_rotary, copy_pages,
+                                                PagedKVCache (paged KV write side)
+  chunk_flash_attention_paged                   flash_attention_chunk_paged (several new tokens per
+                                                sequence over a paged cache)
+  rotary                                        apply_rotary, rotary_frequencies (rotary positions)
 
 All of them run hand-written HIP kernels from libakt_amd.so (built by
 ``python -m attention_kernel_triton_amd.build``) through its C ABI.
@@ -33,4 +37,6 @@ __all__ = [
     "merge_states",
     "sparse_csr",
     "paged_kv",
+    "chunk_flash_attention_paged",
+    "rotary",
 ]

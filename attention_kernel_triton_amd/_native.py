@@ -61,6 +61,18 @@ _SIGNATURES = {
                                                   _i64x, _i64, _p, C.c_size_t, _p]),
     "akt_paged_kv_append": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                       _i64, _i64x, _i64x, _i64x, _p]),
+    "akt_chunk_paged_workspace_size": (C.c_size_t, [_i64] * 7),
+    "akt_chunk_paged_fwd": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                                      _i64, _i64, _i64, _i64, _i64x, _i64x, C.c_float, C.c_int,
+                                      C.c_int, _p, C.c_size_t, _p]),
+    "akt_rotary_fwd": (C.c_int, [_p, _p, _p, _p, _p, _p, C.c_int, _i64, _i64, _i64, _i64, _i64,
+                                 _i64, _i64x, _i64x, _i64x, C.c_int, C.c_int, C.c_float, C.c_int,
+                                 _p]),
+    "akt_paged_kv_append_rotary": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64,
+                                             _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64x,
+                                             _i64x, _i64x, _i64x, C.c_int, C.c_float, C.c_int,
+                                             _p]),
+    "akt_paged_copy": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64x, _p]),
     "akt_kept_index_from_mask": (C.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, C.c_int, _p]),
     "akt_kept_index_from_uniform": (C.c_int, [_p, C.c_float, _i64, _i64, _i64, _p, _p, _i64, _p,
                                               C.c_int, _p]),

@@ -1,0 +1,850 @@
+// Attention of a chunk of new tokens over a paged KV cache (gfx950).
+//
+// Sequence b has n_b query tokens (rows q_indptr[b] .. q_indptr[b + 1] of q) and len_b
+// cached tokens (the page table's count, its new ones among them).  Query i sits at
+// position len_b - n_b + i and sees the keys up to its own position (causal) or all
+// len_b (not causal):
+//   O = softmax(scale q K^T) V,  LSE = ln sum_j exp(scale q.k_j).
+// It serves chunked prefill, the verification of drafted tokens, mixed batches and
+// single-token decode with one kernel: what bounds it is HBM (K and V once) while a
+// kv head has few rows, the matrix pipe when it has many.
+//
+// Units.  The rows of one (sequence, kv head) are its (token, query head of the group)
+// pairs, token major; a unit is a run of up to 128 rows of whole tokens (TR = 128 / G of
+// them), which share every K and V row.  Wave w of a workgroup owns rows 32 w .. 32 w + 31.
+//
+// Ranges.  The units stand one behind another on an axis of keys (sequence by sequence,
+// kv head by kv head, row block by row block), each as long as the keys it sees plus
+// kCkUnitCost for its start and end.  The axis is cut into equal ranges, one to a
+// workgroup, so a launch is balanced whatever the mix of chunk and context lengths, and
+// nothing of it has to be known on the host: every wave computes the axis's length and its
+// own place on it from the tables (a scan over the sequences, 64 at a time).  A unit is
+// cut only at multiples of kCkBlock keys from its start: block kb of a unit that
+// starts at U belongs to the workgroup whose range holds U + kb + kCkBlock - 1.  With
+// ranges of at least kCkBlock that gives every workgroup of a cut unit at least one
+// block, and no two cut units start in the same workgroup, so the first one's
+// number names the unit's arrival counters.  Workgroup x's partial of a unit that started
+// before it is slot 2 x, of one that starts in it slot 2 x + 1.
+//
+// Merge.  Waves store their partial O, m and l with device-scope stores, wait for them,
+// and count themselves on the counter of (unit, wave); the last one merges all partials
+// in the order of the workgroups (not of arrival, so results do not depend on it) and
+// leaves the counter at zero.  Nothing waits for another workgroup.
+//
+// Tiles.  As in the dense prefill kernel: K and V tiles go global -> registers -> one
+// of four LDS buffers, three tiles ahead; both products run transposed so that a lane owns
+// a row; the running max is raised only when a step's sum says so.  The page ids of a tile
+// are loaded by every wave a tile before its rows, one id to a lane; pages of whole
+// 16-token groups put each wave's loads on one page, whose base is then scalar.
+// Keys past the unit's last one and keys of pages outside the pool read as zeros
+// and score -inf.
+//
+// Masked values.  Scores are masked with a select.  V rows are multiplied by
+// probabilities of zero where some of the unit's rows see them and some do not, which an
+// infinity or NaN in V would turn into NaN: where a tile on the diagonal holds one, P.V is
+// computed key by key and added to the rows that see the key (pv_by_key).
+#include <float.h>
+#include <math.h>
+
+#include <cmath>
+
+#include "akt_host.hpp"
+#include "attn_tile.hpp"
+#include "paged_chunk.hpp"
+
+namespace akt {
+namespace {
+
+constexpr int kCkNBuf = 4;  // LDS tile buffers
+constexpr float kCkSlack = 8.0f;  // log2 units a row's max may rise before it is rescaled
+constexpr float kCkStepLimit = 32.0f * 256.0f;  // row sum of a step that stays unchecked
+// Running max of a row that has seen no key: finite, so that exp2(-inf - m) is 0.
+constexpr float kCkFloor = -1e30f;
+#define AKT_C_NEG_INF (-__builtin_inff())
+
+__host__ __device__ constexpr int ck_tile_keys(int D) { return D == 64 ? 64 : 32; }
+__host__ __device__ constexpr int ck_mix_mfma(int D) { return D == 64 ? 8 : (D == 128 ? 10 : 16); }
+__host__ __device__ constexpr int ck_mix_valu(int D) { return D == 128 ? 1 : 2; }
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)uniform((int)(uint32_t)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
+  return (int64_t)(((uint64_t)shfl_u((uint32_t)(v >> 32), src) << 32) | shfl_u((uint32_t)v, src));
+}
+// floor(a / b) for 0 <= a < 2^50, b >= 1: doubles hold both, and the quotient's distance
+// to the next integer (at least 1 / b) is more than its rounding.
+__device__ __forceinline__ int div_range(int64_t a, int64_t b) {
+  return uniform((int)((double)a / (double)b));
+}
+
+struct Seq {
+  int q0, n;    // first query row, query tokens
+  int ip0, len;  // first page table entry, cached tokens
+};
+// Table entries outside their ranges are taken clamped, so nothing outside the arrays is
+// touched.
+__device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b) {
+  Seq s;
+  s.q0 = min(max(p.q_indptr[b], 0), p.total_q);
+  s.n = min(max(p.q_indptr[b + 1], s.q0), p.total_q) - s.q0;
+  s.ip0 = min(max(p.indptr[b], 0), p.total_pages);
+  const int np = min(max(p.indptr[b + 1], s.ip0), p.total_pages) - s.ip0;
+  s.len = np > 0 ? (np - 1) * p.page_size + min(max(p.last_len[b], 0), p.page_size) : 0;
+  return s;
+}
+__device__ __forceinline__ int row_blocks(const ChunkParams& p, int n) {
+  return (int)(((uint32_t)n + p.TR - 1) / (uint32_t)p.TR);
+}
+// Lengths on the axis.  Causal row block r sees min(n, (r + 1) TR) keys past the context;
+// the axis takes the context as at least 0 (a table with n > len breaks the contract).
+__device__ __forceinline__ int64_t unit_start(const ChunkParams& p, const Seq& s, int64_t r) {
+  if (!p.causal) return r * (s.len + kCkUnitCost);
+  return r * (max(s.len - s.n, 0) + kCkUnitCost) + p.TR * (r * (r + 1) / 2);
+}
+__device__ __forceinline__ int64_t head_length(const ChunkParams& p, const Seq& s) {
+  const int64_t R = row_blocks(p, s.n);
+  if (R == 0) return 0;
+  if (!p.causal) return R * (s.len + kCkUnitCost);
+  return unit_start(p, s, R - 1) + max(s.len - s.n, 0) + s.n + kCkUnitCost;
+}
+// n / page_size for 0 <= n < 2^31.
+__device__ __forceinline__ int page_of(const ChunkParams& p, int n) {
+  const int q = (int)__umulhi((uint32_t)n, p.page_magic);
+  return n - q * p.page_size >= p.page_size ? q + 1 : q;
+}
+
+// A unit and the part of its keys that a workgroup serves.
+struct Unit {
+  int q0;     // first query row (token) in q
+  int ntok;   // its tokens
+  int kvh;    // kv head
+  int first;  // position of its first token (non-causal: unused)
+  int len;    // cached tokens of the sequence
+  int kend;   // keys that it sees
+  int ip0;    // first page table entry of the sequence
+};
+
+template <int D, bool BF16, bool GRP, bool LSE>
+__global__ __launch_bounds__(kCkThreads)
+__attribute__((amdgpu_waves_per_eu(chunk_wgs_per_cu(D), chunk_wgs_per_cu(D))))
+void paged_chunk_kernel(ChunkParams p) {
+  typedef Elt<BF16> E;
+  typedef typename E::v8 v8;
+  constexpr int kBN = ck_tile_keys(D);  // keys per staged tile
+  constexpr int SPT = kBN / 32;         // 32-key steps per tile
+  constexpr int KS = D / 16;            // MFMA k-steps over the head dim
+  constexpr int HALF = D / 2;
+  constexpr int NT = D / 32;       // 32-dim output tiles
+  constexpr int CPR = D / 8;       // 16-byte chunks per row
+  constexpr int ROWB = D * 2;      // bytes per row
+  constexpr int TILEB = kBN * ROWB;
+  constexpr int BUFB = 2 * TILEB;  // K then V
+  constexpr int PER_T = kBN * CPR / kCkThreads;  // chunks per thread per matrix
+  constexpr int RPC = 64 / CPR;                  // rows of a wave's 64 chunks
+  static_assert(16 % RPC == 0, "a wave's chunks lie in one 16-key group");
+  __shared__ __attribute__((aligned(16))) char lds[kCkNBuf * BUFB];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int l32 = lane & 31;
+  const int g = lane >> 5;
+
+  // ---- this workgroup's range of the axis.  Workgroup i runs on XCD i % 8, so
+  // consecutive ranges go to one XCD's L2.
+  const int W = p.wgs;
+  const int wg = W % 8 == 0 ? (int)(blockIdx.x % 8) * (W / 8) + (int)(blockIdx.x / 8)
+                            : (int)blockIdx.x;
+  auto seq_length = [&](int b) -> int64_t {
+    if (b >= p.B) return 0;
+    const Seq s = load_seq(p, b);
+    return head_length(p, s) * p.Hkv;
+  };
+  auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t u = shfl64(v, lane - d < 0 ? 0 : lane - d);
+      if (lane >= d) v += u;
+    }
+    return v;
+  };
+  int64_t total = 0;
+  for (int jb = 0; jb < p.B; jb += 64) total += uniform64(shfl64(scan64(seq_length(jb + lane)), 63));
+  int64_t Lw = (total + W - 1) / W;
+  if (Lw < p.min_keys) Lw = p.min_keys;
+  Lw = uniform64(Lw);
+  const int64_t x0 = wg * Lw, x1 = x0 + Lw;
+  if (x0 >= total) return;
+  // The unit that holds x0: sequence, kv head, row block.
+  int b = 0;
+  int64_t U = 0;  // the sequence's start
+  for (int jb = 0;; jb += 64) {
+    const int64_t len = seq_length(jb + lane);
+    const int64_t inc = scan64(len);
+    const uint64_t m = __ballot(U + inc > x0);
+    if (m) {
+      const int l = __builtin_ctzll(m);
+      b = uniform(jb + l);
+      U += uniform64(shfl64(inc - len, l));
+      break;
+    }
+    U += uniform64(shfl64(inc, 63));
+  }
+  Seq s = load_seq(p, b);
+  int64_t hlen = head_length(p, s);
+  int kvh = div_range(x0 - U, hlen);
+  int64_t hs = U + kvh * hlen;  // the head's start
+  int R = uniform(row_blocks(p, s.n)), r = 0;
+  for (int lo = 0, hi = R; lo < hi;) {  // last r with unit_start(r) <= x0 - hs
+    const int mid = (lo + hi) / 2;
+    if (unit_start(p, s, mid) <= x0 - hs) {
+      r = mid;
+      lo = mid + 1;
+    } else {
+      hi = mid;
+    }
+  }
+
+  // ---- per-lane constants
+  const float c = p.qk_scale;
+  // K rows for S^T: key l32 of the step, chunks g * HALF / 8 + s.
+  int koff[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) koff[k] = l32 * ROWB + (((g * HALF / 8) + k) ^ tswz<D>(l32)) * 16;
+  // V^T through the transposing read: see prefill_kernel.
+  const int s16 = lane & 15;
+  const int vrow = 4 * g + (s16 >> 2);
+  const int vcl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+  int voff[NT], voffh[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    voff[n] = TILEB + vrow * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow)) * 16) + (s16 & 1) * 8;
+    voffh[n] =
+        TILEB + (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
+  }
+  const int lrow = 32 * wave + l32;                          // this lane's row of the unit
+  const int ltok = (int)((uint32_t)lrow * p.g_magic >> 16);  // and its token
+
+  // ---- the keys [k0, k1) of a unit, for all four waves.
+  auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
+    const int rows = u.ntok * p.G;
+    const bool active = 32 * wave < rows;
+    const bool whole = k0 == 0 && k1 == u.kend;
+    const int n_tiles = SPT == 2 ? (k1 - k0 + 63) / 64 : 2 * ((k1 - k0 + 63) / 64);
+    const int n_h = active ? 2 * ((k1 - k0 + 63) / 64) : 0;
+    const half_t* const Kh = p.pool + u.kvh * p.sh;
+
+    // Page ids of tile j: lane l holds that of key l (past the unit's keys: of its last one).
+    auto load_ids = [&](int j) -> int {
+      const int key = min(k0 + j * kBN + (lane & (kBN - 1)), u.kend - 1);
+      return p.indices[u.ip0 + page_of(p, key)];
+    };
+    auto id_ok = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pool_pages; };
+    uint4_t kst[PER_T], vst[PER_T];
+    auto load_tile = [&](int j, int ids, uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
+#pragma unroll
+      for (int i = 0; i < PER_T; ++i) {
+        if constexpr (GRP) {
+          // This wave's RPC rows lie in one page.
+          const int row = (wave * 64 + i * kCkThreads) / CPR;
+          const int key = k0 + j * kBN + row;
+          const int id = __builtin_amdgcn_readlane(ids, row);
+          const int left = min(RPC, u.kend - key);
+          const bool ok = left > 0 && id_ok(id);
+          const int slot = key - page_of(p, key) * p.page_size;
+          const half_t* base = Kh + (ok ? id * p.sp + (int64_t)slot * p.ss : 0);
+          const int bytes = ok ? (left - 1) * p.ss * 2 + ROWB : 0;
+          const int off = (lane / CPR) * p.ss * 2 + (lane % CPR) * 16;
+          const auto kr =
+              __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, kBufferWord3);
+          const auto vr =
+              __builtin_amdgcn_make_buffer_rsrc((void*)(base + p.skv), 0, bytes, kBufferWord3);
+          kd[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
+          vd[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
+        } else {
+          const int row = (tid + i * kCkThreads) / CPR;
+          const int key = k0 + j * kBN + row;
+          const int id = (int)shfl_u((uint32_t)ids, row);
+          kd[i] = vd[i] = uint4_t{0, 0, 0, 0};
+          if (key < u.kend && id_ok(id)) {
+            const int slot = key - page_of(p, key) * p.page_size;
+            const half_t* src =
+                Kh + id * p.sp + (int64_t)slot * p.ss + (tid + i * kCkThreads) % CPR * 8;
+            kd[i] = ld16(src);
+            vd[i] = ld16(src + p.skv);
+          }
+        }
+      }
+    };
+    auto store_tile = [&](int j, const uint4_t (&kd)[PER_T], const uint4_t (&vd)[PER_T]) {
+      char* buf = lds + (j % kCkNBuf) * BUFB;
+#pragma unroll
+      for (int i = 0; i < PER_T; ++i) {
+        const int ch = tid + i * kCkThreads;
+        const int row = ch / CPR, cc = ch % CPR;
+        const int off = row * ROWB + ((cc ^ tswz<D>(row)) * 16);
+        *reinterpret_cast<uint4_t*>(buf + off) = kd[i];
+        *reinterpret_cast<uint4_t*>(buf + TILEB + off) = vd[i];
+      }
+    };
+
+    // Last key of this lane's row (rows past the unit's: of its last token), and the
+    // first of the wave's rows' last keys, up to which nothing is masked.
+    const int lim = p.causal ? u.first + min(ltok, u.ntok - 1) : u.len - 1;
+    const int lim_min =
+        p.causal ? u.first + min((int)((uint32_t)(32 * wave) * p.g_magic >> 16), u.ntok - 1)
+                 : u.len - 1;
+
+    // ---- Q^T fragments: lane -> row, dims g*HALF + 8s + e.
+    v8 qf[KS];
+    {
+      const int hl = lrow - ltok * p.G;
+      const half_t* src = p.q + (int64_t)(u.q0 + ltok) * p.q_st +
+                          (int64_t)(u.kvh * p.G + hl) * p.q_sh + g * HALF;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint4_t v = {0, 0, 0, 0};
+        if (lrow < rows) v = ld16(src + 8 * k);
+        if (p.neg_q) v ^= uint4_t{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        qf[k] = E::as8(v);
+      }
+    }
+    float16_t oacc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) oacc[n][i] = 0.f;
+    float m_run = kCkFloor, l_part = 0.f, x_part = 0.f;  // x: the sum of the unrounded P
+
+    float16_t sA, sB;
+    uint32_t pA[8], pB[8];
+    v8 vf[2][NT];
+    // P.V(-1) of step 0 multiplies zeros by zeros.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pB[i] = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) vf[h][n] = E::as8(uint4_t{0, 0, 0, 0});
+
+    auto load_kf = [&](int t, v8 (&kf)[KS]) {
+      const char* kb = lds + ((t / SPT) % kCkNBuf) * BUFB + (t % SPT) * 32 * ROWB;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kf[k] = E::as8(*reinterpret_cast<const uint4_t*>(kb + koff[k]));
+    };
+    auto load_vf = [&](int t) {
+      const char* vb = lds + ((t / SPT) % kCkNBuf) * BUFB + (t % SPT) * 32 * ROWB;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint2 lo = ds_read_tr16(vb + voff[n] + h * 16 * ROWB);
+          const uint2 hi = ds_read_tr16(vb + voffh[n] + h * 16 * ROWB);
+          vf[h][n] = E::as8(uint4_t{lo.x, lo.y, hi.x, hi.y});
+        }
+    };
+    auto qk_mfma = [&](const v8 (&kf)[KS], float16_t& dst) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dst[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) dst = E::mfma(kf[k], qf[k], dst);
+    };
+    auto pv_mfma = [&](const uint32_t (&pk)[8]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v8 bop = E::as8(uint4_t{pk[4 * h], pk[4 * h + 1], pk[4 * h + 2], pk[4 * h + 3]});
+#pragma unroll
+        for (int n = 0; n < NT; ++n) oacc[n] = E::mfma(vf[h][n], bop, oacc[n]);
+      }
+    };
+    // P.V of one step, key by key: each key's product is added to the rows that see it.
+    // Element e of fragment h of lane half g is key 16 h + 8 (e / 4) + 4 g + e % 4.
+    auto pv_by_key = [&](const uint32_t (&pk)[8], int kh0) {
+#pragma clang loop unroll(disable)
+      for (int j = 0; j < 32; ++j) {
+        const bool mine = g == ((j >> 2) & 1);
+        const uint32_t half = (j & 1) ? 0xffff0000u : 0x0000ffffu;
+        const int word = 2 * ((j >> 3) & 1) + ((j >> 1) & 1);
+        v8 bop[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          bop[h] = E::as8(uint4_t{pk[4 * h], pk[4 * h + 1], pk[4 * h + 2], pk[4 * h + 3]});
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float16_t acc;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint4_t v = __builtin_bit_cast(uint4_t, vf[h][n]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              v[w] = (mine && h == (j >> 4) && w == word) ? (v[w] & half) : 0u;
+            acc = E::mfma(E::as8(v), bop[h], acc);
+          }
+          if (kh0 + j <= lim) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[n][i] += acc[i];
+          }
+        }
+      }
+    };
+    auto v_not_finite = [&]() -> bool {
+      constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+      bool bad = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4_t v = __builtin_bit_cast(uint4_t, vf[h][n]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            bad |= (v[w] & kExp) == kExp || (v[w] & (kExp << 16)) == (kExp << 16);
+        }
+      return __any(bad);
+    };
+    auto softmax = [&](const float16_t& ss, uint32_t (&pk)[8], float& l_step, float& x_step) {
+      float ls = 0.f, xs = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = fast_exp2(__builtin_fmaf(ss[i], c, -m_run));
+        const float p1 = fast_exp2(__builtin_fmaf(ss[i + 1], c, -m_run));
+        pk[i >> 1] = E::pack2(p0, p1);
+        if constexpr (LSE) xs += p0 + p1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ls = E::dot2(pk[i], E::kOnes, ls);
+      l_step = ls;
+      x_step = xs;
+    };
+    // Masks step t: keys past a row, and keys (bit of `valid`) of pages outside the pool.
+    auto mask_step = [&](int kh0, uint32_t valid, float16_t& ss) {
+      if (kh0 + 31 > lim_min || valid != 0xffffffffu) {  // wave-uniform
+        const int room = lim - kh0 - 4 * g;
+        const uint32_t vl = valid >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int o = 8 * (i >> 2) + (i & 3);
+          if (o > room || !((vl >> o) & 1)) ss[i] = AKT_C_NEG_INF;
+        }
+      }
+    };
+    auto row_max = [&](const float16_t& sv) {
+      float mx = sv[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, sv[i]);
+      float ma, mb;
+      swap32(mx, ma, mb);
+      return __builtin_elementwise_maximum(ma, mb) * c;
+    };
+    // One step, as in prefill_kernel: with no dependence between them, P.V of the
+    // previous step, S of the next and the softmax of this one.
+    auto step = [&](int t, uint32_t valid, float16_t& scur, float16_t& snext,
+                    const uint32_t (&pprev)[8], uint32_t (&pcur)[8]) {
+      const int kh0 = k0 + 32 * t;
+      mask_step(kh0, valid, scur);
+      v8 kf[KS];
+      load_kf(t + 1, kf);
+      pv_mfma(pprev);
+      qk_mfma(kf, snext);
+      load_vf(t);
+      float l_step, x_step;
+      softmax(scur, pcur, l_step, x_step);
+#pragma unroll
+      for (int i = 0; i < ck_mix_mfma(D); ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, ck_mix_valu(D), 0);
+      }
+      if (__any(!(l_step <= kCkStepLimit))) {  // rare
+        const float mx = row_max(scur);
+        const bool raise = mx > m_run + kCkSlack;
+        const float alpha = raise ? fast_exp2(m_run - mx) : 1.f;
+        l_part *= alpha;
+        x_part *= alpha;
+        if (raise) {
+          m_run = mx;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[n][i] *= alpha;
+        }
+        softmax(scur, pcur, l_step, x_step);
+      }
+      l_part += l_step;
+      x_part += x_step;
+      if (p.causal && kh0 + 31 > lim_min) {  // on the diagonal
+        if (v_not_finite()) {
+          pv_by_key(pcur, kh0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pcur[i] = 0u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) vf[h][n] = E::as8(uint4_t{0, 0, 0, 0});
+        }
+      }
+    };
+
+    // Valid-key bits of tiles j .. j + 3 at tile j (lanes past kBN repeat the first ones).
+    auto valid_of = [&](int ids) -> uint64_t { return __ballot(id_ok(ids)); };
+    uint64_t v0, v1, v2, v3;
+    int ids_next;
+    __syncthreads();  // the last unit's LDS reads are done
+    {
+      const int i0 = load_ids(0), i1 = load_ids(1), i2 = load_ids(2);
+      ids_next = load_ids(3);
+      uint4_t ka[PER_T], va[PER_T], kb[PER_T], vb[PER_T];
+      load_tile(0, i0, ka, va);
+      if (n_tiles > 1) load_tile(1, i1, kb, vb);
+      if (n_tiles > 2) load_tile(2, i2, kst, vst);
+      v0 = 0;
+      v1 = valid_of(i0);
+      v2 = valid_of(i1);
+      v3 = valid_of(i2);
+      store_tile(0, ka, va);
+      if (n_tiles > 1) store_tile(1, kb, vb);
+    }
+    __syncthreads();
+    {
+      v8 kf[KS];
+      load_kf(0, kf);
+      qk_mfma(kf, sA);
+    }
+    mask_step(k0, (uint32_t)v1, sA);
+    {
+      const float mx = row_max(sA);
+      m_run = mx < kCkFloor ? kCkFloor : mx;  // a NaN stays
+    }
+    auto tile_turn = [&](int j) {
+      __syncthreads();
+      v0 = v1;
+      v1 = v2;
+      v2 = v3;
+      if (j + 2 < n_tiles) store_tile(j + 2, kst, vst);
+      if (j + 3 < n_tiles) {
+        load_tile(j + 3, ids_next, kst, vst);
+        v3 = valid_of(ids_next);
+        ids_next = load_ids(j + 4);
+      }
+    };
+#pragma clang loop unroll(disable)
+    for (int j = 0; j < n_tiles; j += 2 / SPT) {
+      tile_turn(j);
+      const int t = SPT * j;
+      if (t < n_h) step(t, (uint32_t)v0, sA, sB, pB, pA);
+      if constexpr (SPT == 1) tile_turn(j + 1);
+      if (t < n_h) {
+        step(t + 1, SPT == 2 ? (uint32_t)(v0 >> 32) : (uint32_t)v0, sB, sA, pA, pB);
+        if (t + 2 == n_h) pv_mfma(pB);
+      }
+    }
+
+    // ---- end of the part: partial or output, each wave for its own rows.
+    __syncthreads();  // every tile read is done
+    if (!active) return;
+    float l_row = xor32_sum(l_part);
+    float x_row = LSE ? xor32_sum(x_part) : 0.f;
+    if (!whole) {
+      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = chunk_slot_bytes(D);
+      const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
+      const int wf = div_range(Ustart + kCkBlock - 1, Lw);
+      const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
+      auto slot_of = [&](int w) -> char* {
+        return p.partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+      };
+      char* mine = slot_of(wg);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          st16_device(mine, (uint32_t)(((4 * n + k) * 64 + lane) * 16),
+                      as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
+                                         oacc[n][4 * k + 3]}));
+      if (g == 0)
+        st16_device(mine, (uint32_t)(NT * 4096 + l32 * 16),
+                    as_uint4f(float4_t{m_run, l_row, x_row, 0.f}));
+      // The stores (device scope) are complete before the count.
+      __builtin_amdgcn_s_waitcnt(0);
+      int prev = 0;
+      if (lane == 0) prev = atomicAdd(&p.arrive[4 * wf + wave], 1);
+      if (uniform(prev) != wl - wf) return;
+      if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
+      float M = AKT_C_NEG_INF;
+      for (int w = wf; w <= wl; ++w)
+        M = __builtin_elementwise_maximum(
+            M, as_float4u(ld16_device(slot_of(w), (uint32_t)(NT * 4096 + l32 * 16)))[0]);
+      m_run = M;
+      l_row = x_row = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[n][i] = 0.f;
+      for (int w = wf; w <= wl; ++w) {
+        const char* src = slot_of(w);
+        const float4_t ml = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
+        const float f = fast_exp2(ml[0] - M);
+        l_row += f * ml[1];
+        x_row += f * ml[2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4_t ov = as_float4u(
+                ld16_device(src, (uint32_t)(((4 * n + k) * 64 + lane) * 16)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[n][4 * k + i] += f * ov[i];
+          }
+      }
+    }
+    // Output rows through LDS, so that every lane stores 16 contiguous bytes.
+    const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
+    if (LSE && g == 0 && lrow < rows)
+      p.lse[(int64_t)(u.q0 + ltok) * p.Hq + u.kvh * p.G + (lrow - ltok * p.G)] =
+          l_row == 0.f ? AKT_C_NEG_INF : (m_run + __log2f(x_row)) * kLn2;
+    char* ost = lds + wave * (32 * ROWB);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float16_t& a = oacc[n];
+        const uint2 hv = {E::pack2(a[4 * k] * inv, a[4 * k + 1] * inv),
+                          E::pack2(a[4 * k + 2] * inv, a[4 * k + 3] * inv)};
+        const int chunk = (4 * n + k) ^ eswz(l32);
+        *reinterpret_cast<uint2*>(ost + l32 * ROWB + chunk * 16 + 8 * g) = hv;
+      }
+#pragma unroll 2
+    for (int idx = lane; idx < 32 * CPR; idx += 64) {
+      const int lr = idx / CPR, cc = idx % CPR;
+      const uint4_t v = *reinterpret_cast<const uint4_t*>(ost + lr * ROWB + ((cc ^ eswz(lr)) * 16));
+      const int row = 32 * wave + lr;
+      const int tok = (int)((uint32_t)row * p.g_magic >> 16);
+      if (row < rows)
+        st16(p.o + ((int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G)) * D + 8 * cc,
+             v);
+    }
+  };
+
+  // ---- the units of the range
+  for (;;) {
+    Unit u;
+    const int t0 = r * p.TR;
+    u.q0 = uniform(s.q0 + t0);
+    u.ntok = uniform(min(p.TR, s.n - t0));
+    u.kvh = kvh;
+    u.first = uniform(s.len - s.n + t0);
+    u.len = uniform(s.len);
+    u.kend = uniform(p.causal ? max(u.first + u.ntok, 0) : s.len);
+    u.ip0 = uniform(s.ip0);
+    const int64_t us = hs + unit_start(p, s, r);
+    // Blocks from the first at or past x - us - (kCkBlock - 1) on are the next range's.
+    auto cut = [&](int64_t x) -> int64_t {
+      const int64_t d = x - us - (kCkBlock - 1);
+      return d <= 0 ? 0 : (d + kCkBlock - 1) / kCkBlock * kCkBlock;
+    };
+    const int64_t e = cut(x1);
+    if (e == 0) break;  // this unit and all after it are later ranges'
+    const int k0 = (int)cut(x0), k1 = uniform((int)(e < u.kend ? e : u.kend));
+    if (u.kend == 0) {
+      // Nothing to see: zeros.
+      const int rows = u.ntok * p.G;
+      if (k0 == 0)
+        for (int idx = tid; idx < rows * CPR; idx += kCkThreads) {
+          const int row = idx / CPR;
+          const int tok = (int)((uint32_t)row * p.g_magic >> 16);
+          const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
+          st16(p.o + at * D + idx % CPR * 8, uint4_t{0, 0, 0, 0});
+          if (LSE && idx % CPR == 0) p.lse[at] = AKT_C_NEG_INF;
+        }
+    } else if (k0 < k1) {
+      serve(u, uniform(k0), k1, us);
+    }
+    if (e < u.kend) break;  // the rest of the unit is the next range's
+    if (++r < R) continue;
+    r = 0;
+    hs += hlen;
+    if (++kvh < p.Hkv) continue;
+    kvh = 0;
+    do {
+      if (++b == p.B) return;
+      s = load_seq(p, b);
+      R = uniform(row_blocks(p, s.n));
+    } while (R == 0);
+    hlen = uniform64(head_length(p, s));
+  }
+}
+
+template <int D, bool BF16, bool GRP>
+int launch_lse(const ChunkParams& p, hipStream_t st) {
+  KernelTimer timer;
+  if (p.lse)
+    timer.launch(paged_chunk_kernel<D, BF16, GRP, true>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
+  else
+    timer.launch(paged_chunk_kernel<D, BF16, GRP, false>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
+  return check_launch("paged_chunk_kernel");
+}
+
+template <int D>
+int launch_chunk(const ChunkParams& p, bool bf16, hipStream_t st) {
+  if (p.page_size % 16 == 0)
+    return bf16 ? launch_lse<D, true, true>(p, st) : launch_lse<D, false, true>(p, st);
+  return bf16 ? launch_lse<D, true, false>(p, st) : launch_lse<D, false, false>(p, st);
+}
+
+}  // namespace
+
+// Each head dim is instantiated in a translation unit of its own (they compile side by
+// side): this one holds D = 128 and the entry points, the others include it.
+#ifndef AKT_CHUNK_TU
+#define AKT_CHUNK_TU 128
+#endif
+#if AKT_CHUNK_TU == 64
+int chunk_launch_64(const ChunkParams& p, bool bf16, hipStream_t st) {
+  return launch_chunk<64>(p, bf16, st);
+}
+#elif AKT_CHUNK_TU == 256
+int chunk_launch_256(const ChunkParams& p, bool bf16, hipStream_t st) {
+  return launch_chunk<256>(p, bf16, st);
+}
+#else
+int chunk_launch_128(const ChunkParams& p, bool bf16, hipStream_t st) {
+  return launch_chunk<128>(p, bf16, st);
+}
+
+namespace {
+
+constexpr int kCkMinKeys = 256;
+
+// Workgroups of a launch: the resident ones, fewer where the axis is too short for them
+// (bounded from above by what the host knows: every sequence as long as all pages).
+int64_t chunk_wgs(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
+                  int64_t page_size, int64_t total_pages) {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus <= 0)
+    cus = 256;  // no device: what an MI355X has
+  const int64_t resident = (int64_t)cus * chunk_wgs_per_cu((int)D);
+  const int64_t units = Hkv * (total_q / (kCkRows / G) + (batch < total_q ? batch : total_q));
+  // units < 2^31 * Hkv and the length < 2^31: as doubles, against overflow.
+  const double axis = (double)units * (double)(total_pages * page_size + kCkUnitCost);
+  const double wgs = ceil(axis / kCkMinKeys);
+  return wgs < (double)resident ? (int64_t)wgs : resident;
+}
+
+}  // namespace
+}  // namespace akt
+
+using namespace akt;
+
+extern "C" size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q,
+                                                 int64_t num_q_heads, int64_t num_kv_heads,
+                                                 int64_t head_dim, int64_t page_size,
+                                                 int64_t total_pages) {
+  if (batch <= 0 || total_q <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || page_size <= 0 ||
+      total_pages < 0 || num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > kCkRows ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return 0;
+  const int64_t wgs = chunk_wgs(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
+                                page_size, total_pages);
+  return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) +
+                  2 * wgs * chunk_slot_bytes((int)head_dim));
+}
+
+extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
+                                   const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+                                   const int32_t* kv_last_page_len, void* o, float* lse,
+                                   int64_t batch, int64_t total_q, int64_t num_q_heads,
+                                   int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                   int64_t total_pages, int64_t num_pool_pages,
+                                   const int64_t q_stride[3], const int64_t kv_stride[5],
+                                   float softmax_scale, int causal, int dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  clear_error();
+  AKT_CHECK(dtype == AKT_DTYPE_F16 || dtype == AKT_DTYPE_BF16,
+            "dtype must be AKT_DTYPE_F16 or AKT_DTYPE_BF16, got %d", dtype);
+  AKT_CHECK(batch >= 0 && total_q >= 0 && total_pages >= 0 && num_pool_pages >= 0,
+            "sizes must be non-negative");
+  AKT_CHECK(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0,
+            "num_q_heads (%lld) must be a positive multiple of num_kv_heads (%lld)",
+            (long long)num_q_heads, (long long)num_kv_heads);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return set_error(AKT_ERR_UNSUPPORTED, "chunk attention head_dim %lld not supported (64, 128, 256)",
+                     (long long)head_dim);
+  if (num_q_heads / num_kv_heads > kCkRows)
+    return set_error(AKT_ERR_UNSUPPORTED, "chunk attention serves up to %d query heads per kv head",
+                     kCkRows);
+  AKT_CHECK(page_size > 0 && page_size < (1 << 20), "page_size out of range");
+  AKT_CHECK(batch < (1ll << 30) && total_q < (1ll << 30) && num_q_heads < (1 << 20),
+            "problem too large");
+  AKT_CHECK(total_pages < (1ll << 31) && total_pages * page_size < (1ll << 30),
+            "the page table spans too many tokens");
+  AKT_CHECK(std::isfinite(softmax_scale), "softmax_scale must be finite");
+  if (batch == 0 || total_q == 0) return AKT_OK;
+  AKT_CHECK(q && q_indptr && kv_cache && kv_page_indptr && kv_last_page_len && o && q_stride &&
+                kv_stride && (kv_page_indices || total_pages == 0),
+            "all pointers are required");
+  AKT_CHECK(q_stride[2] == 1 && kv_stride[4] == 1, "head_dim stride must be 1");
+  AKT_CHECK(rows_aligned16(q, q_stride, 2) && rows_aligned16(kv_cache, kv_stride, 4) &&
+                aligned16(o) && (!lse || aligned4(lse)),
+            "tensors must have 16-byte aligned rows");
+  AKT_CHECK(kv_stride[3] >= 0 && kv_stride[3] < (1 << 22), "slot stride out of range [0, 2^22)");
+  const int64_t G = num_q_heads / num_kv_heads;
+  const int64_t wgs =
+      chunk_wgs(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages);
+  const size_t need = akt_chunk_paged_workspace_size(batch, total_q, num_q_heads, num_kv_heads,
+                                                     head_dim, page_size, total_pages);
+  if (!workspace || workspace_bytes < need)
+    return set_error(AKT_ERR_WORKSPACE, "chunk attention needs a workspace of %zu bytes, got %zu",
+                     need, workspace ? workspace_bytes : (size_t)0);
+  AKT_CHECK(aligned16(workspace), "the workspace must be 16-byte aligned");
+  static_assert(4 * 2 * 1024 <= (AKT_WORKSPACE_ZERO_BYTES - 256) / 4, "arrival counters");
+  AKT_CHECK(4 * wgs <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4, "too many workgroups");
+
+  ChunkParams p = {};
+  p.q = (const half_t*)q;
+  p.pool = (const half_t*)kv_cache;
+  p.o = (half_t*)o;
+  p.lse = lse;
+  p.q_indptr = q_indptr;
+  p.indptr = kv_page_indptr;
+  p.indices = kv_page_indices;
+  p.last_len = kv_last_page_len;
+  p.arrive = (int*)((char*)workspace + 256);
+  p.partials = (char*)workspace + round_up(AKT_WORKSPACE_ZERO_BYTES, 256);
+  p.q_st = q_stride[0];
+  p.q_sh = q_stride[1];
+  p.sp = kv_stride[0];
+  p.skv = kv_stride[1];
+  p.sh = kv_stride[2];
+  p.ss = (int)kv_stride[3];
+  p.total_q = (int)total_q;
+  p.total_pages = (int)total_pages;
+  p.num_pool_pages = (int)(num_pool_pages < (1ll << 31) ? num_pool_pages : (1ll << 31) - 1);
+  p.B = (int)batch;
+  p.Hq = (int)num_q_heads;
+  p.Hkv = (int)num_kv_heads;
+  p.G = (int)G;
+  p.TR = (int)(kCkRows / G);
+  p.g_magic = (uint32_t)((65536 + G - 1) / G);
+  p.page_size = (int)page_size;
+  const uint64_t magic = (1ull << 32) / (uint64_t)page_size;
+  p.page_magic = (uint32_t)(magic < 0xffffffffull ? magic : 0xffffffffull);
+  p.causal = causal ? 1 : 0;
+  // As in prefill: a negative scale flips Q's sign, a zero one becomes FLT_MIN.
+  p.neg_q = softmax_scale < 0.f ? 1 : 0;
+  p.qk_scale = fmaxf(fabsf(softmax_scale) * kLog2e, FLT_MIN);
+  p.wgs = (int)wgs;
+  p.min_keys = kCkMinKeys;
+  hipStream_t st = (hipStream_t)stream;
+  const bool bf16 = dtype == AKT_DTYPE_BF16;
+  if (head_dim == 64) return chunk_launch_64(p, bf16, st);
+  if (head_dim == 256) return chunk_launch_256(p, bf16, st);
+  return chunk_launch_128(p, bf16, st);
+}
+
+namespace akt {
+#endif  // AKT_CHUNK_TU
+}  // namespace akt

@@ -1,5 +1,6 @@
 // Compiled host layer of the hot entry points (prefill, dense / paged /
-// sparse / MagicPIG decode, kept-index selection, paged KV append, LSE merge): the same checks, output allocation, stream and
+// sparse / MagicPIG decode, paged chunk attention, rotary positions, kept-index selection,
+// paged KV append and page copies, LSE merge): the same checks, output allocation, stream and
 // workspace handling as the package's Python wrappers, done in C++ so a
 // drop-in call costs the host a few microseconds.  It calls the C ABI of
 // libakt_amd.so (include/akt_amd.h) and nothing else; there is no fallback.
@@ -10,6 +11,7 @@
 // drop-in modules.
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -80,6 +82,24 @@ at::Tensor half_or_bf16_rows(const char* name, const at::Tensor& t, at::ScalarTy
   return rows16(t);
 }
 
+// Tensor of the given 2-byte type, which is that of the named tensor, as rows16.
+at::Tensor rows_like(const char* name, const at::Tensor& t, at::ScalarType want,
+                     const char* like) {
+  need_gpu(name, t);
+  if (t.scalar_type() != want)
+    throw py::type_error(std::string(name) + " must be " + std::string(c10::toString(want)) +
+                         " like " + like + ", got " + std::string(c10::toString(t.scalar_type())));
+  return rows16(t);
+}
+
+// AKT_DTYPE_* of a 16-bit floating type.
+int dtype16(const char* name, const at::Tensor& t) {
+  if (t.scalar_type() == at::kHalf) return AKT_DTYPE_F16;
+  if (t.scalar_type() == at::kBFloat16) return AKT_DTYPE_BF16;
+  throw py::type_error(std::string(name) + " must be float16 or bfloat16, got " +
+                       std::string(c10::toString(t.scalar_type())));
+}
+
 at::Tensor int32_on(const char* name, const at::Tensor& t, const at::Device& dev) {
   need_gpu(name, t);
   same_device(name, t, dev);
@@ -143,6 +163,21 @@ at::Tensor workspace(size_t nbytes, const at::Device& dev, hipStream_t st) {
   const int64_t size = std::max<int64_t>((int64_t)nbytes, 2 * old);
   at::Tensor buf = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(dev));
   g_ws[key] = buf;
+  return buf;
+}
+
+// Workspace of a call whose launch may be captured into a graph.  A captured launch
+// runs again and again, possibly beside the launches of other graphs captured on the
+// same stream, so it gets a buffer of its own (from the graph's memory pool) whose
+// counters every replay zeroes; any other launch takes the stream's.
+at::Tensor capture_workspace(size_t nbytes, const at::Device& dev, hipStream_t st) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone)
+    return workspace(nbytes, dev, st);
+  if (nbytes == 0) return at::Tensor();
+  at::Tensor buf =
+      at::empty({(int64_t)nbytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  buf.narrow(0, 0, std::min<int64_t>((int64_t)nbytes, AKT_WORKSPACE_ZERO_BYTES)).zero_();
   return buf;
 }
 
@@ -435,6 +470,17 @@ py::tuple kept_indices(int64_t l_max, const c10::optional<at::Tensor>& mask_,
   return py::make_tuple(ind, nnz);
 }
 
+// A pool that a call writes in place: 16-bit elements (the kernels move them whole), rows of
+// unit stride.
+int check_written_pool(const at::Tensor& pool) {
+  const int dtype = dtype16("paged_kv_cache", pool);
+  if (pool.dim() != 5 || pool.size(1) != 2)
+    throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
+  if (pool.stride(-1) != 1)
+    throw py::value_error("paged_kv_cache needs a unit head_dim stride (it is written in place)");
+  return dtype;
+}
+
 // --------------------------------------------------------------------------- paged KV append
 // The write of a decode step's tokens is a few microseconds of GPU time; through
 // ctypes the call cost the host 9.8 us, here 3.8.
@@ -443,14 +489,11 @@ void append_paged_kv(const at::Tensor& k_new_, const at::Tensor& v_new_,
                      const at::Tensor& indptr_, const at::Tensor& indices_,
                      const at::Tensor& last_) {
   need_gpu("paged_kv_cache", pool);
-  if (pool.scalar_type() != at::kHalf)
-    throw py::type_error("paged_kv_cache must be float16, got " +
-                         std::string(c10::toString(pool.scalar_type())));
-  if (pool.dim() != 5) throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
-  if (pool.stride(-1) != 1)
-    throw py::value_error("paged_kv_cache needs a unit head_dim stride (it is written in place)");
+  check_written_pool(pool);
   const at::Device dev = pool.device();
-  at::Tensor k_new = half_rows("k_new", k_new_), v_new = half_rows("v_new", v_new_);
+  const at::ScalarType dt = pool.scalar_type();
+  at::Tensor k_new = rows_like("k_new", k_new_, dt, "paged_kv_cache"),
+             v_new = rows_like("v_new", v_new_, dt, "paged_kv_cache");
   same_device("k_new", k_new, dev);
   same_device("v_new", v_new, dev);
   at::Tensor ap = int32_on("append_indptr", append_indptr, dev).contiguous();
@@ -472,6 +515,183 @@ void append_paged_kv(const at::Tensor& k_new_, const at::Tensor& v_new_,
                                (const int32_t*)ptr(last), B, k_new.size(0), Hkv, D, page, P, ks.v,
                                vs.v, ps.v, stream_of(pool)),
            "akt_paged_kv_append");
+}
+
+// --------------------------------------------------------------------------- chunk attention
+py::object chunk_paged(const at::Tensor& q_, const at::Tensor& q_indptr_, const at::Tensor& pool_,
+                       const at::Tensor& indptr_, const at::Tensor& indices_,
+                       const at::Tensor& last_, bool causal,
+                       const c10::optional<double>& softmax_scale, bool return_lse) {
+  need_gpu("q", q_);
+  const int dtype = dtype16("q", q_);
+  if (q_.dim() != 3) throw py::value_error("q must be [total_q, Hq, D]");
+  if (pool_.dim() != 5 || pool_.size(1) != 2)
+    throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
+  at::Tensor q = rows16(q_), pool = rows_like("paged_kv_cache", pool_, q_.scalar_type(), "q");
+  const at::Device dev = q.device();
+  same_device("paged_kv_cache", pool, dev);
+  at::Tensor q_indptr = int32_on("q_indptr", q_indptr_, dev).contiguous();
+  at::Tensor indptr = int32_on("kv_page_indptr", indptr_, dev).contiguous();
+  at::Tensor indices = int32_on("kv_page_indices", indices_, dev).contiguous();
+  at::Tensor last = int32_on("kv_last_page_len", last_, dev).contiguous();
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
+  const int64_t P = pool.size(0), Hkv = pool.size(2), page = pool.size(3), B = last.numel();
+  if (pool.size(4) != D)
+    throw py::value_error("head_dim mismatch: q has " + std::to_string(D) + ", cache has " +
+                          std::to_string(pool.size(4)));
+  if (q_indptr.numel() != B + 1 || indptr.numel() != B + 1)
+    throw py::value_error("q_indptr and kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  const float scale = softmax_scale.has_value() ? (float)*softmax_scale
+                                                : (float)(1.0 / std::sqrt((double)D));
+  const DeviceGuard guard(dev);
+  at::Tensor o = at::empty({T, Hq, D}, q.options());
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({T, Hq}, q.options().dtype(at::kFloat));
+  const int64_t total = indices.numel();
+  hipStream_t st = stream_of(q);
+  const size_t ws_n = akt_chunk_paged_workspace_size(B, T, Hq, Hkv, D, page, total);
+  at::Tensor ws = capture_workspace(ws_n, dev, st);
+  const Strides qs = strides_of(q), ps = strides_of(pool);
+  check_rc(akt_chunk_paged_fwd(ptr(q), (const int32_t*)ptr(q_indptr), ptr(pool),
+                               (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices),
+                               (const int32_t*)ptr(last), ptr(o), (float*)ptr(lse), B, T, Hq, Hkv,
+                               D, page, total, P, qs.v, ps.v, scale, causal ? 1 : 0, dtype, ptr(ws),
+                               ws_n, st),
+           "akt_chunk_paged_fwd");
+  return result(o, lse, return_lse);
+}
+
+// --------------------------------------------------------------------------- rotary
+at::Tensor frequencies(const at::Tensor& inv_freq, const at::Device& dev) {
+  need_gpu("inv_freq", inv_freq);
+  same_device("inv_freq", inv_freq, dev);
+  if (inv_freq.scalar_type() != at::kDouble)
+    throw py::type_error("inv_freq must be float64, got " +
+                         std::string(c10::toString(inv_freq.scalar_type())));
+  if (inv_freq.dim() != 1) throw py::value_error("inv_freq must be [rotary_dim / 2]");
+  return inv_freq.contiguous();
+}
+
+// Q [B, Hq, S, D] and (unless None) K [B, Hkv, S, D] -> rotated copies.
+py::tuple rotary(const at::Tensor& Q_, const c10::optional<at::Tensor>& K_,
+                 const at::Tensor& inv_freq_, const c10::optional<at::Tensor>& positions_,
+                 bool interleaved, double factor, bool transpose) {
+  need_gpu("Q", Q_);
+  const int dtype = dtype16("Q", Q_);
+  if (Q_.dim() != 4) throw py::value_error("Q must be [B, Hq, S, D]");
+  at::Tensor Q = rows16(Q_), K;
+  const at::Device dev = Q.device();
+  const int64_t B = Q.size(0), Hq = Q.size(1), S = Q.size(2), D = Q.size(3);
+  int64_t Hkv = 0;
+  if (K_.has_value() && K_->defined()) {
+    K = rows_like("K", *K_, Q.scalar_type(), "Q");
+    same_device("K", K, dev);
+    if (K.dim() != 4 || K.size(0) != B || K.size(2) != S || K.size(3) != D)
+      throw py::value_error("K " + c10::str(K.sizes()) + " does not match Q " +
+                            c10::str(Q.sizes()) + " in batch, sequence length or head dim");
+    Hkv = K.size(1);
+  }
+  at::Tensor inv_freq = frequencies(inv_freq_, dev);
+  at::Tensor pos;
+  int64_t pstride[2] = {0, 0};
+  int pbits = 0;
+  if (positions_.has_value() && positions_->defined()) {
+    pos = *positions_;
+    need_gpu("positions", pos);
+    same_device("positions", pos, dev);
+    if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong)
+      throw py::type_error("positions must be int32 or int64, got " +
+                           std::string(c10::toString(pos.scalar_type())));
+    const bool per_row = pos.dim() == 2;
+    if ((pos.dim() != 1 && !per_row) || pos.size(-1) != S || (per_row && pos.size(0) != B))
+      throw py::value_error("positions must be [S] or [B, S] = [" + std::to_string(B) + ", " +
+                            std::to_string(S) + "], got " + c10::str(pos.sizes()));
+    pstride[0] = per_row ? pos.stride(0) : 0;
+    pstride[1] = pos.stride(-1);
+    pbits = pos.scalar_type() == at::kLong ? 64 : 32;
+  }
+  const DeviceGuard guard(dev);
+  at::Tensor Qo = at::empty({B, Hq, S, D}, Q.options()), Ko;
+  if (K.defined()) Ko = at::empty({B, Hkv, S, D}, Q.options());
+  if (Hq == 0 && Hkv > 0) throw py::value_error("Q must have a head");
+  if (Hq > 0) {
+    const Strides qs = strides_of(Q);
+    Strides ks;
+    if (K.defined()) ks = strides_of(K);
+    check_rc(akt_rotary_fwd(ptr(Q), ptr(K), ptr(Qo), ptr(Ko), (const double*)ptr(inv_freq),
+                            ptr(pos), pbits, B, Hq, Hkv, S, D, 2 * inv_freq.numel(), qs.v, ks.v,
+                            pstride, interleaved ? 1 : 0, transpose ? 1 : 0, (float)factor, dtype,
+                            stream_of(Q)),
+             "akt_rotary_fwd");
+  }
+  return py::make_tuple(Qo, K.defined() ? py::cast(Ko) : py::object(py::none()));
+}
+
+// q, k_new rotated by their positions, k_new and v_new appended; returns the rotated q.
+at::Tensor append_paged_kv_rotary(const at::Tensor& q_, const at::Tensor& k_new_,
+                                  const at::Tensor& v_new_, const at::Tensor& append_indptr,
+                                  const at::Tensor& pool, const at::Tensor& indptr_,
+                                  const at::Tensor& indices_, const at::Tensor& last_,
+                                  const at::Tensor& inv_freq_, bool interleaved, double factor) {
+  need_gpu("paged_kv_cache", pool);
+  const int dtype = check_written_pool(pool);
+  const at::Device dev = pool.device();
+  const at::ScalarType dt = pool.scalar_type();
+  at::Tensor q = rows_like("q", q_, dt, "paged_kv_cache"),
+             k_new = rows_like("k_new", k_new_, dt, "paged_kv_cache"),
+             v_new = rows_like("v_new", v_new_, dt, "paged_kv_cache");
+  same_device("q", q, dev);
+  same_device("k_new", k_new, dev);
+  same_device("v_new", v_new, dev);
+  at::Tensor ap = int32_on("append_indptr", append_indptr, dev).contiguous();
+  at::Tensor indptr = int32_on("kv_page_indptr", indptr_, dev).contiguous();
+  at::Tensor indices = int32_on("kv_page_indices", indices_, dev).contiguous();
+  at::Tensor last = int32_on("kv_last_page_len", last_, dev).contiguous();
+  at::Tensor inv_freq = frequencies(inv_freq_, dev);
+  const int64_t P = pool.size(0), Hkv = pool.size(2), page = pool.size(3), D = pool.size(4);
+  if (k_new.dim() != 3 || k_new.size(1) != Hkv || k_new.size(2) != D ||
+      v_new.sizes() != k_new.sizes())
+    throw py::value_error("k_new / v_new must be [total_new, " + std::to_string(Hkv) + ", " +
+                          std::to_string(D) + "]");
+  if (q.dim() != 3 || q.size(0) != k_new.size(0) || q.size(2) != D)
+    throw py::value_error("q must be [" + std::to_string(k_new.size(0)) + ", Hq, " +
+                          std::to_string(D) + "] like k_new");
+  const int64_t B = last.numel();
+  if (ap.numel() != B + 1 || indptr.numel() != B + 1)
+    throw py::value_error("append_indptr and kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  const DeviceGuard guard(dev);
+  at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  const Strides qs = strides_of(q), ks = strides_of(k_new), vs = strides_of(v_new),
+                ps = strides_of(pool);
+  check_rc(akt_paged_kv_append_rotary(
+               ptr(q), ptr(k_new), ptr(v_new), ptr(out), (const int32_t*)ptr(ap), ptr(pool),
+               (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices), (const int32_t*)ptr(last),
+               (const double*)ptr(inv_freq), B, q.size(0), q.size(1), Hkv, D, 2 * inv_freq.numel(),
+               page, indices.numel(), P, qs.v, ks.v, vs.v, ps.v, interleaved ? 1 : 0, (float)factor,
+               dtype, stream_of(pool)),
+           "akt_paged_kv_append_rotary");
+  return out;
+}
+
+// --------------------------------------------------------------------------- page copies
+void copy_pages(const at::Tensor& pool, const at::Tensor& src_, const at::Tensor& dst_,
+                const c10::optional<at::Tensor>& num_tokens) {
+  need_gpu("paged_kv_cache", pool);
+  check_written_pool(pool);
+  const at::Device dev = pool.device();
+  at::Tensor src = int32_on("src", src_, dev).contiguous();
+  at::Tensor dst = int32_on("dst", dst_, dev).contiguous();
+  at::Tensor tok;
+  if (num_tokens.has_value() && num_tokens->defined())
+    tok = int32_on("num_tokens", *num_tokens, dev).contiguous();
+  if (src.dim() != 1 || dst.sizes() != src.sizes() || (tok.defined() && tok.sizes() != src.sizes()))
+    throw py::value_error("src, dst and num_tokens must be 1-D and of one length");
+  const DeviceGuard guard(dev);
+  const Strides ps = strides_of(pool);
+  check_rc(akt_paged_copy(ptr(pool), (const int32_t*)ptr(src), (const int32_t*)ptr(dst),
+                          (const int32_t*)ptr(tok), src.numel(), pool.size(2), pool.size(4),
+                          pool.size(3), pool.size(0), ps.v, stream_of(pool)),
+           "akt_paged_copy");
 }
 
 // --------------------------------------------------------------------------- LSE merge
@@ -555,6 +775,19 @@ PYBIND11_MODULE(_akt_torch, m) {
   m.def("append_paged_kv", &append_paged_kv, py::arg("k_new"), py::arg("v_new"),
         py::arg("append_indptr"), py::arg("paged_kv_cache"), py::arg("kv_page_indptr"),
         py::arg("kv_page_indices"), py::arg("kv_last_page_len"));
+  m.def("chunk_paged", &chunk_paged, py::arg("q"), py::arg("q_indptr"), py::arg("paged_kv_cache"),
+        py::arg("kv_page_indptr"), py::arg("kv_page_indices"), py::arg("kv_last_page_len"),
+        py::arg("causal") = true, py::arg("softmax_scale") = py::none(),
+        py::arg("return_lse") = false);
+  m.def("rotary", &rotary, py::arg("Q"), py::arg("K"), py::arg("inv_freq"),
+        py::arg("positions") = py::none(), py::arg("interleaved") = false,
+        py::arg("factor") = 1.0, py::arg("transpose") = false);
+  m.def("append_paged_kv_rotary", &append_paged_kv_rotary, py::arg("q"), py::arg("k_new"),
+        py::arg("v_new"), py::arg("append_indptr"), py::arg("paged_kv_cache"),
+        py::arg("kv_page_indptr"), py::arg("kv_page_indices"), py::arg("kv_last_page_len"),
+        py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("factor") = 1.0);
+  m.def("copy_pages", &copy_pages, py::arg("paged_kv_cache"), py::arg("src"), py::arg("dst"),
+        py::arg("num_tokens") = py::none());
   m.def("merge_states", &merge_states, py::arg("o"), py::arg("lse"), py::arg("out_f32"));
   m.def("workspaces", &workspaces);
 }

@@ -9,16 +9,22 @@ This module fills them:
 - ``append_paged_kv`` runs the HIP kernel ``akt_paged_kv_append``: each
   sequence's new K/V rows become its last logical positions under an
   already-updated page table.
+- ``append_paged_kv_rotary`` does the same for k that still has to be rotated by
+  its positions, and rotates q with it (``akt_paged_kv_append_rotary``).
+- ``copy_pages`` copies pages within a pool (``akt_paged_copy``).
 - ``PagedKVCache`` owns a pool and a free list on the host, grows each
   sequence's page list as tokens are appended (prefill chunks or one token
   per decode step), and hands out the page table the decode entry points
-  take.  Page bookkeeping is host-side; only the copy runs on the GPU.
+  take.  Sequences may share pages (``fork``); a shared page that is about
+  to be written is copied first.  Page bookkeeping is host-side; only the copies
+  and the attention run on the GPU.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _native as N
+from . import _ops
 
 
 def append_paged_kv(k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
@@ -26,11 +32,36 @@ def append_paged_kv(k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
     """Scatter k_new / v_new [total_new, Hkv, D] into paged_kv_cache [P, 2, Hkv, page, D].
 
     Sequence b's rows append_indptr[b]:append_indptr[b+1] become its last
-    positions under the page table (which must already count them).  Runs
-    asynchronously on the current stream.
+    positions under the page table (which must already count them).  fp16 or
+    bf16, one type.  Runs asynchronously on the current stream.
     """
     N.torch_ext().append_paged_kv(k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
                                   kv_page_indices, kv_last_page_len)
+
+
+def append_paged_kv_rotary(q, k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
+                           kv_page_indices, kv_last_page_len, inv_freq, interleaved=False,
+                           factor=1.0):
+    """append_paged_kv of k_new rotated by its positions; returns q rotated by the same ones.
+
+    q [total_new, Hq, D] has a row for every row of k_new / v_new [total_new, Hkv, D].  A row's
+    position is the one it takes in its sequence; inv_freq (float64 [rotary_dim / 2]),
+    interleaved and factor as in rotary.apply_rotary.  fp16 or bf16, one type.  Rows of q that
+    belong to no sequence are left unwritten.
+    """
+    return N.torch_ext().append_paged_kv_rotary(q, k_new, v_new, append_indptr, paged_kv_cache,
+                                                kv_page_indptr, kv_page_indices, kv_last_page_len,
+                                                inv_freq, interleaved=interleaved, factor=factor)
+
+
+def copy_pages(paged_kv_cache, src, dst, num_tokens=None) -> None:
+    """Copy pages src[i] to dst[i] within paged_kv_cache, K and V of every head.
+
+    src, dst (and num_tokens: the slots to copy of each, default all) are int32 device tensors
+    [N].  The copies run at once: no page may be a destination twice, or a source and a
+    destination.  Pairs that name a page outside the pool are skipped.
+    """
+    N.torch_ext().copy_pages(paged_kv_cache, src, dst, num_tokens=num_tokens)
 
 
 class PagedKVCache:
@@ -40,6 +71,11 @@ class PagedKVCache:
     >>> cache.append([7, 9], k, v, [300, 12])       # prefill chunks
     >>> cache.append([7, 9], k1, v1, [1, 1])        # one decode step
     >>> indptr, indices, last = cache.page_table([7, 9])
+    >>> cache.fork(7, 8)                            # 8 continues 7's tokens, sharing its pages
+    >>> o = cache.extend([7, 8], q, k, v, [4, 1], inv_freq=inv_freq)  # rotate, append, attend
+
+    A page table describes the cache as it is: append, extend, fork, truncate,
+    release and compact make the tables handed out before them stale.
     """
 
     def __init__(self, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
@@ -50,6 +86,7 @@ class PagedKVCache:
         self._free = list(range(num_pages - 1, -1, -1))  # pop() hands out page 0 first
         self._pages: dict = {}
         self._len: dict = {}
+        self._refs = [0] * num_pages  # sequences that hold each page
 
     @property
     def free_pages(self) -> int:
@@ -58,20 +95,104 @@ class PagedKVCache:
     def seq_len(self, seq_id) -> int:
         return self._len.get(seq_id, 0)
 
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._refs[page] = 1
+        return page
+
+    def _drop(self, pages) -> None:
+        for page in pages:
+            self._refs[page] -= 1
+            if self._refs[page] == 0:
+                self._free.append(page)
+
     def release(self, seq_id) -> None:
-        """Return a sequence's pages to the free list."""
-        self._free.extend(reversed(self._pages.pop(seq_id, [])))
+        """Drop a sequence; pages that no other sequence holds return to the free list."""
+        self._drop(reversed(self._pages.pop(seq_id, [])))
         self._len.pop(seq_id, None)
 
-    def _grow(self, seq_id, n: int) -> None:
-        pages = self._pages.setdefault(seq_id, [])
-        new_len = self._len.get(seq_id, 0) + n
-        need = -(-new_len // self.page_size) - len(pages)
+    def truncate(self, seq_id, length: int) -> None:
+        """Forget a sequence's tokens from position `length` on (rejected drafts, say)."""
+        if not 0 <= length <= self.seq_len(seq_id):
+            raise ValueError(f"length {length} is not in [0, {self.seq_len(seq_id)}]")
+        if seq_id not in self._pages:
+            return
+        keep = -(-length // self.page_size)
+        pages = self._pages[seq_id]
+        self._drop(reversed(pages[keep:]))
+        del pages[keep:]
+        self._len[seq_id] = length
+
+    def fork(self, seq_id, new_id) -> None:
+        """Start sequence new_id with seq_id's tokens.  No data moves: the two share pages until
+        one of them writes into a shared one, which it then copies (append, extend)."""
+        if seq_id not in self._pages:
+            raise KeyError(f"no sequence {seq_id!r}")
+        if new_id in self._pages:
+            raise ValueError(f"sequence {new_id!r} exists")
+        for page in self._pages[seq_id]:
+            self._refs[page] += 1
+        self._pages[new_id] = list(self._pages[seq_id])
+        self._len[new_id] = self._len[seq_id]
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool, so that the free ones are its tail
+        (pool[num_pages - free_pages:]).  Returns the number of pages moved."""
+        used = self.pool.shape[0] - len(self._free)
+        holes = sorted(p for p in self._free if p < used)
+        moved = {p: q for p, q in zip((p for p in range(used, len(self._refs)) if self._refs[p]),
+                                      holes)}
+        if not moved:
+            return 0
+        t = torch.tensor([list(moved), list(moved.values())], dtype=torch.int32,
+                         device=self.pool.device)
+        copy_pages(self.pool, t[0], t[1])
+        for src, dst in moved.items():
+            self._refs[dst], self._refs[src] = self._refs[src], 0
+        for pages in self._pages.values():
+            pages[:] = [moved.get(p, p) for p in pages]
+        self._free = list(range(self.pool.shape[0] - 1, used - 1, -1))
+        return len(moved)
+
+    def _grow(self, seq_ids, counts) -> None:
+        """Room for counts[i] more tokens of seq_ids[i].  Last pages that tokens will go into are
+        copied where they are shared.  Nothing changes if the pages do not suffice."""
+        if len(counts) != len(seq_ids):
+            raise ValueError("one count per sequence")
+        if any(n < 0 for n in counts):
+            raise ValueError("counts must be non-negative")
+        growing = [(s, int(n)) for s, n in zip(seq_ids, counts) if n]
+        if len({s for s, _ in growing}) != len(growing):
+            raise ValueError("a sequence can take new tokens once in a call")
+        need, refs = 0, {}
+        for s, n in growing:
+            pages, length = self._pages.get(s, []), self._len.get(s, 0)
+            need += -(-(length + n) // self.page_size) - len(pages)
+            if length % self.page_size:
+                last = pages[-1]
+                refs[last] = refs.get(last, self._refs[last])
+                if refs[last] > 1:  # of the sequences of this call, the last keeps the page
+                    refs[last] -= 1
+                    need += 1
         if need > len(self._free):
             raise MemoryError(f"page pool exhausted: need {need} pages, {len(self._free)} free")
-        for _ in range(need):
-            pages.append(self._free.pop())
-        self._len[seq_id] = new_len
+        for s in seq_ids:
+            self._pages.setdefault(s, [])
+            self._len.setdefault(s, 0)
+        copies = []
+        for s, n in growing:
+            pages, length = self._pages[s], self._len[s]
+            if length % self.page_size and self._refs[pages[-1]] > 1:
+                page = self._take()
+                copies.append((pages[-1], page, length % self.page_size))
+                self._refs[pages[-1]] -= 1
+                pages[-1] = page
+            for _ in range(-(-(length + n) // self.page_size) - len(pages)):
+                pages.append(self._take())
+            self._len[s] = length + n
+        if copies:
+            t = torch.tensor(copies, dtype=torch.int32, device=self.pool.device).t().contiguous()
+            copy_pages(self.pool, t[0], t[1], num_tokens=t[2])
 
     def page_table(self, seq_ids):
         """(kv_page_indptr, kv_page_indices, kv_last_page_len) int32 device tensors."""
@@ -86,24 +207,40 @@ class PagedKVCache:
         mk = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
         return mk(indptr), mk(indices), mk(last)
 
+    def _indptr(self, counts):
+        ap = [0]
+        for n in counts:
+            ap.append(ap[-1] + int(n))
+        return torch.tensor(ap, dtype=torch.int32, device=self.pool.device)
+
     def append(self, seq_ids, k_new, v_new, counts):
         """Append counts[i] rows of k_new / v_new [sum(counts), Hkv, D] to seq_ids[i].
 
         Returns the batch's page table after the append.
         """
-        if len(counts) != len(seq_ids):
-            raise ValueError("one count per sequence")
-        for s, n in zip(seq_ids, counts):
-            if n < 0:
-                raise ValueError("counts must be non-negative")
-            self._grow(s, int(n))
+        self._grow(seq_ids, counts)
         indptr, indices, last = self.page_table(seq_ids)
-        ap = [0]
-        for n in counts:
-            ap.append(ap[-1] + int(n))
-        append_paged_kv(k_new, v_new, torch.tensor(ap, dtype=torch.int32, device=self.pool.device),
-                        self.pool, indptr, indices, last)
+        append_paged_kv(k_new, v_new, self._indptr(counts), self.pool, indptr, indices, last)
         return indptr, indices, last
 
+    def extend(self, seq_ids, q, k_new, v_new, counts, inv_freq=None, interleaved=False,
+               factor=1.0, causal=True, softmax_scale=None, return_lse=False):
+        """One attention step: append counts[i] tokens to seq_ids[i] and attend with them.
 
-__all__ = ["append_paged_kv", "PagedKVCache"]
+        q [sum(counts), Hq, D], k_new and v_new [sum(counts), Hkv, D]; with inv_freq, q and k_new
+        are rotated by the tokens' positions first (append_paged_kv_rotary).  Returns what
+        flash_attention_chunk_paged returns for q over the grown cache.
+        """
+        self._grow(seq_ids, counts)
+        table = self.page_table(seq_ids)
+        q_indptr = self._indptr(counts)
+        if inv_freq is None:
+            append_paged_kv(k_new, v_new, q_indptr, self.pool, *table)
+        else:
+            q = append_paged_kv_rotary(q, k_new, v_new, q_indptr, self.pool, *table, inv_freq,
+                                       interleaved=interleaved, factor=factor)
+        return _ops.chunk_paged(q, q_indptr, self.pool, *table, causal=causal,
+                                softmax_scale=softmax_scale, return_lse=return_lse)
+
+
+__all__ = ["append_paged_kv", "append_paged_kv_rotary", "copy_pages", "PagedKVCache"]

@@ -18,8 +18,9 @@
  * only by calls ordered on one stream (calls that overlap in time must use
  * different workspaces).
  *
- * Tensor element types: q/k/v/o and KV pools are IEEE fp16 (akt_prefill_fwd_ex
- * also takes bf16); page tables, kept-token indices and counts are int32;
+ * Tensor element types: q/k/v/o and KV pools are IEEE fp16 (entry points with a dtype
+ * argument also take bf16, and akt_paged_kv_append and akt_paged_copy move any 2-byte
+ * elements); page tables, kept-token indices and counts are int32;
  * MagicPIG K/L and LSE are fp32.
  * Strides are in elements.  The innermost (head_dim) stride must be 1 and
  * every row must start 16-byte aligned.
@@ -39,6 +40,9 @@
  *   sparse_decode_flash_attention.py:13-15 (CSR index note)   akt_sparse_decode_*csr_fwd
  *   decode_flash_attention_redundant_var_len_paged.py:349-353 (page tables, harness)
  *                                                        akt_paged_kv_append
+ * Without a counterpart there: akt_chunk_paged_fwd, akt_rotary_fwd,
+ * akt_paged_kv_append_rotary and akt_paged_copy, which serve a paged cache beyond
+ * single-token decode.
  */
 #ifndef AKT_AMD_H
 #define AKT_AMD_H
@@ -352,6 +356,94 @@ int akt_paged_kv_append(const void* k_new, const void* v_new, const int32_t* app
                         int64_t head_dim, int64_t page_size, int64_t num_pool_pages,
                         const int64_t k_new_stride[3], const int64_t v_new_stride[3],
                         const int64_t kv_stride[5], void* stream);
+
+/*
+ * Attention of several new tokens per sequence over a paged cache (chunked
+ * prefill, verification of drafted tokens, mixed batches, single tokens).  No
+ * reference counterpart.
+ *   q: [total_q, num_q_heads, head_dim], strides q_stride[3]; sequence b's n_b query
+ *   tokens are rows q_indptr[b] .. q_indptr[b+1] - 1 (int32 [batch+1]).
+ *   kv_cache and page table as akt_decode_paged_fwd; len_b counts the new tokens, whose
+ *   K and V the caller has written (akt_paged_kv_append).
+ *   causal != 0: query i of sequence b sits at position len_b - n_b + i and sees the keys
+ *   0 .. that position; 0: every query sees all len_b keys.
+ *   o: contiguous [total_q, num_q_heads, head_dim]; lse: optional contiguous fp32
+ *   [total_q, num_q_heads], ln sum_j exp(softmax_scale q.k_j).  Rows that see no key get
+ *   o = 0 and lse = -inf; rows of q that belong to no sequence are not written.
+ *   Keys of pages outside [0, num_pool_pages) are skipped.  q_indptr must lie in
+ *   [0, total_q] and kv_page_indptr in [0, total_pages], neither decreasing; entries
+ *   that do not are taken clamped and touch nothing outside the arrays.
+ *   Masked K and V (later tokens, slots past len_b, skipped pages) never reach a row,
+ *   whatever they hold.  dtype: AKT_DTYPE_F16 or AKT_DTYPE_BF16 (q, kv_cache and o; P is
+ *   rounded to it for P.V, the sums are fp32).  head_dim: 64, 128 or 256;
+ *   num_q_heads / num_kv_heads up to 128; total_pages * page_size below 2^30.
+ *   The workspace follows the decode entry points' contract and may be shared with them;
+ *   its size depends on the current device.
+ */
+size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q, int64_t num_q_heads,
+                                      int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                      int64_t total_pages);
+int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
+                        const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+                        const int32_t* kv_last_page_len, void* o, float* lse, int64_t batch,
+                        int64_t total_q, int64_t num_q_heads, int64_t num_kv_heads,
+                        int64_t head_dim, int64_t page_size, int64_t total_pages,
+                        int64_t num_pool_pages, const int64_t q_stride[3],
+                        const int64_t kv_stride[5], float softmax_scale, int causal, int dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions of dense q [batch, num_q_heads, seq_len, head_dim] and, with
+ * num_kv_heads > 0, k [batch, num_kv_heads, seq_len, head_dim], into contiguous q_out and
+ * k_out.  No reference counterpart.
+ *   Frequency f < rotary_dim / 2 turns dims (f, f + rotary_dim / 2), or (2 f, 2 f + 1) when
+ *   interleaved, at position t by the angle t * inv_freq[f] (device fp64
+ *   [rotary_dim / 2]; the angle is formed in 64 bits) and scales them by factor; dims from
+ *   rotary_dim on are copied.  transpose != 0 applies the transposed map: the
+ *   negative angles, the same factor (the gradient of the inputs from that of the
+ *   outputs; at factor 1 the inverse).
+ *   positions: optional device array, element (b, s) at b * position_stride[0] +
+ *   s * position_stride[1], int32 or int64 by position_bits; NULL: 0 .. seq_len - 1.
+ *   head_dim: a multiple of 8 up to 1024; rotary_dim: even, up to head_dim.
+ *   dtype: AKT_DTYPE_F16 or AKT_DTYPE_BF16.
+ */
+int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k_out,
+                   const double* inv_freq, const void* positions, int position_bits,
+                   int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t seq_len,
+                   int64_t head_dim, int64_t rotary_dim, const int64_t q_stride[4],
+                   const int64_t k_stride[4], const int64_t position_stride[2], int interleaved,
+                   int transpose, float factor, int dtype, void* stream);
+
+/*
+ * akt_paged_kv_append with rotary positions: k_new is rotated (as akt_rotary_fwd) by its
+ * token's position in its sequence and written into the pool, v_new is written as it is,
+ * and q [total_new, num_q_heads, head_dim] (rows as k_new's) is rotated by the same
+ * positions into contiguous q_out.  A token whose page lies outside the table or pool is
+ * not stored, its q is rotated; rows that belong to no sequence are not written.
+ * No reference counterpart.
+ */
+int akt_paged_kv_append_rotary(const void* q, const void* k_new, const void* v_new, void* q_out,
+                               const int32_t* append_indptr, void* kv_cache,
+                               const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+                               const int32_t* kv_last_page_len, const double* inv_freq,
+                               int64_t batch, int64_t total_new, int64_t num_q_heads,
+                               int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim,
+                               int64_t page_size, int64_t total_pages, int64_t num_pool_pages,
+                               const int64_t q_stride[3], const int64_t k_new_stride[3],
+                               const int64_t v_new_stride[3], const int64_t kv_stride[5],
+                               int interleaved, float factor, int dtype, void* stream);
+
+/*
+ * Copies the first num_tokens[i] slots (NULL: all page_size; clamped to [0, page_size]) of
+ * page src[i] to page dst[i], K and V of every head, for i < n.  A pair with a page outside
+ * [0, num_pool_pages), or the same page twice, is skipped.  All copies of a call run at
+ * once: no page may be the destination of two of them, or the source of one and
+ * the destination of another.  No reference counterpart.
+ */
+int akt_paged_copy(void* kv_cache, const int32_t* src, const int32_t* dst,
+                   const int32_t* num_tokens, int64_t n, int64_t num_kv_heads, int64_t head_dim,
+                   int64_t page_size, int64_t num_pool_pages, const int64_t kv_stride[5],
+                   void* stream);
 
 /*
  * Kept-token index selection (the reference harness step at
