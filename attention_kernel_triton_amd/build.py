@@ -46,10 +46,12 @@ COMMON_FLAGS = [
 # prefill instances (one wave per SIMD): LLVM's iterative ILP scheduler runs them
 # 8-12% faster than the default one (1-2% slower for the D = 64 instances in
 # prefill.hip), and MFMA results selected into VGPRs save the copies between
-# AGPRs and VGPRs (a further 14% with V read a step ahead).
+# AGPRs and VGPRs (a further 14% with V read a step ahead).  The D = 256 instances of
+# the chunk attention kernels spill without the latter.
 SOURCE_FLAGS = {
     "prefill_wide.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp",
                          "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_chunk_256.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -39,14 +39,15 @@
 // Keys past the unit's last one and keys of pages outside the pool read as zeros
 // and score -inf.
 //
-// Masked values.  Scores are masked with a select.  V rows are multiplied by
-// probabilities of zero where some of the unit's rows see them and some do not, which an
-// infinity or NaN in V would turn into NaN: where a tile on the diagonal holds one, P.V is
-// computed key by key and added to the rows that see the key (pv_by_key).
+// Masked values.  Scores are masked with a select.  V rows that some of the unit's rows see
+// and some do not are multiplied by zeros too, which an infinity or NaN in V would turn into
+// NaN: those are staged as zeros and, in the rare unit that has any, added at its end to
+// the rows that see them (add_not_finite).
 #include <float.h>
 #include <math.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "akt_host.hpp"
 #include "attn_tile.hpp"
@@ -127,7 +128,50 @@ struct Unit {
   int ip0;    // first page table entry of the sequence
 };
 
-template <int D, bool BF16, bool GRP, bool LSE>
+// Replaces the infinities and NaNs of a 16-byte chunk by zeros; true if there were any.
+template <bool BF16>
+__device__ __forceinline__ bool zero_not_finite(uint4_t& v) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  bool any = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const bool lo = (v[w] & kExp) == kExp, hi = (v[w] & (kExp << 16)) == (kExp << 16);
+    v[w] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+    any |= lo || hi;
+  }
+  return any;
+}
+
+// Adds the infinities and NaNs of keys j0 .. j1 - 1 of V, which were staged as zeros, to the O
+// of the rows that see them (a key's probability is positive).  Lane (l32, g) holds dims 32 n + 8 k + 4 g .. + 3 of row l32, whose last key is lim.
+template <int D, bool BF16>
+__device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit& u, int j0, int j1,
+                                               int g, int lim, float16_t (&oacc)[D / 32]) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+#pragma clang loop unroll(disable)
+  for (int j = j0; j < j1; ++j) {
+    const int lp = page_of(p, j), id = p.indices[u.ip0 + lp];
+    if ((uint32_t)id >= (uint32_t)p.num_pool_pages || j > lim) continue;
+    const half_t* row = p.pool + id * p.sp + p.skv + u.kvh * p.sh +
+                        (int64_t)(j - lp * p.page_size) * p.ss + 4 * g;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint2 v = *reinterpret_cast<const uint2*>(row + 32 * n + 8 * k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = ((i < 2 ? v.x : v.y) >> (16 * (i & 1))) & 0xffffu;
+          float f;
+          if constexpr (BF16) f = __uint_as_float(x << 16);
+          else f = (float)__builtin_bit_cast(half_t, (uint16_t)x);
+          oacc[n][4 * k + i] += (x & kExp) == kExp ? f : 0.f;
+        }
+      }
+  }
+}
+
+template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT>
 __global__ __launch_bounds__(kCkThreads)
 __attribute__((amdgpu_waves_per_eu(chunk_wgs_per_cu(D), chunk_wgs_per_cu(D))))
 void paged_chunk_kernel(ChunkParams p) {
@@ -146,33 +190,35 @@ void paged_chunk_kernel(ChunkParams p) {
   constexpr int RPC = 64 / CPR;                  // rows of a wave's 64 chunks
   static_assert(16 % RPC == 0, "a wave's chunks lie in one 16-key group");
   __shared__ __attribute__((aligned(16))) char lds[kCkNBuf * BUFB];
+  __shared__ float4_t sm_ml[4][32];
+  __shared__ int sm_bad[4];
 
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int wave = uniform(tid >> 6);
-  const int l32 = lane & 31;
-  const int g = lane >> 5;
+  const int tid0 = threadIdx.x;
+  const int wave = uniform(tid0 >> 6);
 
   // ---- this workgroup's range of the axis.  Workgroup i runs on XCD i % 8, so
   // consecutive ranges go to one XCD's L2.
   const int W = p.wgs;
   const int wg = W % 8 == 0 ? (int)(blockIdx.x % 8) * (W / 8) + (int)(blockIdx.x / 8)
                             : (int)blockIdx.x;
+  const int lane0 = tid0 & 63;
+  // The sequences that this kernel serves.
+  auto mine = [&](const Seq& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
   auto seq_length = [&](int b) -> int64_t {
     if (b >= p.B) return 0;
     const Seq s = load_seq(p, b);
-    return head_length(p, s) * p.Hkv;
+    return mine(s) ? head_length(p, s) * p.Hkv : 0;
   };
   auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int64_t u = shfl64(v, lane - d < 0 ? 0 : lane - d);
-      if (lane >= d) v += u;
+      const int64_t u = shfl64(v, lane0 - d < 0 ? 0 : lane0 - d);
+      if (lane0 >= d) v += u;
     }
     return v;
   };
   int64_t total = 0;
-  for (int jb = 0; jb < p.B; jb += 64) total += uniform64(shfl64(scan64(seq_length(jb + lane)), 63));
+  for (int jb = 0; jb < p.B; jb += 64) total += uniform64(shfl64(scan64(seq_length(jb + lane0)), 63));
   int64_t Lw = (total + W - 1) / W;
   if (Lw < p.min_keys) Lw = p.min_keys;
   Lw = uniform64(Lw);
@@ -182,7 +228,7 @@ void paged_chunk_kernel(ChunkParams p) {
   int b = 0;
   int64_t U = 0;  // the sequence's start
   for (int jb = 0;; jb += 64) {
-    const int64_t len = seq_length(jb + lane);
+    const int64_t len = seq_length(jb + lane0);
     const int64_t inc = scan64(len);
     const uint64_t m = __ballot(U + inc > x0);
     if (m) {
@@ -208,28 +254,31 @@ void paged_chunk_kernel(ChunkParams p) {
     }
   }
 
-  // ---- per-lane constants
   const float c = p.qk_scale;
-  // K rows for S^T: key l32 of the step, chunks g * HALF / 8 + s.
-  int koff[KS];
-#pragma unroll
-  for (int k = 0; k < KS; ++k) koff[k] = l32 * ROWB + (((g * HALF / 8) + k) ^ tswz<D>(l32)) * 16;
-  // V^T through the transposing read: see prefill_kernel.
-  const int s16 = lane & 15;
-  const int vrow = 4 * g + (s16 >> 2);
-  const int vcl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
-  int voff[NT], voffh[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    voff[n] = TILEB + vrow * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow)) * 16) + (s16 & 1) * 8;
-    voffh[n] =
-        TILEB + (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
-  }
-  const int lrow = 32 * wave + l32;                          // this lane's row of the unit
-  const int ltok = (int)((uint32_t)lrow * p.g_magic >> 16);  // and its token
-
   // ---- the keys [k0, k1) of a unit, for all four waves.
   auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
+    // The lane number is opaque here, so that what is derived from it lives no longer than
+    // this part (held across the units' loop it would not fit the registers).
+    int lane = tid0 & 63;
+    asm volatile("" : "+v"(lane));
+    const int l32 = lane & 31, g = lane >> 5, tid = 64 * wave + lane;
+    // K rows for S^T: key l32 of the step, chunks g * HALF / 8 + s.
+    int koff[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) koff[k] = l32 * ROWB + (((g * HALF / 8) + k) ^ tswz<D>(l32)) * 16;
+    // V^T through the transposing read: see prefill_kernel.
+    const int s16 = lane & 15;
+    const int vrow = 4 * g + (s16 >> 2);
+    const int vcl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+    int voff[NT], voffh[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      voff[n] = TILEB + vrow * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow)) * 16) + (s16 & 1) * 8;
+      voffh[n] =
+          TILEB + (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
+    }
+    const int lrow = 32 * wave + l32;                          // this lane's row of the unit
+    const int ltok = (int)((uint32_t)lrow * p.g_magic >> 16);  // and its token
     const int rows = u.ntok * p.G;
     const bool active = 32 * wave < rows;
     const bool whole = k0 == 0 && k1 == u.kend;
@@ -279,8 +328,15 @@ void paged_chunk_kernel(ChunkParams p) {
         }
       }
     };
-    auto store_tile = [&](int j, const uint4_t (&kd)[PER_T], const uint4_t (&vd)[PER_T]) {
+    bool bad = false;
+    auto store_tile = [&](int j, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
       char* buf = lds + (j % kCkNBuf) * BUFB;
+      if (p.causal && k0 + (j + 1) * kBN > u.first + 1) {  // keys that not every row sees
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < PER_T; ++i) any |= zero_not_finite<BF16>(vd[i]);
+        bad = bad || __any(any);
+      }
 #pragma unroll
       for (int i = 0; i < PER_T; ++i) {
         const int ch = tid + i * kCkThreads;
@@ -360,52 +416,6 @@ void paged_chunk_kernel(ChunkParams p) {
         for (int n = 0; n < NT; ++n) oacc[n] = E::mfma(vf[h][n], bop, oacc[n]);
       }
     };
-    // P.V of one step, key by key: each key's product is added to the rows that see it.
-    // Element e of fragment h of lane half g is key 16 h + 8 (e / 4) + 4 g + e % 4.
-    auto pv_by_key = [&](const uint32_t (&pk)[8], int kh0) {
-#pragma clang loop unroll(disable)
-      for (int j = 0; j < 32; ++j) {
-        const bool mine = g == ((j >> 2) & 1);
-        const uint32_t half = (j & 1) ? 0xffff0000u : 0x0000ffffu;
-        const int word = 2 * ((j >> 3) & 1) + ((j >> 1) & 1);
-        v8 bop[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          bop[h] = E::as8(uint4_t{pk[4 * h], pk[4 * h + 1], pk[4 * h + 2], pk[4 * h + 3]});
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float16_t acc;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint4_t v = __builtin_bit_cast(uint4_t, vf[h][n]);
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-              v[w] = (mine && h == (j >> 4) && w == word) ? (v[w] & half) : 0u;
-            acc = E::mfma(E::as8(v), bop[h], acc);
-          }
-          if (kh0 + j <= lim) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) oacc[n][i] += acc[i];
-          }
-        }
-      }
-    };
-    auto v_not_finite = [&]() -> bool {
-      constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-      bool bad = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4_t v = __builtin_bit_cast(uint4_t, vf[h][n]);
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            bad |= (v[w] & kExp) == kExp || (v[w] & (kExp << 16)) == (kExp << 16);
-        }
-      return __any(bad);
-    };
     auto softmax = [&](const float16_t& ss, uint32_t (&pk)[8], float& l_step, float& x_step) {
       float ls = 0.f, xs = 0.f;
 #pragma unroll
@@ -475,17 +485,6 @@ void paged_chunk_kernel(ChunkParams p) {
       }
       l_part += l_step;
       x_part += x_step;
-      if (p.causal && kh0 + 31 > lim_min) {  // on the diagonal
-        if (v_not_finite()) {
-          pv_by_key(pcur, kh0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pcur[i] = 0u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) vf[h][n] = E::as8(uint4_t{0, 0, 0, 0});
-        }
-      }
     };
 
     // Valid-key bits of tiles j .. j + 3 at tile j (lanes past kBN repeat the first ones).
@@ -543,8 +542,11 @@ void paged_chunk_kernel(ChunkParams p) {
     }
 
     // ---- end of the part: partial or output, each wave for its own rows.
+    if (lane == 0) sm_bad[wave] = bad;
     __syncthreads();  // every tile read is done
     if (!active) return;
+    if (uniform(sm_bad[0] | sm_bad[1] | sm_bad[2] | sm_bad[3]))
+      add_not_finite<D, BF16>(p, u, max(k0, u.first + 1), k1, g, lim, oacc);
     float l_row = xor32_sum(l_part);
     float x_row = LSE ? xor32_sum(x_part) : 0.f;
     if (!whole) {
@@ -627,6 +629,305 @@ void paged_chunk_kernel(ChunkParams p) {
     }
   };
 
+  // ---- the keys [k0, k1) of a unit of up to 32 RG rows: few rows, so the keys are what is
+  // shared out.  Wave w has rows 32 (w % RG) .. and takes the 32-key steps w / RG, + KG, ...
+  // of the part, each on its own: K goes from global memory straight into the fragments'
+  // registers, V through the wave's own LDS for the transposing reads, both loaded again as
+  // soon as the step has used them, with no barrier before the waves' results are merged.
+  auto serve_split = [&](const Unit& u, int k0, int k1, int64_t Ustart, auto rg_c) {
+    // The lane number is opaque here, so that what is derived from it lives no longer than
+    // this part (held across the units' loop it would not fit the registers).
+    int lane = tid0 & 63;
+    asm volatile("" : "+v"(lane));
+    const int l32 = lane & 31, g = lane >> 5;
+    // V^T through the transposing read: see prefill_kernel.
+    const int s16 = lane & 15;
+    const int vrow = 4 * g + (s16 >> 2);
+    const int vcl = 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1);
+    int voff[NT], voffh[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      voff[n] = vrow * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow)) * 16) + (s16 & 1) * 8;
+      voffh[n] =
+          (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
+    }
+    constexpr int RG = decltype(rg_c)::value, KG = 4 / RG;
+    constexpr int VPL = CPR / 2;      // V chunks per lane and step
+    constexpr int OB = 32 * D * 4;    // bytes of a wave's O
+    constexpr int NQ = 4 * NT / KG;   // 4-element pieces of O that a wave merges
+    static_assert(4 * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
+    const int rg = wave % RG, kg = wave / RG;
+    const int rows = u.ntok * p.G;
+    const bool active = 32 * rg < rows;
+    const int n_steps = active ? (k1 - k0 + 31) / 32 : 0;
+    const half_t* const Kh = p.pool + u.kvh * p.sh;
+    const int row = 32 * rg + l32;
+    const int tok = (int)((uint32_t)row * p.g_magic >> 16);
+    const int lim = p.causal ? u.first + min(tok, u.ntok - 1) : u.len - 1;
+    const int lim_min =
+        p.causal ? u.first + min((int)((uint32_t)(32 * rg) * p.g_magic >> 16), u.ntok - 1)
+                 : u.len - 1;
+    char* const vst = lds + wave * OB;
+
+    auto id_ok = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pool_pages; };
+    // Lane l holds the page id of key l32 of step t (past the unit's keys: of its last one).
+    auto load_ids = [&](int t) -> int {
+      const int key = min(k0 + 32 * t + l32, u.kend - 1);
+      return p.indices[u.ip0 + page_of(p, key)];
+    };
+    uint4_t kf[KS], vr[VPL];
+    // K fragment k: key l32, dims 16 k + 8 g + e.  A key that nothing sees is read from q (any
+    // readable row does: its score is masked).
+    auto load_k = [&](int t, int ids) {
+      const int key = min(k0 + 32 * t + l32, u.kend - 1);
+      const int slot = key - page_of(p, key) * p.page_size;
+      const half_t* src =
+          (id_ok(ids) ? Kh + ids * p.sp + (int64_t)slot * p.ss : p.q) + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kf[k] = ld16(src + 16 * k);
+    };
+    // V chunk i: 16-byte chunk lane + 64 i of the step's rows; rows that nothing sees are zeros.
+    auto load_v = [&](int t, int ids) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if constexpr (GRP) {
+          const int r0 = RPC * i, key = k0 + 32 * t + r0;
+          const int id = __builtin_amdgcn_readlane(ids, r0);
+          const int left = min(RPC, u.kend - key);
+          const bool ok = left > 0 && id_ok(id);
+          const int slot = key - page_of(p, key) * p.page_size;
+          const half_t* base = Kh + p.skv + (ok ? id * p.sp + (int64_t)slot * p.ss : 0);
+          const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)base, 0, ok ? (left - 1) * p.ss * 2 + ROWB : 0, kBufferWord3);
+          vr[i] = __builtin_bit_cast(
+              uint4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                           rs, (lane / CPR) * p.ss * 2 + (lane % CPR) * 16, 0, 0));
+        } else {
+          const int r = (lane + 64 * i) / CPR, key = k0 + 32 * t + r;
+          const int id = (int)shfl_u((uint32_t)ids, r);
+          vr[i] = uint4_t{0, 0, 0, 0};
+          if (key < u.kend && id_ok(id))
+            vr[i] = ld16(Kh + p.skv + id * p.sp +
+                         (int64_t)(key - page_of(p, key) * p.page_size) * p.ss + lane % CPR * 8);
+        }
+      }
+    };
+
+    v8 qf[KS];
+    {
+      const half_t* src = p.q + (int64_t)(u.q0 + tok) * p.q_st +
+                          (int64_t)(u.kvh * p.G + row - tok * p.G) * p.q_sh + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint4_t v = {0, 0, 0, 0};
+        if (row < rows) v = ld16(src + 16 * k);
+        if (p.neg_q) v ^= uint4_t{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+        qf[k] = E::as8(v);
+      }
+    }
+    float16_t oacc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) oacc[n][i] = 0.f;
+    float m_run = kCkFloor, l_part = 0.f, x_part = 0.f;
+    auto frag = [&](int h, int n) -> v8 {  // V^T of the staged rows
+      const uint2 lo = ds_read_tr16(vst + voff[n] + h * 16 * ROWB);
+      const uint2 hi = ds_read_tr16(vst + voffh[n] + h * 16 * ROWB);
+      return E::as8(uint4_t{lo.x, lo.y, hi.x, hi.y});
+    };
+
+    __syncthreads();  // the last unit's LDS reads are done
+    bool bad = false;
+    int ids = 0, ids_next = 0;
+    if (kg < n_steps) {
+      ids = load_ids(kg);
+      ids_next = load_ids(kg + KG);
+      load_k(kg, ids);
+      load_v(kg, ids);
+    }
+#pragma clang loop unroll(disable)
+    for (int t = kg; t < n_steps; t += KG) {
+      const int kh0 = k0 + 32 * t;
+      const bool more = t + KG < n_steps;
+      const uint32_t valid = (uint32_t)__ballot(id_ok(ids));
+      float16_t sv;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sv[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) sv = E::mfma(E::as8(kf[k]), qf[k], sv);
+      if (more) load_k(t + KG, ids_next);
+      if (p.causal && kh0 + 31 > u.first) {  // keys that not every row sees
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) any |= zero_not_finite<BF16>(vr[i]);
+        bad = bad || __any(any);
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const int ch = lane + 64 * i, r = ch / CPR, cc = ch % CPR;
+        *reinterpret_cast<uint4_t*>(vst + r * ROWB + ((cc ^ tswz<D>(r)) * 16)) = vr[i];
+      }
+      if (more) {
+        load_v(t + KG, ids_next);
+        ids = ids_next;
+        ids_next = load_ids(t + 2 * KG);
+      }
+      if (kh0 + 31 > lim_min || valid != 0xffffffffu) {  // wave-uniform
+        const int room = lim - kh0 - 4 * g;
+        const uint32_t vl = valid >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int o = 8 * (i >> 2) + (i & 3);
+          if (o > room || !((vl >> o) & 1)) sv[i] = AKT_C_NEG_INF;
+        }
+      }
+      float mx = sv[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, sv[i]);
+      float ma, mb;
+      swap32(mx, ma, mb);
+      const float m_new =
+          __builtin_elementwise_maximum(m_run, __builtin_elementwise_maximum(ma, mb) * c);
+      if (__any(!(m_new <= m_run + kCkSlack))) {
+        // The slack leaves P below 2^kCkSlack.  The first keys' rise from the floor scales zeros.
+        const float alpha = fast_exp2(m_run - m_new);
+        l_part *= alpha;
+        x_part *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) oacc[n][i] *= alpha;
+        m_run = m_new;
+      }
+      uint32_t pk[8];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = fast_exp2(__builtin_fmaf(sv[i], c, -m_run));
+        const float p1 = fast_exp2(__builtin_fmaf(sv[i + 1], c, -m_run));
+        pk[i >> 1] = E::pack2(p0, p1);
+        if constexpr (LSE) x_part += p0 + p1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l_part = E::dot2(pk[i], E::kOnes, l_part);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v8 bop = E::as8(uint4_t{pk[4 * h], pk[4 * h + 1], pk[4 * h + 2], pk[4 * h + 3]});
+#pragma unroll
+        for (int n = 0; n < NT; ++n) oacc[n] = E::mfma(frag(h, n), bop, oacc[n]);
+      }
+    }
+    if (bad)
+      for (int t = kg; t < n_steps; t += KG)
+        add_not_finite<D, BF16>(p, u, max(k0 + 32 * t, u.first + 1), min(k0 + 32 * t + 32, u.kend),
+                                g, lim, oacc);
+
+    // ---- merge of the KG waves that share rows: piece 4 n + k of O (dims 32 n + 8 k + 4 g ..
+    // + 3 of row l32) of every lane lies at [wave][piece][lane]; the wave with key group kg
+    // then sums pieces NQ kg .. of all.
+    float l_row = xor32_sum(l_part);
+    float x_row = LSE ? xor32_sum(x_part) : 0.f;
+    if (g == 0) sm_ml[wave][l32] = float4_t{m_run, l_row, x_row, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4_t*>(vst + ((4 * n + k) * 64 + lane) * 16) =
+            as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
+                               oacc[n][4 * k + 3]});
+    __syncthreads();
+    if (!active) return;
+    float4_t acc[NQ];
+    {
+      float f[KG];
+      m_run = AKT_C_NEG_INF;
+#pragma unroll
+      for (int w = 0; w < KG; ++w)
+        m_run = __builtin_elementwise_maximum(m_run, sm_ml[w * RG + rg][l32][0]);
+      l_row = x_row = 0.f;
+#pragma unroll
+      for (int w = 0; w < KG; ++w) {
+        const float4_t ml = sm_ml[w * RG + rg][l32];
+        f[w] = fast_exp2(ml[0] - m_run);
+        l_row += f[w] * ml[1];
+        x_row += f[w] * ml[2];
+      }
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KG; ++w)
+          acc[i] += f[w] * as_float4u(*reinterpret_cast<const uint4_t*>(
+                               lds + (w * RG + rg) * OB + ((NQ * kg + i) * 64 + lane) * 16));
+      }
+    }
+    if (!(k0 == 0 && k1 == u.kend)) {
+      // Partial: this wave's pieces and the row's (m, l); the last of the unit's workgroups
+      // merges them, wave by wave.
+      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = chunk_slot_bytes(D);
+      const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
+      const int wf = div_range(Ustart + kCkBlock - 1, Lw);
+      const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
+      auto slot_of = [&](int w) -> char* {
+        return p.partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+      };
+      char* mine = slot_of(wg);
+      if (row < rows) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          st16_device(mine, (uint32_t)((i * 64 + lane) * 16), as_uint4f(acc[i]));
+        if (g == 0)
+          st16_device(mine, (uint32_t)(NT * 4096 + l32 * 16),
+                      as_uint4f(float4_t{m_run, l_row, x_row, 0.f}));
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      int prev = 0;
+      if (lane == 0) prev = atomicAdd(&p.arrive[4 * wf + wave], 1);
+      if (uniform(prev) != wl - wf) return;
+      if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
+      if (row < rows) {
+        float M = AKT_C_NEG_INF;
+        for (int w = wf; w <= wl; ++w)
+          M = __builtin_elementwise_maximum(
+              M, as_float4u(ld16_device(slot_of(w), (uint32_t)(NT * 4096 + l32 * 16)))[0]);
+        m_run = M;
+        l_row = x_row = 0.f;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int w = wf; w <= wl; ++w) {
+          const char* src = slot_of(w);
+          const float4_t ml = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
+          const float f = fast_exp2(ml[0] - M);
+          l_row += f * ml[1];
+          x_row += f * ml[2];
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            acc[i] += f * as_float4u(ld16_device(src, (uint32_t)((i * 64 + lane) * 16)));
+        }
+      }
+    }
+    const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
+    const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
+    if (LSE && kg == 0 && g == 0 && row < rows)
+      p.lse[at] = l_row == 0.f ? AKT_C_NEG_INF : (m_run + __log2f(x_row)) * kLn2;
+    // The lane halves hold 8-byte halves of a row's 16-byte chunks: half 0 takes chunk i
+    // whole, half 1 chunk i + 1.
+#pragma unroll
+    for (int i = 0; i < NQ; i += 2) {
+      uint2 hv[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        hv[k] = uint2{E::pack2(acc[i + k][0] * inv, acc[i + k][1] * inv),
+                      E::pack2(acc[i + k][2] * inv, acc[i + k][3] * inv)};
+      const uint2 send = g == 0 ? hv[1] : hv[0];
+      const uint2 recv = {(uint32_t)__shfl_xor((int)send.x, 32, 64),
+                          (uint32_t)__shfl_xor((int)send.y, 32, 64)};
+      const uint4_t v = g == 0 ? uint4_t{hv[0].x, hv[0].y, recv.x, recv.y}
+                               : uint4_t{recv.x, recv.y, hv[1].x, hv[1].y};
+      if (row < rows) st16(p.o + at * D + 8 * (NQ * kg + i + g), v);
+    }
+  };
+
   // ---- the units of the range
   for (;;) {
     Unit u;
@@ -651,7 +952,7 @@ void paged_chunk_kernel(ChunkParams p) {
       // Nothing to see: zeros.
       const int rows = u.ntok * p.G;
       if (k0 == 0)
-        for (int idx = tid; idx < rows * CPR; idx += kCkThreads) {
+        for (int idx = tid0; idx < rows * CPR; idx += kCkThreads) {
           const int row = idx / CPR;
           const int tok = (int)((uint32_t)row * p.g_magic >> 16);
           const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
@@ -659,7 +960,9 @@ void paged_chunk_kernel(ChunkParams p) {
           if (LSE && idx % CPR == 0) p.lse[at] = AKT_C_NEG_INF;
         }
     } else if (k0 < k1) {
-      serve(u, uniform(k0), k1, us);
+      if constexpr (!SPLIT) serve(u, uniform(k0), k1, us);
+      else if (u.ntok * p.G <= 32) serve_split(u, uniform(k0), k1, us, std::integral_constant<int, 1>{});
+      else serve_split(u, uniform(k0), k1, us, std::integral_constant<int, 2>{});
     }
     if (e < u.kend) break;  // the rest of the unit is the next range's
     if (++r < R) continue;
@@ -670,20 +973,30 @@ void paged_chunk_kernel(ChunkParams p) {
     do {
       if (++b == p.B) return;
       s = load_seq(p, b);
-      R = uniform(row_blocks(p, s.n));
-    } while (R == 0);
+    } while (!mine(s));
+    R = uniform(row_blocks(p, s.n));
     hlen = uniform64(head_length(p, s));
   }
 }
 
+template <int D, bool BF16, bool GRP, bool LSE>
+int launch_paths(const ChunkParams& p, hipStream_t st) {
+  if (p.paths & kCkSplit) {
+    KernelTimer timer;
+    timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, true>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
+    if (int rc = check_launch("paged_chunk_kernel (few rows)")) return rc;
+  }
+  if (p.paths & kCkTiles) {
+    KernelTimer timer;
+    timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, false>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
+    return check_launch("paged_chunk_kernel (many rows)");
+  }
+  return AKT_OK;
+}
+
 template <int D, bool BF16, bool GRP>
 int launch_lse(const ChunkParams& p, hipStream_t st) {
-  KernelTimer timer;
-  if (p.lse)
-    timer.launch(paged_chunk_kernel<D, BF16, GRP, true>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
-  else
-    timer.launch(paged_chunk_kernel<D, BF16, GRP, false>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
-  return check_launch("paged_chunk_kernel");
+  return p.lse ? launch_paths<D, BF16, GRP, true>(p, st) : launch_paths<D, BF16, GRP, false>(p, st);
 }
 
 template <int D>
@@ -838,6 +1151,12 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   p.qk_scale = fmaxf(fabsf(softmax_scale) * kLog2e, FLT_MIN);
   p.wgs = (int)wgs;
   p.min_keys = kCkMinKeys;
+  // Sequences of up to 64 rows to a kv head share out their keys.  How many tokens a
+  // sequence has is known on the device alone, unless there is one, or all are few.
+  p.split_tokens = (int)(kCkSplitRows / G);
+  p.paths = kCkSplit | kCkTiles;
+  if (total_q <= p.split_tokens) p.paths = kCkSplit;
+  else if (batch == 1 || p.split_tokens == 0) p.split_tokens = 0, p.paths = kCkTiles;
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == AKT_DTYPE_BF16;
   if (head_dim == 64) return chunk_launch_64(p, bf16, st);

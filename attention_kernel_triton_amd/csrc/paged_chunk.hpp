@@ -13,6 +13,9 @@ constexpr int kCkThreads = 256;  // four waves
 constexpr int kCkRows = 128;     // rows (token, query head of the group) of a unit
 constexpr int kCkBlock = 128;    // keys of a block, the grain in which units are cut
 constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
+// Rows of a sequence and kv head up to which the waves of a workgroup share out the keys.
+constexpr int kCkSplitRows = 64;
+constexpr int kCkSplit = 1, kCkTiles = 2;  // the kernels of a launch
 
 struct ChunkParams {
   const half_t* q;     // [total_q, Hq, D] rows (strides q_st, q_sh)
@@ -38,6 +41,8 @@ struct ChunkParams {
   int neg_q;       // 1: softmax_scale < 0, computed as (-Q) K^T at |softmax_scale|
   float qk_scale;  // |softmax_scale| * log2(e), at least FLT_MIN
   int wgs;         // workgroups of the launch
+  int split_tokens;  // sequences of up to so many new tokens are the split kernel's
+  int paths;         // kCkSplit | kCkTiles
   int min_keys;    // fewest keys (with unit costs) of a workgroup's range, at least kCkBlock
 };
 
