@@ -96,6 +96,11 @@ __device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b) {
   s.len = np > 0 ? (np - 1) * p.page_size + min(max(p.last_len[b], 0), p.page_size) : 0;
   return s;
 }
+// The same for a wave-uniform b, in scalar registers.
+__device__ __forceinline__ Seq load_seq_uniform(const ChunkParams& p, int b) {
+  const Seq s = load_seq(p, b);
+  return Seq{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len)};
+}
 __device__ __forceinline__ int row_blocks(const ChunkParams& p, int n) {
   return (int)(((uint32_t)n + p.TR - 1) / (uint32_t)p.TR);
 }
@@ -128,16 +133,56 @@ struct Unit {
   int ip0;    // first page table entry of the sequence
 };
 
-// Replaces the infinities and NaNs of a 16-byte chunk by zeros; true if there were any.
-template <bool BF16>
-__device__ __forceinline__ bool zero_not_finite(uint4_t& v) {
-  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-  bool any = false;
+// Scores of the keys that a row does not see become -inf: of the step's 32 those past its
+// first room + 1, and those whose bit of `valid` is 0.
+__device__ __forceinline__ void mask_scores(float16_t& s, uint32_t valid, int room, int g) {
+  const uint32_t see = room < 0 ? 0u : valid & (0xffffffffu >> (31 - min(room, 31)));
+  const uint32_t mine = see >> (4 * g);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const bool lo = (v[w] & kExp) == kExp, hi = (v[w] & (kExp << 16)) == (kExp << 16);
-    v[w] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
-    any |= lo || hi;
+  for (int i = 0; i < 16; ++i) {
+    const int keep = __builtin_amdgcn_sbfe((int)mine, 8 * (i >> 2) + (i & 3), 1);  // 0 or -1
+    s[i] = __int_as_float((__float_as_int(s[i]) & keep) | (0xff800000 & ~keep));
+  }
+}
+
+// Takes a partial's (m, l, x) into a row's running ones, rescaling what is summed so far where
+// m is a new maximum; returns the factor of the partial's O.
+template <typename F>
+__device__ __forceinline__ float merge_in(float4_t ml, float& m, float& l, float& x, F rescale) {
+  if (ml[0] > m) {
+    const float sc = fast_exp2(m - ml[0]);  // 0 for the first
+    rescale(sc);
+    l *= sc;
+    x *= sc;
+    m = ml[0];
+  }
+  const float f = fast_exp2(ml[0] - m);
+  l += f * ml[1];
+  x += f * ml[2];
+  return f;
+}
+
+// Replaces infinities and NaNs by zeros; returns whether any lane of the wave had one.
+template <bool BF16, int N>
+__device__ __forceinline__ bool zero_not_finite(uint4_t (&v)[N]) {
+  typedef unsigned short ushort2_v __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  ushort2_v top = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_v, v[i][w] & 0x7fff7fffu));
+  const bool any = __any(top.x >= kExp || top.y >= kExp);
+  if (any) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t lo = (v[i][w] & kExp) == kExp ? 0xffff0000u : ~0u;
+        const uint32_t hi = (v[i][w] & (kExp << 16)) == (kExp << 16) ? 0x0000ffffu : ~0u;
+        v[i][w] &= lo & hi;
+      }
   }
   return any;
 }
@@ -217,43 +262,7 @@ void paged_chunk_kernel(ChunkParams p) {
     }
     return v;
   };
-  int64_t total = 0;
-  for (int jb = 0; jb < p.B; jb += 64) total += uniform64(shfl64(scan64(seq_length(jb + lane0)), 63));
-  int64_t Lw = (total + W - 1) / W;
-  if (Lw < p.min_keys) Lw = p.min_keys;
-  Lw = uniform64(Lw);
-  const int64_t x0 = wg * Lw, x1 = x0 + Lw;
-  if (x0 >= total) return;
-  // The unit that holds x0: sequence, kv head, row block.
-  int b = 0;
-  int64_t U = 0;  // the sequence's start
-  for (int jb = 0;; jb += 64) {
-    const int64_t len = seq_length(jb + lane0);
-    const int64_t inc = scan64(len);
-    const uint64_t m = __ballot(U + inc > x0);
-    if (m) {
-      const int l = __builtin_ctzll(m);
-      b = uniform(jb + l);
-      U += uniform64(shfl64(inc - len, l));
-      break;
-    }
-    U += uniform64(shfl64(inc, 63));
-  }
-  Seq s = load_seq(p, b);
-  int64_t hlen = head_length(p, s);
-  int kvh = div_range(x0 - U, hlen);
-  int64_t hs = U + kvh * hlen;  // the head's start
-  int R = uniform(row_blocks(p, s.n)), r = 0;
-  for (int lo = 0, hi = R; lo < hi;) {  // last r with unit_start(r) <= x0 - hs
-    const int mid = (lo + hi) / 2;
-    if (unit_start(p, s, mid) <= x0 - hs) {
-      r = mid;
-      lo = mid + 1;
-    } else {
-      hi = mid;
-    }
-  }
-
+  int64_t Lw = 0, x0 = 0, x1 = 0;
   const float c = p.qk_scale;
   // ---- the keys [k0, k1) of a unit, for all four waves.
   auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
@@ -332,10 +341,7 @@ void paged_chunk_kernel(ChunkParams p) {
     auto store_tile = [&](int j, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
       char* buf = lds + (j % kCkNBuf) * BUFB;
       if (p.causal && k0 + (j + 1) * kBN > u.first + 1) {  // keys that not every row sees
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < PER_T; ++i) any |= zero_not_finite<BF16>(vd[i]);
-        bad = bad || __any(any);
+        bad |= zero_not_finite<BF16>(vd);
       }
 #pragma unroll
       for (int i = 0; i < PER_T; ++i) {
@@ -433,13 +439,7 @@ void paged_chunk_kernel(ChunkParams p) {
     // Masks step t: keys past a row, and keys (bit of `valid`) of pages outside the pool.
     auto mask_step = [&](int kh0, uint32_t valid, float16_t& ss) {
       if (kh0 + 31 > lim_min || valid != 0xffffffffu) {  // wave-uniform
-        const int room = lim - kh0 - 4 * g;
-        const uint32_t vl = valid >> (4 * g);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int o = 8 * (i >> 2) + (i & 3);
-          if (o > room || !((vl >> o) & 1)) ss[i] = AKT_C_NEG_INF;
-        }
+        mask_scores(ss, valid, lim - kh0, g);
       }
     };
     auto row_max = [&](const float16_t& sv) {
@@ -574,31 +574,38 @@ void paged_chunk_kernel(ChunkParams p) {
       if (lane == 0) prev = atomicAdd(&p.arrive[4 * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
       if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
-      float M = AKT_C_NEG_INF;
-      for (int w = wf; w <= wl; ++w)
-        M = __builtin_elementwise_maximum(
-            M, as_float4u(ld16_device(slot_of(w), (uint32_t)(NT * 4096 + l32 * 16)))[0]);
-      m_run = M;
+      constexpr int UB = D == 64 ? 4 : 2;  // partials in flight
+      m_run = AKT_C_NEG_INF;
       l_row = x_row = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[n][i] = 0.f;
-      for (int w = wf; w <= wl; ++w) {
-        const char* src = slot_of(w);
-        const float4_t ml = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
-        const float f = fast_exp2(ml[0] - M);
-        l_row += f * ml[1];
-        x_row += f * ml[2];
+#pragma clang loop unroll(disable)
+      for (int w = wf; w <= wl; w += UB) {
+        float4_t ml[UB], ov[UB][4 * NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int k = 0; k < UB; ++k) {
+          const char* src = slot_of(min(w + k, wl));
+          ml[k] = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float4_t ov = as_float4u(
-                ld16_device(src, (uint32_t)(((4 * n + k) * 64 + lane) * 16)));
+          for (int i = 0; i < 4 * NT; ++i)
+            ov[k][i] = as_float4u(ld16_device(src, (uint32_t)((i * 64 + lane) * 16)));
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) oacc[n][4 * k + i] += f * ov[i];
-          }
+        for (int k = 0; k < UB; ++k) {
+          if (w + k > wl) break;
+          const float f = merge_in(ml[k], m_run, l_row, x_row, [&](float sc) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) oacc[n][i] *= sc;
+          });
+#pragma unroll
+          for (int i = 0; i < 4 * NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) oacc[i / 4][4 * (i % 4) + j] += f * ov[k][i][j];
+        }
       }
     }
     // Output rows through LDS, so that every lane stores 16 contiguous bytes.
@@ -758,10 +765,7 @@ void paged_chunk_kernel(ChunkParams p) {
       for (int k = 0; k < KS; ++k) sv = E::mfma(E::as8(kf[k]), qf[k], sv);
       if (more) load_k(t + KG, ids_next);
       if (p.causal && kh0 + 31 > u.first) {  // keys that not every row sees
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) any |= zero_not_finite<BF16>(vr[i]);
-        bad = bad || __any(any);
+        bad |= zero_not_finite<BF16>(vr);
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
@@ -774,13 +778,7 @@ void paged_chunk_kernel(ChunkParams p) {
         ids_next = load_ids(t + 2 * KG);
       }
       if (kh0 + 31 > lim_min || valid != 0xffffffffu) {  // wave-uniform
-        const int room = lim - kh0 - 4 * g;
-        const uint32_t vl = valid >> (4 * g);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int o = 8 * (i >> 2) + (i & 3);
-          if (o > room || !((vl >> o) & 1)) sv[i] = AKT_C_NEG_INF;
-        }
+        mask_scores(sv, valid, lim - kh0, g);
       }
       float mx = sv[0];
 #pragma unroll
@@ -886,23 +884,32 @@ void paged_chunk_kernel(ChunkParams p) {
       if (uniform(prev) != wl - wf) return;
       if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
       if (row < rows) {
-        float M = AKT_C_NEG_INF;
-        for (int w = wf; w <= wl; ++w)
-          M = __builtin_elementwise_maximum(
-              M, as_float4u(ld16_device(slot_of(w), (uint32_t)(NT * 4096 + l32 * 16)))[0]);
-        m_run = M;
+        constexpr int UB = 32 / NQ < 8 ? 32 / NQ : 8;  // partials in flight
+        m_run = AKT_C_NEG_INF;
         l_row = x_row = 0.f;
 #pragma unroll
         for (int i = 0; i < NQ; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-        for (int w = wf; w <= wl; ++w) {
-          const char* src = slot_of(w);
-          const float4_t ml = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
-          const float f = fast_exp2(ml[0] - M);
-          l_row += f * ml[1];
-          x_row += f * ml[2];
+#pragma clang loop unroll(disable)
+        for (int w = wf; w <= wl; w += UB) {
+          float4_t ml[UB], ov[UB][NQ];
 #pragma unroll
-          for (int i = 0; i < NQ; ++i)
-            acc[i] += f * as_float4u(ld16_device(src, (uint32_t)((i * 64 + lane) * 16)));
+          for (int k = 0; k < UB; ++k) {
+            const char* src = slot_of(min(w + k, wl));
+            ml[k] = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+              ov[k][i] = as_float4u(ld16_device(src, (uint32_t)((i * 64 + lane) * 16)));
+          }
+#pragma unroll
+          for (int k = 0; k < UB; ++k) {
+            if (w + k > wl) break;
+            const float f = merge_in(ml[k], m_run, l_row, x_row, [&](float sc) {
+#pragma unroll
+              for (int i = 0; i < NQ; ++i) acc[i] *= sc;
+            });
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) acc[i] += f * ov[k][i];
+          }
         }
       }
     }
@@ -928,54 +935,112 @@ void paged_chunk_kernel(ChunkParams p) {
     }
   };
 
-  // ---- the units of the range
-  for (;;) {
-    Unit u;
-    const int t0 = r * p.TR;
-    u.q0 = uniform(s.q0 + t0);
-    u.ntok = uniform(min(p.TR, s.n - t0));
-    u.kvh = kvh;
-    u.first = uniform(s.len - s.n + t0);
-    u.len = uniform(s.len);
-    u.kend = uniform(p.causal ? max(u.first + u.ntok, 0) : s.len);
-    u.ip0 = uniform(s.ip0);
-    const int64_t us = hs + unit_start(p, s, r);
-    // Blocks from the first at or past x - us - (kCkBlock - 1) on are the next range's.
-    auto cut = [&](int64_t x) -> int64_t {
-      const int64_t d = x - us - (kCkBlock - 1);
-      return d <= 0 ? 0 : (d + kCkBlock - 1) / kCkBlock * kCkBlock;
-    };
-    const int64_t e = cut(x1);
-    if (e == 0) break;  // this unit and all after it are later ranges'
-    const int k0 = (int)cut(x0), k1 = uniform((int)(e < u.kend ? e : u.kend));
-    if (u.kend == 0) {
-      // Nothing to see: zeros.
-      const int rows = u.ntok * p.G;
-      if (k0 == 0)
-        for (int idx = tid0; idx < rows * CPR; idx += kCkThreads) {
-          const int row = idx / CPR;
-          const int tok = (int)((uint32_t)row * p.g_magic >> 16);
-          const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
-          st16(p.o + at * D + idx % CPR * 8, uint4_t{0, 0, 0, 0});
-          if (LSE && idx % CPR == 0) p.lse[at] = AKT_C_NEG_INF;
-        }
-    } else if (k0 < k1) {
-      if constexpr (!SPLIT) serve(u, uniform(k0), k1, us);
-      else if (u.ntok * p.G <= 32) serve_split(u, uniform(k0), k1, us, std::integral_constant<int, 1>{});
-      else serve_split(u, uniform(k0), k1, us, std::integral_constant<int, 2>{});
+  // ---- the units of the range: first the one that reaches out of its end, then the others
+  // from its start on.  A range that is about as long as a unit then goes through a unit's
+  // head and the tail of the unit before it in the order of their keys, so the
+  // workgroups of one kv head, which share an L2, read the same keys at the same time.
+  int last_b = -1, last_kvh = 0, last_r = 0;
+#pragma clang loop unroll(disable)
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t len = seq_length(lane0), inc = scan64(len);
+    if (pass == 0) {
+      int64_t total = uniform64(shfl64(inc, 63));
+      for (int jb = 64; jb < p.B; jb += 64)
+        total += uniform64(shfl64(scan64(seq_length(jb + lane0)), 63));
+      Lw = (total + W - 1) / W;
+      if (Lw < p.min_keys) Lw = p.min_keys;
+      Lw = uniform64(Lw);
+      x0 = wg * Lw;
+      if (x0 >= total) return;
+      x1 = x0 + Lw < total ? x0 + Lw : total;
     }
-    if (e < u.kend) break;  // the rest of the unit is the next range's
-    if (++r < R) continue;
-    r = 0;
-    hs += hlen;
-    if (++kvh < p.Hkv) continue;
-    kvh = 0;
-    do {
-      if (++b == p.B) return;
-      s = load_seq(p, b);
-    } while (!mine(s));
-    R = uniform(row_blocks(p, s.n));
-    hlen = uniform64(head_length(p, s));
+    // The unit that holds x: sequence, kv head, row block.
+    const int64_t x = pass == 0 ? x1 - 1 : x0;
+    int b = 0;
+    int64_t U = 0;  // the sequence's start
+    for (int jb = 0;;) {
+      const uint64_t m = __ballot(U + inc > x);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        b = uniform(jb + l);
+        U += uniform64(shfl64(inc - len, l));
+        break;
+      }
+      U += uniform64(shfl64(inc, 63));
+      jb += 64;
+      len = seq_length(jb + lane0);
+      inc = scan64(len);
+    }
+    Seq s = load_seq_uniform(p, b);
+    int64_t hlen = uniform64(head_length(p, s));
+    int kvh = div_range(x - U, hlen);
+    int64_t hs = uniform64(U + kvh * hlen);  // the head's start
+    int R = uniform(row_blocks(p, s.n)), r = 0;
+    for (int lo = 1, hi = R; lo < hi;) {  // last r with unit_start(r) <= x - hs
+      const int mid = (lo + hi) / 2;
+      if (unit_start(p, s, mid) <= x - hs) {
+        r = mid;
+        lo = mid + 1;
+      } else {
+        hi = mid;
+      }
+    }
+    for (;;) {
+      if (b == last_b && kvh == last_kvh && r == last_r) return;
+      Unit u;
+      const int t0 = r * p.TR;
+      u.q0 = uniform(s.q0 + t0);
+      u.ntok = uniform(min(p.TR, s.n - t0));
+      u.kvh = kvh;
+      u.first = uniform(s.len - s.n + t0);
+      u.len = uniform(s.len);
+      u.kend = uniform(p.causal ? max(u.first + u.ntok, 0) : s.len);
+      u.ip0 = uniform(s.ip0);
+      const int64_t us = uniform64(hs + unit_start(p, s, r));
+      // Blocks from the first at or past x - us - (kCkBlock - 1) on are those of the ranges
+      // from x on.
+      auto cut = [&](int64_t x) -> int {
+        const int64_t d = x - us;
+        return uniform(d >= u.kend + kCkBlock ? u.kend
+                       : d < kCkBlock         ? 0
+                                              : min((int)d / kCkBlock * kCkBlock, u.kend));
+      };
+      const int k0 = cut(x0), k1 = cut(x1);
+      if (u.kend == 0) {
+        // Nothing to see: zeros, by the workgroup of what would be the first block.
+        const int rows = u.ntok * p.G;
+        if (x0 - us < kCkBlock && x1 - us >= kCkBlock)
+          for (int idx = tid0; idx < rows * CPR; idx += kCkThreads) {
+            const int row = idx / CPR;
+            const int tok = (int)((uint32_t)row * p.g_magic >> 16);
+            const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
+            st16(p.o + at * D + idx % CPR * 8, uint4_t{0, 0, 0, 0});
+            if (LSE && idx % CPR == 0) p.lse[at] = AKT_C_NEG_INF;
+          }
+      } else if (k0 < k1) {
+        if constexpr (!SPLIT) serve(u, k0, k1, us);
+        else if (u.ntok * p.G <= 32) serve_split(u, k0, k1, us, std::integral_constant<int, 1>{});
+        else serve_split(u, k0, k1, us, std::integral_constant<int, 2>{});
+      }
+      if (pass == 0) {
+        if (us <= x0) return;  // the range lies in this unit
+        last_b = b;
+        last_kvh = kvh;
+        last_r = r;
+        break;
+      }
+      if (++r < R) continue;
+      r = 0;
+      hs += hlen;
+      if (++kvh < p.Hkv) continue;
+      kvh = 0;
+      do {
+        if (++b == p.B) return;
+        s = load_seq_uniform(p, b);
+      } while (!mine(s));
+      R = uniform(row_blocks(p, s.n));
+      hlen = uniform64(head_length(p, s));
+    }
   }
 }
 
