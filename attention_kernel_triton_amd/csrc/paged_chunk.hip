@@ -10,8 +10,8 @@
 // kv head has few rows, the matrix pipe when it has many.
 //
 // Units.  The rows of one (sequence, kv head) are its (token, query head of the group)
-// pairs, token major; a unit is a run of up to 128 rows of whole tokens (TR = 128 / G of
-// them), which share every K and V row.  Wave w of a workgroup owns rows 32 w .. 32 w + 31.
+// pairs, token major; a unit is a run of up to 128 (256) rows of whole tokens, TR = 128 / G of
+// them, which share every K and V row.  Wave w of a workgroup owns rows 32 w .. 32 w + 31.
 //
 // Ranges.  The units stand one behind another on an axis of keys (sequence by sequence,
 // kv head by kv head, row block by row block), each as long as the keys it sees plus
@@ -63,7 +63,9 @@ constexpr float kCkStepLimit = 32.0f * 256.0f;  // row sum of a step that stays 
 constexpr float kCkFloor = -1e30f;
 #define AKT_C_NEG_INF (-__builtin_inff())
 
-__host__ __device__ constexpr int ck_tile_keys(int D) { return D == 64 ? 64 : 32; }
+__host__ __device__ constexpr int ck_tile_keys(int D, int WAVES) {
+  return D == 64 || WAVES == 8 ? 64 : 32;
+}
 __host__ __device__ constexpr int ck_mix_mfma(int D) { return D == 64 ? 8 : (D == 128 ? 10 : 16); }
 __host__ __device__ constexpr int ck_mix_valu(int D) { return D == 128 ? 1 : 2; }
 
@@ -216,14 +218,14 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit&
   }
 }
 
-template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT>
-__global__ __launch_bounds__(kCkThreads)
-__attribute__((amdgpu_waves_per_eu(chunk_wgs_per_cu(D), chunk_wgs_per_cu(D))))
+template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES)
+__attribute__((amdgpu_waves_per_eu(chunk_waves_per_simd(D), chunk_waves_per_simd(D))))
 void paged_chunk_kernel(ChunkParams p) {
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
-  constexpr int kBN = ck_tile_keys(D);  // keys per staged tile
-  constexpr int SPT = kBN / 32;         // 32-key steps per tile
+  constexpr int kThreads = 64 * WAVES;
+  constexpr int kBN = ck_tile_keys(D, WAVES);  // keys per staged tile
   constexpr int KS = D / 16;            // MFMA k-steps over the head dim
   constexpr int HALF = D / 2;
   constexpr int NT = D / 32;       // 32-dim output tiles
@@ -231,12 +233,12 @@ void paged_chunk_kernel(ChunkParams p) {
   constexpr int ROWB = D * 2;      // bytes per row
   constexpr int TILEB = kBN * ROWB;
   constexpr int BUFB = 2 * TILEB;  // K then V
-  constexpr int PER_T = kBN * CPR / kCkThreads;  // chunks per thread per matrix
+  constexpr int PER_T = kBN * CPR / kThreads;  // chunks per thread per matrix
   constexpr int RPC = 64 / CPR;                  // rows of a wave's 64 chunks
   static_assert(16 % RPC == 0, "a wave's chunks lie in one 16-key group");
   __shared__ __attribute__((aligned(16))) char lds[kCkNBuf * BUFB];
   __shared__ float4_t sm_ml[4][32];
-  __shared__ int sm_bad[4];
+  __shared__ int sm_bad[WAVES];
 
   const int tid0 = threadIdx.x;
   const int wave = uniform(tid0 >> 6);
@@ -291,65 +293,92 @@ void paged_chunk_kernel(ChunkParams p) {
     const int rows = u.ntok * p.G;
     const bool active = 32 * wave < rows;
     const bool whole = k0 == 0 && k1 == u.kend;
-    const int n_tiles = SPT == 2 ? (k1 - k0 + 63) / 64 : 2 * ((k1 - k0 + 63) / 64);
-    const int n_h = active ? 2 * ((k1 - k0 + 63) / 64) : 0;
+    const int nb = (k1 - k0 + 63) / 64;  // blocks of 64 keys: two steps
+    const int n_tiles = 64 / kBN * nb;
     const half_t* const Kh = p.pool + u.kvh * p.sh;
 
-    // Page ids of tile j: lane l holds that of key l (past the unit's keys: of its last one).
-    auto load_ids = [&](int j) -> int {
-      const int key = min(k0 + j * kBN + (lane & (kBN - 1)), u.kend - 1);
-      return p.indices[u.ip0 + page_of(p, key)];
+    // Places of the keys, a block of 64 at a time: lane l holds key l's.
+    struct Keys {
+      int lo, hi;   // byte offset of its K row from Kh
+      uint64_t ok;  // keys that can be read: before the unit's end, on pages of the pool
     };
-    auto id_ok = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pool_pages; };
+    int id_next, slot_next;  // of the block whose ids are on their way
+    auto load_ids = [&](int m) {
+      const int key = min(k0 + 64 * m + lane, u.kend - 1);
+      const int lp = page_of(p, key);
+      slot_next = key - lp * p.page_size;
+      id_next = p.indices[u.ip0 + lp];
+    };
+    auto place = [&](int m) -> Keys {
+      const bool ok =
+          k0 + 64 * m + lane < u.kend && (uint32_t)id_next < (uint32_t)p.num_pool_pages;
+      const int64_t off = ok ? 2 * (id_next * p.sp + (int64_t)slot_next * p.ss) : 0;
+      return Keys{(int)(uint32_t)off, (int)(uint32_t)((uint64_t)off >> 32), __ballot(ok)};
+    };
     uint4_t kst[PER_T], vst[PER_T];
-    auto load_tile = [&](int j, int ids, uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
+    // Rows of a tile whose first key is key `first` (0 or 32) of its block.
+    auto load_tile = [&](const Keys& keys, int first, uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
+      if constexpr (GRP) {
+        // Each of this wave's loads takes RPC rows, which lie in one page.
+        const uint32_t off = (uint32_t)((lane / CPR) * p.ss * 2 + (lane % CPR) * 16);
+        const char* base[PER_T];
 #pragma unroll
-      for (int i = 0; i < PER_T; ++i) {
-        if constexpr (GRP) {
-          // This wave's RPC rows lie in one page.
-          const int row = (wave * 64 + i * kCkThreads) / CPR;
-          const int key = k0 + j * kBN + row;
-          const int id = __builtin_amdgcn_readlane(ids, row);
-          const int left = min(RPC, u.kend - key);
-          const bool ok = left > 0 && id_ok(id);
-          const int slot = key - page_of(p, key) * p.page_size;
-          const half_t* base = Kh + (ok ? id * p.sp + (int64_t)slot * p.ss : 0);
-          const int bytes = ok ? (left - 1) * p.ss * 2 + ROWB : 0;
-          const int off = (lane / CPR) * p.ss * 2 + (lane % CPR) * 16;
-          const auto kr =
-              __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, kBufferWord3);
-          const auto vr =
-              __builtin_amdgcn_make_buffer_rsrc((void*)(base + p.skv), 0, bytes, kBufferWord3);
-          kd[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
-          vd[i] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
+        for (int i = 0; i < PER_T; ++i) {
+          const int row = first + (wave * 64 + i * kThreads) / CPR;
+          base[i] = (const char*)Kh +
+                    (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(keys.hi, row) << 32) |
+                              (uint32_t)__builtin_amdgcn_readlane(keys.lo, row));
+        }
+        const bool full = kBN == 64 ? keys.ok == ~0ull : (uint32_t)(keys.ok >> first) == ~0u;
+        if (full) {
+#pragma unroll
+          for (int i = 0; i < PER_T; ++i) {
+            kd[i] = ld16(base[i] + off);
+            vd[i] = ld16(base[i] + 2 * p.skv + off);
+          }
         } else {
-          const int row = (tid + i * kCkThreads) / CPR;
-          const int key = k0 + j * kBN + row;
-          const int id = (int)shfl_u((uint32_t)ids, row);
+#pragma unroll
+          for (int i = 0; i < PER_T; ++i) {
+            const int row = first + (wave * 64 + i * kThreads) / CPR;
+            const int n = __builtin_popcount((uint32_t)(keys.ok >> row) & ((1u << RPC) - 1));
+            const int bytes = n > 0 ? (n - 1) * p.ss * 2 + ROWB : 0;
+            const auto kr =
+                __builtin_amdgcn_make_buffer_rsrc((void*)base[i], 0, bytes, kBufferWord3);
+            const auto vr = __builtin_amdgcn_make_buffer_rsrc((void*)(base[i] + 2 * p.skv), 0,
+                                                              bytes, kBufferWord3);
+            kd[i] =
+                __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
+            vd[i] =
+                __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER_T; ++i) {
+          const int row = first + (tid + i * kThreads) / CPR;
+          const uint32_t lo = shfl_u((uint32_t)keys.lo, row), hi = shfl_u((uint32_t)keys.hi, row);
           kd[i] = vd[i] = uint4_t{0, 0, 0, 0};
-          if (key < u.kend && id_ok(id)) {
-            const int slot = key - page_of(p, key) * p.page_size;
-            const half_t* src =
-                Kh + id * p.sp + (int64_t)slot * p.ss + (tid + i * kCkThreads) % CPR * 8;
+          if ((keys.ok >> row) & 1) {
+            const char* src = (const char*)Kh + (int64_t)(((uint64_t)hi << 32) | lo) +
+                              (tid + i * kThreads) % CPR * 16;
             kd[i] = ld16(src);
-            vd[i] = ld16(src + p.skv);
+            vd[i] = ld16(src + 2 * p.skv);
           }
         }
       }
     };
+    // Tile j, whose first key is k0 + kBN j, into buffer buf.
     bool bad = false;
-    auto store_tile = [&](int j, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
-      char* buf = lds + (j % kCkNBuf) * BUFB;
-      if (p.causal && k0 + (j + 1) * kBN > u.first + 1) {  // keys that not every row sees
+    auto store_tile = [&](int j, int buf, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
+      if (p.causal && k0 + (j + 1) * kBN > u.first + 1)  // keys that not every row sees
         bad |= zero_not_finite<BF16>(vd);
-      }
 #pragma unroll
       for (int i = 0; i < PER_T; ++i) {
-        const int ch = tid + i * kCkThreads;
+        const int ch = tid + i * kThreads;
         const int row = ch / CPR, cc = ch % CPR;
-        const int off = row * ROWB + ((cc ^ tswz<D>(row)) * 16);
-        *reinterpret_cast<uint4_t*>(buf + off) = kd[i];
-        *reinterpret_cast<uint4_t*>(buf + TILEB + off) = vd[i];
+        const int off = buf * BUFB + row * ROWB + ((cc ^ tswz<D>(row)) * 16);
+        *reinterpret_cast<uint4_t*>(lds + off) = kd[i];
+        *reinterpret_cast<uint4_t*>(lds + TILEB + off) = vd[i];
       }
     };
 
@@ -392,19 +421,19 @@ void paged_chunk_kernel(ChunkParams p) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) vf[h][n] = E::as8(uint4_t{0, 0, 0, 0});
 
-    auto load_kf = [&](int t, v8 (&kf)[KS]) {
-      const char* kb = lds + ((t / SPT) % kCkNBuf) * BUFB + (t % SPT) * 32 * ROWB;
+    // Fragments from LDS offset `at` of a step's rows.
+    auto load_kf = [&](int at, v8 (&kf)[KS]) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) kf[k] = E::as8(*reinterpret_cast<const uint4_t*>(kb + koff[k]));
+      for (int k = 0; k < KS; ++k)
+        kf[k] = E::as8(*reinterpret_cast<const uint4_t*>(lds + at + koff[k]));
     };
-    auto load_vf = [&](int t) {
-      const char* vb = lds + ((t / SPT) % kCkNBuf) * BUFB + (t % SPT) * 32 * ROWB;
+    auto load_vf = [&](int at) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint2 lo = ds_read_tr16(vb + voff[n] + h * 16 * ROWB);
-          const uint2 hi = ds_read_tr16(vb + voffh[n] + h * 16 * ROWB);
+          const uint2 lo = ds_read_tr16(lds + at + voff[n] + h * 16 * ROWB);
+          const uint2 hi = ds_read_tr16(lds + at + voffh[n] + h * 16 * ROWB);
           vf[h][n] = E::as8(uint4_t{lo.x, lo.y, hi.x, hi.y});
         }
     };
@@ -451,16 +480,16 @@ void paged_chunk_kernel(ChunkParams p) {
       return __builtin_elementwise_maximum(ma, mb) * c;
     };
     // One step, as in prefill_kernel: with no dependence between them, P.V of the
-    // previous step, S of the next and the softmax of this one.
-    auto step = [&](int t, uint32_t valid, float16_t& scur, float16_t& snext,
-                    const uint32_t (&pprev)[8], uint32_t (&pcur)[8]) {
-      const int kh0 = k0 + 32 * t;
+    // previous step, S of the next (K at LDS offset knext) and the softmax of this one (V at
+    // vcur).
+    auto step = [&](int kh0, uint32_t valid, int knext, int vcur, float16_t& scur,
+                    float16_t& snext, const uint32_t (&pprev)[8], uint32_t (&pcur)[8]) {
       mask_step(kh0, valid, scur);
       v8 kf[KS];
-      load_kf(t + 1, kf);
+      load_kf(knext, kf);
       pv_mfma(pprev);
       qk_mfma(kf, snext);
-      load_vf(t);
+      load_vf(vcur);
       float l_step, x_step;
       softmax(scur, pcur, l_step, x_step);
 #pragma unroll
@@ -487,24 +516,39 @@ void paged_chunk_kernel(ChunkParams p) {
       x_part += x_step;
     };
 
-    // Valid-key bits of tiles j .. j + 3 at tile j (lanes past kBN repeat the first ones).
-    auto valid_of = [&](int ids) -> uint64_t { return __ballot(id_ok(ids)); };
-    uint64_t v0, v1, v2, v3;
-    int ids_next;
+    // ---- the walk.  While tile j is computed, tile j + 1 is published, j + 2 is written and
+    // j + 3 is on its way; the ids of the block after it too.
+    Keys keys;                 // of the last block placed
+    uint64_t ok0, ok1, ok2;    // readable keys of the block of the next body and those after it
+    load_ids(0);
     __syncthreads();  // the last unit's LDS reads are done
     {
-      const int i0 = load_ids(0), i1 = load_ids(1), i2 = load_ids(2);
-      ids_next = load_ids(3);
       uint4_t ka[PER_T], va[PER_T], kb[PER_T], vb[PER_T];
-      load_tile(0, i0, ka, va);
-      if (n_tiles > 1) load_tile(1, i1, kb, vb);
-      if (n_tiles > 2) load_tile(2, i2, kst, vst);
-      v0 = 0;
-      v1 = valid_of(i0);
-      v2 = valid_of(i1);
-      v3 = valid_of(i2);
-      store_tile(0, ka, va);
-      if (n_tiles > 1) store_tile(1, kb, vb);
+      keys = place(0);
+      load_ids(1);
+      ok0 = keys.ok;
+      load_tile(keys, 0, ka, va);
+      if constexpr (kBN == 32) {
+        load_tile(keys, 32, kb, vb);
+        keys = place(1);
+        ok1 = keys.ok;
+        ok2 = 0;
+        load_ids(2);
+        if (n_tiles > 2) load_tile(keys, 0, kst, vst);
+        store_tile(0, 0, ka, va);
+        store_tile(1, 1, kb, vb);
+      } else {
+        keys = place(1);
+        ok1 = keys.ok;
+        load_ids(2);
+        if (n_tiles > 1) load_tile(keys, 0, kb, vb);
+        keys = place(2);
+        ok2 = keys.ok;
+        load_ids(3);
+        if (n_tiles > 2) load_tile(keys, 0, kst, vst);
+        store_tile(0, 0, ka, va);
+        if (n_tiles > 1) store_tile(1, 1, kb, vb);
+      }
     }
     __syncthreads();
     {
@@ -512,45 +556,78 @@ void paged_chunk_kernel(ChunkParams p) {
       load_kf(0, kf);
       qk_mfma(kf, sA);
     }
-    mask_step(k0, (uint32_t)v1, sA);
+    mask_step(k0, (uint32_t)ok0, sA);
     {
       const float mx = row_max(sA);
       m_run = mx < kCkFloor ? kCkFloor : mx;  // a NaN stays
     }
-    auto tile_turn = [&](int j) {
-      __syncthreads();
-      v0 = v1;
-      v1 = v2;
-      v2 = v3;
-      if (j + 2 < n_tiles) store_tile(j + 2, kst, vst);
-      if (j + 3 < n_tiles) {
-        load_tile(j + 3, ids_next, kst, vst);
-        v3 = valid_of(ids_next);
-        ids_next = load_ids(j + 4);
+    // Keys 64 m .. 64 m + 63 of the part; PH: m modulo the bodies that go round the buffers, so
+    // that every LDS offset is a constant.
+    auto body = [&](int m, auto ph_c) {
+      constexpr int PH = decltype(ph_c)::value;
+      const uint64_t ok = ok0;
+      ok0 = ok1;
+      if constexpr (kBN == 32) {
+        constexpr int B0 = 2 * PH, B1 = B0 + 1, B2 = (B0 + 2) % 4, B3 = (B0 + 3) % 4;
+        __syncthreads();
+        if (m + 1 < nb) {
+          store_tile(2 * m + 2, B2, kst, vst);
+          load_tile(keys, 32, kst, vst);
+        }
+        if (m + 2 < nb) {
+          keys = place(m + 2);
+          ok1 = keys.ok;
+          load_ids(m + 3);
+        }
+        if (active) step(k0 + 64 * m, (uint32_t)ok, B1 * BUFB, B0 * BUFB, sA, sB, pB, pA);
+        __syncthreads();
+        if (m + 1 < nb) store_tile(2 * m + 3, B3, kst, vst);
+        if (m + 2 < nb) load_tile(keys, 0, kst, vst);
+        if (active)
+          step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), B2 * BUFB, B1 * BUFB, sB, sA, pA, pB);
+      } else {
+        constexpr int B0 = PH, B1 = (B0 + 1) % 4, B2 = (B0 + 2) % 4;
+        constexpr int kHalf = 32 * ROWB;
+        ok1 = ok2;
+        __syncthreads();
+        if (m + 2 < nb) store_tile(m + 2, B2, kst, vst);
+        if (m + 3 < nb) {
+          keys = place(m + 3);
+          ok2 = keys.ok;
+          load_tile(keys, 0, kst, vst);
+          load_ids(m + 4);
+        }
+        if (active) {
+          step(k0 + 64 * m, (uint32_t)ok, B0 * BUFB + kHalf, B0 * BUFB, sA, sB, pB, pA);
+          step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), B1 * BUFB, B0 * BUFB + kHalf, sB, sA, pA, pB);
+        }
       }
     };
+    constexpr int kRound = kBN == 32 ? 2 : 4;
 #pragma clang loop unroll(disable)
-    for (int j = 0; j < n_tiles; j += 2 / SPT) {
-      tile_turn(j);
-      const int t = SPT * j;
-      if (t < n_h) step(t, (uint32_t)v0, sA, sB, pB, pA);
-      if constexpr (SPT == 1) tile_turn(j + 1);
-      if (t < n_h) {
-        step(t + 1, SPT == 2 ? (uint32_t)(v0 >> 32) : (uint32_t)v0, sB, sA, pA, pB);
-        if (t + 2 == n_h) pv_mfma(pB);
+    for (int m = 0; m < nb; m += kRound) {
+      body(m, std::integral_constant<int, 0>{});
+      if (m + 1 < nb) body(m + 1, std::integral_constant<int, 1>{});
+      if constexpr (kRound == 4) {
+        if (m + 2 < nb) body(m + 2, std::integral_constant<int, 2>{});
+        if (m + 3 < nb) body(m + 3, std::integral_constant<int, 3>{});
       }
     }
+    if (active) pv_mfma(pB);  // P.V of the last step
 
     // ---- end of the part: partial or output, each wave for its own rows.
     if (lane == 0) sm_bad[wave] = bad;
     __syncthreads();  // every tile read is done
     if (!active) return;
-    if (uniform(sm_bad[0] | sm_bad[1] | sm_bad[2] | sm_bad[3]))
+    int any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any_bad |= sm_bad[w];
+    if (uniform(any_bad))
       add_not_finite<D, BF16>(p, u, max(k0, u.first + 1), k1, g, lim, oacc);
     float l_row = xor32_sum(l_part);
     float x_row = LSE ? xor32_sum(x_part) : 0.f;
     if (!whole) {
-      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = chunk_slot_bytes(D);
+      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = WAVES * kWaveB;
       const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
@@ -571,9 +648,9 @@ void paged_chunk_kernel(ChunkParams p) {
       // The stores (device scope) are complete before the count.
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[4 * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
+      if (lane == 0) atomicExch(&p.arrive[WAVES * wf + wave], 0);
       constexpr int UB = D == 64 ? 4 : 2;  // partials in flight
       m_run = AKT_C_NEG_INF;
       l_row = x_row = 0.f;
@@ -662,7 +739,7 @@ void paged_chunk_kernel(ChunkParams p) {
     constexpr int VPL = CPR / 2;      // V chunks per lane and step
     constexpr int OB = 32 * D * 4;    // bytes of a wave's O
     constexpr int NQ = 4 * NT / KG;   // 4-element pieces of O that a wave merges
-    static_assert(4 * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
+    static_assert(WAVES == 4 && 4 * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
     const int rg = wave % RG, kg = wave / RG;
     const int rows = u.ntok * p.G;
     const bool active = 32 * rg < rows;
@@ -862,7 +939,7 @@ void paged_chunk_kernel(ChunkParams p) {
     if (!(k0 == 0 && k1 == u.kend)) {
       // Partial: this wave's pieces and the row's (m, l); the last of the unit's workgroups
       // merges them, wave by wave.
-      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = chunk_slot_bytes(D);
+      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = WAVES * kWaveB;
       const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
@@ -880,9 +957,9 @@ void paged_chunk_kernel(ChunkParams p) {
       }
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[4 * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[4 * wf + wave], 0);
+      if (lane == 0) atomicExch(&p.arrive[WAVES * wf + wave], 0);
       if (row < rows) {
         constexpr int UB = 32 / NQ < 8 ? 32 / NQ : 8;  // partials in flight
         m_run = AKT_C_NEG_INF;
@@ -1010,7 +1087,7 @@ void paged_chunk_kernel(ChunkParams p) {
         // Nothing to see: zeros, by the workgroup of what would be the first block.
         const int rows = u.ntok * p.G;
         if (x0 - us < kCkBlock && x1 - us >= kCkBlock)
-          for (int idx = tid0; idx < rows * CPR; idx += kCkThreads) {
+          for (int idx = tid0; idx < rows * CPR; idx += kThreads) {
             const int row = idx / CPR;
             const int tok = (int)((uint32_t)row * p.g_magic >> 16);
             const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
@@ -1044,19 +1121,22 @@ void paged_chunk_kernel(ChunkParams p) {
   }
 }
 
+template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT, int WAVES>
+int launch_one(const ChunkParams& p, int wgs, hipStream_t st) {
+  ChunkParams q = p;
+  q.wgs = wgs;
+  KernelTimer timer;
+  timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, SPLIT, WAVES>, dim3(wgs), dim3(64 * WAVES), 0,
+               st, q);
+  return check_launch("paged_chunk_kernel");
+}
+
 template <int D, bool BF16, bool GRP, bool LSE>
 int launch_paths(const ChunkParams& p, hipStream_t st) {
-  if (p.paths & kCkSplit) {
-    KernelTimer timer;
-    timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, true>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
-    if (int rc = check_launch("paged_chunk_kernel (few rows)")) return rc;
-  }
-  if (p.paths & kCkTiles) {
-    KernelTimer timer;
-    timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, false>, dim3(p.wgs), dim3(kCkThreads), 0, st, p);
-    return check_launch("paged_chunk_kernel (many rows)");
-  }
-  return AKT_OK;
+  if (p.split_wgs > 0)
+    if (int rc = launch_one<D, BF16, GRP, LSE, true, 4>(p, p.split_wgs, st)) return rc;
+  if (p.tile_wgs == 0) return AKT_OK;
+  return launch_one<D, BF16, GRP, LSE, false, chunk_tile_waves(D)>(p, p.tile_wgs, st);
 }
 
 template <int D, bool BF16, bool GRP>
@@ -1095,21 +1175,45 @@ namespace {
 
 constexpr int kCkMinKeys = 256;
 
+// How a call is served: the workgroups of both kernels (0: not launched).
+struct ChunkPlan {
+  int waves;  // of the tile kernel's workgroups
+  int split_tokens;
+  int64_t split_wgs, tile_wgs, slots;
+};
+
 // Workgroups of a launch: the resident ones, fewer where the axis is too short for them
 // (bounded from above by what the host knows: every sequence as long as all pages).
-int64_t chunk_wgs(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
-                  int64_t page_size, int64_t total_pages) {
+int64_t axis_wgs(double units, int64_t tokens, int64_t resident) {
+  const double wgs = ceil(units * (double)(tokens + kCkUnitCost) / kCkMinKeys);
+  return wgs < (double)resident ? (int64_t)wgs : resident;
+}
+
+ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
+                     int64_t page_size, int64_t total_pages) {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-      cus <= 0)
+      cus <= 0 || cus > 1024)
     cus = 256;  // no device: what an MI355X has
-  const int64_t resident = (int64_t)cus * chunk_wgs_per_cu((int)D);
-  const int64_t units = Hkv * (total_q / (kCkRows / G) + (batch < total_q ? batch : total_q));
-  // units < 2^31 * Hkv and the length < 2^31: as doubles, against overflow.
-  const double axis = (double)units * (double)(total_pages * page_size + kCkUnitCost);
-  const double wgs = ceil(axis / kCkMinKeys);
-  return wgs < (double)resident ? (int64_t)wgs : resident;
+  const int64_t tokens = page_size * total_pages;
+  const int64_t seqs = batch < total_q ? batch : total_q;
+  ChunkPlan c = {};
+  c.waves = chunk_tile_waves((int)D);
+  const int64_t rows = 32 * c.waves;
+  // Sequences of up to kCkSplitRows rows to a kv head share out their keys.  How many tokens a
+  // sequence has is known on the device alone, unless there is one, or all are few.
+  c.split_tokens = (int)(kCkSplitRows / G);
+  const bool few = total_q <= c.split_tokens;
+  if (!few && batch == 1) c.split_tokens = 0;
+  const int64_t resident = (int64_t)cus * chunk_waves_per_simd((int)D);
+  if (c.split_tokens > 0) c.split_wgs = axis_wgs((double)Hkv * seqs, tokens, resident);
+  if (!few)
+    c.tile_wgs = axis_wgs((double)Hkv * (total_q / (rows / G) + seqs), tokens,
+                          resident * 4 / c.waves);
+  const int64_t a = 4 * c.split_wgs, b = c.waves * c.tile_wgs;
+  c.slots = 2 * (a > b ? a : b);  // two a wave
+  return c;
 }
 
 }  // namespace
@@ -1125,10 +1229,10 @@ extern "C" size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q,
       total_pages < 0 || num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > kCkRows ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  const int64_t wgs = chunk_wgs(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
-                                page_size, total_pages);
+  const ChunkPlan c = chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
+                                 page_size, total_pages);
   return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) +
-                  2 * wgs * chunk_slot_bytes((int)head_dim));
+                  c.slots * chunk_wave_bytes((int)head_dim));
 }
 
 extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
@@ -1170,16 +1274,16 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
             "tensors must have 16-byte aligned rows");
   AKT_CHECK(kv_stride[3] >= 0 && kv_stride[3] < (1 << 22), "slot stride out of range [0, 2^22)");
   const int64_t G = num_q_heads / num_kv_heads;
-  const int64_t wgs =
-      chunk_wgs(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages);
+  const ChunkPlan plan =
+      chunk_plan(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages);
   const size_t need = akt_chunk_paged_workspace_size(batch, total_q, num_q_heads, num_kv_heads,
                                                      head_dim, page_size, total_pages);
   if (!workspace || workspace_bytes < need)
     return set_error(AKT_ERR_WORKSPACE, "chunk attention needs a workspace of %zu bytes, got %zu",
                      need, workspace ? workspace_bytes : (size_t)0);
   AKT_CHECK(aligned16(workspace), "the workspace must be 16-byte aligned");
-  static_assert(4 * 2 * 1024 <= (AKT_WORKSPACE_ZERO_BYTES - 256) / 4, "arrival counters");
-  AKT_CHECK(4 * wgs <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4, "too many workgroups");
+  AKT_CHECK(plan.slots / 2 <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4,
+            "too many workgroups");
 
   ChunkParams p = {};
   p.q = (const half_t*)q;
@@ -1205,7 +1309,7 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   p.Hq = (int)num_q_heads;
   p.Hkv = (int)num_kv_heads;
   p.G = (int)G;
-  p.TR = (int)(kCkRows / G);
+  p.TR = (int)(32 * plan.waves / G);
   p.g_magic = (uint32_t)((65536 + G - 1) / G);
   p.page_size = (int)page_size;
   const uint64_t magic = (1ull << 32) / (uint64_t)page_size;
@@ -1214,14 +1318,10 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   // As in prefill: a negative scale flips Q's sign, a zero one becomes FLT_MIN.
   p.neg_q = softmax_scale < 0.f ? 1 : 0;
   p.qk_scale = fmaxf(fabsf(softmax_scale) * kLog2e, FLT_MIN);
-  p.wgs = (int)wgs;
   p.min_keys = kCkMinKeys;
-  // Sequences of up to 64 rows to a kv head share out their keys.  How many tokens a
-  // sequence has is known on the device alone, unless there is one, or all are few.
-  p.split_tokens = (int)(kCkSplitRows / G);
-  p.paths = kCkSplit | kCkTiles;
-  if (total_q <= p.split_tokens) p.paths = kCkSplit;
-  else if (batch == 1 || p.split_tokens == 0) p.split_tokens = 0, p.paths = kCkTiles;
+  p.split_tokens = plan.split_tokens;
+  p.split_wgs = (int)plan.split_wgs;
+  p.tile_wgs = (int)plan.tile_wgs;
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == AKT_DTYPE_BF16;
   if (head_dim == 64) return chunk_launch_64(p, bf16, st);

@@ -9,13 +9,11 @@
 
 namespace akt {
 
-constexpr int kCkThreads = 256;  // four waves
-constexpr int kCkRows = 128;     // rows (token, query head of the group) of a unit
+constexpr int kCkRows = 128;  // query heads that a kv head may have: a token's rows are in one unit
 constexpr int kCkBlock = 128;    // keys of a block, the grain in which units are cut
 constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
 // Rows of a sequence and kv head up to which the waves of a workgroup share out the keys.
 constexpr int kCkSplitRows = 64;
-constexpr int kCkSplit = 1, kCkTiles = 2;  // the kernels of a launch
 
 struct ChunkParams {
   const half_t* q;     // [total_q, Hq, D] rows (strides q_st, q_sh)
@@ -27,14 +25,14 @@ struct ChunkParams {
   const int32_t* indices;
   const int32_t* last_len;
   int* arrive;     // [4 * workgroups] arrival counters (zero between launches)
-  char* partials;  // two slots of slot_bytes to a workgroup
+  char* partials;  // two slots to a workgroup
   int64_t q_st, q_sh;
   int64_t sp, skv, sh;  // page, K/V and head strides of the pool (elements)
   int ss;               // slot stride (elements, < 2^22)
   int total_q, total_pages, num_pool_pages;
   int B, Hq, Hkv, G;
-  int TR;              // tokens of a unit: kCkRows / G
-  uint32_t g_magic;    // ceil(2^16 / G): n / G = n * g_magic >> 16 for n < kCkRows
+  int TR;              // tokens of a unit: 32 waves / G
+  uint32_t g_magic;    // ceil(2^16 / G): n / G = n * g_magic >> 16 for n < 256
   int page_size;
   uint32_t page_magic;  // min(2^32 - 1, floor(2^32 / page_size))
   int causal;
@@ -42,17 +40,22 @@ struct ChunkParams {
   float qk_scale;  // |softmax_scale| * log2(e), at least FLT_MIN
   int wgs;         // workgroups of the launch
   int split_tokens;  // sequences of up to so many new tokens are the split kernel's
-  int paths;         // kCkSplit | kCkTiles
+  int split_wgs, tile_wgs;  // workgroups of the two kernels, 0: not launched
   int min_keys;    // fewest keys (with unit costs) of a workgroup's range, at least kCkBlock
 };
 
-// Bytes of a partial slot: per wave the fp32 O of 32 rows as it sits in registers
+// Bytes of a wave's part of a partial slot: the fp32 O of 32 rows as it sits in registers
 // and a 16-byte (m, l, exact l, -) row for each.
 __host__ __device__ constexpr int64_t chunk_wave_bytes(int D) { return 32 * D * 4 + 32 * 16; }
-__host__ __device__ constexpr int64_t chunk_slot_bytes(int D) { return 4 * chunk_wave_bytes(D); }
 
-// Workgroups to a CU.
-__host__ __device__ constexpr int chunk_wgs_per_cu(int D) { return D <= 128 ? 2 : 1; }
+// Waves to a SIMD, and workgroups of four waves to a CU.
+__host__ __device__ constexpr int chunk_waves_per_simd(int D) { return D <= 128 ? 2 : 1; }
+
+// Waves of the tile kernel's workgroups.  At D = 128 eight share a tile of 64 keys (one
+// workgroup to a CU): half the loads, LDS stores and barriers a wave, and faster at every size
+// measured (us, four waves / eight, 32 heads over 8): 32 tokens after 200 26.6 / 24.6, 777
+// after 0 41.0 / 36.2, 777 after 8000 153 / 142, 2048 after 30000 1239 / 1101.
+__host__ __device__ constexpr int chunk_tile_waves(int D) { return D == 128 ? 8 : 4; }
 
 int chunk_launch_64(const ChunkParams& p, bool bf16, hipStream_t st);
 int chunk_launch_128(const ChunkParams& p, bool bf16, hipStream_t st);
