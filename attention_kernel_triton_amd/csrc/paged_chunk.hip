@@ -367,7 +367,7 @@ void paged_chunk_kernel(ChunkParams p) {
         }
       }
     };
-    // Tile j, whose first key is k0 + kBN j, into buffer buf.
+    // Tile j, whose first key is k0 + kBN j, into the buffer at LDS offset buf.
     bool bad = false;
     auto store_tile = [&](int j, int buf, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
       if (p.causal && k0 + (j + 1) * kBN > u.first + 1)  // keys that not every row sees
@@ -376,7 +376,7 @@ void paged_chunk_kernel(ChunkParams p) {
       for (int i = 0; i < PER_T; ++i) {
         const int ch = tid + i * kThreads;
         const int row = ch / CPR, cc = ch % CPR;
-        const int off = buf * BUFB + row * ROWB + ((cc ^ tswz<D>(row)) * 16);
+        const int off = buf + row * ROWB + ((cc ^ tswz<D>(row)) * 16);
         *reinterpret_cast<uint4_t*>(lds + off) = kd[i];
         *reinterpret_cast<uint4_t*>(lds + TILEB + off) = vd[i];
       }
@@ -536,7 +536,7 @@ void paged_chunk_kernel(ChunkParams p) {
         load_ids(2);
         if (n_tiles > 2) load_tile(keys, 0, kst, vst);
         store_tile(0, 0, ka, va);
-        store_tile(1, 1, kb, vb);
+        store_tile(1, BUFB, kb, vb);
       } else {
         keys = place(1);
         ok1 = keys.ok;
@@ -547,7 +547,7 @@ void paged_chunk_kernel(ChunkParams p) {
         load_ids(3);
         if (n_tiles > 2) load_tile(keys, 0, kst, vst);
         store_tile(0, 0, ka, va);
-        if (n_tiles > 1) store_tile(1, 1, kb, vb);
+        if (n_tiles > 1) store_tile(1, BUFB, kb, vb);
       }
     }
     __syncthreads();
@@ -561,17 +561,15 @@ void paged_chunk_kernel(ChunkParams p) {
       const float mx = row_max(sA);
       m_run = mx < kCkFloor ? kCkFloor : mx;  // a NaN stays
     }
-    // Keys 64 m .. 64 m + 63 of the part; PH: m modulo the bodies that go round the buffers, so
-    // that every LDS offset is a constant.
-    auto body = [&](int m, auto ph_c) {
-      constexpr int PH = decltype(ph_c)::value;
+#pragma clang loop unroll(disable)
+    for (int m = 0; m < nb; ++m) {  // keys 64 m .. 64 m + 63 of the part
       const uint64_t ok = ok0;
       ok0 = ok1;
       if constexpr (kBN == 32) {
-        constexpr int B0 = 2 * PH, B1 = B0 + 1, B2 = (B0 + 2) % 4, B3 = (B0 + 3) % 4;
+        const int b0 = 2 * (m & 1) * BUFB, b1 = b0 + BUFB, b2 = 2 * BUFB - b0;
         __syncthreads();
         if (m + 1 < nb) {
-          store_tile(2 * m + 2, B2, kst, vst);
+          store_tile(2 * m + 2, b2, kst, vst);
           load_tile(keys, 32, kst, vst);
         }
         if (m + 2 < nb) {
@@ -579,18 +577,17 @@ void paged_chunk_kernel(ChunkParams p) {
           ok1 = keys.ok;
           load_ids(m + 3);
         }
-        if (active) step(k0 + 64 * m, (uint32_t)ok, B1 * BUFB, B0 * BUFB, sA, sB, pB, pA);
+        if (active) step(k0 + 64 * m, (uint32_t)ok, b1, b0, sA, sB, pB, pA);
         __syncthreads();
-        if (m + 1 < nb) store_tile(2 * m + 3, B3, kst, vst);
+        if (m + 1 < nb) store_tile(2 * m + 3, b2 + BUFB, kst, vst);
         if (m + 2 < nb) load_tile(keys, 0, kst, vst);
-        if (active)
-          step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), B2 * BUFB, B1 * BUFB, sB, sA, pA, pB);
+        if (active) step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), b2, b1, sB, sA, pA, pB);
       } else {
-        constexpr int B0 = PH, B1 = (B0 + 1) % 4, B2 = (B0 + 2) % 4;
+        const int b0 = (m & 3) * BUFB, b1 = ((m + 1) & 3) * BUFB, b2 = ((m + 2) & 3) * BUFB;
         constexpr int kHalf = 32 * ROWB;
         ok1 = ok2;
         __syncthreads();
-        if (m + 2 < nb) store_tile(m + 2, B2, kst, vst);
+        if (m + 2 < nb) store_tile(m + 2, b2, kst, vst);
         if (m + 3 < nb) {
           keys = place(m + 3);
           ok2 = keys.ok;
@@ -598,19 +595,9 @@ void paged_chunk_kernel(ChunkParams p) {
           load_ids(m + 4);
         }
         if (active) {
-          step(k0 + 64 * m, (uint32_t)ok, B0 * BUFB + kHalf, B0 * BUFB, sA, sB, pB, pA);
-          step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), B1 * BUFB, B0 * BUFB + kHalf, sB, sA, pA, pB);
+          step(k0 + 64 * m, (uint32_t)ok, b0 + kHalf, b0, sA, sB, pB, pA);
+          step(k0 + 64 * m + 32, (uint32_t)(ok >> 32), b1, b0 + kHalf, sB, sA, pA, pB);
         }
-      }
-    };
-    constexpr int kRound = kBN == 32 ? 2 : 4;
-#pragma clang loop unroll(disable)
-    for (int m = 0; m < nb; m += kRound) {
-      body(m, std::integral_constant<int, 0>{});
-      if (m + 1 < nb) body(m + 1, std::integral_constant<int, 1>{});
-      if constexpr (kRound == 4) {
-        if (m + 2 < nb) body(m + 2, std::integral_constant<int, 2>{});
-        if (m + 3 < nb) body(m + 3, std::integral_constant<int, 3>{});
       }
     }
     if (active) pv_mfma(pB);  // P.V of the last step
