@@ -63,9 +63,7 @@ constexpr float kCkStepLimit = 32.0f * 256.0f;  // row sum of a step that stays 
 constexpr float kCkFloor = -1e30f;
 #define AKT_C_NEG_INF (-__builtin_inff())
 
-__host__ __device__ constexpr int ck_tile_keys(int D, int WAVES) {
-  return D == 64 || WAVES == 8 ? 64 : 32;
-}
+__host__ __device__ constexpr int ck_tile_keys(int D) { return D <= 128 ? 64 : 32; }
 __host__ __device__ constexpr int ck_mix_mfma(int D) { return D == 64 ? 8 : (D == 128 ? 10 : 16); }
 __host__ __device__ constexpr int ck_mix_valu(int D) { return D == 128 ? 1 : 2; }
 
@@ -218,14 +216,16 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit&
   }
 }
 
-template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES)
-__attribute__((amdgpu_waves_per_eu(chunk_waves_per_simd(D), chunk_waves_per_simd(D))))
-void paged_chunk_kernel(ChunkParams p) {
+// The units of one of the W ranges of the axis of the sequences of few tokens (SPLIT) or of
+// many.  lds: the workgroup's tile buffers.
+template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT>
+__device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int block, int W,
+                                            int* arrive, char* partials) {
+  constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
   constexpr int kThreads = 64 * WAVES;
-  constexpr int kBN = ck_tile_keys(D, WAVES);  // keys per staged tile
+  constexpr int kBN = ck_tile_keys(D);  // keys per staged tile
   constexpr int KS = D / 16;            // MFMA k-steps over the head dim
   constexpr int HALF = D / 2;
   constexpr int NT = D / 32;       // 32-dim output tiles
@@ -236,8 +236,7 @@ void paged_chunk_kernel(ChunkParams p) {
   constexpr int PER_T = kBN * CPR / kThreads;  // chunks per thread per matrix
   constexpr int RPC = 64 / CPR;                  // rows of a wave's 64 chunks
   static_assert(16 % RPC == 0, "a wave's chunks lie in one 16-key group");
-  __shared__ __attribute__((aligned(16))) char lds[kCkNBuf * BUFB];
-  __shared__ float4_t sm_ml[4][32];
+  __shared__ float4_t sm_ml[WAVES][32];
   __shared__ int sm_bad[WAVES];
 
   const int tid0 = threadIdx.x;
@@ -245,9 +244,7 @@ void paged_chunk_kernel(ChunkParams p) {
 
   // ---- this workgroup's range of the axis.  Workgroup i runs on XCD i % 8, so
   // consecutive ranges go to one XCD's L2.
-  const int W = p.wgs;
-  const int wg = W % 8 == 0 ? (int)(blockIdx.x % 8) * (W / 8) + (int)(blockIdx.x / 8)
-                            : (int)blockIdx.x;
+  const int wg = (block % 8) * (W / 8) + block / 8;
   const int lane0 = tid0 & 63;
   // The sequences that this kernel serves.
   auto mine = [&](const Seq& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
@@ -619,7 +616,7 @@ void paged_chunk_kernel(ChunkParams p) {
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return p.partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+        return partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
       };
       char* mine = slot_of(wg);
 #pragma unroll
@@ -635,9 +632,9 @@ void paged_chunk_kernel(ChunkParams p) {
       // The stores (device scope) are complete before the count.
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[WAVES * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&arrive[WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[WAVES * wf + wave], 0);
+      if (lane == 0) atomicExch(&arrive[WAVES * wf + wave], 0);
       constexpr int UB = D == 64 ? 4 : 2;  // partials in flight
       m_run = AKT_C_NEG_INF;
       l_row = x_row = 0.f;
@@ -722,11 +719,11 @@ void paged_chunk_kernel(ChunkParams p) {
       voffh[n] =
           (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
     }
-    constexpr int RG = decltype(rg_c)::value, KG = 4 / RG;
-    constexpr int VPL = CPR / 2;      // V chunks per lane and step
-    constexpr int OB = 32 * D * 4;    // bytes of a wave's O
-    constexpr int NQ = 4 * NT / KG;   // 4-element pieces of O that a wave merges
-    static_assert(WAVES == 4 && 4 * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
+    constexpr int RG = decltype(rg_c)::value, KG = WAVES / RG;
+    constexpr int OB = 32 * D * 4;   // bytes of a wave's O
+    constexpr int NQ = 4 * NT / KG;  // 4-element pieces of O that a wave merges
+    static_assert(WAVES * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
+    static_assert(NQ % 2 == 0, "whole 16-byte chunks");
     const int rg = wave % RG, kg = wave / RG;
     const int rows = u.ntok * p.G;
     const bool active = 32 * rg < rows;
@@ -740,47 +737,38 @@ void paged_chunk_kernel(ChunkParams p) {
                  : u.len - 1;
     char* const vst = lds + wave * OB;
 
-    auto id_ok = [&](int id) { return (uint32_t)id < (uint32_t)p.num_pool_pages; };
-    // Lane l holds the page id of key l32 of step t (past the unit's keys: of its last one).
-    auto load_ids = [&](int t) -> int {
+    // Lane (l32, g) loads chunks 2 k + g of the K and V rows of key l32 of a step.  Ids are loaded
+    // a step before the rows.
+    int id_next = 0, slot_next = 0;
+    auto load_ids = [&](int t) {
       const int key = min(k0 + 32 * t + l32, u.kend - 1);
-      return p.indices[u.ip0 + page_of(p, key)];
+      const int lp = page_of(p, key);
+      slot_next = key - lp * p.page_size;
+      id_next = p.indices[u.ip0 + lp];
     };
-    uint4_t kf[KS], vr[VPL];
-    // K fragment k: key l32, dims 16 k + 8 g + e.  A key that nothing sees is read from q (any
-    // readable row does: its score is masked).
-    auto load_k = [&](int t, int ids) {
-      const int key = min(k0 + 32 * t + l32, u.kend - 1);
-      const int slot = key - page_of(p, key) * p.page_size;
-      const half_t* src =
-          (id_ok(ids) ? Kh + ids * p.sp + (int64_t)slot * p.ss : p.q) + 8 * g;
+    uint32_t valid = 0, valid_next = 0;  // keys that can be read: in the pool, before the unit's end
+    const half_t* src = p.q;
+    // The place of a step's row.  A key that cannot be read takes a row of q (any readable row
+    // does: its score is masked, its V zeroed).
+    auto place = [&](int t) {
+      const bool ok =
+          k0 + 32 * t + l32 < u.kend && (uint32_t)id_next < (uint32_t)p.num_pool_pages;
+      valid_next = (uint32_t)__ballot(ok);
+      src = (ok ? Kh + id_next * p.sp + (int64_t)slot_next * p.ss : p.q) + 8 * g;
+    };
+    uint4_t kf[KS], vr[KS];
+    auto load_k = [&]() {
 #pragma unroll
       for (int k = 0; k < KS; ++k) kf[k] = ld16(src + 16 * k);
     };
-    // V chunk i: 16-byte chunk lane + 64 i of the step's rows; rows that nothing sees are zeros.
-    auto load_v = [&](int t, int ids) {
+    auto load_v = [&]() {
+      if (valid_next == 0xffffffffu) {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        if constexpr (GRP) {
-          const int r0 = RPC * i, key = k0 + 32 * t + r0;
-          const int id = __builtin_amdgcn_readlane(ids, r0);
-          const int left = min(RPC, u.kend - key);
-          const bool ok = left > 0 && id_ok(id);
-          const int slot = key - page_of(p, key) * p.page_size;
-          const half_t* base = Kh + p.skv + (ok ? id * p.sp + (int64_t)slot * p.ss : 0);
-          const auto rs = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)base, 0, ok ? (left - 1) * p.ss * 2 + ROWB : 0, kBufferWord3);
-          vr[i] = __builtin_bit_cast(
-              uint4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                           rs, (lane / CPR) * p.ss * 2 + (lane % CPR) * 16, 0, 0));
-        } else {
-          const int r = (lane + 64 * i) / CPR, key = k0 + 32 * t + r;
-          const int id = (int)shfl_u((uint32_t)ids, r);
-          vr[i] = uint4_t{0, 0, 0, 0};
-          if (key < u.kend && id_ok(id))
-            vr[i] = ld16(Kh + p.skv + id * p.sp +
-                         (int64_t)(key - page_of(p, key) * p.page_size) * p.ss + lane % CPR * 8);
-        }
+        for (int k = 0; k < KS; ++k) vr[k] = ld16(src + p.skv + 16 * k);
+      } else {
+        const bool ok = (valid_next >> l32) & 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) vr[k] = ok ? ld16(src + p.skv + 16 * k) : uint4_t{0, 0, 0, 0};
       }
     };
 
@@ -810,36 +798,35 @@ void paged_chunk_kernel(ChunkParams p) {
 
     __syncthreads();  // the last unit's LDS reads are done
     bool bad = false;
-    int ids = 0, ids_next = 0;
     if (kg < n_steps) {
-      ids = load_ids(kg);
-      ids_next = load_ids(kg + KG);
-      load_k(kg, ids);
-      load_v(kg, ids);
+      load_ids(kg);
+      place(kg);
+      load_k();
+      load_v();
+      load_ids(kg + KG);
     }
 #pragma clang loop unroll(disable)
     for (int t = kg; t < n_steps; t += KG) {
       const int kh0 = k0 + 32 * t;
       const bool more = t + KG < n_steps;
-      const uint32_t valid = (uint32_t)__ballot(id_ok(ids));
+      valid = valid_next;
       float16_t sv;
 #pragma unroll
       for (int i = 0; i < 16; ++i) sv[i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) sv = E::mfma(E::as8(kf[k]), qf[k], sv);
-      if (more) load_k(t + KG, ids_next);
-      if (p.causal && kh0 + 31 > u.first) {  // keys that not every row sees
-        bad |= zero_not_finite<BF16>(vr);
-      }
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int ch = lane + 64 * i, r = ch / CPR, cc = ch % CPR;
-        *reinterpret_cast<uint4_t*>(vst + r * ROWB + ((cc ^ tswz<D>(r)) * 16)) = vr[i];
-      }
       if (more) {
-        load_v(t + KG, ids_next);
-        ids = ids_next;
-        ids_next = load_ids(t + 2 * KG);
+        place(t + KG);
+        load_k();
+      }
+      if (p.causal && kh0 + 31 > u.first)  // keys that not every row sees
+        bad |= zero_not_finite<BF16>(vr);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        *reinterpret_cast<uint4_t*>(vst + l32 * ROWB + (((2 * k + g) ^ tswz<D>(l32)) * 16)) = vr[k];
+      if (more) {
+        load_v();
+        load_ids(t + 2 * KG);
       }
       if (kh0 + 31 > lim_min || valid != 0xffffffffu) {  // wave-uniform
         mask_scores(sv, valid, lim - kh0, g);
@@ -926,12 +913,13 @@ void paged_chunk_kernel(ChunkParams p) {
     if (!(k0 == 0 && k1 == u.kend)) {
       // Partial: this wave's pieces and the row's (m, l); the last of the unit's workgroups
       // merges them, wave by wave.
-      constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = WAVES * kWaveB;
+      constexpr int64_t kWaveB = chunk_split_wave_bytes(D), kSlotB = WAVES * kWaveB;
+      constexpr uint32_t kMl = (uint32_t)kWaveB - 512;  // the rows' (m, l)
       const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return p.partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+        return partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
       };
       char* mine = slot_of(wg);
       if (row < rows) {
@@ -939,14 +927,14 @@ void paged_chunk_kernel(ChunkParams p) {
         for (int i = 0; i < NQ; ++i)
           st16_device(mine, (uint32_t)((i * 64 + lane) * 16), as_uint4f(acc[i]));
         if (g == 0)
-          st16_device(mine, (uint32_t)(NT * 4096 + l32 * 16),
+          st16_device(mine, kMl + l32 * 16,
                       as_uint4f(float4_t{m_run, l_row, x_row, 0.f}));
       }
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[WAVES * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&arrive[WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[WAVES * wf + wave], 0);
+      if (lane == 0) atomicExch(&arrive[WAVES * wf + wave], 0);
       if (row < rows) {
         constexpr int UB = 32 / NQ < 8 ? 32 / NQ : 8;  // partials in flight
         m_run = AKT_C_NEG_INF;
@@ -959,7 +947,7 @@ void paged_chunk_kernel(ChunkParams p) {
 #pragma unroll
           for (int k = 0; k < UB; ++k) {
             const char* src = slot_of(min(w + k, wl));
-            ml[k] = as_float4u(ld16_device(src, (uint32_t)(NT * 4096 + l32 * 16)));
+            ml[k] = as_float4u(ld16_device(src, kMl + l32 * 16));
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
               ov[k][i] = as_float4u(ld16_device(src, (uint32_t)((i * 64 + lane) * 16)));
@@ -1108,27 +1096,29 @@ void paged_chunk_kernel(ChunkParams p) {
   }
 }
 
-template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT, int WAVES>
-int launch_one(const ChunkParams& p, int wgs, hipStream_t st) {
-  ChunkParams q = p;
-  q.wgs = wgs;
-  KernelTimer timer;
-  timer.launch(paged_chunk_kernel<D, BF16, GRP, LSE, SPLIT, WAVES>, dim3(wgs), dim3(64 * WAVES), 0,
-               st, q);
-  return check_launch("paged_chunk_kernel");
-}
-
 template <int D, bool BF16, bool GRP, bool LSE>
-int launch_paths(const ChunkParams& p, hipStream_t st) {
-  if (p.split_wgs > 0)
-    if (int rc = launch_one<D, BF16, GRP, LSE, true, 4>(p, p.split_wgs, st)) return rc;
-  if (p.tile_wgs == 0) return AKT_OK;
-  return launch_one<D, BF16, GRP, LSE, false, chunk_tile_waves(D)>(p, p.tile_wgs, st);
+__global__ __launch_bounds__(64 * chunk_waves(D))
+__attribute__((amdgpu_waves_per_eu(chunk_waves_per_simd(D), chunk_waves_per_simd(D))))
+void paged_chunk_kernel(ChunkParams p) {
+  constexpr int WAVES = chunk_waves(D);
+  __shared__ __attribute__((aligned(16)))
+  char lds[kCkNBuf * 2 * ck_tile_keys(D) * D * 2];
+  const int block = blockIdx.x;
+  if (block < p.split_wgs)
+    chunk_range<D, BF16, GRP, LSE, true>(p, lds, block, p.split_wgs, p.arrive, p.partials);
+  else
+    chunk_range<D, BF16, GRP, LSE, false>(
+        p, lds, block - p.split_wgs, p.tile_wgs, p.arrive + WAVES * p.split_wgs,
+        p.partials + 2 * (int64_t)p.split_wgs * WAVES * chunk_split_wave_bytes(D));
 }
 
 template <int D, bool BF16, bool GRP>
 int launch_lse(const ChunkParams& p, hipStream_t st) {
-  return p.lse ? launch_paths<D, BF16, GRP, true>(p, st) : launch_paths<D, BF16, GRP, false>(p, st);
+  KernelTimer timer;
+  const dim3 grid(p.split_wgs + p.tile_wgs), block(64 * chunk_waves(D));
+  if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true>, grid, block, 0, st, p);
+  else timer.launch(paged_chunk_kernel<D, BF16, GRP, false>, grid, block, 0, st, p);
+  return check_launch("paged_chunk_kernel");
 }
 
 template <int D>
@@ -1162,18 +1152,19 @@ namespace {
 
 constexpr int kCkMinKeys = 256;
 
-// How a call is served: the workgroups of both kernels (0: not launched).
+// How a call is served: the workgroups of the sequences of few tokens and of many (0: there
+// can be none).
 struct ChunkPlan {
-  int waves;  // of the tile kernel's workgroups
   int split_tokens;
-  int64_t split_wgs, tile_wgs, slots;
+  int64_t split_wgs, tile_wgs;
+  int64_t counters, partial_bytes;
 };
 
-// Workgroups of a launch: the resident ones, fewer where the axis is too short for them
-// (bounded from above by what the host knows: every sequence as long as all pages).
+// Workgroups of an axis: as many as are resident, fewer where it is too short for them (bounded
+// from above by what the host knows: every sequence as long as all pages).
 int64_t axis_wgs(double units, int64_t tokens, int64_t resident) {
   const double wgs = ceil(units * (double)(tokens + kCkUnitCost) / kCkMinKeys);
-  return wgs < (double)resident ? (int64_t)wgs : resident;
+  return wgs < (double)resident ? round_up((int64_t)wgs, 8) : resident;
 }
 
 ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
@@ -1185,21 +1176,20 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
     cus = 256;  // no device: what an MI355X has
   const int64_t tokens = page_size * total_pages;
   const int64_t seqs = batch < total_q ? batch : total_q;
+  const int waves = chunk_waves((int)D);
+  const int64_t resident = round_up((int64_t)cus * chunk_waves_per_simd((int)D) * 4 / waves, 8);
   ChunkPlan c = {};
-  c.waves = chunk_tile_waves((int)D);
-  const int64_t rows = 32 * c.waves;
   // Sequences of up to kCkSplitRows rows to a kv head share out their keys.  How many tokens a
   // sequence has is known on the device alone, unless there is one, or all are few.
   c.split_tokens = (int)(kCkSplitRows / G);
   const bool few = total_q <= c.split_tokens;
   if (!few && batch == 1) c.split_tokens = 0;
-  const int64_t resident = (int64_t)cus * chunk_waves_per_simd((int)D);
   if (c.split_tokens > 0) c.split_wgs = axis_wgs((double)Hkv * seqs, tokens, resident);
   if (!few)
-    c.tile_wgs = axis_wgs((double)Hkv * (total_q / (rows / G) + seqs), tokens,
-                          resident * 4 / c.waves);
-  const int64_t a = 4 * c.split_wgs, b = c.waves * c.tile_wgs;
-  c.slots = 2 * (a > b ? a : b);  // two a wave
+    c.tile_wgs = axis_wgs((double)Hkv * (total_q / (32 * waves / G) + seqs), tokens, resident);
+  c.counters = waves * (c.split_wgs + c.tile_wgs);
+  c.partial_bytes = 2 * waves * (c.split_wgs * chunk_split_wave_bytes((int)D) +
+                                 c.tile_wgs * chunk_wave_bytes((int)D));
   return c;
 }
 
@@ -1219,7 +1209,7 @@ extern "C" size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q,
   const ChunkPlan c = chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
                                  page_size, total_pages);
   return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) +
-                  c.slots * chunk_wave_bytes((int)head_dim));
+                  c.partial_bytes);
 }
 
 extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
@@ -1269,7 +1259,7 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
     return set_error(AKT_ERR_WORKSPACE, "chunk attention needs a workspace of %zu bytes, got %zu",
                      need, workspace ? workspace_bytes : (size_t)0);
   AKT_CHECK(aligned16(workspace), "the workspace must be 16-byte aligned");
-  AKT_CHECK(plan.slots / 2 <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4,
+  AKT_CHECK(plan.counters <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4,
             "too many workgroups");
 
   ChunkParams p = {};
@@ -1296,7 +1286,7 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   p.Hq = (int)num_q_heads;
   p.Hkv = (int)num_kv_heads;
   p.G = (int)G;
-  p.TR = (int)(32 * plan.waves / G);
+  p.TR = (int)(32 * chunk_waves((int)head_dim) / G);
   p.g_magic = (uint32_t)((65536 + G - 1) / G);
   p.page_size = (int)page_size;
   const uint64_t magic = (1ull << 32) / (uint64_t)page_size;

@@ -38,24 +38,27 @@ struct ChunkParams {
   int causal;
   int neg_q;       // 1: softmax_scale < 0, computed as (-Q) K^T at |softmax_scale|
   float qk_scale;  // |softmax_scale| * log2(e), at least FLT_MIN
-  int wgs;         // workgroups of the launch
-  int split_tokens;  // sequences of up to so many new tokens are the split kernel's
-  int split_wgs, tile_wgs;  // workgroups of the two kernels, 0: not launched
+  int split_tokens;  // sequences of up to so many new tokens share out their keys
+  int split_wgs, tile_wgs;  // workgroups of the sequences of few tokens and of many
   int min_keys;    // fewest keys (with unit costs) of a workgroup's range, at least kCkBlock
 };
 
-// Bytes of a wave's part of a partial slot: the fp32 O of 32 rows as it sits in registers
-// and a 16-byte (m, l, exact l, -) row for each.
+// Waves of a workgroup.  At D = 128 eight share a tile of 64 keys (one workgroup to a CU):
+// half the loads, LDS stores and barriers a wave, and faster at every size measured (us, four
+// waves / eight, 32 heads over 8): 32 tokens after 200 26.6 / 24.6, 777 after 0 41.0 / 36.2,
+// 777 after 8000 153 / 142, 2048 after 30000 1239 / 1101.
+__host__ __device__ constexpr int chunk_waves(int D) { return D == 128 ? 8 : 4; }
+
+// Bytes of a wave's part of a partial slot: fp32 O of 32 rows as it sits in registers and a
+// 16-byte (m, l, exact l, -) row for each.  Where the waves share out the keys, a wave
+// holds its share of the pieces of O, at most half as many waves sharing as there are.
 __host__ __device__ constexpr int64_t chunk_wave_bytes(int D) { return 32 * D * 4 + 32 * 16; }
+__host__ __device__ constexpr int64_t chunk_split_wave_bytes(int D) {
+  return 32 * D * 4 * 2 / chunk_waves(D) + 32 * 16;
+}
 
-// Waves to a SIMD, and workgroups of four waves to a CU.
+// Waves to a SIMD.
 __host__ __device__ constexpr int chunk_waves_per_simd(int D) { return D <= 128 ? 2 : 1; }
-
-// Waves of the tile kernel's workgroups.  At D = 128 eight share a tile of 64 keys (one
-// workgroup to a CU): half the loads, LDS stores and barriers a wave, and faster at every size
-// measured (us, four waves / eight, 32 heads over 8): 32 tokens after 200 26.6 / 24.6, 777
-// after 0 41.0 / 36.2, 777 after 8000 153 / 142, 2048 after 30000 1239 / 1101.
-__host__ __device__ constexpr int chunk_tile_waves(int D) { return D == 128 ? 8 : 4; }
 
 int chunk_launch_64(const ChunkParams& p, bool bf16, hipStream_t st);
 int chunk_launch_128(const ChunkParams& p, bool bf16, hipStream_t st);
