@@ -216,11 +216,10 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit&
   }
 }
 
-// The units of one of the W ranges of the axis of the sequences of few tokens (SPLIT) or of
-// many.  lds: the workgroup's tile buffers.
+// The units of the ranges of workgroup `block` of W, on the axis of the sequences of few tokens
+// (SPLIT) or of many.  lds: the workgroup's tile buffers.
 template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT>
-__device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int block, int W,
-                                            int* arrive, char* partials) {
+__device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int block, int W) {
   constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
@@ -236,15 +235,20 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   constexpr int PER_T = kBN * CPR / kThreads;  // chunks per thread per matrix
   constexpr int RPC = 64 / CPR;                  // rows of a wave's 64 chunks
   static_assert(16 % RPC == 0, "a wave's chunks lie in one 16-key group");
+  // Waves that serve a range: all of a workgroup's, or, where they share out the keys, four, so
+  // that one range's start and merge overlap with another's loads on the same CU.
+  constexpr int TW = SPLIT ? 4 : WAVES;
   __shared__ float4_t sm_ml[WAVES][32];
   __shared__ int sm_bad[WAVES];
+  __shared__ int sm_team[WAVES / TW];  // arrivals of each team at its barriers
 
   const int tid0 = threadIdx.x;
   const int wave = uniform(tid0 >> 6);
 
   // ---- this workgroup's range of the axis.  Workgroup i runs on XCD i % 8, so
   // consecutive ranges go to one XCD's L2.
-  const int wg = (block % 8) * (W / 8) + block / 8;
+  const int team = SPLIT ? wave / TW : 0, twave = wave - team * TW;
+  const int wg = team * W + (block % 8) * (W / 8) + block / 8;
   const int lane0 = tid0 & 63;
   // The sequences that this kernel serves.
   auto mine = [&](const Seq& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
@@ -262,6 +266,26 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     return v;
   };
   int64_t Lw = 0, x0 = 0, x1 = 0;
+  const int ranges = W * (WAVES / TW);
+  if (SPLIT && WAVES > TW) {
+    if (tid0 < WAVES / TW) sm_team[tid0] = 0;
+    __syncthreads();
+  }
+  // Barrier of a team's waves: each counts itself in, and waits until all have (they are of
+  // one workgroup, and none waits for anything but its team).
+  int team_target = 0;
+  auto team_sync = [&]() {
+    if constexpr (WAVES == TW) {
+      __syncthreads();
+    } else {
+      team_target += TW;
+      if (lane0 == 0)
+        __hip_atomic_fetch_add(&sm_team[team], 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
+      while (uniform(__hip_atomic_load(&sm_team[team], __ATOMIC_ACQUIRE,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP)) < team_target)
+        __builtin_amdgcn_s_sleep(1);
+    }
+  };
   const float c = p.qk_scale;
   // ---- the keys [k0, k1) of a unit, for all four waves.
   auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
@@ -616,7 +640,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+        return p.partials + (SPLIT ? 0 : p.many_partial) + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
       };
       char* mine = slot_of(wg);
 #pragma unroll
@@ -632,9 +656,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       // The stores (device scope) are complete before the count.
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&arrive[WAVES * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[(SPLIT ? 0 : p.many_counter) + WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&arrive[WAVES * wf + wave], 0);
+      if (lane == 0) atomicExch(&p.arrive[(SPLIT ? 0 : p.many_counter) + WAVES * wf + wave], 0);
       constexpr int UB = D == 64 ? 4 : 2;  // partials in flight
       m_run = AKT_C_NEG_INF;
       l_row = x_row = 0.f;
@@ -719,12 +743,12 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       voffh[n] =
           (vrow + 8) * ROWB + (((4 * n + vcl) ^ tswz<D>(vrow + 8)) * 16) + (s16 & 1) * 8;
     }
-    constexpr int RG = decltype(rg_c)::value, KG = WAVES / RG;
+    constexpr int RG = decltype(rg_c)::value, KG = TW / RG;
     constexpr int OB = 32 * D * 4;   // bytes of a wave's O
     constexpr int NQ = 4 * NT / KG;  // 4-element pieces of O that a wave merges
     static_assert(WAVES * OB <= kCkNBuf * BUFB, "the waves' O fit the tile buffers");
     static_assert(NQ % 2 == 0, "whole 16-byte chunks");
-    const int rg = wave % RG, kg = wave / RG;
+    const int rg = twave % RG, kg = twave / RG;
     const int rows = u.ntok * p.G;
     const bool active = 32 * rg < rows;
     const int n_steps = active ? (k1 - k0 + 31) / 32 : 0;
@@ -796,7 +820,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       return E::as8(uint4_t{lo.x, lo.y, hi.x, hi.y});
     };
 
-    __syncthreads();  // the last unit's LDS reads are done
+    team_sync();  // the last unit's LDS reads are done
     bool bad = false;
     if (kg < n_steps) {
       load_ids(kg);
@@ -884,7 +908,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         *reinterpret_cast<uint4_t*>(vst + ((4 * n + k) * 64 + lane) * 16) =
             as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
                                oacc[n][4 * k + 3]});
-    __syncthreads();
+    team_sync();
     if (!active) return;
     float4_t acc[NQ];
     {
@@ -892,11 +916,11 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       m_run = AKT_C_NEG_INF;
 #pragma unroll
       for (int w = 0; w < KG; ++w)
-        m_run = __builtin_elementwise_maximum(m_run, sm_ml[w * RG + rg][l32][0]);
+        m_run = __builtin_elementwise_maximum(m_run, sm_ml[team * TW + w * RG + rg][l32][0]);
       l_row = x_row = 0.f;
 #pragma unroll
       for (int w = 0; w < KG; ++w) {
-        const float4_t ml = sm_ml[w * RG + rg][l32];
+        const float4_t ml = sm_ml[team * TW + w * RG + rg][l32];
         f[w] = fast_exp2(ml[0] - m_run);
         l_row += f[w] * ml[1];
         x_row += f[w] * ml[2];
@@ -907,19 +931,19 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
 #pragma unroll
         for (int w = 0; w < KG; ++w)
           acc[i] += f[w] * as_float4u(*reinterpret_cast<const uint4_t*>(
-                               lds + (w * RG + rg) * OB + ((NQ * kg + i) * 64 + lane) * 16));
+                               lds + (team * TW + w * RG + rg) * OB + ((NQ * kg + i) * 64 + lane) * 16));
       }
     }
     if (!(k0 == 0 && k1 == u.kend)) {
       // Partial: this wave's pieces and the row's (m, l); the last of the unit's workgroups
       // merges them, wave by wave.
-      constexpr int64_t kWaveB = chunk_split_wave_bytes(D), kSlotB = WAVES * kWaveB;
+      constexpr int64_t kWaveB = chunk_split_wave_bytes(D), kSlotB = TW * kWaveB;
       constexpr uint32_t kMl = (uint32_t)kWaveB - 512;  // the rows' (m, l)
       const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+        return p.partials + (SPLIT ? 0 : p.many_partial) + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + twave * kWaveB;
       };
       char* mine = slot_of(wg);
       if (row < rows) {
@@ -932,9 +956,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       }
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&arrive[WAVES * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[(SPLIT ? 0 : p.many_counter) + TW * wf + twave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&arrive[WAVES * wf + wave], 0);
+      if (lane == 0) atomicExch(&p.arrive[(SPLIT ? 0 : p.many_counter) + TW * wf + twave], 0);
       if (row < rows) {
         constexpr int UB = 32 / NQ < 8 ? 32 / NQ : 8;  // partials in flight
         m_run = AKT_C_NEG_INF;
@@ -999,7 +1023,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       int64_t total = uniform64(shfl64(inc, 63));
       for (int jb = 64; jb < p.B; jb += 64)
         total += uniform64(shfl64(scan64(seq_length(jb + lane0)), 63));
-      Lw = (total + W - 1) / W;
+      Lw = (total + ranges - 1) / ranges;
       if (Lw < p.min_keys) Lw = p.min_keys;
       Lw = uniform64(Lw);
       x0 = wg * Lw;
@@ -1062,7 +1086,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         // Nothing to see: zeros, by the workgroup of what would be the first block.
         const int rows = u.ntok * p.G;
         if (x0 - us < kCkBlock && x1 - us >= kCkBlock)
-          for (int idx = tid0; idx < rows * CPR; idx += kThreads) {
+          for (int idx = 64 * twave + lane0; idx < rows * CPR; idx += 64 * TW) {
             const int row = idx / CPR;
             const int tok = (int)((uint32_t)row * p.g_magic >> 16);
             const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
@@ -1096,26 +1120,54 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   }
 }
 
+// Workgroups (of all W, a multiple of 8) for the sequences of few tokens, where a launch may hold
+// both kinds: in proportion to the lengths of the two axes, a key of the other weighing
+// chunk_tile_cost.
+template <int D>
+__device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
+  const int lane = threadIdx.x & 63;
+  double few = 0, many = 0;
+  for (int b = lane; b < p.B; b += 64) {
+    const Seq s = load_seq(p, b);
+    const double len = (double)head_length(p, s);
+    if (s.n <= p.split_tokens) few += len;
+    else many += len;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    few += __shfl_xor(few, d, 64);
+    many += __shfl_xor(many, d, 64);
+  }
+  if (many == 0) return W;
+  if (few == 0) return 0;
+  const int s = 8 * (int)(W / 8 * (few / (few + chunk_tile_cost(D) * many)) + 0.5);
+  return uniform(min(max(s, 8), W - 8));
+}
+
 template <int D, bool BF16, bool GRP, bool LSE>
 __global__ __launch_bounds__(64 * chunk_waves(D))
 __attribute__((amdgpu_waves_per_eu(chunk_waves_per_simd(D), chunk_waves_per_simd(D))))
 void paged_chunk_kernel(ChunkParams p) {
-  constexpr int WAVES = chunk_waves(D);
   __shared__ __attribute__((aligned(16)))
   char lds[kCkNBuf * 2 * ck_tile_keys(D) * D * 2];
-  const int block = blockIdx.x;
-  if (block < p.split_wgs)
-    chunk_range<D, BF16, GRP, LSE, true>(p, lds, block, p.split_wgs, p.arrive, p.partials);
+  const int block = blockIdx.x, W = gridDim.x;
+  // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
+  // of them in what follows.
+  __shared__ int sm_share;
+  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D>(p, W) : p.kinds == kCkFew ? W : 0;
+  if (threadIdx.x == 0) sm_share = share;
+  __syncthreads();
+  const int S = uniform(sm_share);
+  if (block < S)
+    chunk_range<D, BF16, GRP, LSE, true>(p, lds, block, S);
   else
-    chunk_range<D, BF16, GRP, LSE, false>(
-        p, lds, block - p.split_wgs, p.tile_wgs, p.arrive + WAVES * p.split_wgs,
-        p.partials + 2 * (int64_t)p.split_wgs * WAVES * chunk_split_wave_bytes(D));
+    chunk_range<D, BF16, GRP, LSE, false>(p, lds, block - S, W - S);
 }
 
 template <int D, bool BF16, bool GRP>
 int launch_lse(const ChunkParams& p, hipStream_t st) {
   KernelTimer timer;
-  const dim3 grid(p.split_wgs + p.tile_wgs), block(64 * chunk_waves(D));
+  const dim3 grid(p.wgs), block(64 * chunk_waves(D));
   if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true>, grid, block, 0, st, p);
   else timer.launch(paged_chunk_kernel<D, BF16, GRP, false>, grid, block, 0, st, p);
   return check_launch("paged_chunk_kernel");
@@ -1152,11 +1204,10 @@ namespace {
 
 constexpr int kCkMinKeys = 256;
 
-// How a call is served: the workgroups of the sequences of few tokens and of many (0: there
-// can be none).
+// How a call is served.
 struct ChunkPlan {
-  int split_tokens;
-  int64_t split_wgs, tile_wgs;
+  int split_tokens, kinds;
+  int64_t wgs, many_counter, many_partial;  // where the counters and partials of the second kind begin
   int64_t counters, partial_bytes;
 };
 
@@ -1184,12 +1235,21 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   c.split_tokens = (int)(kCkSplitRows / G);
   const bool few = total_q <= c.split_tokens;
   if (!few && batch == 1) c.split_tokens = 0;
-  if (c.split_tokens > 0) c.split_wgs = axis_wgs((double)Hkv * seqs, tokens, resident);
-  if (!few)
-    c.tile_wgs = axis_wgs((double)Hkv * (total_q / (32 * waves / G) + seqs), tokens, resident);
-  c.counters = waves * (c.split_wgs + c.tile_wgs);
-  c.partial_bytes = 2 * waves * (c.split_wgs * chunk_split_wave_bytes((int)D) +
-                                 c.tile_wgs * chunk_wave_bytes((int)D));
+  if (c.split_tokens > 0) c.kinds |= kCkFew;
+  if (!few) c.kinds |= kCkMany;
+  double units = 0;
+  if (c.kinds & kCkFew) units += (double)Hkv * seqs;
+  if (c.kinds & kCkMany) units += (double)Hkv * (total_q / (32 * waves / G) + seqs);
+  c.wgs = axis_wgs(units, tokens, resident);
+  if (c.kinds == (kCkFew | kCkMany) && c.wgs < 16) c.wgs = 16;  // eight of each kind
+  // Two partial slots to a range, whichever kind a workgroup serves.
+  if (c.kinds & kCkFew) {
+    c.many_counter = c.wgs * waves;
+    c.many_partial = 2 * c.wgs * waves * chunk_split_wave_bytes((int)D);
+  }
+  c.counters = c.many_counter + (c.kinds & kCkMany ? c.wgs * waves : 0);
+  c.partial_bytes =
+      c.many_partial + (c.kinds & kCkMany ? 2 * c.wgs * waves * chunk_wave_bytes((int)D) : 0);
   return c;
 }
 
@@ -1297,8 +1357,10 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   p.qk_scale = fmaxf(fabsf(softmax_scale) * kLog2e, FLT_MIN);
   p.min_keys = kCkMinKeys;
   p.split_tokens = plan.split_tokens;
-  p.split_wgs = (int)plan.split_wgs;
-  p.tile_wgs = (int)plan.tile_wgs;
+  p.kinds = plan.kinds;
+  p.wgs = (int)plan.wgs;
+  p.many_counter = (int)plan.many_counter;
+  p.many_partial = plan.many_partial;
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == AKT_DTYPE_BF16;
   if (head_dim == 64) return chunk_launch_64(p, bf16, st);

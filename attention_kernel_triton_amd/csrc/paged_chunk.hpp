@@ -14,6 +14,11 @@ constexpr int kCkBlock = 128;    // keys of a block, the grain in which units ar
 constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
 // Rows of a sequence and kv head up to which the waves of a workgroup share out the keys.
 constexpr int kCkSplitRows = 64;
+constexpr int kCkFew = 1, kCkMany = 2;
+// A key of a unit of many rows costs a workgroup as much as so many of a unit of few (us at 1.4,
+// 2 and 3, 777 new tokens beside 15 single ones: D = 128 73.9 / 69.4 / 72.4, D = 256 77.6 / 83.6
+// / 97.8, D = 64 75.2 / 69.8 / 67.9; 2000 beside 7 after 3000 to 9000, D = 128 327 / 334 / 592).
+__host__ __device__ constexpr double chunk_tile_cost(int D) { return D <= 128 ? 2.0 : 1.4; }
 
 struct ChunkParams {
   const half_t* q;     // [total_q, Hq, D] rows (strides q_st, q_sh)
@@ -39,22 +44,26 @@ struct ChunkParams {
   int neg_q;       // 1: softmax_scale < 0, computed as (-Q) K^T at |softmax_scale|
   float qk_scale;  // |softmax_scale| * log2(e), at least FLT_MIN
   int split_tokens;  // sequences of up to so many new tokens share out their keys
-  int split_wgs, tile_wgs;  // workgroups of the sequences of few tokens and of many
+  int kinds;         // sequences that there can be: kCkFew | kCkMany
+  int wgs;
+  int many_counter;      // where the second kind's arrival counters
+  int64_t many_partial;  // and partials begin
   int min_keys;    // fewest keys (with unit costs) of a workgroup's range, at least kCkBlock
 };
 
-// Waves of a workgroup.  At D = 128 eight share a tile of 64 keys (one workgroup to a CU):
-// half the loads, LDS stores and barriers a wave, and faster at every size measured (us, four
-// waves / eight, 32 heads over 8): 32 tokens after 200 26.6 / 24.6, 777 after 0 41.0 / 36.2,
-// 777 after 8000 153 / 142, 2048 after 30000 1239 / 1101.
-__host__ __device__ constexpr int chunk_waves(int D) { return D == 128 ? 8 : 4; }
+// Waves of a workgroup.  Up to D = 128 eight share a tile of 64 keys (one workgroup to a CU):
+// half the loads, LDS stores and barriers a wave, and faster for most sizes (us, four waves /
+// eight): D = 128, 32 heads over 8: 32 tokens after 200 26.6 / 24.6, 777 after 0 41.0 / 36.2,
+// 777 after 8000 153 / 142, 2048 after 30000 1239 / 1101; D = 64, 64 heads over 16: 8 x 1024
+// after 0 150 / 144, 1024 after 10000 250 / 226, 100 after 1000 22.7 / 24.3.
+__host__ __device__ constexpr int chunk_waves(int D) { return D <= 128 ? 8 : 4; }
 
 // Bytes of a wave's part of a partial slot: fp32 O of 32 rows as it sits in registers and a
-// 16-byte (m, l, exact l, -) row for each.  Where the waves share out the keys, a wave
-// holds its share of the pieces of O, at most half as many waves sharing as there are.
+// 16-byte (m, l, exact l, -) row for each.  Where four waves share out the keys, a wave
+// holds its share of the pieces of O: a quarter, or half where two share each half of them.
 __host__ __device__ constexpr int64_t chunk_wave_bytes(int D) { return 32 * D * 4 + 32 * 16; }
 __host__ __device__ constexpr int64_t chunk_split_wave_bytes(int D) {
-  return 32 * D * 4 * 2 / chunk_waves(D) + 32 * 16;
+  return 32 * D * 4 * 2 / 4 + 32 * 16;
 }
 
 // Waves to a SIMD.

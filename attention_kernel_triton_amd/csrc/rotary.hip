@@ -224,103 +224,115 @@ struct AppendRotaryParams {
   const double* inv_freq;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
   int64_t sp, skv, sh, ss;
-  int64_t total;
+  int total;
   int B, Hq, Hkv, D, rot, inter;
   float factor;
   int page_size, num_pool_pages, total_pages;
 };
 
 struct Place {
-  int64_t pos;  // -1: the token belongs to no sequence
+  int pos;         // -1: the token belongs to no sequence
   int page, slot;  // page -1: not stored
 };
-// Sequence, position, page and slot of token tok, wave-uniform.
-__device__ __forceinline__ Place place_of(const AppendRotaryParams& p, int64_t tok, int lane) {
+// Sequence, position, page and slot of token tok, wave-uniform.  Page table entries outside
+// their range are taken clamped.
+__device__ __forceinline__ Place place_of(const AppendRotaryParams& p, int tok, int lane) {
   int cnt = 0;  // sequences that start at or before tok
   for (int jb = 0; jb < p.B; jb += 64) {
     const int j = jb + lane;
-    const int64_t aj = j < p.B ? (int64_t)p.append_indptr[j] : INT64_MAX;
+    const int aj = j < p.B ? p.append_indptr[j] : INT32_MAX;
     cnt += __popcll(__ballot(aj <= tok));
   }
   Place r = {-1, -1, 0};
-  const int b = cnt - 1;
+  const int b = uniform(cnt) - 1;
   if (b < 0) return r;
-  const int64_t a0 = p.append_indptr[b], a1 = p.append_indptr[b + 1];
-  const int ip0 = p.indptr[b], np = p.indptr[b + 1] - ip0;
+  const int a0 = p.append_indptr[b], a1 = p.append_indptr[b + 1];
+  const int ip0 = min(max(p.indptr[b], 0), p.total_pages);
+  const int np = min(max(p.indptr[b + 1], ip0), p.total_pages) - ip0;
   const int last = min(max(p.last_len[b], 0), p.page_size);
-  const int64_t len = (int64_t)(np - 1) * p.page_size + last;
-  const int64_t pos = len - (a1 - a0) + (tok - a0);
-  if (tok < a0 || tok >= a1 || np <= 0 || pos < 0 || pos >= len) return r;
-  r.pos = pos;
-  const int lp = (int)(pos / p.page_size);
-  r.slot = (int)(pos - (int64_t)lp * p.page_size);
-  const int64_t at = (int64_t)ip0 + lp;
-  if (at >= 0 && at < p.total_pages) {
-    const int pg = p.indices[at];
-    if (pg >= 0 && pg < p.num_pool_pages) r.page = pg;
-  }
+  const int len = (np - 1) * p.page_size + last;  // total_pages * page_size < 2^30
+  const int64_t pos = (int64_t)len - ((int64_t)a1 - tok);
+  if (tok < a0 || tok >= a1 || np <= 0 || pos < 0) return r;
+  r.pos = (int)pos;
+  const int lp = (int)((uint32_t)r.pos / (uint32_t)p.page_size);
+  r.slot = r.pos - lp * p.page_size;
+  const int pg = p.indices[ip0 + lp];
+  if ((uint32_t)pg < (uint32_t)p.num_pool_pages) r.page = pg;
   return r;
 }
 
-// Source and destination of row h of token tok (q heads, then k, then v); no destination
-// for a k or v row of a token without a page.
-struct Rows {
-  const half_t* src;
-  half_t* dst;
-  bool rotated;
-};
-__device__ __forceinline__ Rows rows_of(const AppendRotaryParams& p, int64_t tok, const Place& pl,
-                                        int h) {
-  Rows r;
+// Rows of a token: q heads, then k, then v.
+__device__ __forceinline__ const half_t* row_src(const AppendRotaryParams& p, int tok, int h) {
+  const int hk = h - p.Hq, hv = hk - p.Hkv;
+  if (hk < 0) return p.q + tok * p.q_st + h * p.q_sh;
+  return hv < 0 ? p.k + tok * p.k_st + hk * p.k_sh : p.v + tok * p.v_st + hv * p.v_sh;
+}
+// Destination of row h; none for a k or v row of a token without a page.
+__device__ __forceinline__ half_t* row_dst(const AppendRotaryParams& p, int tok, const Place& pl,
+                                           int h) {
+  const int hk = h - p.Hq, hv = hk - p.Hkv;
+  if (hk < 0) return p.qo + ((int64_t)tok * p.Hq + h) * p.D;
+  if (pl.page < 0) return nullptr;
   half_t* slot = p.pool + pl.page * p.sp + pl.slot * p.ss;
-  if (h < p.Hq) {
-    r.src = p.q + tok * p.q_st + h * p.q_sh;
-    r.dst = p.qo + (tok * p.Hq + h) * p.D;
-    r.rotated = true;
-    return r;
-  }
-  h -= p.Hq;
-  r.rotated = h < p.Hkv;
-  if (!r.rotated) h -= p.Hkv;
-  r.src = r.rotated ? p.k + tok * p.k_st + h * p.k_sh : p.v + tok * p.v_st + h * p.v_sh;
-  r.dst = pl.page < 0 ? nullptr : slot + (r.rotated ? 0 : p.skv) + h * p.sh;
-  return r;
+  return hv < 0 ? slot + hk * p.sh : slot + p.skv + hv * p.sh;
 }
 
-// One wave to a token.
+// One wave to a token.  The rows are loaded before the token's place is known: its look-up,
+// three dependent loads, runs meanwhile.
+constexpr int kRBatch = 3;  // steps in flight
+
 template <bool BF16, bool INTER>
 __global__ __launch_bounds__(kRThreads) void append_rotary_kernel(AppendRotaryParams p) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  const int64_t tok = (int64_t)blockIdx.x * kRWaves + wave;
+  const int tok = (int)blockIdx.x * kRWaves + wave;
   if (tok >= p.total) return;
+  const int upr = p.D / 16;
+  const int col = lane % upr, h_lane = lane / upr;
+  const bool turned = 16 * col < p.rot;
+  const int heads = p.Hq + 2 * p.Hkv, rotated = p.Hq + p.Hkv;
+  const int hpw = 64 / upr;  // rows to a step
+  // Chunks of a unit, in elements (rotated rows of the half layout, others).
+  const int d0 = !INTER && turned ? 8 * col : 16 * col;
+  const int d1 = !INTER && turned ? p.rot / 2 + 8 * col : 16 * col + 8;
+  uint4_t x[kRBatch], y[kRBatch];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kRBatch; ++k) {
+      const int h = h0 + k * hpw + h_lane;
+      if (h < heads) {
+        const half_t* src = row_src(p, tok, h);
+        const bool r = h < rotated;
+        x[k] = ld16(src + (r ? d0 : 16 * col));
+        y[k] = ld16(src + (r ? d1 : 16 * col + 8));
+      }
+    }
+  };
+  load(0);
   const Place pl = place_of(p, tok, lane);
   if (pl.pos < 0) return;
-  const int upr = p.D / 16;
-  const int col = lane % upr;
-  const bool turned = 16 * col < p.rot;
   float cs[8], sn[8];
   if (turned) {
 #pragma unroll
     for (int f = 0; f < 8; ++f)
       turn_of(p.inv_freq[8 * col + f] * kTurn, (double)pl.pos, p.factor, cs[f], sn[f]);
   }
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int hpw = 64 / upr;  // rows to a step
-#pragma unroll 4
-  for (int h0 = 0; h0 < heads; h0 += hpw) {
-    const int h = h0 + lane / upr;
-    if (h >= heads) break;
-    const Rows r = rows_of(p, tok, pl, h);
-    const bool turn = turned && r.rotated;
-    const int d0 = !INTER && turn ? 8 * col : 16 * col;
-    const int d1 = !INTER && turn ? p.rot / 2 + 8 * col : 16 * col + 8;
-    uint4_t x = ld16(r.src + d0), y = ld16(r.src + d1);
-    if (turn) rotate8<BF16, INTER>(x, y, cs, sn);
-    if (r.dst) {
-      st16(r.dst + d0, x);
-      st16(r.dst + d1, y);
+  for (int h0 = 0;;) {
+#pragma unroll
+    for (int k = 0; k < kRBatch; ++k) {
+      const int h = h0 + k * hpw + h_lane;
+      if (h < heads) {
+        const bool r = h < rotated;
+        if (turned && r) rotate8<BF16, INTER>(x[k], y[k], cs, sn);
+        if (half_t* dst = row_dst(p, tok, pl, h)) {
+          st16(dst + (r ? d0 : 16 * col), x[k]);
+          st16(dst + (r ? d1 : 16 * col + 8), y[k]);
+        }
+      }
     }
+    h0 += kRBatch * hpw;
+    if (h0 >= heads) break;  // wave-uniform
+    load(h0);
   }
 }
 
@@ -328,12 +340,12 @@ template <bool BF16>
 __global__ __launch_bounds__(kRThreads) void append_rotary_gen_kernel(AppendRotaryParams p) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  const int64_t tok = (int64_t)blockIdx.x * kRWaves + wave;
+  const int tok = (int)blockIdx.x * kRWaves + wave;
   if (tok >= p.total) return;
   const Place pl = place_of(p, tok, lane);
   if (pl.pos < 0) return;
   const int cpr = p.D / 8;
-  const int heads = p.Hq + 2 * p.Hkv;
+  const int heads = p.Hq + 2 * p.Hkv, rotated = p.Hq + p.Hkv;
   // Column by column (64 at a time where a row has more): a lane keeps its plan.
   const int cw = min(cpr, 64), hpw = 64 / cw;
   if (lane >= cw * hpw) return;
@@ -341,9 +353,9 @@ __global__ __launch_bounds__(kRThreads) void append_rotary_gen_kernel(AppendRota
     Gen8 g;
     gen_plan(g, col, p.rot, p.inter, p.inv_freq, (double)pl.pos, p.factor);
     for (int h = lane / cw; h < heads; h += hpw) {
-      const Rows r = rows_of(p, tok, pl, h);
-      const uint4_t x = r.rotated ? gen_apply<BF16>(g, r.src, col) : ld16(r.src + 8 * col);
-      if (r.dst) st16(r.dst + 8 * col, x);
+      const half_t* src = row_src(p, tok, h);
+      const uint4_t x = h < rotated ? gen_apply<BF16>(g, src, col) : ld16(src + 8 * col);
+      if (half_t* dst = row_dst(p, tok, pl, h)) st16(dst + 8 * col, x);
     }
   }
 }
@@ -462,10 +474,11 @@ extern "C" int akt_paged_kv_append_rotary(
   AKT_CHECK(batch >= 0 && total_new >= 0 && total_pages >= 0 && num_pool_pages >= 0 &&
                 num_q_heads > 0 && num_kv_heads > 0,
             "sizes must be non-negative");
-  AKT_CHECK(batch < (1ll << 30) && total_new < (1ll << 31) && total_pages < (1ll << 31) &&
+  AKT_CHECK(batch < (1ll << 30) && total_new < (1ll << 30) && total_pages < (1ll << 31) &&
                 num_q_heads < (1 << 20) && num_kv_heads < (1 << 20),
             "problem too large");
   AKT_CHECK(page_size > 0 && page_size < (1 << 20), "page_size out of range");
+  AKT_CHECK(total_pages * page_size < (1ll << 30), "the page table spans too many tokens");
   if (batch == 0 || total_new == 0) return AKT_OK;
   AKT_CHECK(q && k_new && v_new && q_out && append_indptr && kv_cache && kv_page_indptr &&
                 (kv_page_indices || total_pages == 0) && kv_last_page_len && inv_freq && q_stride &&
@@ -495,7 +508,7 @@ extern "C" int akt_paged_kv_append_rotary(
   p.skv = kv_stride[1];
   p.sh = kv_stride[2];
   p.ss = kv_stride[3];
-  p.total = total_new;
+  p.total = (int)total_new;
   p.B = (int)batch;
   p.Hq = (int)num_q_heads;
   p.Hkv = (int)num_kv_heads;
