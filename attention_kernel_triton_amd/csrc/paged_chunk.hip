@@ -245,8 +245,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   const int tid0 = threadIdx.x;
   const int wave = uniform(tid0 >> 6);
 
-  // ---- this workgroup's range of the axis.  Workgroup i runs on XCD i % 8, so
-  // consecutive ranges go to one XCD's L2.
+  // ---- this workgroup's (team's) range of the axis.  Workgroup i runs on XCD i % 8, so
+  // consecutive ranges go to one XCD's L2; the second teams have the axis's second half, which
+  // leaves them idle where it is cut into one range to a workgroup.
   const int team = SPLIT ? wave / TW : 0, twave = wave - team * TW;
   const int wg = team * W + (block % 8) * (W / 8) + block / 8;
   const int lane0 = tid0 & 63;
@@ -1021,9 +1022,18 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     int64_t len = seq_length(lane0), inc = scan64(len);
     if (pass == 0) {
       int64_t total = uniform64(shfl64(inc, 63));
-      for (int jb = 64; jb < p.B; jb += 64)
-        total += uniform64(shfl64(scan64(seq_length(jb + lane0)), 63));
-      Lw = (total + ranges - 1) / ranges;
+      int seqs = __builtin_popcountll(__ballot(len > 0));
+      for (int jb = 64; jb < p.B; jb += 64) {
+        const int64_t more = seq_length(jb + lane0);
+        total += uniform64(shfl64(scan64(more), 63));
+        seqs += __builtin_popcountll(__ballot(more > 0));
+      }
+      // Where few units share the axis, one range to a workgroup, not one to a team: half the
+      // partials to a unit (us, D = 128 over 8 kv heads, a team / a workgroup: one token after
+      // 30000 54.5 / 42.8, two of those 71.5 / 62.0, four after 10000 49.8 / 45.9; eight after
+      // 10000, past the limit, 76 either way).
+      const int used = SPLIT && seqs * p.Hkv <= W / 8 ? W : ranges;
+      Lw = (total + used - 1) / used;
       if (Lw < p.min_keys) Lw = p.min_keys;
       Lw = uniform64(Lw);
       x0 = wg * Lw;
