@@ -229,18 +229,32 @@ class PagedKVCache:
 
         q [sum(counts), Hq, D], k_new and v_new [sum(counts), Hkv, D]; with inv_freq, q and k_new
         are rotated by the tokens' positions first (append_paged_kv_rotary).  Returns what
-        flash_attention_chunk_paged returns for q over the grown cache.
+        flash_attention_chunk_paged returns for q over the grown cache.  A call that is refused
+        leaves the sequences with the tokens they had.
         """
+        total = sum(int(n) for n in counts)
+        for name, x in (("q", q), ("k_new", k_new), ("v_new", v_new)):
+            if x.shape[0] != total:
+                raise ValueError(f"{name} has {x.shape[0]} rows, the counts make {total}")
+        before = {s: self._len.get(s) for s in seq_ids}
         self._grow(seq_ids, counts)
-        table = self.page_table(seq_ids)
-        q_indptr = self._indptr(counts)
-        if inv_freq is None:
-            append_paged_kv(k_new, v_new, q_indptr, self.pool, *table)
-        else:
-            q = append_paged_kv_rotary(q, k_new, v_new, q_indptr, self.pool, *table, inv_freq,
-                                       interleaved=interleaved, factor=factor)
-        return _ops.chunk_paged(q, q_indptr, self.pool, *table, causal=causal,
-                                softmax_scale=softmax_scale, return_lse=return_lse)
+        try:
+            table = self.page_table(seq_ids)
+            q_indptr = self._indptr(counts)
+            if inv_freq is None:
+                append_paged_kv(k_new, v_new, q_indptr, self.pool, *table)
+            else:
+                q = append_paged_kv_rotary(q, k_new, v_new, q_indptr, self.pool, *table, inv_freq,
+                                           interleaved=interleaved, factor=factor)
+            return _ops.chunk_paged(q, q_indptr, self.pool, *table, causal=causal,
+                                    softmax_scale=softmax_scale, return_lse=return_lse)
+        except Exception:
+            for s, n in before.items():
+                if n is None:
+                    self.release(s)
+                else:
+                    self.truncate(s, n)
+            raise
 
 
 __all__ = ["append_paged_kv", "append_paged_kv_rotary", "copy_pages", "PagedKVCache"]

@@ -110,6 +110,29 @@ def test_bookkeeping_refusals(host):
     assert cache.free_pages == 3
 
 
+def test_a_refused_extend_leaves_the_sequences_as_they_were(host):
+    cache = PagedKVCache(8, 1, 4, 64, device="cpu")
+    z = lambda n, d=64: torch.zeros(n, 1, d).half()  # noqa: E731
+    cache.append(["a"], torch.ones(6, 1, 64).half(), torch.ones(6, 1, 64).half(), [6])
+    cache.fork("a", "b")
+    for q, k, v, counts in ((z(3), z(4), z(4), [3, 1]), (z(4), z(3), z(4), [3, 1]),
+                            (z(4), z(4), z(5), [3, 1]), (z(5), z(5), z(5), [3, 1])):
+        with pytest.raises(ValueError):  # rows that are not those of the counts
+            cache.extend(["a", "c"], q, k, v, counts)
+        assert cache.free_pages == 6 and cache.seq_len("a") == 6 and "c" not in cache._pages
+    # Attention refuses (here: tensors that are not on a GPU) after pages were taken.
+    with pytest.raises(Exception):
+        cache.extend(["a", "c"], z(4), z(4), z(4), [3, 1])
+    assert cache.seq_len("a") == 6 and cache.seq_len("b") == 6 and "c" not in cache._pages
+    assert cache.free_pages == 5  # the copy of the page that a and b shared stays a's
+    for s in ("a", "b"):
+        for t in range(6):
+            assert float(cache.pool[cache._pages[s][t // 4], :, :, t % 4].min()) == 1
+    cache.release("a")
+    cache.release("b")
+    assert cache.free_pages == 8
+
+
 def _i64(*v):
     return (C.c_int64 * len(v))(*v)
 
