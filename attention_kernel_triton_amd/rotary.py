@@ -65,7 +65,7 @@ def apply_rotary(Q, K, inv_freq, positions=None, interleaved=False, factor=1.0, 
     inv_freq: float64 [rotary_dim / 2] on their device; positions: int32 or int64 [S] or [B, S],
     default 0 .. S - 1.  transpose=True applies the transposed map (negative angles, the same
     factor): it takes the gradient of Q' to that of Q, and undoes a rotation of factor 1.
-    D is a multiple of 8.
+    D is a multiple of 8 up to 1024.
     """
     return N.torch_ext().rotary(Q, K, inv_freq, positions=positions, interleaved=interleaved,
                                 factor=factor, transpose=transpose)

@@ -420,6 +420,7 @@ int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k_out,
  * and q [total_new, num_q_heads, head_dim] (rows as k_new's) is rotated by the same
  * positions into contiguous q_out.  A token whose page lies outside the table or pool is
  * not stored, its q is rotated; rows that belong to no sequence are not written.
+ * total_pages * page_size must be below 2^30.
  * No reference counterpart.
  */
 int akt_paged_kv_append_rotary(const void* q, const void* k_new, const void* v_new, void* q_out,

@@ -301,6 +301,40 @@ def test_another_stream(dev):
     assert torch.equal(o.cpu(), ref)
 
 
+@pytest.mark.parametrize("B,n,D,Hq,Hkv", [(1, 1, 128, 8, 8), (2, 16, 128, 32, 8), (4, 7, 64, 8, 8),
+                                          (5, 1, 128, 8, 8), (3, 3, 128, 4, 1)])
+def test_few_units_share_the_workgroups(dev, B, n, D, Hq, Hkv):
+    """Few units over all workgroups, on both sides of an eighth of them."""
+    Case([6000 + 131 * i for i in range(B)], [n] * B, Hq, Hkv, D, 16).check(dev)
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap on two streams each have a workspace of their own."""
+    cases = [Case([9000, 50, 2000], [1, 300, 5], 16, 4, 128, 16, seed=s) for s in range(2)]
+    args = [c.args(dev) for c in cases]
+    want = [flash_attention_chunk_paged(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    out = []
+    for _ in range(8):
+        for st, a in zip(streams, args):
+            with torch.cuda.stream(st):
+                out.append(flash_attention_chunk_paged(*a))
+    torch.cuda.synchronize()
+    for i, o in enumerate(out):
+        assert torch.equal(o, want[i % 2])
+
+
+def test_padded_batch(dev):
+    """Sequences with neither tokens nor pages between the others, rows of q past the last one."""
+    c = Case([300, 0, 0, 2000, 0, 77, 0], [200, 0, 1, 2, 0, 0, 0], 8, 2, 64, 16, slack=5)
+    o, lse, _ = c.run(dev)
+    O, L, A, C = c.oracle()
+    m = sum(c.n)
+    c.q = c.q[:m]
+    compare(c, o[:m], lse[:m], (O[:m], L[:m], A[:m], C[:m]))
+
+
 def test_graph_replays_follow_the_tables(dev):
     """A captured call replayed on changed tables and inputs, beside eager calls and a second
     graph captured on the same stream."""
