@@ -11,12 +11,12 @@
 //
 // Units.  The rows of one (sequence, kv head) are its (token, query head of the group)
 // pairs, token major; a unit is a run of up to 32 chunk_waves rows (256; 128 at D = 256) of
-// whole tokens, which share every K and V row.  Sequences of up to kCkSplitRows rows to a kv head
+// whole tokens, which share every K and V row.  Sequences of up to chunk_split_rows rows to a kv head
 // (few tokens) and those of more (many) are served differently:
 // - many: wave w of a workgroup owns rows 32 w .. 32 w + 31, and all waves walk the same keys,
 //   staged in LDS once for all of them;
-// - few: there are rows for one or two waves only, so four waves (a team) share out the keys,
-//   each loading its own, and merge at the part's end.
+// - few: there are rows for one wave only (two at D = 256), so four waves (a team) share out the
+//   keys, each loading its own, and merge at the part's end.
 //
 // Ranges.  The units of a kind stand one behind another on an axis of keys (sequence by sequence,
 // kv head by kv head, row block by row block), each as long as the keys it sees plus
@@ -52,11 +52,10 @@
 // the rows that see them (add_not_finite).
 //
 // Measured (us a call among others; D = 128, 8 kv heads unless said): 32 single tokens over 255
-// to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 60
-// (2.6 TB/s: up to 56 rows, so two waves of a team load each key); 777 new
-// tokens beside 15 single ones 64; 2048 tokens after 30000, 32 query heads, bf16 1012 (1.03
-// PFLOP/s, matrix pipe 48% busy); D = 256, 4 kv heads, 100 to 300 tokens, not causal, 61 (293
-// TFLOP/s: one wave a SIMD, 17% busy).
+// to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 56
+// (2.8 TB/s: starts and merges beside a few steps a wave); 777 new tokens beside 15 single ones
+// 65; 2048 tokens after 30000, 32 query heads, bf16 1012 (1.03 PFLOP/s, matrix pipe 48% busy);
+// D = 256, 4 kv heads, 100 to 300 tokens, not causal, 61 (293 TFLOP/s: one wave a SIMD, 17% busy).
 #include <float.h>
 #include <math.h>
 
@@ -1119,8 +1118,10 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
           }
       } else if (k0 < k1) {
         if constexpr (!SPLIT) serve(u, k0, k1, us);
-        else if (u.ntok * p.G <= 32) serve_split(u, k0, k1, us, std::integral_constant<int, 1>{});
-        else serve_split(u, k0, k1, us, std::integral_constant<int, 2>{});
+        else if (chunk_split_rows(D) <= 32 || u.ntok * p.G <= 32)
+          serve_split(u, k0, k1, us, std::integral_constant<int, 1>{});
+        else if constexpr (chunk_split_rows(D) > 32)
+          serve_split(u, k0, k1, us, std::integral_constant<int, 2>{});
       }
       if (pass == 0) {
         if (us <= x0) return;  // the range lies in this unit
@@ -1145,17 +1146,19 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
 }
 
 // Workgroups (of all W, a multiple of 8) for the sequences of few tokens, where a launch may hold
-// both kinds: in proportion to the lengths of the two axes, a key of the other weighing
-// chunk_tile_cost.
+// both kinds: in proportion to the lengths of the two axes, a key of the other weighing 1 for a
+// unit of hardly any rows up to chunk_tile_cost for one of all rows.
 template <int D>
 __device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
+  constexpr int kRows = 32 * chunk_waves(D);
   const int lane = threadIdx.x & 63;
   double few = 0, many = 0;
   for (int b = lane; b < p.B; b += 64) {
     const Seq s = load_seq(p, b);
     const double len = (double)head_length(p, s);
     if (s.n <= p.split_tokens) few += len;
-    else many += len;
+    else
+      many += len * (1 + (chunk_tile_cost(D) - 1) / kRows * min((double)s.n * p.G, (double)kRows));
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -1164,7 +1167,7 @@ __device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
   }
   if (many == 0) return W;
   if (few == 0) return 0;
-  const int s = 8 * (int)(W / 8 * (few / (few + chunk_tile_cost(D) * many)) + 0.5);
+  const int s = 8 * (int)(W / 8 * (few / (few + many)) + 0.5);
   return uniform(min(max(s, 8), W - 8));
 }
 
@@ -1254,9 +1257,9 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   const int waves = chunk_waves((int)D);
   const int64_t resident = round_up((int64_t)cus * chunk_waves_per_simd((int)D) * 4 / waves, 8);
   ChunkPlan c = {};
-  // Sequences of up to kCkSplitRows rows to a kv head share out their keys.  How many tokens a
+  // Sequences of up to chunk_split_rows rows to a kv head share out their keys.  How many tokens a
   // sequence has is known on the device alone, unless there is one, or all are few.
-  c.split_tokens = (int)(kCkSplitRows / G);
+  c.split_tokens = (int)(chunk_split_rows((int)D) / G);
   const bool few = total_q <= c.split_tokens;
   if (!few && batch == 1) c.split_tokens = 0;
   if (c.split_tokens > 0) c.kinds |= kCkFew;

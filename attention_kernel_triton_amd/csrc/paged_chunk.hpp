@@ -12,8 +12,12 @@ namespace akt {
 constexpr int kCkRows = 128;  // query heads that a kv head may have: a token's rows are in one unit
 constexpr int kCkBlock = 128;    // keys of a block, the grain in which units are cut
 constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
-// Rows of a sequence and kv head up to which waves share out the keys.
-constexpr int kCkSplitRows = 64;
+// Rows of a sequence and kv head up to which waves share out the keys.  Past 32, two waves of a
+// team would load each key, and tiles of mostly idle rows are faster up to D = 128 (us, shared
+// out / tiles: 40 rows, 16 sequences over 500 to 4000 keys 59.4 / 54.1, 64 sequences of 64 rows
+// 164 / 143, two of 64 rows over 30000 90 / 64); at D = 256, where a tile has half the waves, one
+// of 64 rows over 30000 takes 88 / 117, 16 over 500 to 4000 67 / 65.
+__host__ __device__ constexpr int chunk_split_rows(int D) { return D <= 128 ? 32 : 64; }
 constexpr int kCkFew = 1, kCkMany = 2;
 // A key of a unit of many rows costs a workgroup as much as so many of a unit of few (us at 1.4,
 // 2 and 3, 777 new tokens beside 15 single ones: D = 128 73.9 / 69.4 / 72.4, D = 256 77.6 / 83.6
@@ -60,10 +64,10 @@ __host__ __device__ constexpr int chunk_waves(int D) { return D <= 128 ? 8 : 4; 
 
 // Bytes of a wave's part of a partial slot: fp32 O of 32 rows as it sits in registers and a
 // 16-byte (m, l, exact l, -) row for each.  Where four waves share out the keys, a wave
-// holds its share of the pieces of O: a quarter, or half where two share each half of them.
+// holds its share of the pieces of O: a quarter, or (rows for two waves) half.
 __host__ __device__ constexpr int64_t chunk_wave_bytes(int D) { return 32 * D * 4 + 32 * 16; }
 __host__ __device__ constexpr int64_t chunk_split_wave_bytes(int D) {
-  return 32 * D * 4 * 2 / 4 + 32 * 16;
+  return 32 * D * 4 / (chunk_split_rows(D) > 32 ? 2 : 4) + 32 * 16;
 }
 
 // Waves to a SIMD.

@@ -166,15 +166,18 @@ def test_chunk_refusals(kw, rc, word):
 def test_chunk_workspace_sizes():
     """Small calls ask for little, large ones for two partial slots to each resident workgroup (256
     of eight waves, at D = 256 of four, as assumed without a device), for sequences of many tokens
-    and, smaller ones, of few."""
+    and, smaller ones, of few: up to 32 rows to a kv head, whose waves hold a quarter of O each, at
+    D = 256 up to 64 and half."""
     ws = N.load().akt_chunk_paged_workspace_size
     zero = -(-N.WORKSPACE_ZERO_BYTES // 256) * 256
     for D, wgs, waves in ((64, 256, 8), (128, 256, 8), (256, 256, 4)):
         o = 32 * D * 4
-        many, few = waves * (o + 512), waves * (o // 2 + 512)
+        many, few = waves * (o + 512), waves * (o // (2 if D == 256 else 4) + 512)
         assert ws(64, 10 ** 4, 32, 8, D, 16, 10 ** 5) == zero + 2 * wgs * (many + few)
         assert ws(1, 10 ** 4, 32, 8, D, 16, 10 ** 5) == zero + 2 * wgs * many
-        assert ws(64, 10, 32, 8, D, 16, 10 ** 5) == zero + 2 * wgs * few
+        # 10 tokens of 4 heads: 40 rows, few at D = 256 only.
+        assert ws(64, 10, 32, 8, D, 16, 10 ** 5) == zero + 2 * wgs * (few + (0 if D == 256 else many))
+        assert ws(64, 8, 32, 8, D, 16, 10 ** 5) == zero + 2 * wgs * few
     slot = lambda D: 8 * (32 * D * 4 + 512)  # noqa: E731
     assert zero < ws(1, 1, 8, 2, 64, 16, 2) < zero + 20 * slot(64)
     assert ws(0, 4, 8, 2, 64, 16, 2) == ws(1, 0, 8, 2, 64, 16, 2) == ws(1, 4, 8, 2, 96, 16, 2) == 0
