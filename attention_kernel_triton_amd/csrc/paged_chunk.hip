@@ -52,9 +52,9 @@
 // the rows that see them (add_not_finite).
 //
 // Measured (us a call among others; D = 128, 8 kv heads unless said): 32 single tokens over 255
-// to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 56
+// to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 58
 // (2.8 TB/s: starts and merges beside a few steps a wave); 777 new tokens beside 15 single ones
-// 65; 2048 tokens after 30000, 32 query heads, bf16 1012 (1.03 PFLOP/s, matrix pipe 48% busy);
+// 65; 2048 tokens after 30000, 32 query heads, bf16 993 to 1045 (1.0 PFLOP/s, matrix pipe 48% busy);
 // D = 256, 4 kv heads, 100 to 300 tokens, not causal, 61 (293 TFLOP/s: one wave a SIMD, 17% busy).
 #include <float.h>
 #include <math.h>

@@ -18,7 +18,7 @@
 // Rows whose rotated part does not fill units (rot % 16 != 0, or other head dims) take
 // the generic kernels: a lane handles 8 elements of a row and loads each one's partner.
 //
-// Measured: dense Q and K of 8 x 1024 tokens, 64 + 16 heads, D = 64: 35.8 us (168 MB, 4.7 TB/s,
+// Measured: dense Q and K of 8 x 1024 tokens, 64 + 16 heads, D = 64: 36 to 37 us (168 MB, 4.6 TB/s,
 // where a large copy reaches 5.1); 4 appended prompts of 1000 to 3001 tokens, 32 + 8 heads,
 // D = 128: 51.8 us (219 MB, 4.2 TB/s); 64 single tokens: 6.5 us, launch and look-ups.
 #include <math.h>

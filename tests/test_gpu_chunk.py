@@ -308,6 +308,13 @@ def test_few_units_share_the_workgroups(dev, B, n, D, Hq, Hkv):
     Case([6000 + 131 * i for i in range(B)], [n] * B, Hq, Hkv, D, 16).check(dev)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_around_the_borders(dev, D, dtype):
+    """Sequences of few and of many rows to a kv head beside each other."""
+    Case([900, 40, 2000, 0, 500, 1300, 70], [31, 32, 33, 63, 64, 65, 1], 2, 2, D, 16, dtype).check(dev)
+
+
 def test_two_streams_at_once(dev):
     """Calls that overlap on two streams each have a workspace of their own."""
     cases = [Case([9000, 50, 2000], [1, 300, 5], 16, 4, 128, 16, seed=s) for s in range(2)]
