@@ -48,8 +48,10 @@
 //
 // Masked values.  Scores are masked with a select.  V rows that some of the unit's rows see
 // and some do not are multiplied by zeros too, which an infinity or NaN in V would turn into
-// NaN: those are staged as zeros and, in the rare unit that has any, added at its end to
-// the rows that see them (add_not_finite).
+// NaN: in tiles (steps, where waves share out the keys) that hold such rows, infinities and NaNs
+// are staged as zeros, and in the rare unit that has any they are added at its end to the rows that
+// see them (add_not_finite), from the first key of the first such tile on.  Elsewhere they go
+// through the product (where an infinity whose probability rounds to 0 in the type becomes NaN).
 //
 // Measured (us a call among others; D = 128, 8 kv heads unless said): 32 single tokens over 255
 // to 8191 keys 89 (389 MB, 4.36 TB/s); 3 to 7 drafted tokens of 16 sequences, 64 query heads, 58
@@ -201,7 +203,8 @@ __device__ __forceinline__ bool zero_not_finite(uint4_t (&v)[N]) {
 }
 
 // Adds the infinities and NaNs of keys j0 .. j1 - 1 of V, which were staged as zeros, to the O
-// of the rows that see them (a key's probability is positive).  Lane (l32, g) holds dims 32 n + 8 k + 4 g .. + 3 of row l32, whose last key is lim.
+// of the rows that see them (a key's probability is positive).  Lane (l32, g) holds dims
+// 32 n + 8 k + 4 g .. + 3 of row l32, whose last key is lim.
 template <int D, bool BF16>
 __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit& u, int j0, int j1,
                                                int g, int lim, float16_t (&oacc)[D / 32]) {
@@ -644,8 +647,8 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     int any_bad = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) any_bad |= sm_bad[w];
-    if (uniform(any_bad))
-      add_not_finite<D, BF16>(p, u, max(k0, u.first + 1), k1, g, lim, oacc);
+    if (uniform(any_bad))  // from the first tile that store_tile took the values out of
+      add_not_finite<D, BF16>(p, u, k0 + max(u.first + 1 - k0, 0) / kBN * kBN, k1, g, lim, oacc);
     float l_row = xor32_sum(l_part);
     float x_row = LSE ? xor32_sum(x_part) : 0.f;
     if (!whole) {
@@ -906,8 +909,8 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     }
     if (bad)
       for (int t = kg; t < n_steps; t += KG)
-        add_not_finite<D, BF16>(p, u, max(k0 + 32 * t, u.first + 1), min(k0 + 32 * t + 32, u.kend),
-                                g, lim, oacc);
+        if (k0 + 32 * t + 31 > u.first)  // a step that the values were taken out of
+          add_not_finite<D, BF16>(p, u, k0 + 32 * t, min(k0 + 32 * t + 32, u.kend), g, lim, oacc);
 
     // ---- merge of the KG waves that share rows: piece 4 n + k of O (dims 32 n + 8 k + 4 g ..
     // + 3 of row l32) of every lane lies at [wave][piece][lane]; the wave with key group kg

@@ -374,7 +374,8 @@ int akt_paged_kv_append(const void* k_new, const void* v_new, const int32_t* app
  *   [0, total_q] and kv_page_indptr in [0, total_pages], neither decreasing; entries
  *   that do not are taken clamped and touch nothing outside the arrays.
  *   Masked K and V (later tokens, slots past len_b, skipped pages) never reach a row,
- *   whatever they hold.  dtype: AKT_DTYPE_F16 or AKT_DTYPE_BF16 (q, kv_cache and o; P is
+ *   whatever they hold; infinities and NaNs of V that a row sees reach it (as NaN where
+ *   the probability rounds to 0).  dtype: AKT_DTYPE_F16 or AKT_DTYPE_BF16 (q, kv_cache and o; P is
  *   rounded to it for P.V, the sums are fp32).  head_dim: 64, 128 or 256;
  *   num_q_heads / num_kv_heads up to 128; total_pages * page_size below 2^30.
  *   The workspace follows the decode entry points' contract and may be shared with them;

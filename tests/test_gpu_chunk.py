@@ -379,3 +379,58 @@ def test_graph_replays_follow_the_tables(dev):
                 gb.replay()
             torch.cuda.synchronize()
             assert torch.equal(oa, want) and torch.equal(ob, wantb)
+
+
+def plant(c, b, heads, first, bad):
+    """Writes `bad` into V of keys first .. first + 43 of sequence b (those that it has) for each kv
+    head in `heads`, a dim of its own for every key.  Returns (key, kv head, dim) of each."""
+    out = []
+    for h in heads:
+        for i in range(44):
+            t = first + i
+            if 0 <= t < c.lens[b]:
+                p, s = c.slot(b, t)
+                c.pool[p, 1, h, s, i] = bad
+                out.append((t, h, i))
+    return out
+
+
+# Keys on both sides of the last one that every row of a unit sees: up to 40 before it, 3 after.
+# 300 tokens of 4 heads to a kv head are several units, of which the `unit`-th is looked at.
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 24), (256, 16)])
+@pytest.mark.parametrize("n,ctx,unit", [(1, 200, 0), (1, 95, 0), (1, 4100, 0), (3, 45, 0), (3, 128, 0),
+                                        (3, 3001, 0), (12, 250, 0), (40, 7, 0), (40, 190, 0),
+                                        (300, 101, 0), (300, 101, 2), (300, 3000, 1)])
+def test_values_that_rows_see_come_through_at_the_diagonal(dev, n, ctx, unit, D, page, dtype, bad):
+    """A value of V that is not finite reaches the rows that see its key, and no others.  A positive
+    probability times it is the value itself, so each dim of O is finite or exactly that."""
+    c = Case([ctx, 33], [n, 1], 8, 2, D, page, dtype)
+    clean = c.pool.clone()
+    tokens = 32 * (8 if D <= 128 else 4) // 4
+    planted = plant(c, 0, (0, 1), ctx + unit * tokens - 40, bad)
+    planted = [(0, n, ctx, *x) for x in planted]
+    planted += [(n, 1, 33, *x) for x in plant(c, 1, (1,), 33 - 40, bad)]  # a single token beside it
+    o, lse, only = c.run(dev)
+    c.pool, clean = clean, c.pool
+    O, L, A, C = c.oracle()
+    for row, m, pos, t, h, i in planted:
+        O[row + max(0, t - pos):row + m, 4 * h:4 * h + 4, i] = bad
+    compare(c, o, lse, (O, L, A, C))
+    compare(c, only, None, (O, L, A, C))
+
+
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_values_come_through_where_every_token_sees_all(dev, n, D):
+    c = Case([150], [n], 8, 2, D, 16)
+    clean = c.pool.clone()
+    planted = plant(c, 0, (0, 1), 150 - 40, math.inf)
+    o, lse, only = c.run(dev, causal=False)
+    c.pool = clean
+    O, L, A, C = c.oracle(False)
+    for t, h, i in planted:
+        O[:, 4 * h:4 * h + 4, i] = math.inf
+    compare(c, o, lse, (O, L, A, C))
+    compare(c, only, None, (O, L, A, C))
