@@ -95,11 +95,6 @@ class PagedKVCache:
     def seq_len(self, seq_id) -> int:
         return self._len.get(seq_id, 0)
 
-    def _take(self) -> int:
-        page = self._free.pop()
-        self._refs[page] = 1
-        return page
-
     def _drop(self, pages) -> None:
         for page in pages:
             self._refs[page] -= 1
@@ -156,7 +151,7 @@ class PagedKVCache:
 
     def _grow(self, seq_ids, counts) -> None:
         """Room for counts[i] more tokens of seq_ids[i].  Last pages that tokens will go into are
-        copied where they are shared.  Nothing changes if the pages do not suffice."""
+        copied where they are shared.  Nothing changes if the pages do not suffice or the copy fails."""
         if len(counts) != len(seq_ids):
             raise ValueError("one count per sequence")
         if any(n < 0 for n in counts):
@@ -176,23 +171,35 @@ class PagedKVCache:
                     need += 1
         if need > len(self._free):
             raise MemoryError(f"page pool exhausted: need {need} pages, {len(self._free)} free")
-        for s in seq_ids:
-            self._pages.setdefault(s, [])
-            self._len.setdefault(s, 0)
-        copies = []
+        # Into free pages first: until the copies are made, the sequences stay as they are.
+        taken = iter(self._free[len(self._free) - need:][::-1])
+        copies, plan, left = [], [], {}  # left: how many of this call give up a shared page
         for s, n in growing:
-            pages, length = self._pages[s], self._len[s]
-            if length % self.page_size and self._refs[pages[-1]] > 1:
-                page = self._take()
-                copies.append((pages[-1], page, length % self.page_size))
-                self._refs[pages[-1]] -= 1
-                pages[-1] = page
-            for _ in range(-(-(length + n) // self.page_size) - len(pages)):
-                pages.append(self._take())
-            self._len[s] = length + n
+            pages, length = self._pages.get(s, []), self._len.get(s, 0)
+            own = None  # takes the place of a shared last page
+            if length % self.page_size and self._refs[pages[-1]] - left.get(pages[-1], 0) > 1:
+                left[pages[-1]] = left.get(pages[-1], 0) + 1
+                own = next(taken)
+                copies.append((pages[-1], own, length % self.page_size))
+            more = -(-(length + n) // self.page_size) - len(pages)
+            plan.append((s, own, [next(taken) for _ in range(more)], length + n))
         if copies:
             t = torch.tensor(copies, dtype=torch.int32, device=self.pool.device).t().contiguous()
             copy_pages(self.pool, t[0], t[1], num_tokens=t[2])
+        del self._free[len(self._free) - need:]
+        for s in seq_ids:
+            self._pages.setdefault(s, [])
+            self._len.setdefault(s, 0)
+        for s, own, new, length in plan:
+            pages = self._pages[s]
+            if own is not None:
+                self._refs[pages[-1]] -= 1
+                self._refs[own] = 1
+                pages[-1] = own
+            for page in new:
+                self._refs[page] = 1
+            pages.extend(new)
+            self._len[s] = length
 
     def page_table(self, seq_ids):
         """(kv_page_indptr, kv_page_indices, kv_last_page_len) int32 device tensors."""

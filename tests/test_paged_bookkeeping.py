@@ -289,3 +289,36 @@ def test_argument_refusals_on_the_device(dev):
         with pytest.raises(err):
             fn(*args[:n], bad, *args[n + 1:])
     torch.cuda.synchronize()
+
+
+def _state(cache):
+    return (list(cache._free), {s: list(p) for s, p in cache._pages.items()}, dict(cache._len),
+            list(cache._refs))
+
+
+def _shared(n=6):
+    """Sequences a and b that share n tokens (two pages, the second one partly filled)."""
+    cache = PagedKVCache(8, 1, 4, 8, device="cpu")
+    cache.append(["a"], torch.ones(n, 1, 8).half(), torch.ones(n, 1, 8).half(), [n])
+    cache.fork("a", "b")
+    return cache
+
+
+def _refuse(*args, **kw):
+    raise TypeError("refused")
+
+
+@pytest.mark.parametrize("call", ["append", "extend"])
+def test_a_failed_page_copy_changes_nothing(host, monkeypatch, call):
+    """The copy of a shared page may be refused (a stream under capture, say): neither sequence then
+    holds the page that was meant for it."""
+    cache = _shared()
+    before, pool = _state(cache), cache.pool.clone()
+    x = torch.zeros(3, 1, 8).half()
+    monkeypatch.setattr(paged_kv, "copy_pages", _refuse)
+    with pytest.raises(TypeError):
+        if call == "append":
+            cache.append(["a", "c"], x, x, [2, 1])
+        else:
+            cache.extend(["a", "c"], x, x, x, [2, 1])
+    assert _state(cache) == before and torch.equal(cache.pool, pool)
