@@ -220,14 +220,28 @@ class PagedKVCache:
             ap.append(ap[-1] + int(n))
         return torch.tensor(ap, dtype=torch.int32, device=self.pool.device)
 
+    def _restore(self, before) -> None:
+        """Gives sequences back the lengths (None: no sequence) that they had."""
+        for s, n in before.items():
+            if n is None:
+                self.release(s)
+            else:
+                self.truncate(s, n)
+
     def append(self, seq_ids, k_new, v_new, counts):
         """Append counts[i] rows of k_new / v_new [sum(counts), Hkv, D] to seq_ids[i].
 
-        Returns the batch's page table after the append.
+        Returns the batch's page table after the append.  A call that is refused leaves the
+        sequences with the tokens they had.
         """
+        before = {s: self._len.get(s) for s in seq_ids}
         self._grow(seq_ids, counts)
-        indptr, indices, last = self.page_table(seq_ids)
-        append_paged_kv(k_new, v_new, self._indptr(counts), self.pool, indptr, indices, last)
+        try:
+            indptr, indices, last = self.page_table(seq_ids)
+            append_paged_kv(k_new, v_new, self._indptr(counts), self.pool, indptr, indices, last)
+        except BaseException:
+            self._restore(before)
+            raise
         return indptr, indices, last
 
     def extend(self, seq_ids, q, k_new, v_new, counts, inv_freq=None, interleaved=False,
@@ -255,12 +269,8 @@ class PagedKVCache:
                                            interleaved=interleaved, factor=factor)
             return _ops.chunk_paged(q, q_indptr, self.pool, *table, causal=causal,
                                     softmax_scale=softmax_scale, return_lse=return_lse)
-        except Exception:
-            for s, n in before.items():
-                if n is None:
-                    self.release(s)
-                else:
-                    self.truncate(s, n)
+        except BaseException:
+            self._restore(before)
             raise
 
 

@@ -308,6 +308,21 @@ def _refuse(*args, **kw):
     raise TypeError("refused")
 
 
+def test_a_refused_append_leaves_the_sequences_as_they_were(host, monkeypatch):
+    cache = PagedKVCache(8, 1, 4, 8, device="cpu")
+    z = lambda n: torch.zeros(n, 1, 8).half()  # noqa: E731
+    cache.append(["a"], z(6), z(6), [6])
+    before = _state(cache)
+    monkeypatch.setattr(paged_kv, "append_paged_kv", _refuse)  # as for a wrong type or head dim
+    with pytest.raises(TypeError):
+        cache.append(["a", "c"], z(9), z(9), [4, 5])
+    after = _state(cache)
+    assert sorted(after[0]) == sorted(before[0]) and after[1:] == before[1:]
+    with pytest.raises(TypeError):
+        cache.append(["a", "c"], z(0), z(0), [0, 0])
+    assert _state(cache)[1:] == before[1:]
+
+
 @pytest.mark.parametrize("call", ["append", "extend"])
 def test_a_failed_page_copy_changes_nothing(host, monkeypatch, call):
     """The copy of a shared page may be refused (a stream under capture, say): neither sequence then
