@@ -231,9 +231,13 @@ class PagedKVCache:
     def append(self, seq_ids, k_new, v_new, counts):
         """Append counts[i] rows of k_new / v_new [sum(counts), Hkv, D] to seq_ids[i].
 
-        Returns the batch's page table after the append.  A call that is refused leaves the
-        sequences with the tokens they had.
+        Returns the batch's page table after the append.  Rows past sum(counts) belong to no
+        sequence.  A call that is refused leaves the sequences with the tokens they had.
         """
+        total = sum(int(n) for n in counts)
+        for name, x in (("k_new", k_new), ("v_new", v_new)):
+            if x.shape[0] < total:
+                raise ValueError(f"{name} has {x.shape[0]} rows, the counts make {total}")
         before = {s: self._len.get(s) for s in seq_ids}
         self._grow(seq_ids, counts)
         try:

@@ -323,6 +323,18 @@ def test_a_refused_append_leaves_the_sequences_as_they_were(host, monkeypatch):
     assert _state(cache)[1:] == before[1:]
 
 
+def test_an_append_of_too_few_rows_is_refused(host):
+    cache = _shared()
+    before = _state(cache)
+    z = lambda n: torch.zeros(n, 1, 8).half()  # noqa: E731
+    for k, v in ((z(3), z(3)), (z(3), z(4)), (z(4), z(3))):
+        with pytest.raises(ValueError, match="rows"):
+            cache.append(["a", "c"], k, v, [3, 1])
+        assert _state(cache) == before
+    cache.append(["a", "c"], z(7), z(7), [3, 1])  # rows past the counts belong to no sequence
+    assert cache.seq_len("a") == 9 and cache.seq_len("c") == 1
+
+
 @pytest.mark.parametrize("call", ["append", "extend"])
 def test_a_failed_page_copy_changes_nothing(host, monkeypatch, call):
     """The copy of a shared page may be refused (a stream under capture, say): neither sequence then
