@@ -471,10 +471,10 @@ py::tuple kept_indices(int64_t l_max, const c10::optional<at::Tensor>& mask_,
 }
 
 // A pool that a call writes in place: 16-bit elements (the kernels move them whole), rows of
-// unit stride.
-int check_written_pool(const at::Tensor& pool) {
+// unit stride.  `more`: planes behind K and V are allowed, and left alone.
+int check_written_pool(const at::Tensor& pool, bool more = false) {
   const int dtype = dtype16("paged_kv_cache", pool);
-  if (pool.dim() != 5 || pool.size(1) != 2)
+  if (pool.dim() != 5 || pool.size(1) < 2 || (pool.size(1) > 2 && !more))
     throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
   if (pool.stride(-1) != 1)
     throw py::value_error("paged_kv_cache needs a unit head_dim stride (it is written in place)");
@@ -489,7 +489,7 @@ void append_paged_kv(const at::Tensor& k_new_, const at::Tensor& v_new_,
                      const at::Tensor& indptr_, const at::Tensor& indices_,
                      const at::Tensor& last_) {
   need_gpu("paged_kv_cache", pool);
-  check_written_pool(pool);
+  check_written_pool(pool, true);
   const at::Device dev = pool.device();
   const at::ScalarType dt = pool.scalar_type();
   at::Tensor k_new = rows_like("k_new", k_new_, dt, "paged_kv_cache"),

@@ -127,3 +127,18 @@ def test_paged_cache_rejects_overflow(dev):
     with pytest.raises(MemoryError):
         cache.append([0], torch.zeros(9, 1, 64, dtype=torch.float16, device=dev),
                       torch.zeros(9, 1, 64, dtype=torch.float16, device=dev), [9])
+
+
+def test_planes_behind_k_and_v_are_left_alone(dev):
+    """A pool of more than two planes to a page: K and V go to the first two; one of fewer is refused."""
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(3, 2, 64, generator=g).half().to(dev) for _ in range(2))
+    i32 = dict(dtype=torch.int32, device=dev)
+    table = (torch.tensor([0, 1], **i32), torch.tensor([1], **i32), torch.tensor([3], **i32))
+    pool = torch.full((2, 3, 2, 4, 64), 7.0, dtype=torch.float16, device=dev)
+    want = pool.clone()
+    want[1, 0, :, :3], want[1, 1, :, :3] = k.transpose(0, 1), v.transpose(0, 1)
+    append_paged_kv(k, v, torch.tensor([0, 3], **i32), pool, *table)
+    assert torch.equal(pool, want)
+    with pytest.raises(ValueError):
+        append_paged_kv(k, v, torch.tensor([0, 3], **i32), pool[:, :1], *table)
