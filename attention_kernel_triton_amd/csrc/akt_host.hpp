@@ -65,6 +65,12 @@ inline bool rows_aligned16(const void* base, const int64_t* strides, int n) {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
+// Whether a launch of so many blocks of `threads` in a row is one that the runtime takes: fewer
+// than 2^32 work items.
+inline bool grid_fits(int64_t blocks, int64_t threads) {
+  return blocks < (1ll << 32) && blocks * threads < (1ll << 32);
+}
+
 constexpr int kMaxResidentDevices = 64;
 
 // Workgroups of `Kernel` (blocks of `threads`) that fit the current device at

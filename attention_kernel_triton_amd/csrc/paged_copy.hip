@@ -96,7 +96,7 @@ extern "C" int akt_paged_copy(void* kv_cache, const int32_t* src, const int32_t*
   p.per_head = (int)per_head;
   p.per_page = (int)(2 * num_kv_heads * per_head);
   p.blocks = (int)ceil_div(p.per_page, kPThreads * kPPerLane);
-  AKT_CHECK(n < (1ll << 31) && n * p.blocks < (1ll << 31), "too many pages");
+  AKT_CHECK(n < (1ll << 31) && grid_fits(n * p.blocks, kPThreads), "too many pages");
   KernelTimer timer;
   timer.launch(paged_copy_kernel, dim3((unsigned)(n * p.blocks)), dim3(kPThreads), 0,
                (hipStream_t)stream, p);

@@ -440,7 +440,7 @@ extern "C" int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k
   p.tpb = units ? (int)(64 / (head_dim / 16)) : 0;
   const int64_t blocks = units ? ceil_div(tokens, (int64_t)p.tpb * kRWaves)
                                : ceil_div(tokens * (head_dim / 8), kRThreads);
-  AKT_CHECK(blocks < (1ll << 31), "problem too large");
+  AKT_CHECK(grid_fits(blocks, kRThreads), "problem too large");
   // Heads of a block: as many as leave about four workgroups to a CU, so that cos and sin
   // serve many heads in a large launch and a small one fills the chip.
   const int64_t heads = num_q_heads + num_kv_heads;
@@ -494,6 +494,7 @@ extern "C" int akt_paged_kv_append_rotary(
                 rows_aligned16(v_new, v_new_stride, 2) && rows_aligned16(kv_cache, kv_stride, 4) &&
                 aligned16(q_out),
             "tensors must have 16-byte aligned rows");
+  AKT_CHECK(grid_fits(ceil_div(total_new, kRWaves), kRThreads), "too many tokens");
   AppendRotaryParams p = {};
   p.q = (const half_t*)q;
   p.k = (const half_t*)k_new;

@@ -405,7 +405,9 @@ int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_c
  *   outputs; at factor 1 the inverse).
  *   positions: optional device array, element (b, s) at b * position_stride[0] +
  *   s * position_stride[1], int32 or int64 by position_bits; NULL: 0 .. seq_len - 1.
- *   head_dim: a multiple of 8 up to 1024; rotary_dim: even, up to head_dim.
+ *   head_dim: a multiple of 8 up to 1024; rotary_dim: even, up to head_dim.  A launch has
+ *   fewer than 2^32 work items: calls of batch * seq_len * head_dim from 2^35 on may be
+ *   refused.
  *   dtype: AKT_DTYPE_F16 or AKT_DTYPE_BF16.
  */
 int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k_out,
@@ -421,7 +423,7 @@ int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k_out,
  * and q [total_new, num_q_heads, head_dim] (rows as k_new's) is rotated by the same
  * positions into contiguous q_out.  A token whose page lies outside the table or pool is
  * not stored, its q is rotated; rows that belong to no sequence are not written.
- * total_pages * page_size must be below 2^30.
+ * total_pages * page_size must be below 2^30, total_new at most 2^26 - 4.
  * No reference counterpart.
  */
 int akt_paged_kv_append_rotary(const void* q, const void* k_new, const void* v_new, void* q_out,
@@ -440,7 +442,8 @@ int akt_paged_kv_append_rotary(const void* q, const void* k_new, const void* v_n
  * page src[i] to page dst[i], K and V of every head, for i < n.  A pair with a page outside
  * [0, num_pool_pages), or the same page twice, is skipped.  All copies of a call run at
  * once: no page may be the destination of two of them, or the source of one and
- * the destination of another.  No reference counterpart.
+ * the destination of another.  Up to 2^24 - 1 blocks of 16 KiB (a page takes one at
+ * least) are copied by a call; more are refused.  No reference counterpart.
  */
 int akt_paged_copy(void* kv_cache, const int32_t* src, const int32_t* dst,
                    const int32_t* num_tokens, int64_t n, int64_t num_kv_heads, int64_t head_dim,

@@ -349,3 +349,12 @@ def test_a_failed_page_copy_changes_nothing(host, monkeypatch, call):
         else:
             cache.extend(["a", "c"], x, x, x, [2, 1])
     assert _state(cache) == before and torch.equal(cache.pool, pool)
+
+
+def test_launches_past_the_runtimes_limit_are_refused():
+    """Grids of 2^32 work items and more."""
+    lib = N.load()
+    assert _copy(lib, n=1 << 24) == 1 and b"too many pages" in lib.akt_last_error()
+    assert _rotary(lib, S=1 << 30) == 1 and b"too large" in lib.akt_last_error()
+    assert _rotary(lib, S=1 << 29, D=72, rot=72) == 1 and b"too large" in lib.akt_last_error()
+    assert _append(lib, total=1 << 26) == 1 and b"too many tokens" in lib.akt_last_error()
