@@ -38,8 +38,10 @@ struct Elt<true> {
   }
 };
 
-// Chunk-position swizzle of a K / V tile row (see the header comment); a
-// function of r mod 16, with tswz(r + 8) = tswz(r) ^ 2.
+// Chunk-position swizzle of a K / V tile row: chunk c (16 bytes) of row r lies at position
+// c ^ tswz(r) of the row, so that the K reads (16 consecutive rows, one chunk each) and the
+// transposing V reads (four rows, four chunks) use all LDS banks.  A function of r mod 16, with
+// tswz(r + 8) = tswz(r) ^ 2.
 // - 64- and 192-dim rows (128 / 384 bytes) start on bank 0 or 32 by row
 //   parity: over 16 consecutive rows the even rows' values are a permutation
 //   of 0..7, and so are the odd rows' (K reads), and rows 4i + j and 4i + j + 2

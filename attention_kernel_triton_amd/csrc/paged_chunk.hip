@@ -657,7 +657,8 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return p.partials + (SPLIT ? 0 : p.many_partial) + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + wave * kWaveB;
+        return p.partials + p.many_partial + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB +
+               wave * kWaveB;
       };
       char* mine = slot_of(wg);
 #pragma unroll
@@ -673,9 +674,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       // The stores (device scope) are complete before the count.
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[(SPLIT ? 0 : p.many_counter) + WAVES * wf + wave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[p.many_counter + WAVES * wf + wave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[(SPLIT ? 0 : p.many_counter) + WAVES * wf + wave], 0);
+      if (lane == 0) atomicExch(&p.arrive[p.many_counter + WAVES * wf + wave], 0);
       constexpr int UB = D == 64 ? 4 : 2;  // partials in flight
       m_run = AKT_C_NEG_INF;
       l_row = x_row = 0.f;
@@ -960,7 +961,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       const int wf = div_range(Ustart + kCkBlock - 1, Lw);
       const int wl = div_range(Ustart + kb_last + kCkBlock - 1, Lw);
       auto slot_of = [&](int w) -> char* {
-        return p.partials + (SPLIT ? 0 : p.many_partial) + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + twave * kWaveB;
+        return p.partials + (2 * (int64_t)w + (w == wf ? 1 : 0)) * kSlotB + twave * kWaveB;
       };
       char* mine = slot_of(wg);
       if (row < rows) {
@@ -973,9 +974,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       }
       __builtin_amdgcn_s_waitcnt(0);
       int prev = 0;
-      if (lane == 0) prev = atomicAdd(&p.arrive[(SPLIT ? 0 : p.many_counter) + TW * wf + twave], 1);
+      if (lane == 0) prev = atomicAdd(&p.arrive[TW * wf + twave], 1);
       if (uniform(prev) != wl - wf) return;
-      if (lane == 0) atomicExch(&p.arrive[(SPLIT ? 0 : p.many_counter) + TW * wf + twave], 0);
+      if (lane == 0) atomicExch(&p.arrive[TW * wf + twave], 0);
       if (row < rows) {
         constexpr int UB = 32 / NQ < 8 ? 32 / NQ : 8;  // partials in flight
         m_run = AKT_C_NEG_INF;
