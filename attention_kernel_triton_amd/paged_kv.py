@@ -159,46 +159,35 @@ class PagedKVCache:
         growing = [(s, int(n)) for s, n in zip(seq_ids, counts) if n]
         if len({s for s, _ in growing}) != len(growing):
             raise ValueError("a sequence can take new tokens once in a call")
-        need, refs = 0, {}
+        need, plan, copies, left = 0, [], [], {}  # left: how often this call gives up a shared page
         for s, n in growing:
-            pages, length = self._pages.get(s, []), self._len.get(s, 0)
-            need += -(-(length + n) // self.page_size) - len(pages)
-            if length % self.page_size:
-                last = pages[-1]
-                refs[last] = refs.get(last, self._refs[last])
-                if refs[last] > 1:  # of the sequences of this call, the last keeps the page
-                    refs[last] -= 1
-                    need += 1
+            pages, length = self._pages.get(s, ()), self._len.get(s, 0)
+            more, fill = -(-(length + n) // self.page_size) - len(pages), length % self.page_size
+            own = False  # whether the last page is replaced; the last holder keeps it
+            if fill and self._refs[pages[-1]] - left.get(pages[-1], 0) > 1:
+                left[pages[-1]] = left.get(pages[-1], 0) + 1
+                copies.append((pages[-1], need, fill))
+                own, more = True, more + 1
+            plan.append((s, own, need, need + more, length + n))
+            need += more
         if need > len(self._free):
             raise MemoryError(f"page pool exhausted: need {need} pages, {len(self._free)} free")
-        # Into free pages first: until the copies are made, the sequences stay as they are.
-        taken = iter(self._free[len(self._free) - need:][::-1])
-        copies, plan, left = [], [], {}  # left: how many of this call give up a shared page
-        for s, n in growing:
-            pages, length = self._pages.get(s, []), self._len.get(s, 0)
-            own = None  # takes the place of a shared last page
-            if length % self.page_size and self._refs[pages[-1]] - left.get(pages[-1], 0) > 1:
-                left[pages[-1]] = left.get(pages[-1], 0) + 1
-                own = next(taken)
-                copies.append((pages[-1], own, length % self.page_size))
-            more = -(-(length + n) // self.page_size) - len(pages)
-            plan.append((s, own, [next(taken) for _ in range(more)], length + n))
-        if copies:
-            t = torch.tensor(copies, dtype=torch.int32, device=self.pool.device).t().contiguous()
+        taken = self._free[len(self._free) - need:][::-1]
+        if copies:  # into free pages: until they are made, the sequences stay as they are
+            t = torch.tensor([(src, taken[at], fill) for src, at, fill in copies],
+                             dtype=torch.int32, device=self.pool.device).t().contiguous()
             copy_pages(self.pool, t[0], t[1], num_tokens=t[2])
         del self._free[len(self._free) - need:]
         for s in seq_ids:
             self._pages.setdefault(s, [])
             self._len.setdefault(s, 0)
-        for s, own, new, length in plan:
+        for s, own, i, j, length in plan:
             pages = self._pages[s]
-            if own is not None:
-                self._refs[pages[-1]] -= 1
-                self._refs[own] = 1
-                pages[-1] = own
-            for page in new:
+            if own:
+                self._refs[pages.pop()] -= 1
+            for page in taken[i:j]:
                 self._refs[page] = 1
-            pages.extend(new)
+                pages.append(page)
             self._len[s] = length
 
     def page_table(self, seq_ids):
