@@ -24,7 +24,9 @@ def flash_attention_chunk_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_
     causal=True: a query sees the keys up to its own position; causal=False: all len_b keys.
     softmax_scale defaults to 1/sqrt(D).  Any page_size; D = 64, 128 or 256; up to 128 query
     heads per kv head.  Rows that see no key get zeros (lse -inf); rows of q that belong to no
-    sequence are left unwritten.  A call under graph capture takes a workspace of its own from
+    sequence are left unwritten.  Probabilities are rounded to q's type for the product with V and
+    in the normaliser (sums are fp32), so a single token's output may be a little less exact than
+    flash_attention_decode_paged's.  A call under graph capture takes a workspace of its own from
     the graph's memory pool, so captured calls may replay side by side.
     """
     return _ops.chunk_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices,

@@ -20,7 +20,9 @@
 //
 // Measured: dense Q and K of 8 x 1024 tokens, 64 + 16 heads, D = 64: 36 to 37 us (168 MB, 4.6 TB/s,
 // where a large copy reaches 5.1); 4 appended prompts of 1000 to 3001 tokens, 32 + 8 heads,
-// D = 128: 51.8 us (219 MB, 4.2 TB/s); 64 single tokens: 6.5 us, launch and look-ups.
+// D = 128: 51.6 us (219 MB, 4.2 TB/s); 64 single tokens: 6.5 us, launch and look-ups.  Generic:
+// dense 8 x 1024 tokens, 32 + 8 heads, D = 192: 92 us (252 MB, 2.7 TB/s; D = 128, whole units,
+// 168 MB in 30 us); 4 x 2000 appended tokens, D = 80: 67 us (123 MB, 1.8 TB/s).
 #include <math.h>
 
 #include <cmath>
