@@ -11,13 +11,18 @@ Modules mirror the reference repository's files (KiritoHugh/attention_kernel_tri
                                                 sparsetoken_flash_attention_decode_paged
   magicpig_sparsetoken_decode_flash_attention_redundant_var_len_paged_with_norm
                                                 magicpig_sparsetoken_flash_attention_decode_paged
-  kept_index                                    select_kept (device kept-index selection)
+  kept_index                                    select_kept, select_heaviest (device kept-index
+                                                selection)
   merge_states                                  merge_states (LSE merge of partial results)
   sparse_csr                                    sparse decodes over CSR kept indices (inds + ptr)
   paged_kv                                      append_paged_kv, append_paged_kv_rotary, copy_pages,
-                                                PagedKVCache (paged KV write side)
+                                                keep_tokens, PagedKVCache (paged KV write side)
   chunk_flash_attention_paged                   flash_attention_chunk_paged (several new tokens per
                                                 sequence over a paged cache)
+  shared_prefix_flash_attention_paged           flash_attention_shared_prefix_paged (a prefix read
+                                                once for all sequences that share it)
+  attention_weights_paged                       accumulate_attention_weights_paged (attention that
+                                                cached tokens draw)
   rotary                                        apply_rotary, rotary_frequencies (rotary positions)
 
 All of them run hand-written HIP kernels from libakt_amd.so (built by
@@ -38,5 +43,7 @@ __all__ = [
     "sparse_csr",
     "paged_kv",
     "chunk_flash_attention_paged",
+    "shared_prefix_flash_attention_paged",
+    "attention_weights_paged",
     "rotary",
 ]

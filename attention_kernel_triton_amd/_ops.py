@@ -47,13 +47,13 @@ def _same_device(dev, **tensors) -> None:
 
 
 # --------------------------------------------------------------------------- hot paths
-# prefill, decode, decode_paged, chunk_paged, sparse_decode and sparse_decode_paged run in
-# the compiled host layer (csrc/torch_ops.cpp): the same checks, allocation,
+# prefill, decode, decode_paged, chunk_paged, shared_prefix_paged, sparse_decode and
+# sparse_decode_paged run in the compiled host layer (csrc/torch_ops.cpp): the same checks, allocation,
 # stream and workspace handling as the wrappers below, at a few microseconds
 # of host time per call.  The first call of each name binds this module's
 # attribute to the compiled function.
-_HOT = ("prefill", "decode", "decode_paged", "chunk_paged", "sparse_decode",
-        "sparse_decode_paged")
+_HOT = ("prefill", "decode", "decode_paged", "chunk_paged", "shared_prefix_paged",
+        "sparse_decode", "sparse_decode_paged")
 
 
 def _hot(name):
@@ -109,6 +109,17 @@ def chunk_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices, kv
     return _hot("chunk_paged")(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices,
                                kv_last_page_len, causal=causal, softmax_scale=softmax_scale,
                                return_lse=return_lse)
+
+
+def shared_prefix_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices,
+                        kv_last_page_len, group_indptr, prefix_page_indptr, prefix_page_indices,
+                        prefix_last_page_len, causal=True, softmax_scale=None, return_lse=False):
+    """Attention of q [total_q,Hq,D] over groups' prefixes and own keys: o [total_q,Hq,D] (, lse)."""
+    return _hot("shared_prefix_paged")(q, q_indptr, paged_kv_cache, kv_page_indptr,
+                                       kv_page_indices, kv_last_page_len, group_indptr,
+                                       prefix_page_indptr, prefix_page_indices,
+                                       prefix_last_page_len, causal=causal,
+                                       softmax_scale=softmax_scale, return_lse=return_lse)
 
 
 def sparse_decode(q, K, V, sparse_ind, sparse_nnz, softmax_scale, return_lse=False,

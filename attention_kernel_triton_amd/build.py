@@ -52,6 +52,7 @@ SOURCE_FLAGS = {
     "prefill_wide.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp",
                          "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "paged_chunk_256.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_shared_256.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -104,14 +104,46 @@ __device__ __forceinline__ int div_range(int64_t a, int64_t b) {
   return uniform((int)((double)a / (double)b));
 }
 
+template <bool SHARED>
 struct Seq {
   int q0, n;    // first query row, query tokens
   int ip0, len;  // first page table entry, cached tokens
 };
+// In a launch with shared prefixes a group's tokens together are a sequence too, whose keys are
+// the prefix: it has a table of its own, and every token sees all of it.
+template <>
+struct Seq<true> {
+  int q0, n, ip0, len;
+  int prefix;
+};
+template <typename S>
+__device__ __forceinline__ int is_prefix(const S& s) {
+  return s.prefix;
+}
+__device__ __forceinline__ int is_prefix(const Seq<false>&) { return 0; }
+template <bool SHARED>
+__device__ __forceinline__ int num_seqs(const ChunkParams& p) {
+  return SHARED ? p.B + p.groups : p.B;
+}
 // Table entries outside their ranges are taken clamped, so nothing outside the arrays is
 // touched.
-__device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b) {
-  Seq s;
+template <bool SHARED>
+__device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b) {
+  Seq<SHARED> s;
+  if constexpr (SHARED) {
+    s.prefix = b >= p.B;
+    if (s.prefix) {
+      const int i = b - p.B;
+      const int b0 = min(max(p.group_indptr[i], 0), p.B);
+      const int b1 = min(max(p.group_indptr[i + 1], b0), p.B);
+      s.q0 = min(max(p.q_indptr[b0], 0), p.total_q);
+      s.n = b1 > b0 ? min(max(p.q_indptr[b1], s.q0), p.total_q) - s.q0 : 0;
+      s.ip0 = min(max(p.prefix_indptr[i], 0), p.prefix_pages);
+      const int np = min(max(p.prefix_indptr[i + 1], s.ip0), p.prefix_pages) - s.ip0;
+      s.len = np > 0 ? (np - 1) * p.page_size + min(max(p.prefix_last[i], 0), p.page_size) : 0;
+      return s;
+    }
+  }
   s.q0 = min(max(p.q_indptr[b], 0), p.total_q);
   s.n = min(max(p.q_indptr[b + 1], s.q0), p.total_q) - s.q0;
   s.ip0 = min(max(p.indptr[b], 0), p.total_pages);
@@ -120,23 +152,34 @@ __device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b) {
   return s;
 }
 // The same for a wave-uniform b, in scalar registers.
-__device__ __forceinline__ Seq load_seq_uniform(const ChunkParams& p, int b) {
-  const Seq s = load_seq(p, b);
-  return Seq{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len)};
+template <bool SHARED>
+__device__ __forceinline__ Seq<SHARED> load_seq_uniform(const ChunkParams& p, int b) {
+  const Seq<SHARED> s = load_seq<SHARED>(p, b);
+  if constexpr (SHARED)
+    return Seq<SHARED>{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len), uniform(s.prefix)};
+  else
+    return Seq<SHARED>{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len)};
 }
 __device__ __forceinline__ int row_blocks(const ChunkParams& p, int n) {
   return (int)(((uint32_t)n + p.TR - 1) / (uint32_t)p.TR);
 }
+// Whether a row of the sequence (unit) sees the keys up to its own position only.
+template <typename S>
+__device__ __forceinline__ bool is_causal(const ChunkParams& p, const S& s) {
+  return p.causal && !is_prefix(s);
+}
 // Lengths on the axis.  Causal row block r sees min(n, (r + 1) TR) keys past the context;
 // the axis takes the context as at least 0 (a table with n > len breaks the contract).
-__device__ __forceinline__ int64_t unit_start(const ChunkParams& p, const Seq& s, int64_t r) {
-  if (!p.causal) return r * (s.len + kCkUnitCost);
+template <bool SHARED>
+__device__ __forceinline__ int64_t unit_start(const ChunkParams& p, const Seq<SHARED>& s, int64_t r) {
+  if (!is_causal(p, s)) return r * (s.len + kCkUnitCost);
   return r * (max(s.len - s.n, 0) + kCkUnitCost) + p.TR * (r * (r + 1) / 2);
 }
-__device__ __forceinline__ int64_t head_length(const ChunkParams& p, const Seq& s) {
+template <bool SHARED>
+__device__ __forceinline__ int64_t head_length(const ChunkParams& p, const Seq<SHARED>& s) {
   const int64_t R = row_blocks(p, s.n);
   if (R == 0) return 0;
-  if (!p.causal) return R * (s.len + kCkUnitCost);
+  if (!is_causal(p, s)) return R * (s.len + kCkUnitCost);
   return unit_start(p, s, R - 1) + max(s.len - s.n, 0) + s.n + kCkUnitCost;
 }
 // n / page_size for 0 <= n < 2^31.
@@ -146,6 +189,7 @@ __device__ __forceinline__ int page_of(const ChunkParams& p, int n) {
 }
 
 // A unit and the part of its keys that a workgroup serves.
+template <bool SHARED>
 struct Unit {
   int q0;     // first query row (token) in q
   int ntok;   // its tokens
@@ -155,6 +199,30 @@ struct Unit {
   int kend;   // keys that it sees
   int ip0;    // first page table entry of the sequence
 };
+template <>
+struct Unit<true> {
+  int q0, ntok, kvh, first, len, kend, ip0;
+  int prefix;  // a group's rows and its prefix's keys
+  int more;    // the rows have a prefix's state too (own keys)
+};
+__device__ __forceinline__ int is_prefix(const Unit<false>&) { return 0; }
+__device__ __forceinline__ const int32_t* page_ids(const ChunkParams& p, const Unit<false>&) {
+  return p.indices;
+}
+__device__ __forceinline__ const int32_t* page_ids(const ChunkParams& p, const Unit<true>& u) {
+  return u.prefix ? p.prefix_indices : p.indices;
+}
+
+// Where the state (m, l, exact l, whether a prefix's state goes with it) and the sums of P.V of
+// a row go that attends in two parts: row (token, query head) of the own keys' or the prefixes'.
+__device__ __forceinline__ float4_t* state_ml(const ChunkParams& p, const Unit<true>& u) {
+  return reinterpret_cast<float4_t*>(p.states) + (u.prefix ? (int64_t)p.total_q * p.Hq : 0);
+}
+template <int D>
+__device__ __forceinline__ float* state_o(const ChunkParams& p, const Unit<true>& u) {
+  const int64_t rows = (int64_t)p.total_q * p.Hq;
+  return reinterpret_cast<float*>(p.states + rows * 32) + (u.prefix ? rows * D : 0);
+}
 
 // Scores of the keys that a row does not see become -inf: of the step's 32 those past its
 // first room + 1, and those whose bit of `valid` is 0.
@@ -213,13 +281,13 @@ __device__ __forceinline__ bool zero_not_finite(uint4_t (&v)[N]) {
 // Adds the infinities and NaNs of keys j0 .. j1 - 1 of V, which were staged as zeros, to the O
 // of the rows that see them (a key's probability is positive).  Lane (l32, g) holds dims
 // 32 n + 8 k + 4 g .. + 3 of row l32, whose last key is lim.
-template <int D, bool BF16>
-__device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit& u, int j0, int j1,
+template <int D, bool BF16, bool SHARED>
+__device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit<SHARED>& u, int j0, int j1,
                                                int g, int lim, float16_t (&oacc)[D / 32]) {
   constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
 #pragma clang loop unroll(disable)
   for (int j = j0; j < j1; ++j) {
-    const int lp = page_of(p, j), id = p.indices[u.ip0 + lp];
+    const int lp = page_of(p, j), id = page_ids(p, u)[u.ip0 + lp];
     if ((uint32_t)id >= (uint32_t)p.num_pool_pages || j > lim) continue;
     const half_t* row = p.pool + id * p.sp + p.skv + u.kvh * p.sh +
                         (int64_t)(j - lp * p.page_size) * p.ss + 4 * g;
@@ -242,7 +310,7 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit&
 
 // The units of the ranges of workgroup `block` of W, on the axis of the sequences of few tokens
 // (SPLIT) or of many.  lds: the workgroup's tile buffers.
-template <int D, bool BF16, bool GRP, bool LSE, bool SPLIT>
+template <int D, bool BF16, bool GRP, bool LSE, bool SHARED, bool SPLIT>
 __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int block, int W) {
   constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
@@ -276,10 +344,10 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   const int wg = team * W + (block % 8) * (W / 8) + block / 8;
   const int lane0 = tid0 & 63;
   // The sequences that this kernel serves.
-  auto mine = [&](const Seq& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
+  auto mine = [&](const Seq<SHARED>& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
   auto seq_length = [&](int b) -> int64_t {
-    if (b >= p.B) return 0;
-    const Seq s = load_seq(p, b);
+    if (b >= num_seqs<SHARED>(p)) return 0;
+    const Seq<SHARED> s = load_seq<SHARED>(p, b);
     return mine(s) ? head_length(p, s) * p.Hkv : 0;
   };
   auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
@@ -313,7 +381,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   };
   const float c = p.qk_scale;
   // ---- the keys [k0, k1) of a unit of many rows, by all waves.
-  auto serve = [&](const Unit& u, int k0, int k1, int64_t Ustart) {
+  auto serve = [&](const Unit<SHARED>& u, int k0, int k1, int64_t Ustart) {
     // The lane number is opaque here, so that what is derived from it lives no longer than
     // this part (held across the units' loop it would not fit the registers).
     int lane = tid0 & 63;
@@ -353,7 +421,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       const int key = min(k0 + 64 * m + lane, u.kend - 1);
       const int lp = page_of(p, key);
       slot_next = key - lp * p.page_size;
-      id_next = p.indices[u.ip0 + lp];
+      id_next = page_ids(p, u)[u.ip0 + lp];
     };
     auto place = [&](int m) -> Keys {
       const bool ok =
@@ -416,7 +484,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     // Tile j, whose first key is k0 + kBN j, into the buffer at LDS offset buf.
     bool bad = false;
     auto store_tile = [&](int j, int buf, const uint4_t (&kd)[PER_T], uint4_t (&vd)[PER_T]) {
-      if (p.causal && k0 + (j + 1) * kBN > u.first + 1)  // keys that not every row sees
+      if (is_causal(p, u) && k0 + (j + 1) * kBN > u.first + 1)  // keys that not every row sees
         bad |= zero_not_finite<BF16>(vd);
 #pragma unroll
       for (int i = 0; i < PER_T; ++i) {
@@ -430,9 +498,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
 
     // Last key of this lane's row (rows past the unit's: of its last token), and the
     // first of the wave's rows' last keys, up to which nothing is masked.
-    const int lim = p.causal ? u.first + min(ltok, u.ntok - 1) : u.len - 1;
+    const int lim = is_causal(p, u) ? u.first + min(ltok, u.ntok - 1) : u.len - 1;
     const int lim_min =
-        p.causal ? u.first + min((int)((uint32_t)(32 * wave) * p.g_magic >> 16), u.ntok - 1)
+        is_causal(p, u) ? u.first + min((int)((uint32_t)(32 * wave) * p.g_magic >> 16), u.ntok - 1)
                  : u.len - 1;
 
     // ---- Q^T fragments: lane -> row, dims g*HALF + 8s + e.
@@ -656,7 +724,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) any_bad |= sm_bad[w];
     if (uniform(any_bad))  // from the first tile that store_tile took the values out of
-      add_not_finite<D, BF16>(p, u, k0 + max(u.first + 1 - k0, 0) / kBN * kBN, k1, g, lim, oacc);
+      add_not_finite<D, BF16, SHARED>(p, u, k0 + max(u.first + 1 - k0, 0) / kBN * kBN, k1, g, lim, oacc);
     float l_row = xor32_sum(l_part);
     float x_row = LSE ? xor32_sum(x_part) : 0.f;
     if (!whole) {
@@ -719,6 +787,22 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         }
       }
     }
+    if constexpr (SHARED) {
+      if (lrow < rows) {
+        const int64_t at =
+            (int64_t)(u.q0 + ltok) * p.Hq + u.kvh * p.G + (lrow - ltok * p.G);
+        if (g == 0) state_ml(p, u)[at] = float4_t{m_run, l_row, x_row, (float)u.more};
+        float* const so = state_o<D>(p, u) + at * D + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            st16(so + 32 * n + 8 * k,
+                 as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
+                                    oacc[n][4 * k + 3]}));
+      }
+      return;
+    }
     // Output rows through LDS, so that every lane stores 16 contiguous bytes.
     const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
     if (LSE && g == 0 && lrow < rows)
@@ -752,7 +836,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   // of the part, each on its own: K goes from global memory straight into the fragments'
   // registers, V through the wave's own LDS for the transposing reads, both loaded again as
   // soon as the step has used them, with no barrier before the waves' results are merged.
-  auto serve_split = [&](const Unit& u, int k0, int k1, int64_t Ustart, auto rg_c) {
+  auto serve_split = [&](const Unit<SHARED>& u, int k0, int k1, int64_t Ustart, auto rg_c) {
     // The lane number is opaque here, so that what is derived from it lives no longer than
     // this part (held across the units' loop it would not fit the registers).
     int lane = tid0 & 63;
@@ -781,9 +865,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     const half_t* const Kh = p.pool + u.kvh * p.sh;
     const int row = 32 * rg + l32;
     const int tok = (int)((uint32_t)row * p.g_magic >> 16);
-    const int lim = p.causal ? u.first + min(tok, u.ntok - 1) : u.len - 1;
+    const int lim = is_causal(p, u) ? u.first + min(tok, u.ntok - 1) : u.len - 1;
     const int lim_min =
-        p.causal ? u.first + min((int)((uint32_t)(32 * rg) * p.g_magic >> 16), u.ntok - 1)
+        is_causal(p, u) ? u.first + min((int)((uint32_t)(32 * rg) * p.g_magic >> 16), u.ntok - 1)
                  : u.len - 1;
     char* const vst = lds + wave * OB;
 
@@ -794,7 +878,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       const int key = min(k0 + 32 * t + l32, u.kend - 1);
       const int lp = page_of(p, key);
       slot_next = key - lp * p.page_size;
-      id_next = p.indices[u.ip0 + lp];
+      id_next = page_ids(p, u)[u.ip0 + lp];
     };
     uint32_t valid = 0, valid_next = 0;  // keys that can be read: in the pool, before the unit's end
     const half_t* src = p.q;
@@ -869,7 +953,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         place(t + KG);
         load_k();
       }
-      if (p.causal && kh0 + 31 > u.first)  // keys that not every row sees
+      if (is_causal(p, u) && kh0 + 31 > u.first)  // keys that not every row sees
         bad |= zero_not_finite<BF16>(vr);
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -919,7 +1003,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     if (bad)
       for (int t = kg; t < n_steps; t += KG)
         if (k0 + 32 * t + 31 > u.first)  // a step that the values were taken out of
-          add_not_finite<D, BF16>(p, u, k0 + 32 * t, min(k0 + 32 * t + 32, u.kend), g, lim, oacc);
+          add_not_finite<D, BF16, SHARED>(p, u, k0 + 32 * t, min(k0 + 32 * t + 32, u.kend), g, lim, oacc);
 
     // ---- merge of the KG waves that share rows: piece 4 n + k of O (dims 32 n + 8 k + 4 g ..
     // + 3 of row l32) of every lane lies at [wave][piece][lane]; the wave with key group kg
@@ -1015,8 +1099,17 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         }
       }
     }
-    const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
     const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
+    if constexpr (SHARED) {
+      if (row < rows) {
+        if (kg == 0 && g == 0) state_ml(p, u)[at] = float4_t{m_run, l_row, x_row, (float)u.more};
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          st16(state_o<D>(p, u) + at * D + 8 * (NQ * kg + i) + 4 * g, as_uint4f(acc[i]));
+      }
+      return;
+    }
+    const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
     if (LSE && kg == 0 && g == 0 && row < rows)
       p.lse[at] = l_row == 0.f ? AKT_C_NEG_INF : (m_run + __log2f(x_row)) * kLn2;
     // The lane halves hold 8-byte halves of a row's 16-byte chunks: half 0 takes chunk i
@@ -1048,7 +1141,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     if (pass == 0) {
       int64_t total = uniform64(shfl64(inc, 63));
       int seqs = __builtin_popcountll(__ballot(len > 0));
-      for (int jb = 64; jb < p.B; jb += 64) {
+      for (int jb = 64; jb < num_seqs<SHARED>(p); jb += 64) {
         const int64_t more = seq_length(jb + lane0);
         total += uniform64(shfl64(scan64(more), 63));
         seqs += __builtin_popcountll(__ballot(more > 0));
@@ -1082,7 +1175,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       len = seq_length(jb + lane0);
       inc = scan64(len);
     }
-    Seq s = load_seq_uniform(p, b);
+    Seq<SHARED> s = load_seq_uniform<SHARED>(p, b);
     int64_t hlen = uniform64(head_length(p, s));
     int kvh = div_range(x - U, hlen);
     int64_t hs = uniform64(U + kvh * hlen);  // the head's start
@@ -1098,15 +1191,20 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
     }
     for (;;) {
       if (b == last_b && kvh == last_kvh && r == last_r) return;
-      Unit u;
+      Unit<SHARED> u;
       const int t0 = r * p.TR;
       u.q0 = uniform(s.q0 + t0);
       u.ntok = uniform(min(p.TR, s.n - t0));
       u.kvh = kvh;
       u.first = uniform(s.len - s.n + t0);
       u.len = uniform(s.len);
-      u.kend = uniform(p.causal ? max(u.first + u.ntok, 0) : s.len);
+      u.kend = uniform(is_causal(p, s) ? max(u.first + u.ntok, 0) : s.len);
       u.ip0 = uniform(s.ip0);
+      if constexpr (SHARED) {
+        u.prefix = uniform(s.prefix);
+        u.more = uniform(!s.prefix && p.groups > 0 && b >= p.group_indptr[0] &&
+                         b < p.group_indptr[p.groups]);
+      }
       const int64_t us = uniform64(hs + unit_start(p, s, r));
       // Blocks from the first at or past x - us - (kCkBlock - 1) on are those of the ranges
       // from x on.
@@ -1125,6 +1223,10 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
             const int row = idx / CPR;
             const int tok = (int)((uint32_t)row * p.g_magic >> 16);
             const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
+            if constexpr (SHARED) {
+              if (idx % CPR == 0) state_ml(p, u)[at] = float4_t{AKT_C_NEG_INF, 0.f, 0.f, (float)u.more};
+              continue;
+            }
             st16(p.o + at * D + idx % CPR * 8, uint4_t{0, 0, 0, 0});
             if (LSE && idx % CPR == 0) p.lse[at] = AKT_C_NEG_INF;
           }
@@ -1148,8 +1250,8 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       if (++kvh < p.Hkv) continue;
       kvh = 0;
       do {
-        if (++b == p.B) return;
-        s = load_seq_uniform(p, b);
+        if (++b == num_seqs<SHARED>(p)) return;
+        s = load_seq_uniform<SHARED>(p, b);
       } while (!mine(s));
       R = uniform(row_blocks(p, s.n));
       hlen = uniform64(head_length(p, s));
@@ -1160,13 +1262,13 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
 // Workgroups (of all W, a multiple of 8) for the sequences of few tokens, where a launch may hold
 // both kinds: in proportion to the lengths of the two axes, a key of the other weighing 1 for a
 // unit of hardly any rows up to chunk_tile_cost for one of all rows.
-template <int D>
+template <int D, bool SHARED>
 __device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
   constexpr int kRows = 32 * chunk_waves(D);
   const int lane = threadIdx.x & 63;
   double few = 0, many = 0;
-  for (int b = lane; b < p.B; b += 64) {
-    const Seq s = load_seq(p, b);
+  for (int b = lane; b < num_seqs<SHARED>(p); b += 64) {
+    const Seq<SHARED> s = load_seq<SHARED>(p, b);
     const double len = (double)head_length(p, s);
     if (s.n <= p.split_tokens) few += len;
     else
@@ -1183,7 +1285,7 @@ __device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
   return uniform(min(max(s, 8), W - 8));
 }
 
-template <int D, bool BF16, bool GRP, bool LSE>
+template <int D, bool BF16, bool GRP, bool LSE, bool SHARED>
 __global__ __launch_bounds__(64 * chunk_waves(D))
 __attribute__((amdgpu_waves_per_eu(chunk_waves_per_simd(D), chunk_waves_per_simd(D))))
 void paged_chunk_kernel(ChunkParams p) {
@@ -1193,22 +1295,31 @@ void paged_chunk_kernel(ChunkParams p) {
   // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
   // of them in what follows.
   __shared__ int sm_share;
-  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D>(p, W) : p.kinds == kCkFew ? W : 0;
+  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D, SHARED>(p, W) : p.kinds == kCkFew ? W : 0;
   if (threadIdx.x == 0) sm_share = share;
   __syncthreads();
   const int S = uniform(sm_share);
   if (block < S)
-    chunk_range<D, BF16, GRP, LSE, true>(p, lds, block, S);
+    chunk_range<D, BF16, GRP, LSE, SHARED, true>(p, lds, block, S);
   else
-    chunk_range<D, BF16, GRP, LSE, false>(p, lds, block - S, W - S);
+    chunk_range<D, BF16, GRP, LSE, SHARED, false>(p, lds, block - S, W - S);
 }
+
+// The instances of this translation unit: with or without shared prefixes.
+#ifdef AKT_CHUNK_SHARED
+constexpr bool kShared = true;
+#else
+constexpr bool kShared = false;
+#endif
 
 template <int D, bool BF16, bool GRP>
 int launch_lse(const ChunkParams& p, hipStream_t st) {
   KernelTimer timer;
   const dim3 grid(p.wgs), block(64 * chunk_waves(D));
-  if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true>, grid, block, 0, st, p);
-  else timer.launch(paged_chunk_kernel<D, BF16, GRP, false>, grid, block, 0, st, p);
+  if constexpr (kShared)
+    timer.launch(paged_chunk_kernel<D, BF16, GRP, true, true>, grid, block, 0, st, p);
+  else if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true, false>, grid, block, 0, st, p);
+  else timer.launch(paged_chunk_kernel<D, BF16, GRP, false, false>, grid, block, 0, st, p);
   return check_launch("paged_chunk_kernel");
 }
 
@@ -1222,22 +1333,23 @@ int launch_chunk(const ChunkParams& p, bool bf16, hipStream_t st) {
 }  // namespace
 
 // Each head dim is instantiated in a translation unit of its own (they compile side by
-// side): this one holds D = 128 and the entry points, the others include it.
+// side), with shared prefixes and without: this one holds D = 128 and the entry points, the
+// others include it.
 #ifndef AKT_CHUNK_TU
 #define AKT_CHUNK_TU 128
 #endif
-#if AKT_CHUNK_TU == 64
-int chunk_launch_64(const ChunkParams& p, bool bf16, hipStream_t st) {
-  return launch_chunk<64>(p, bf16, st);
-}
-#elif AKT_CHUNK_TU == 256
-int chunk_launch_256(const ChunkParams& p, bool bf16, hipStream_t st) {
-  return launch_chunk<256>(p, bf16, st);
+#define AKT_CAT_(a, b) a##b
+#define AKT_CAT(a, b) AKT_CAT_(a, b)
+#ifdef AKT_CHUNK_SHARED
+int AKT_CAT(shared_launch_, AKT_CHUNK_TU)(const ChunkParams& p, bool bf16, hipStream_t st) {
+  return launch_chunk<AKT_CHUNK_TU>(p, bf16, st);
 }
 #else
-int chunk_launch_128(const ChunkParams& p, bool bf16, hipStream_t st) {
-  return launch_chunk<128>(p, bf16, st);
+int AKT_CAT(chunk_launch_, AKT_CHUNK_TU)(const ChunkParams& p, bool bf16, hipStream_t st) {
+  return launch_chunk<AKT_CHUNK_TU>(p, bf16, st);
 }
+#endif
+#if AKT_CHUNK_TU == 128 && !defined(AKT_CHUNK_SHARED)
 
 namespace {
 
@@ -1257,15 +1369,23 @@ int64_t axis_wgs(double units, int64_t tokens, int64_t resident) {
   return wgs < (double)resident ? round_up((int64_t)wgs, 8) : resident;
 }
 
+// groups < 0: no shared prefixes.
 ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
-                     int64_t page_size, int64_t total_pages) {
+                     int64_t page_size, int64_t total_pages, int64_t groups,
+                     int64_t prefix_pages) {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
       cus <= 0 || cus > 1024)
     cus = 256;  // no device: what an MI355X has
-  const int64_t tokens = page_size * total_pages;
-  const int64_t seqs = batch < total_q ? batch : total_q;
+  const bool shared = groups >= 0;
+  const int64_t tokens = page_size * (total_pages + (shared ? prefix_pages : 0));
+  // Sequences with new tokens, and their new tokens; a group's once more.
+  int64_t seqs = batch < total_q ? batch : total_q, rows = total_q;
+  if (shared) {
+    seqs += groups < total_q ? groups : total_q;
+    rows += total_q;
+  }
   const int waves = chunk_waves((int)D);
   const int64_t resident = round_up((int64_t)cus * chunk_waves_per_simd((int)D) * 4 / waves, 8);
   ChunkPlan c = {};
@@ -1278,7 +1398,7 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   if (!few) c.kinds |= kCkMany;
   double units = 0;
   if (c.kinds & kCkFew) units += (double)Hkv * seqs;
-  if (c.kinds & kCkMany) units += (double)Hkv * (total_q / (32 * waves / G) + seqs);
+  if (c.kinds & kCkMany) units += (double)Hkv * (rows / (32 * waves / G) + seqs);
   c.wgs = axis_wgs(units, tokens, resident);
   if (c.kinds == (kCkFew | kCkMany) && c.wgs < 16) c.wgs = 16;  // eight of each kind
   // Two partial slots to a range, whichever kind a workgroup serves.
@@ -1292,38 +1412,37 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   return c;
 }
 
-}  // namespace
-}  // namespace akt
+// Bytes of the states of rows that attend in two parts.
+int64_t state_bytes(int64_t total_q, int64_t Hq, int64_t D) { return total_q * Hq * (32 + 8 * D); }
 
-using namespace akt;
-
-extern "C" size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q,
-                                                 int64_t num_q_heads, int64_t num_kv_heads,
-                                                 int64_t head_dim, int64_t page_size,
-                                                 int64_t total_pages) {
-  if (batch <= 0 || total_q <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || page_size <= 0 ||
-      total_pages < 0 || num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > kCkRows ||
-      (head_dim != 64 && head_dim != 128 && head_dim != 256))
-    return 0;
-  const ChunkPlan c = chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
-                                 page_size, total_pages);
-  return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) +
-                  c.partial_bytes);
+bool sizes_served(int64_t Hq, int64_t Hkv, int64_t D) {
+  return Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kCkRows &&
+         (D == 64 || D == 128 || D == 256);
 }
 
-extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
-                                   const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
-                                   const int32_t* kv_last_page_len, void* o, float* lse,
-                                   int64_t batch, int64_t total_q, int64_t num_q_heads,
-                                   int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
-                                   int64_t total_pages, int64_t num_pool_pages,
-                                   const int64_t q_stride[3], const int64_t kv_stride[5],
-                                   float softmax_scale, int causal, int dtype, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+size_t workspace_bytes_of(const ChunkPlan& c, int64_t states) {
+  return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) + round_up(c.partial_bytes, 256) + states);
+}
+
+// What a call with shared prefixes has besides.
+struct SharedArgs {
+  const int32_t *group_indptr, *prefix_indptr, *prefix_indices, *prefix_last;
+  int64_t groups, prefix_pages;
+};
+
+int chunk_call(const void* q, const int32_t* q_indptr, const void* kv_cache,
+               const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+               const int32_t* kv_last_page_len, const SharedArgs* shared, void* o, float* lse,
+               int64_t batch, int64_t total_q, int64_t num_q_heads, int64_t num_kv_heads,
+               int64_t head_dim, int64_t page_size, int64_t total_pages, int64_t num_pool_pages,
+               const int64_t q_stride[3], const int64_t kv_stride[5], float softmax_scale,
+               int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   AKT_CHECK(dtype == AKT_DTYPE_F16 || dtype == AKT_DTYPE_BF16,
             "dtype must be AKT_DTYPE_F16 or AKT_DTYPE_BF16, got %d", dtype);
   AKT_CHECK(batch >= 0 && total_q >= 0 && total_pages >= 0 && num_pool_pages >= 0,
+            "sizes must be non-negative");
+  AKT_CHECK(!shared || (shared->groups >= 0 && shared->prefix_pages >= 0),
             "sizes must be non-negative");
   AKT_CHECK(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0,
             "num_q_heads (%lld) must be a positive multiple of num_kv_heads (%lld)",
@@ -1339,10 +1458,18 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
             "problem too large");
   AKT_CHECK(total_pages < (1ll << 31) && total_pages * page_size < (1ll << 30),
             "the page table spans too many tokens");
+  AKT_CHECK(!shared || (shared->groups < (1ll << 30) && shared->prefix_pages < (1ll << 31) &&
+                        shared->prefix_pages * page_size < (1ll << 30)),
+            "the prefixes' page table spans too many tokens");
+  AKT_CHECK(!shared || total_q * num_q_heads < (1ll << 31) / 64, "too many query rows");
   AKT_CHECK(std::isfinite(softmax_scale), "softmax_scale must be finite");
   if (batch == 0 || total_q == 0) return AKT_OK;
   AKT_CHECK(q && q_indptr && kv_cache && kv_page_indptr && kv_last_page_len && o && q_stride &&
                 kv_stride && (kv_page_indices || total_pages == 0),
+            "all pointers are required");
+  AKT_CHECK(!shared || (shared->group_indptr && shared->prefix_indptr &&
+                        (shared->prefix_last || shared->groups == 0) &&
+                        (shared->prefix_indices || shared->prefix_pages == 0)),
             "all pointers are required");
   AKT_CHECK(q_stride[2] == 1 && kv_stride[4] == 1, "head_dim stride must be 1");
   AKT_CHECK(rows_aligned16(q, q_stride, 2) && rows_aligned16(kv_cache, kv_stride, 4) &&
@@ -1351,9 +1478,10 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   AKT_CHECK(kv_stride[3] >= 0 && kv_stride[3] < (1 << 22), "slot stride out of range [0, 2^22)");
   const int64_t G = num_q_heads / num_kv_heads;
   const ChunkPlan plan =
-      chunk_plan(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages);
-  const size_t need = akt_chunk_paged_workspace_size(batch, total_q, num_q_heads, num_kv_heads,
-                                                     head_dim, page_size, total_pages);
+      chunk_plan(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages,
+                 shared ? shared->groups : -1, shared ? shared->prefix_pages : 0);
+  const size_t need =
+      workspace_bytes_of(plan, shared ? state_bytes(total_q, num_q_heads, head_dim) : 0);
   if (!workspace || workspace_bytes < need)
     return set_error(AKT_ERR_WORKSPACE, "chunk attention needs a workspace of %zu bytes, got %zu",
                      need, workspace ? workspace_bytes : (size_t)0);
@@ -1402,9 +1530,83 @@ extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const
   p.many_partial = plan.many_partial;
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == AKT_DTYPE_BF16;
-  if (head_dim == 64) return chunk_launch_64(p, bf16, st);
-  if (head_dim == 256) return chunk_launch_256(p, bf16, st);
-  return chunk_launch_128(p, bf16, st);
+  if (!shared) {
+    if (head_dim == 64) return chunk_launch_64(p, bf16, st);
+    if (head_dim == 256) return chunk_launch_256(p, bf16, st);
+    return chunk_launch_128(p, bf16, st);
+  }
+  p.group_indptr = shared->group_indptr;
+  p.prefix_indptr = shared->prefix_indptr;
+  p.prefix_indices = shared->prefix_indices;
+  p.prefix_last = shared->prefix_last;
+  p.groups = (int)shared->groups;
+  p.prefix_pages = (int)shared->prefix_pages;
+  p.states = p.partials + round_up(plan.partial_bytes, 256);
+  const int rc = head_dim == 64    ? shared_launch_64(p, bf16, st)
+                 : head_dim == 256 ? shared_launch_256(p, bf16, st)
+                                   : shared_launch_128(p, bf16, st);
+  return rc != AKT_OK ? rc : shared_merge_launch(p, (int)head_dim, bf16, st);
+}
+
+}  // namespace
+}  // namespace akt
+
+using namespace akt;
+
+extern "C" size_t akt_chunk_paged_workspace_size(int64_t batch, int64_t total_q,
+                                                 int64_t num_q_heads, int64_t num_kv_heads,
+                                                 int64_t head_dim, int64_t page_size,
+                                                 int64_t total_pages) {
+  if (batch <= 0 || total_q <= 0 || page_size <= 0 || total_pages < 0 ||
+      !sizes_served(num_q_heads, num_kv_heads, head_dim))
+    return 0;
+  return workspace_bytes_of(chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads,
+                                       head_dim, page_size, total_pages, -1, 0), 0);
+}
+
+extern "C" int akt_chunk_paged_fwd(const void* q, const int32_t* q_indptr, const void* kv_cache,
+                                   const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+                                   const int32_t* kv_last_page_len, void* o, float* lse,
+                                   int64_t batch, int64_t total_q, int64_t num_q_heads,
+                                   int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                   int64_t total_pages, int64_t num_pool_pages,
+                                   const int64_t q_stride[3], const int64_t kv_stride[5],
+                                   float softmax_scale, int causal, int dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  return chunk_call(q, q_indptr, kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len,
+                    nullptr, o, lse, batch, total_q, num_q_heads, num_kv_heads, head_dim, page_size,
+                    total_pages, num_pool_pages, q_stride, kv_stride, softmax_scale, causal, dtype,
+                    workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t akt_shared_prefix_paged_workspace_size(int64_t batch, int64_t total_q,
+                                                         int64_t num_q_heads, int64_t num_kv_heads,
+                                                         int64_t head_dim, int64_t page_size,
+                                                         int64_t total_pages, int64_t groups,
+                                                         int64_t prefix_pages) {
+  if (batch <= 0 || total_q <= 0 || page_size <= 0 || total_pages < 0 || groups < 0 ||
+      prefix_pages < 0 || !sizes_served(num_q_heads, num_kv_heads, head_dim))
+    return 0;
+  return workspace_bytes_of(chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads,
+                                       head_dim, page_size, total_pages, groups, prefix_pages),
+                            state_bytes(total_q, num_q_heads, head_dim));
+}
+
+extern "C" int akt_shared_prefix_paged_fwd(
+    const void* q, const int32_t* q_indptr, const void* kv_cache, const int32_t* kv_page_indptr,
+    const int32_t* kv_page_indices, const int32_t* kv_last_page_len, const int32_t* group_indptr,
+    const int32_t* prefix_page_indptr, const int32_t* prefix_page_indices,
+    const int32_t* prefix_last_page_len, void* o, float* lse, int64_t batch, int64_t total_q,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+    int64_t total_pages, int64_t groups, int64_t prefix_pages, int64_t num_pool_pages,
+    const int64_t q_stride[3], const int64_t kv_stride[5], float softmax_scale, int causal,
+    int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const SharedArgs shared = {group_indptr, prefix_page_indptr, prefix_page_indices,
+                             prefix_last_page_len, groups, prefix_pages};
+  return chunk_call(q, q_indptr, kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len,
+                    &shared, o, lse, batch, total_q, num_q_heads, num_kv_heads, head_dim, page_size,
+                    total_pages, num_pool_pages, q_stride, kv_stride, softmax_scale, causal, dtype,
+                    workspace, workspace_bytes, stream);
 }
 
 namespace akt {

@@ -53,6 +53,16 @@ struct ChunkParams {
   int many_counter;      // where the second kind's arrival counters
   int64_t many_partial;  // and partials begin
   int min_keys;    // fewest keys (with unit costs) of a range, at least kCkBlock
+  // Shared prefixes: group i is sequences group_indptr[i] .. group_indptr[i + 1] - 1 and has the
+  // keys of row i of the prefixes' page table.
+  const int32_t* group_indptr;
+  const int32_t* prefix_indptr;
+  const int32_t* prefix_indices;
+  const int32_t* prefix_last;
+  int groups, prefix_pages;
+  // States of the rows, (m, l, exact l, -) and the sums of P.V, fp32: [2][total_q * Hq] rows of
+  // 16 bytes, then [2][total_q * Hq] of 4 D, own keys' first.
+  char* states;
 };
 
 // Waves of a workgroup.  Up to D = 128 eight share a tile of 64 keys (one workgroup to a CU):
@@ -73,8 +83,15 @@ __host__ __device__ constexpr int64_t chunk_split_wave_bytes(int D) {
 // Waves to a SIMD.
 __host__ __device__ constexpr int chunk_waves_per_simd(int D) { return D <= 128 ? 2 : 1; }
 
+// Each head dim is compiled in a file of its own, with shared prefixes and without.
 int chunk_launch_64(const ChunkParams& p, bool bf16, hipStream_t st);
 int chunk_launch_128(const ChunkParams& p, bool bf16, hipStream_t st);
 int chunk_launch_256(const ChunkParams& p, bool bf16, hipStream_t st);
+
+int shared_launch_64(const ChunkParams& p, bool bf16, hipStream_t st);
+int shared_launch_128(const ChunkParams& p, bool bf16, hipStream_t st);
+int shared_launch_256(const ChunkParams& p, bool bf16, hipStream_t st);
+// Joins the two states of every row (paged_shared.hip).
+int shared_merge_launch(const ChunkParams& p, int head_dim, bool bf16, hipStream_t st);
 
 }  // namespace akt

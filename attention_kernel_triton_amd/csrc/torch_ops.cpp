@@ -1,6 +1,6 @@
 // Compiled host layer of the hot entry points (prefill, dense / paged /
-// sparse / MagicPIG decode, paged chunk attention, rotary positions, kept-index selection,
-// paged KV append and page copies, LSE merge): the same checks, output allocation, stream and
+// sparse / MagicPIG decode, paged chunk and shared-prefix attention, attention weights, rotary
+// positions, kept-index selection, paged KV append, page copies and kept tokens, LSE merge): the same checks, output allocation, stream and
 // workspace handling as the package's Python wrappers, done in C++ so a
 // drop-in call costs the host a few microseconds.  It calls the C ABI of
 // libakt_amd.so (include/akt_amd.h) and nothing else; there is no fallback.
@@ -561,6 +561,167 @@ py::object chunk_paged(const at::Tensor& q_, const at::Tensor& q_indptr_, const 
   return result(o, lse, return_lse);
 }
 
+// --------------------------------------------------------------------------- shared prefixes
+py::object shared_prefix_paged(const at::Tensor& q_, const at::Tensor& q_indptr_,
+                               const at::Tensor& pool_, const at::Tensor& indptr_,
+                               const at::Tensor& indices_, const at::Tensor& last_,
+                               const at::Tensor& group_indptr_, const at::Tensor& prefix_indptr_,
+                               const at::Tensor& prefix_indices_, const at::Tensor& prefix_last_,
+                               bool causal, const c10::optional<double>& softmax_scale,
+                               bool return_lse) {
+  need_gpu("q", q_);
+  const int dtype = dtype16("q", q_);
+  if (q_.dim() != 3) throw py::value_error("q must be [total_q, Hq, D]");
+  if (pool_.dim() != 5 || pool_.size(1) != 2)
+    throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
+  at::Tensor q = rows16(q_), pool = rows_like("paged_kv_cache", pool_, q_.scalar_type(), "q");
+  const at::Device dev = q.device();
+  same_device("paged_kv_cache", pool, dev);
+  at::Tensor q_indptr = int32_on("q_indptr", q_indptr_, dev).contiguous();
+  at::Tensor indptr = int32_on("kv_page_indptr", indptr_, dev).contiguous();
+  at::Tensor indices = int32_on("kv_page_indices", indices_, dev).contiguous();
+  at::Tensor last = int32_on("kv_last_page_len", last_, dev).contiguous();
+  at::Tensor group_indptr = int32_on("group_indptr", group_indptr_, dev).contiguous();
+  at::Tensor prefix_indptr = int32_on("prefix_page_indptr", prefix_indptr_, dev).contiguous();
+  at::Tensor prefix_indices = int32_on("prefix_page_indices", prefix_indices_, dev).contiguous();
+  at::Tensor prefix_last = int32_on("prefix_last_page_len", prefix_last_, dev).contiguous();
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
+  const int64_t P = pool.size(0), Hkv = pool.size(2), page = pool.size(3), B = last.numel();
+  const int64_t groups = prefix_last.numel();
+  if (pool.size(4) != D)
+    throw py::value_error("head_dim mismatch: q has " + std::to_string(D) + ", cache has " +
+                          std::to_string(pool.size(4)));
+  if (q_indptr.numel() != B + 1 || indptr.numel() != B + 1)
+    throw py::value_error("q_indptr and kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  if (group_indptr.numel() != groups + 1 || prefix_indptr.numel() != groups + 1)
+    throw py::value_error(
+        "group_indptr and prefix_page_indptr must have groups+1 and prefix_last_page_len groups entries");
+  const float scale = softmax_scale.has_value() ? (float)*softmax_scale
+                                                : (float)(1.0 / std::sqrt((double)D));
+  const DeviceGuard guard(dev);
+  at::Tensor o = at::empty({T, Hq, D}, q.options());
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({T, Hq}, q.options().dtype(at::kFloat));
+  const int64_t total = indices.numel(), prefix_pages = prefix_indices.numel();
+  hipStream_t st = stream_of(q);
+  const size_t ws_n =
+      akt_shared_prefix_paged_workspace_size(B, T, Hq, Hkv, D, page, total, groups, prefix_pages);
+  at::Tensor ws = capture_workspace(ws_n, dev, st);
+  const Strides qs = strides_of(q), ps = strides_of(pool);
+  check_rc(akt_shared_prefix_paged_fwd(
+               ptr(q), (const int32_t*)ptr(q_indptr), ptr(pool), (const int32_t*)ptr(indptr),
+               (const int32_t*)ptr(indices), (const int32_t*)ptr(last),
+               (const int32_t*)ptr(group_indptr), (const int32_t*)ptr(prefix_indptr),
+               (const int32_t*)ptr(prefix_indices), (const int32_t*)ptr(prefix_last), ptr(o),
+               (float*)ptr(lse), B, T, Hq, Hkv, D, page, total, groups, prefix_pages, P, qs.v,
+               ps.v, scale, causal ? 1 : 0, dtype, ptr(ws), ws_n, st),
+           "akt_shared_prefix_paged_fwd");
+  return result(o, lse, return_lse);
+}
+
+// --------------------------------------------------------------------------- attention weights
+// Sums fp32 [N, H, L] with a unit last stride, and the row of each of B sequences.
+struct WeightRows {
+  int64_t stride[2];
+  at::Tensor rows;
+};
+WeightRows weight_rows(const at::Tensor& weights, const c10::optional<at::Tensor>& rows_,
+                       const at::Device& dev, int64_t B, int64_t H) {
+  need_gpu("weights", weights);
+  same_device("weights", weights, dev);
+  if (weights.scalar_type() != at::kFloat)
+    throw py::type_error("weights must be float32, got " +
+                         std::string(c10::toString(weights.scalar_type())));
+  if (weights.dim() != 3 || (H >= 0 && weights.size(1) != H))
+    throw py::value_error("weights must be [N, Hkv, L], got " + c10::str(weights.sizes()));
+  if (weights.size(2) > 1 && weights.stride(2) != 1)
+    throw py::value_error("weights need a unit last stride");
+  WeightRows r{{weights.stride(0), weights.stride(1)}, at::Tensor()};
+  if (rows_.has_value() && rows_->defined()) {
+    r.rows = int32_on("rows", *rows_, dev).contiguous();
+    if (r.rows.dim() != 1 || r.rows.numel() != B)
+      throw py::value_error("rows must have " + std::to_string(B) + " entries, got " +
+                            std::to_string(r.rows.numel()));
+  } else if (weights.size(0) < B) {
+    throw py::value_error("weights have " + std::to_string(weights.size(0)) + " rows for " +
+                          std::to_string(B) + " sequences");
+  }
+  return r;
+}
+
+void attention_weights_paged(const at::Tensor& weights, const at::Tensor& q_,
+                             const at::Tensor& q_indptr_, const at::Tensor& lse_,
+                             const at::Tensor& pool_, const at::Tensor& indptr_,
+                             const at::Tensor& indices_, const at::Tensor& last_,
+                             const c10::optional<at::Tensor>& rows, bool causal,
+                             const c10::optional<double>& softmax_scale,
+                             const c10::optional<int64_t>& window) {
+  need_gpu("q", q_);
+  const int dtype = dtype16("q", q_);
+  if (q_.dim() != 3) throw py::value_error("q must be [total_q, Hq, D]");
+  if (pool_.dim() != 5 || pool_.size(1) != 2)
+    throw py::value_error("paged_kv_cache must be [P, 2, Hkv, page, D]");
+  at::Tensor q = rows16(q_), pool = rows_like("paged_kv_cache", pool_, q_.scalar_type(), "q");
+  const at::Device dev = q.device();
+  same_device("paged_kv_cache", pool, dev);
+  at::Tensor q_indptr = int32_on("q_indptr", q_indptr_, dev).contiguous();
+  at::Tensor indptr = int32_on("kv_page_indptr", indptr_, dev).contiguous();
+  at::Tensor indices = int32_on("kv_page_indices", indices_, dev).contiguous();
+  at::Tensor last = int32_on("kv_last_page_len", last_, dev).contiguous();
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
+  const int64_t P = pool.size(0), Hkv = pool.size(2), page = pool.size(3), B = last.numel();
+  if (pool.size(4) != D)
+    throw py::value_error("head_dim mismatch: q has " + std::to_string(D) + ", cache has " +
+                          std::to_string(pool.size(4)));
+  if (q_indptr.numel() != B + 1 || indptr.numel() != B + 1)
+    throw py::value_error("q_indptr and kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  need_gpu("lse", lse_);
+  same_device("lse", lse_, dev);
+  if (lse_.scalar_type() != at::kFloat)
+    throw py::type_error("lse must be float32, got " +
+                         std::string(c10::toString(lse_.scalar_type())));
+  if (lse_.dim() != 2 || lse_.size(0) != T || lse_.size(1) != Hq)
+    throw py::value_error("lse must be [" + std::to_string(T) + ", " + std::to_string(Hq) + "]");
+  at::Tensor lse = lse_.contiguous();
+  const WeightRows wr = weight_rows(weights, rows, dev, B, Hkv);
+  if (window.has_value() && *window < 0) throw py::value_error("window must be non-negative");
+  const float scale = softmax_scale.has_value() ? (float)*softmax_scale
+                                                : (float)(1.0 / std::sqrt((double)D));
+  const DeviceGuard guard(dev);
+  const Strides qs = strides_of(q), ps = strides_of(pool);
+  check_rc(akt_attention_weights_paged(
+               ptr(q), (const int32_t*)ptr(q_indptr), (const float*)ptr(lse), ptr(pool),
+               (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices),
+               (const int32_t*)ptr(last), (float*)ptr(weights), (const int32_t*)ptr(wr.rows), B, T,
+               Hq, Hkv, D, page, indices.numel(), P, weights.size(0), weights.size(2), qs.v, ps.v,
+               wr.stride, scale, causal ? 1 : 0, window.has_value() ? *window : INT64_MAX, dtype,
+               stream_of(q)),
+           "akt_attention_weights_paged");
+}
+
+// The heaviest tokens of each sequence and head, as kept-token lists.
+py::tuple kept_heaviest(const at::Tensor& weights, const at::Tensor& lengths_, int64_t keep,
+                        int64_t first, int64_t recent, const c10::optional<at::Tensor>& rows) {
+  need_gpu("weights", weights);
+  const at::Device dev = weights.device();
+  at::Tensor lengths = int32_on("lengths", lengths_, dev).contiguous();
+  if (lengths.dim() != 1) throw py::value_error("lengths must be [B]");
+  const int64_t B = lengths.numel();
+  const WeightRows wr = weight_rows(weights, rows, dev, B, -1);
+  if (keep < 0 || first < 0 || recent < 0 || first > keep || recent > keep - first)
+    throw py::value_error("keep must be at least first + recent, and none negative");
+  const DeviceGuard guard(dev);
+  const int64_t H = weights.size(1);
+  at::Tensor ind = at::empty({B, H, keep}, lengths.options());
+  at::Tensor nnz = at::empty({B, H, 1}, lengths.options());
+  check_rc(akt_kept_index_heaviest((const float*)ptr(weights), (const int32_t*)ptr(lengths),
+                                   (const int32_t*)ptr(wr.rows), (int32_t*)ptr(ind),
+                                   (int32_t*)ptr(nnz), B, H, weights.size(0), weights.size(2),
+                                   wr.stride, keep, first, recent, stream_of(weights)),
+           "akt_kept_index_heaviest");
+  return py::make_tuple(ind, nnz);
+}
+
 // --------------------------------------------------------------------------- rotary
 at::Tensor frequencies(const at::Tensor& inv_freq, const at::Device& dev) {
   need_gpu("inv_freq", inv_freq);
@@ -694,6 +855,50 @@ void copy_pages(const at::Tensor& pool, const at::Tensor& src_, const at::Tensor
            "akt_paged_copy");
 }
 
+// Kept tokens (and their sums) to the front of their sequences.
+void keep_tokens(const at::Tensor& pool, const at::Tensor& indptr_, const at::Tensor& indices_,
+                 const at::Tensor& last_, const at::Tensor& ind_, const at::Tensor& nnz_,
+                 const c10::optional<at::Tensor>& dst_, const c10::optional<at::Tensor>& weights,
+                 const c10::optional<at::Tensor>& rows) {
+  need_gpu("paged_kv_cache", pool);
+  check_written_pool(pool);
+  const at::Device dev = pool.device();
+  at::Tensor indptr = int32_on("kv_page_indptr", indptr_, dev).contiguous();
+  at::Tensor indices = int32_on("kv_page_indices", indices_, dev).contiguous();
+  at::Tensor last = int32_on("kv_last_page_len", last_, dev).contiguous();
+  at::Tensor ind = int32_on("sparse_ind", ind_, dev).contiguous();
+  at::Tensor nnz = int32_on("sparse_nnz", nnz_, dev).contiguous();
+  const int64_t P = pool.size(0), Hkv = pool.size(2), page = pool.size(3), D = pool.size(4);
+  const int64_t B = last.numel();
+  if (indptr.numel() != B + 1)
+    throw py::value_error("kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  if (ind.dim() != 3 || ind.size(0) != B || ind.size(1) != Hkv)
+    throw py::value_error("sparse_ind must be [B=" + std::to_string(B) + ", Hkv=" +
+                          std::to_string(Hkv) + ", keep], got " + c10::str(ind.sizes()));
+  if (nnz.dim() < 2 || nnz.size(0) != B || nnz.size(1) != Hkv || nnz.numel() != B * Hkv)
+    throw py::value_error("sparse_nnz must be [B=" + std::to_string(B) + ", Hkv=" +
+                          std::to_string(Hkv) + "(, 1)]");
+  at::Tensor dst;
+  if (dst_.has_value() && dst_->defined()) {
+    dst = int32_on("dst_page_indices", *dst_, dev).contiguous();
+    if (dst.numel() != indices.numel())
+      throw py::value_error("dst_page_indices must have an entry for each of kv_page_indices");
+  }
+  const bool sums = weights.has_value() && weights->defined();
+  WeightRows wr{{0, 0}, at::Tensor()};
+  if (sums) wr = weight_rows(*weights, rows, dev, B, Hkv);
+  const DeviceGuard guard(dev);
+  const Strides ps = strides_of(pool);
+  check_rc(akt_paged_keep(ptr(pool), (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices),
+                          (const int32_t*)ptr(last), (const int32_t*)ptr(dst),
+                          (const int32_t*)ptr(ind), (const int32_t*)ptr(nnz),
+                          sums ? (float*)weights->data_ptr() : nullptr,
+                          (const int32_t*)ptr(wr.rows), B, Hkv, D, page, indices.numel(), P,
+                          ind.size(2), sums ? weights->size(0) : 0, sums ? weights->size(2) : 0,
+                          ps.v, wr.stride, stream_of(pool)),
+           "akt_paged_keep");
+}
+
 // --------------------------------------------------------------------------- LSE merge
 int merge_dtype(const char* name, at::ScalarType t) {
   if (t == at::kHalf) return AKT_DTYPE_F16;
@@ -779,6 +984,22 @@ PYBIND11_MODULE(_akt_torch, m) {
         py::arg("kv_page_indptr"), py::arg("kv_page_indices"), py::arg("kv_last_page_len"),
         py::arg("causal") = true, py::arg("softmax_scale") = py::none(),
         py::arg("return_lse") = false);
+  m.def("shared_prefix_paged", &shared_prefix_paged, py::arg("q"), py::arg("q_indptr"),
+        py::arg("paged_kv_cache"), py::arg("kv_page_indptr"), py::arg("kv_page_indices"),
+        py::arg("kv_last_page_len"), py::arg("group_indptr"), py::arg("prefix_page_indptr"),
+        py::arg("prefix_page_indices"), py::arg("prefix_last_page_len"), py::arg("causal") = true,
+        py::arg("softmax_scale") = py::none(), py::arg("return_lse") = false);
+  m.def("attention_weights_paged", &attention_weights_paged, py::arg("weights"), py::arg("q"),
+        py::arg("q_indptr"), py::arg("lse"), py::arg("paged_kv_cache"), py::arg("kv_page_indptr"),
+        py::arg("kv_page_indices"), py::arg("kv_last_page_len"), py::arg("rows") = py::none(),
+        py::arg("causal") = true, py::arg("softmax_scale") = py::none(),
+        py::arg("window") = py::none());
+  m.def("kept_heaviest", &kept_heaviest, py::arg("weights"), py::arg("lengths"), py::arg("keep"),
+        py::arg("first") = 0, py::arg("recent") = 0, py::arg("rows") = py::none());
+  m.def("keep_tokens", &keep_tokens, py::arg("paged_kv_cache"), py::arg("kv_page_indptr"),
+        py::arg("kv_page_indices"), py::arg("kv_last_page_len"), py::arg("sparse_ind"),
+        py::arg("sparse_nnz"), py::arg("dst_page_indices") = py::none(),
+        py::arg("weights") = py::none(), py::arg("rows") = py::none());
   m.def("rotary", &rotary, py::arg("Q"), py::arg("K"), py::arg("inv_freq"),
         py::arg("positions") = py::none(), py::arg("interleaved") = false,
         py::arg("factor") = 1.0, py::arg("transpose") = false);

@@ -12,6 +12,8 @@ This module fills them:
 - ``append_paged_kv_rotary`` does the same for k that still has to be rotated by
   its positions, and rotates q with it (``akt_paged_kv_append_rotary``).
 - ``copy_pages`` copies pages within a pool (``akt_paged_copy``).
+- ``keep_tokens`` moves the tokens that a selection keeps to the front of their sequences
+  (``akt_paged_keep``).
 - ``PagedKVCache`` owns a pool and a free list on the host, grows each
   sequence's page list as tokens are appended (prefill chunks or one token
   per decode step), and hands out the page table the decode entry points
@@ -62,6 +64,26 @@ def copy_pages(paged_kv_cache, src, dst, num_tokens=None) -> None:
     destination.  Pairs that name a page outside the pool are skipped.
     """
     N.torch_ext().copy_pages(paged_kv_cache, src, dst, num_tokens=num_tokens)
+
+
+def keep_tokens(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len, sparse_ind,
+                sparse_nnz, dst_page_indices=None, weights=None, rows=None) -> None:
+    """Move kept tokens' K and V to the front of their sequences, in place, and their sums along.
+
+    sparse_ind int32 [B, Hkv, keep], sparse_nnz int32 [B, Hkv(, 1)]: ascending token indices, as
+    kept_index.select_heaviest returns them.  Slot j of a (sequence, kv head) takes token
+    sparse_ind[b, h, j]; an entry that names a token before its own slot, or past the sequence's
+    end, is skipped.  The table still describes the sequences before the call; afterwards head h of
+    sequence b has sparse_nnz[b, h] tokens.
+    dst_page_indices: int32, in the place of kv_page_indices for the slots written, where a page
+    must not be (it is shared); the pages that differ must be in no sequence of the call.  No page
+    may be written for two sequences, nor written for one and read for another.
+    weights float32 [N, Hkv, L] and rows as in select_heaviest, no row twice: the kept tokens' sums
+    move with them, and those behind become 0.
+    """
+    N.torch_ext().keep_tokens(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len,
+                              sparse_ind, sparse_nnz, dst_page_indices=dst_page_indices,
+                              weights=weights, rows=rows)
 
 
 class PagedKVCache:
@@ -267,4 +289,5 @@ class PagedKVCache:
             raise
 
 
-__all__ = ["append_paged_kv", "append_paged_kv_rotary", "copy_pages", "PagedKVCache"]
+__all__ = ["append_paged_kv", "append_paged_kv_rotary", "copy_pages", "keep_tokens",
+           "PagedKVCache"]

@@ -42,7 +42,8 @@
  *                                                        akt_paged_kv_append
  * Without a counterpart there: akt_chunk_paged_fwd, akt_rotary_fwd,
  * akt_paged_kv_append_rotary and akt_paged_copy, which serve a paged cache beyond
- * single-token decode.
+ * single-token decode; akt_shared_prefix_paged_fwd, akt_attention_weights_paged,
+ * akt_kept_index_heaviest and akt_paged_keep, which keep what is read and held of one small.
  */
 #ifndef AKT_AMD_H
 #define AKT_AMD_H
@@ -449,6 +450,91 @@ int akt_paged_copy(void* kv_cache, const int32_t* src, const int32_t* dst,
                    const int32_t* num_tokens, int64_t n, int64_t num_kv_heads, int64_t head_dim,
                    int64_t page_size, int64_t num_pool_pages, const int64_t kv_stride[5],
                    void* stream);
+
+/*
+ * akt_chunk_paged_fwd for sequences that share prefixes: each prefix's K and V are read once for
+ * all of its group.  No reference counterpart.
+ *   group_indptr int32 [groups + 1]: group i is sequences group_indptr[i] .. group_indptr[i + 1]
+ *   - 1 (a sequence outside [group_indptr[0], group_indptr[groups]) has no prefix).
+ *   prefix_page_indptr [groups + 1], prefix_page_indices [prefix_pages], prefix_last_page_len
+ *   [groups]: the prefixes' page table, in the form of the sequences' own.
+ * A sequence's keys are its group's prefix, then its own (the table kv_page_*, which counts its new
+ * tokens).  Every query token sees the whole prefix; of the own keys query i of n_b, at own
+ * position len_b - n_b + i, sees those up to its own position (causal) or all.
+ * The rest is as in akt_chunk_paged_fwd; so is the workspace, and the first
+ * AKT_WORKSPACE_ZERO_BYTES of it that every call leaves zero.  Two launches.
+ */
+size_t akt_shared_prefix_paged_workspace_size(int64_t batch, int64_t total_q, int64_t num_q_heads,
+                                              int64_t num_kv_heads, int64_t head_dim,
+                                              int64_t page_size, int64_t total_pages,
+                                              int64_t groups, int64_t prefix_pages);
+int akt_shared_prefix_paged_fwd(
+    const void* q, const int32_t* q_indptr, const void* kv_cache, const int32_t* kv_page_indptr,
+    const int32_t* kv_page_indices, const int32_t* kv_last_page_len, const int32_t* group_indptr,
+    const int32_t* prefix_page_indptr, const int32_t* prefix_page_indices,
+    const int32_t* prefix_last_page_len, void* o, float* lse, int64_t batch, int64_t total_q,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+    int64_t total_pages, int64_t groups, int64_t prefix_pages, int64_t num_pool_pages,
+    const int64_t q_stride[3], const int64_t kv_stride[5], float softmax_scale, int causal,
+    int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Adds the attention that cached tokens draw to sums over calls.  No reference counterpart.
+ *   weights[rows[b], h, j] += sum over the tokens i of sequence b that see key j and the query
+ *   heads of kv head h of exp(softmax_scale * q_i . k_j - lse_i)
+ * for the keys j < min(len_b, row_len).  q [total_q, num_q_heads, head_dim], q_indptr, the page
+ * table and causal are those of an attention call, lse (contiguous fp32 [total_q, num_q_heads]) what
+ * it returned; rows of q with lse -inf count nothing.
+ *   weights: fp32 [num_rows, num_kv_heads, row_len], strides weight_stride[0..1], unit in the last.
+ *   rows: int32 [batch], the row of each sequence (NULL: b); no row may be named twice, and a
+ *   sequence whose row is outside [0, num_rows) is left out.
+ *   window: only the last `window` tokens of each sequence count.
+ * Keys on pages outside the pool are skipped.  head_dim: 64, 128 or 256; dtype AKT_DTYPE_F16 or
+ * AKT_DTYPE_BF16 (q and the cache).
+ */
+int akt_attention_weights_paged(
+    const void* q, const int32_t* q_indptr, const float* lse, const void* kv_cache,
+    const int32_t* kv_page_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len,
+    float* weights, const int32_t* rows, int64_t batch, int64_t total_q, int64_t num_q_heads,
+    int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t total_pages,
+    int64_t num_pool_pages, int64_t num_rows, int64_t row_len, const int64_t q_stride[3],
+    const int64_t kv_stride[5], const int64_t weight_stride[2], float softmax_scale, int causal,
+    int64_t window, int dtype, void* stream);
+
+/*
+ * Kept tokens close up within a cache, in place.  For each (sequence b, kv head h) and j <
+ * min(sparse_nnz[b, h], keep, len_b): slot j takes K and V of token sparse_ind[b, h, j], which must
+ * be at or behind slot j and before len_b (other entries are skipped: their slots stay).
+ *   sparse_ind: contiguous int32 [batch, num_kv_heads, keep]; sparse_nnz: [batch, num_kv_heads].
+ *   dst_page_indices: NULL, or int32 [total_pages] in the place of kv_page_indices for the slots
+ *   written; where the two differ the page must be in no sequence of the call.
+ *   weights: NULL, or sums as in akt_attention_weights_paged, which move along; those of slots from
+ *   the count on, up to len_b, become 0.
+ * No page may be written for two sequences, nor written for one and read for another.  The cache
+ * is moved as 16-bit words; head_dim a multiple of 8 up to 1024.
+ */
+int akt_paged_keep(void* kv_cache, const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+                   const int32_t* kv_last_page_len, const int32_t* dst_page_indices,
+                   const int32_t* sparse_ind, const int32_t* sparse_nnz, float* weights,
+                   const int32_t* rows, int64_t batch, int64_t num_kv_heads, int64_t head_dim,
+                   int64_t page_size, int64_t total_pages, int64_t num_pool_pages, int64_t keep,
+                   int64_t num_rows, int64_t row_len, const int64_t kv_stride[5],
+                   const int64_t weight_stride[2], void* stream);
+
+/*
+ * The heaviest entries of rows of sums, as kept-token lists.  For each (sequence b, head h), of
+ * the first len = min(lengths[b], row_len) entries of weights[rows[b], h]: the first `first`, the
+ * last `recent` and the heaviest of the others, `keep` in all (all len where there are no more),
+ * ascending in sparse_ind [batch, num_heads, keep], -1 behind them; their number in sparse_nnz
+ * [batch, num_heads].  Of equal sums the lower index is kept; NaN counts as the heaviest.
+ * weights, num_rows, row_len, weight_stride and rows as in akt_attention_weights_paged (a row may
+ * be named twice here; a sequence whose row is outside [0, num_rows) keeps nothing).
+ */
+int akt_kept_index_heaviest(const float* weights, const int32_t* lengths, const int32_t* rows,
+                            int32_t* sparse_ind, int32_t* sparse_nnz, int64_t batch,
+                            int64_t num_heads, int64_t num_rows, int64_t row_len,
+                            const int64_t weight_stride[2], int64_t keep, int64_t first,
+                            int64_t recent, void* stream);
 
 /*
  * Kept-token index selection (the reference harness step at
