@@ -72,6 +72,9 @@ _SIGNATURES = {
                                              _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64x,
                                              _i64x, _i64x, _i64x, C.c_int, C.c_float, C.c_int,
                                              _p]),
+    "akt_paged_kv_append_rotary_at": (C.c_int, [_p] * 11 + [_i64] * 9 +
+                                      [_i64x, _i64x, _i64x, _i64x, C.c_int, C.c_float, C.c_int,
+                                       _p]),
     "akt_paged_copy": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64x, _p]),
     "akt_shared_prefix_paged_workspace_size": (C.c_size_t, [_i64] * 9),
     "akt_shared_prefix_paged_fwd": (C.c_int, [_p] * 12 + [_i64] * 10 +

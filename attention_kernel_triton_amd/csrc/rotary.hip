@@ -228,6 +228,7 @@ struct AppendRotaryParams {
   const int32_t* indices;
   const int32_t* last_len;
   const double* inv_freq;
+  const int32_t* offset;  // added to the positions of each sequence; may be null
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
   int64_t sp, skv, sh, ss;
   int total;
@@ -237,7 +238,8 @@ struct AppendRotaryParams {
 };
 
 struct Place {
-  int pos;         // -1: the token belongs to no sequence
+  int pos;         // place in its sequence, -1: the token belongs to no sequence
+  int64_t at;      // position that it is rotated by
   int page, slot;  // page -1: not stored
 };
 // Sequence, position, page and slot of token tok, wave-uniform.  Page table entries outside
@@ -249,7 +251,7 @@ __device__ __forceinline__ Place place_of(const AppendRotaryParams& p, int tok, 
     const int aj = j < p.B ? p.append_indptr[j] : INT32_MAX;
     cnt += __popcll(__ballot(aj <= tok));
   }
-  Place r = {-1, -1, 0};
+  Place r = {-1, 0, -1, 0};
   const int b = uniform(cnt) - 1;
   if (b < 0) return r;
   const int a0 = p.append_indptr[b], a1 = p.append_indptr[b + 1];
@@ -260,6 +262,7 @@ __device__ __forceinline__ Place place_of(const AppendRotaryParams& p, int tok, 
   const int64_t pos = (int64_t)len - ((int64_t)a1 - tok);
   if (tok < a0 || tok >= a1 || np <= 0 || pos < 0) return r;
   r.pos = (int)pos;
+  r.at = pos + (p.offset ? p.offset[b] : 0);
   const int lp = (int)((uint32_t)r.pos / (uint32_t)p.page_size);
   r.slot = r.pos - lp * p.page_size;
   const int pg = p.indices[ip0 + lp];
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(kRThreads) void append_rotary_kernel(AppendRotaryPa
   if (turned) {
 #pragma unroll
     for (int f = 0; f < 8; ++f)
-      turn_of(p.inv_freq[8 * col + f] * kTurn, (double)pl.pos, p.factor, cs[f], sn[f]);
+      turn_of(p.inv_freq[8 * col + f] * kTurn, (double)pl.at, p.factor, cs[f], sn[f]);
   }
   for (int h0 = 0;;) {
 #pragma unroll
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(kRThreads) void append_rotary_gen_kernel(AppendRota
   if (lane >= cw * hpw) return;
   for (int col = lane % cw; col < cpr; col += cw) {
     Gen8 g;
-    gen_plan(g, col, p.rot, p.inter, p.inv_freq, (double)pl.pos, p.factor);
+    gen_plan(g, col, p.rot, p.inter, p.inv_freq, (double)pl.at, p.factor);
     for (int h = lane / cw; h < heads; h += hpw) {
       const half_t* src = row_src(p, tok, h);
       const uint4_t x = h < rotated ? gen_apply<BF16>(g, src, col) : ld16(src + 8 * col);
@@ -467,10 +470,11 @@ extern "C" int akt_rotary_fwd(const void* q, const void* k, void* q_out, void* k
   return check_launch("rotary_dense_kernel");
 }
 
-extern "C" int akt_paged_kv_append_rotary(
+extern "C" int akt_paged_kv_append_rotary_at(
     const void* q, const void* k_new, const void* v_new, void* q_out, const int32_t* append_indptr,
     void* kv_cache, const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
-    const int32_t* kv_last_page_len, const double* inv_freq, int64_t batch, int64_t total_new,
+    const int32_t* kv_last_page_len, const int32_t* position_offset, const double* inv_freq,
+    int64_t batch, int64_t total_new,
     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim,
     int64_t page_size, int64_t total_pages, int64_t num_pool_pages, const int64_t q_stride[3],
     const int64_t k_new_stride[3], const int64_t v_new_stride[3], const int64_t kv_stride[5],
@@ -508,6 +512,7 @@ extern "C" int akt_paged_kv_append_rotary(
   p.indices = kv_page_indices;
   p.last_len = kv_last_page_len;
   p.inv_freq = inv_freq;
+  p.offset = position_offset;
   p.q_st = q_stride[0]; p.q_sh = q_stride[1];
   p.k_st = k_new_stride[0]; p.k_sh = k_new_stride[1];
   p.v_st = v_new_stride[0]; p.v_sh = v_new_stride[1];
@@ -541,4 +546,19 @@ extern "C" int akt_paged_kv_append_rotary(
     else timer.launch(append_rotary_kernel<false, false>, grid, blk, 0, st, p);
   }
   return check_launch("append_rotary_kernel");
+}
+
+extern "C" int akt_paged_kv_append_rotary(
+    const void* q, const void* k_new, const void* v_new, void* q_out, const int32_t* append_indptr,
+    void* kv_cache, const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+    const int32_t* kv_last_page_len, const double* inv_freq, int64_t batch, int64_t total_new,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim,
+    int64_t page_size, int64_t total_pages, int64_t num_pool_pages, const int64_t q_stride[3],
+    const int64_t k_new_stride[3], const int64_t v_new_stride[3], const int64_t kv_stride[5],
+    int interleaved, float factor, int dtype, void* stream) {
+  return akt_paged_kv_append_rotary_at(
+      q, k_new, v_new, q_out, append_indptr, kv_cache, kv_page_indptr, kv_page_indices,
+      kv_last_page_len, nullptr, inv_freq, batch, total_new, num_q_heads, num_kv_heads, head_dim,
+      rotary_dim, page_size, total_pages, num_pool_pages, q_stride, k_new_stride, v_new_stride,
+      kv_stride, interleaved, factor, dtype, stream);
 }

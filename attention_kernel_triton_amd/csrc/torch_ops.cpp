@@ -793,7 +793,8 @@ at::Tensor append_paged_kv_rotary(const at::Tensor& q_, const at::Tensor& k_new_
                                   const at::Tensor& v_new_, const at::Tensor& append_indptr,
                                   const at::Tensor& pool, const at::Tensor& indptr_,
                                   const at::Tensor& indices_, const at::Tensor& last_,
-                                  const at::Tensor& inv_freq_, bool interleaved, double factor) {
+                                  const at::Tensor& inv_freq_, bool interleaved, double factor,
+                                  const c10::optional<at::Tensor>& position_offset) {
   need_gpu("paged_kv_cache", pool);
   const int dtype = check_written_pool(pool);
   const at::Device dev = pool.device();
@@ -820,14 +821,21 @@ at::Tensor append_paged_kv_rotary(const at::Tensor& q_, const at::Tensor& k_new_
   const int64_t B = last.numel();
   if (ap.numel() != B + 1 || indptr.numel() != B + 1)
     throw py::value_error("append_indptr and kv_page_indptr must have B+1 and kv_last_page_len B entries");
+  at::Tensor offset;
+  if (position_offset.has_value() && position_offset->defined()) {
+    offset = int32_on("position_offset", *position_offset, dev).contiguous();
+    if (offset.dim() != 1 || offset.numel() != B)
+      throw py::value_error("position_offset must have " + std::to_string(B) + " entries, got " +
+                            std::to_string(offset.numel()));
+  }
   const DeviceGuard guard(dev);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   const Strides qs = strides_of(q), ks = strides_of(k_new), vs = strides_of(v_new),
                 ps = strides_of(pool);
-  check_rc(akt_paged_kv_append_rotary(
+  check_rc(akt_paged_kv_append_rotary_at(
                ptr(q), ptr(k_new), ptr(v_new), ptr(out), (const int32_t*)ptr(ap), ptr(pool),
                (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices), (const int32_t*)ptr(last),
-               (const double*)ptr(inv_freq), B, q.size(0), q.size(1), Hkv, D, 2 * inv_freq.numel(),
+               (const int32_t*)ptr(offset), (const double*)ptr(inv_freq), B, q.size(0), q.size(1), Hkv, D, 2 * inv_freq.numel(),
                page, indices.numel(), P, qs.v, ks.v, vs.v, ps.v, interleaved ? 1 : 0, (float)factor,
                dtype, stream_of(pool)),
            "akt_paged_kv_append_rotary");
@@ -1006,7 +1014,8 @@ PYBIND11_MODULE(_akt_torch, m) {
   m.def("append_paged_kv_rotary", &append_paged_kv_rotary, py::arg("q"), py::arg("k_new"),
         py::arg("v_new"), py::arg("append_indptr"), py::arg("paged_kv_cache"),
         py::arg("kv_page_indptr"), py::arg("kv_page_indices"), py::arg("kv_last_page_len"),
-        py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("factor") = 1.0);
+        py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("factor") = 1.0,
+        py::arg("position_offset") = py::none());
   m.def("copy_pages", &copy_pages, py::arg("paged_kv_cache"), py::arg("src"), py::arg("dst"),
         py::arg("num_tokens") = py::none());
   m.def("merge_states", &merge_states, py::arg("o"), py::arg("lse"), py::arg("out_f32"));

@@ -18,8 +18,9 @@ This module fills them:
   sequence's page list as tokens are appended (prefill chunks or one token
   per decode step), and hands out the page table the decode entry points
   take.  Sequences may share pages (``fork``); a shared page that is about
-  to be written is copied first.  Page bookkeeping is host-side; only the copies
-  and the attention run on the GPU.
+  to be written is copied first.  Sequences that grow too long can be cut down to the
+  tokens that draw attention (``evict``).  Page bookkeeping is host-side; only the copies,
+  the selections and the attention run on the GPU.
 """
 from __future__ import annotations
 
@@ -27,6 +28,8 @@ import torch
 
 from . import _native as N
 from . import _ops
+from .attention_weights_paged import accumulate_attention_weights_paged
+from .kept_index import select_heaviest
 
 
 def append_paged_kv(k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
@@ -43,17 +46,19 @@ def append_paged_kv(k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
 
 def append_paged_kv_rotary(q, k_new, v_new, append_indptr, paged_kv_cache, kv_page_indptr,
                            kv_page_indices, kv_last_page_len, inv_freq, interleaved=False,
-                           factor=1.0):
+                           factor=1.0, position_offset=None):
     """append_paged_kv of k_new rotated by its positions; returns q rotated by the same ones.
 
     q [total_new, Hq, D] has a row for every row of k_new / v_new [total_new, Hkv, D].  A row's
-    position is the one it takes in its sequence; inv_freq (float64 [rotary_dim / 2]),
+    position is the one it takes in its sequence, plus position_offset[b] (int32 [B]) where given:
+    the tokens that sequence b has lost (keep_tokens).  inv_freq (float64 [rotary_dim / 2]),
     interleaved and factor as in rotary.apply_rotary.  fp16 or bf16, one type.  Rows of q that
     belong to no sequence are left unwritten.
     """
     return N.torch_ext().append_paged_kv_rotary(q, k_new, v_new, append_indptr, paged_kv_cache,
                                                 kv_page_indptr, kv_page_indices, kv_last_page_len,
-                                                inv_freq, interleaved=interleaved, factor=factor)
+                                                inv_freq, interleaved=interleaved, factor=factor,
+                                                position_offset=position_offset)
 
 
 def copy_pages(paged_kv_cache, src, dst, num_tokens=None) -> None:
@@ -95,13 +100,17 @@ class PagedKVCache:
     >>> indptr, indices, last = cache.page_table([7, 9])
     >>> cache.fork(7, 8)                            # 8 continues 7's tokens, sharing its pages
     >>> o = cache.extend([7, 8], q, k, v, [4, 1], inv_freq=inv_freq)  # rotate, append, attend
+    >>> cache.evict([7], keep=256, first=4, recent=64)  # with weight_rows: drop what draws little
 
-    A page table describes the cache as it is: append, extend, fork, truncate,
+    With weight_rows, `weights` [weight_rows, Hkv, weight_len] keeps for as many sequences the
+    attention that each token has drawn from the steps so far (extend), by which evict chooses.
+
+    A page table describes the cache as it is: append, extend, fork, truncate, evict,
     release and compact make the tables handed out before them stale.
     """
 
     def __init__(self, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
-                 device="cuda", dtype=torch.float16):
+                 device="cuda", dtype=torch.float16, weight_rows: int = 0, weight_len: int = 0):
         self.page_size = page_size
         self.pool = torch.zeros((num_pages, 2, num_kv_heads, page_size, head_dim), dtype=dtype,
                                 device=device)
@@ -109,6 +118,14 @@ class PagedKVCache:
         self._pages: dict = {}
         self._len: dict = {}
         self._refs = [0] * num_pages  # sequences that hold each page
+        self._dropped: dict = {}  # tokens that evict took from each sequence
+        # Sums of attention weight; those behind a sequence's last token are 0.
+        self.weights = None
+        if weight_rows:
+            self.weights = torch.zeros((weight_rows, num_kv_heads, weight_len),
+                                       dtype=torch.float32, device=device)
+        self._free_rows = list(range(weight_rows - 1, -1, -1))
+        self._rows: dict = {}  # each sequence's row of the sums, once it has any
 
     @property
     def free_pages(self) -> int:
@@ -116,6 +133,10 @@ class PagedKVCache:
 
     def seq_len(self, seq_id) -> int:
         return self._len.get(seq_id, 0)
+
+    def next_position(self, seq_id) -> int:
+        """Position of the sequence's next token: its length and what evict took from it."""
+        return self._len.get(seq_id, 0) + self._dropped.get(seq_id, 0)
 
     def _drop(self, pages) -> None:
         for page in pages:
@@ -127,6 +148,9 @@ class PagedKVCache:
         """Drop a sequence; pages that no other sequence holds return to the free list."""
         self._drop(reversed(self._pages.pop(seq_id, [])))
         self._len.pop(seq_id, None)
+        self._dropped.pop(seq_id, None)
+        if seq_id in self._rows:
+            self._free_rows.append(self._rows.pop(seq_id))
 
     def truncate(self, seq_id, length: int) -> None:
         """Forget a sequence's tokens from position `length` on (rejected drafts, say)."""
@@ -138,6 +162,10 @@ class PagedKVCache:
         pages = self._pages[seq_id]
         self._drop(reversed(pages[keep:]))
         del pages[keep:]
+        if seq_id in self._rows and length < self._len[seq_id]:
+            self.weights[self._rows[seq_id], :, length:self._len[seq_id]].zero_()
+        if length == 0:
+            self._dropped.pop(seq_id, None)  # positions begin anew
         self._len[seq_id] = length
 
     def fork(self, seq_id, new_id) -> None:
@@ -147,6 +175,13 @@ class PagedKVCache:
             raise KeyError(f"no sequence {seq_id!r}")
         if new_id in self._pages:
             raise ValueError(f"sequence {new_id!r} exists")
+        if seq_id in self._rows:
+            row, n = self._take_row(), self._len[seq_id]
+            self.weights[row].zero_()
+            self.weights[row, :, :n] = self.weights[self._rows[seq_id], :, :n]
+            self._rows[new_id] = row
+        if seq_id in self._dropped:
+            self._dropped[new_id] = self._dropped[seq_id]
         for page in self._pages[seq_id]:
             self._refs[page] += 1
         self._pages[new_id] = list(self._pages[seq_id])
@@ -212,24 +247,88 @@ class PagedKVCache:
                 pages.append(page)
             self._len[s] = length
 
-    def page_table(self, seq_ids):
-        """(kv_page_indptr, kv_page_indices, kv_last_page_len) int32 device tensors."""
+    def _ints(self, v):
+        return torch.tensor(v, dtype=torch.int32, device=self.pool.device)
+
+    def _table(self, held):
+        """Page table of (pages, tokens) pairs."""
         indptr, indices, last = [0], [], []
-        for s in seq_ids:
-            pages = self._pages.get(s, [])
+        for pages, n in held:
             indices.extend(pages)
             indptr.append(len(indices))
-            n = self._len.get(s, 0)
             last.append(0 if n == 0 else (n - 1) % self.page_size + 1)
-        dev = self.pool.device
-        mk = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
-        return mk(indptr), mk(indices), mk(last)
+        return self._ints(indptr), self._ints(indices), self._ints(last)
+
+    def page_table(self, seq_ids):
+        """(kv_page_indptr, kv_page_indices, kv_last_page_len) int32 device tensors."""
+        return self._table([(self._pages.get(s, []), self._len.get(s, 0)) for s in seq_ids])
+
+    def _groups(self, seq_ids, counts):
+        """Neighbours that share leading pages: [first, end, pages shared] of each group.
+
+        A page counts as shared where it holds no new token of either.  A sequence joins the group before
+        it unless that would save less than the group saves without it."""
+        room = [max(self._len.get(s, 0) - int(n), 0) // self.page_size
+                for s, n in zip(seq_ids, counts)]
+        groups = []
+        for i, s in enumerate(seq_ids):
+            pages = self._pages.get(s, [])
+            if groups and groups[-1][1] == i:
+                a, end, held = groups[-1]
+                other = self._pages.get(seq_ids[a], [])
+                lo, hi = 0, min(held if end - a > 1 else room[a], room[i])
+                if pages[:hi] == other[:hi]:
+                    lo = hi
+                while lo < hi:  # pages[:lo] are shared, pages[:hi + 1] are not
+                    mid = (lo + hi + 1) // 2
+                    if pages[lo:mid] == other[lo:mid]:
+                        lo = mid
+                    else:
+                        hi = mid - 1
+                if lo and lo * (end - a) >= held * (end - a - 1):
+                    groups[-1] = [a, i + 1, lo]
+                    continue
+            groups.append([i, i + 1, 0])
+        return groups
+
+    def split_table(self, seq_ids, counts=None):
+        """(kv_page_indptr, kv_page_indices, kv_last_page_len, group_indptr, prefix_page_indptr,
+        prefix_page_indices, prefix_last_page_len) as flash_attention_shared_prefix_paged takes them.
+
+        Neighbours in seq_ids that share leading pages form groups; the last counts[i] tokens of each
+        sequence (default: one) are its queries and stay out of the prefixes."""
+        counts = [1] * len(seq_ids) if counts is None else counts
+        group, prefixes, own = [0], [], []
+        for a, end, held in self._groups(seq_ids, counts):
+            group.append(end)
+            prefixes.append((self._pages.get(seq_ids[a], [])[:held], held * self.page_size))
+            for s in seq_ids[a:end]:
+                own.append((self._pages.get(s, [])[held:],
+                            self._len.get(s, 0) - held * self.page_size))
+        prefix = self._table(prefixes)
+        return (*self._table(own), self._ints(group), *prefix)
+
+    def _take_row(self) -> int:
+        if not self._free_rows:
+            raise MemoryError(f"all {self.weights.shape[0]} rows of weights are taken")
+        return self._free_rows.pop()
+
+    def _row_table(self, seq_ids):
+        """The sequences' rows of the sums, int32; those that have none get one, all or none."""
+        new = [s for s in dict.fromkeys(seq_ids) if s not in self._rows]
+        if len(new) > len(self._free_rows):
+            raise MemoryError(f"all {self.weights.shape[0]} rows of weights are taken")
+        for s in new:
+            row = self._take_row()
+            self.weights[row].zero_()
+            self._rows[s] = row
+        return self._ints([self._rows[s] for s in seq_ids])
 
     def _indptr(self, counts):
         ap = [0]
         for n in counts:
             ap.append(ap[-1] + int(n))
-        return torch.tensor(ap, dtype=torch.int32, device=self.pool.device)
+        return self._ints(ap)
 
     def _restore(self, before) -> None:
         """Gives sequences back the lengths (None: no sequence) that they had."""
@@ -260,33 +359,110 @@ class PagedKVCache:
         return indptr, indices, last
 
     def extend(self, seq_ids, q, k_new, v_new, counts, inv_freq=None, interleaved=False,
-               factor=1.0, causal=True, softmax_scale=None, return_lse=False):
+               factor=1.0, causal=True, softmax_scale=None, return_lse=False,
+               shared_prefix=False, observe=None):
         """One attention step: append counts[i] tokens to seq_ids[i] and attend with them.
 
         q [sum(counts), Hq, D], k_new and v_new [sum(counts), Hkv, D]; with inv_freq, q and k_new
         are rotated by the tokens' positions first (append_paged_kv_rotary).  Returns what
         flash_attention_chunk_paged returns for q over the grown cache.  A call that is refused
         leaves the sequences with the tokens they had.
+        shared_prefix: leading pages that neighbours in seq_ids share (fork) are read once for all
+        of them (flash_attention_shared_prefix_paged).
+        observe: where the cache keeps sums of attention weight, the last `observe` of each
+        sequence's new tokens add theirs (default: all; 0: none).  A whole prompt's cost is about half its
+        attention again.
         """
+        watch = self.weights is not None and observe != 0
+        if observe is not None and observe < 0:
+            raise ValueError("observe must be non-negative")
         total = sum(int(n) for n in counts)
         for name, x in (("q", q), ("k_new", k_new), ("v_new", v_new)):
             if x.shape[0] != total:
                 raise ValueError(f"{name} has {x.shape[0]} rows, the counts make {total}")
-        before = {s: self._len.get(s) for s in seq_ids}
+        before, rows_before = {s: self._len.get(s) for s in seq_ids}, set(self._rows)
         self._grow(seq_ids, counts)
         try:
+            rows = self._row_table(seq_ids) if watch else None
             table = self.page_table(seq_ids)
             q_indptr = self._indptr(counts)
             if inv_freq is None:
                 append_paged_kv(k_new, v_new, q_indptr, self.pool, *table)
             else:
+                lost = [self._dropped.get(s, 0) for s in seq_ids]
+                at = {"position_offset": self._ints(lost)} if any(lost) else {}
                 q = append_paged_kv_rotary(q, k_new, v_new, q_indptr, self.pool, *table, inv_freq,
-                                           interleaved=interleaved, factor=factor)
-            return _ops.chunk_paged(q, q_indptr, self.pool, *table, causal=causal,
-                                    softmax_scale=softmax_scale, return_lse=return_lse)
+                                           interleaved=interleaved, factor=factor, **at)
+            kw = dict(causal=causal, softmax_scale=softmax_scale, return_lse=return_lse or watch)
+            if shared_prefix:
+                own = self.split_table(seq_ids, counts)
+                out = _ops.shared_prefix_paged(q, q_indptr, self.pool, *own, **kw)
+            else:
+                out = _ops.chunk_paged(q, q_indptr, self.pool, *table, **kw)
+            if watch:
+                accumulate_attention_weights_paged(self.weights, q, q_indptr, out[1], self.pool,
+                                                   *table, rows=rows, causal=causal,
+                                                   softmax_scale=softmax_scale, window=observe)
+            return out if return_lse or not watch else out[0]
         except BaseException:
+            for s in seq_ids:
+                if s in self._rows and s not in rows_before:
+                    self._free_rows.append(self._rows.pop(s))
             self._restore(before)
             raise
+
+    def evict(self, seq_ids, keep: int, first: int = 0, recent: int = 0) -> int:
+        """Cut sequences of more than `keep` tokens down to so many; returns the tokens dropped.
+
+        Each kv head keeps the first `first` tokens, the last `recent`, and of the others those that
+        drew most attention (select_heaviest over the cache's sums), in their order; K, V and sums
+        move to the front of the sequence's pages, and the pages behind return to the free list.
+        New tokens keep counting positions from the tokens there were (next_position).  Shared pages are
+        left to the other sequences: the kept tokens go into free ones.  A call that is refused
+        changes nothing.
+        """
+        if self.weights is None:
+            raise ValueError("the cache keeps no sums of attention weight (weight_rows)")
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise ValueError("keep must be positive and at least first + recent")
+        seqs = [s for s in dict.fromkeys(seq_ids) if self.seq_len(s) > keep]
+        if not seqs:
+            return 0
+        for s in seqs:
+            if self._len[s] > self.weights.shape[2]:
+                raise ValueError(f"sequence {s!r} has {self._len[s]} tokens, the sums hold "
+                                 f"{self.weights.shape[2]}")
+        held = -(-keep // self.page_size)  # pages of a sequence afterwards
+        shared = [(s, i) for s in seqs for i in range(held) if self._refs[self._pages[s][i]] > 1]
+        if len(shared) > len(self._free):
+            raise MemoryError(f"page pool exhausted: need {len(shared)} pages, "
+                              f"{len(self._free)} free")
+        fresh = dict(zip(shared, self._free[len(self._free) - len(shared):][::-1]))
+        rows = self._row_table(seqs)
+        table = self.page_table(seqs)
+        dst = None
+        if fresh:
+            dst = self._ints([fresh.get((s, i), p) for s in seqs
+                              for i, p in enumerate(self._pages[s])])
+        ind, nnz = select_heaviest(self.weights, self._ints([self._len[s] for s in seqs]), keep,
+                                   first=first, recent=recent, rows=rows)
+        keep_tokens(self.pool, *table, ind, nnz, dst_page_indices=dst, weights=self.weights,
+                    rows=rows)
+        del self._free[len(self._free) - len(shared):]
+        dropped = 0
+        for s in seqs:
+            pages = self._pages[s]
+            self._drop(reversed(pages[held:]))
+            for i in range(held):
+                if (s, i) in fresh:
+                    self._drop([pages[i]])
+                    pages[i] = fresh[s, i]
+                    self._refs[pages[i]] = 1
+            del pages[held:]
+            dropped += self._len[s] - keep
+            self._dropped[s] = self._dropped.get(s, 0) + self._len[s] - keep
+            self._len[s] = keep
+        return dropped
 
 
 __all__ = ["append_paged_kv", "append_paged_kv_rotary", "copy_pages", "keep_tokens",

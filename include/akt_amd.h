@@ -439,6 +439,19 @@ int akt_paged_kv_append_rotary(const void* q, const void* k_new, const void* v_n
                                int interleaved, float factor, int dtype, void* stream);
 
 /*
+ * akt_paged_kv_append_rotary for sequences that have lost tokens: position_offset[b] (int32
+ * [batch]; NULL: 0) is added to the positions of sequence b's tokens.
+ */
+int akt_paged_kv_append_rotary_at(
+    const void* q, const void* k_new, const void* v_new, void* q_out, const int32_t* append_indptr,
+    void* kv_cache, const int32_t* kv_page_indptr, const int32_t* kv_page_indices,
+    const int32_t* kv_last_page_len, const int32_t* position_offset, const double* inv_freq,
+    int64_t batch, int64_t total_new, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+    int64_t rotary_dim, int64_t page_size, int64_t total_pages, int64_t num_pool_pages,
+    const int64_t q_stride[3], const int64_t k_new_stride[3], const int64_t v_new_stride[3],
+    const int64_t kv_stride[5], int interleaved, float factor, int dtype, void* stream);
+
+/*
  * Copies the first num_tokens[i] slots (NULL: all page_size; clamped to [0, page_size]) of
  * page src[i] to page dst[i], K and V of every head, for i < n.  A pair with a page outside
  * [0, num_pool_pages), or the same page twice, is skipped.  All copies of a call run at
