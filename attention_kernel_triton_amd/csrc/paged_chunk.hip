@@ -114,7 +114,8 @@ struct Seq {
 template <>
 struct Seq<true> {
   int q0, n, ip0, len;
-  int prefix;
+  int prefix;  // a group and its prefix
+  int more;    // a sequence of a group: its rows have a prefix's state too
 };
 template <typename S>
 __device__ __forceinline__ int is_prefix(const S& s) {
@@ -125,13 +126,24 @@ template <bool SHARED>
 __device__ __forceinline__ int num_seqs(const ChunkParams& p) {
   return SHARED ? p.B + p.groups : p.B;
 }
+// With shared prefixes a workgroup keeps the sequences' places in LDS, unless there are too many.
+constexpr int kCkTable = 1024;
+__device__ __forceinline__ bool in_table(const ChunkParams& p) {
+  return p.B + p.groups <= kCkTable;
+}
 // Table entries outside their ranges are taken clamped, so nothing outside the arrays is
 // touched.
 template <bool SHARED>
-__device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b) {
+__device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b,
+                                                const int4* table = nullptr) {
   Seq<SHARED> s;
   if constexpr (SHARED) {
     s.prefix = b >= p.B;
+    if (table) {
+      const int4 t = table[b];
+      return Seq<SHARED>{t.x, t.y & 0x3fffffff, t.z, t.w, s.prefix, t.y >> 30};
+    }
+    s.more = !s.prefix && p.groups > 0 && b >= p.group_indptr[0] && b < p.group_indptr[p.groups];
     if (s.prefix) {
       const int i = b - p.B;
       const int b0 = min(max(p.group_indptr[i], 0), p.B);
@@ -153,10 +165,12 @@ __device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b) {
 }
 // The same for a wave-uniform b, in scalar registers.
 template <bool SHARED>
-__device__ __forceinline__ Seq<SHARED> load_seq_uniform(const ChunkParams& p, int b) {
-  const Seq<SHARED> s = load_seq<SHARED>(p, b);
+__device__ __forceinline__ Seq<SHARED> load_seq_uniform(const ChunkParams& p, int b,
+                                                        const int4* table) {
+  const Seq<SHARED> s = load_seq<SHARED>(p, b, table);
   if constexpr (SHARED)
-    return Seq<SHARED>{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len), uniform(s.prefix)};
+    return Seq<SHARED>{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len), uniform(s.prefix),
+                       uniform(s.more)};
   else
     return Seq<SHARED>{uniform(s.q0), uniform(s.n), uniform(s.ip0), uniform(s.len)};
 }
@@ -168,19 +182,23 @@ template <typename S>
 __device__ __forceinline__ bool is_causal(const ChunkParams& p, const S& s) {
   return p.causal && !is_prefix(s);
 }
+template <bool SHARED>
+__device__ __forceinline__ constexpr int unit_cost() {
+  return SHARED ? kSharedUnitCost : kCkUnitCost;
+}
 // Lengths on the axis.  Causal row block r sees min(n, (r + 1) TR) keys past the context;
 // the axis takes the context as at least 0 (a table with n > len breaks the contract).
 template <bool SHARED>
 __device__ __forceinline__ int64_t unit_start(const ChunkParams& p, const Seq<SHARED>& s, int64_t r) {
-  if (!is_causal(p, s)) return r * (s.len + kCkUnitCost);
-  return r * (max(s.len - s.n, 0) + kCkUnitCost) + p.TR * (r * (r + 1) / 2);
+  if (!is_causal(p, s)) return r * (s.len + unit_cost<SHARED>());
+  return r * (max(s.len - s.n, 0) + unit_cost<SHARED>()) + p.TR * (r * (r + 1) / 2);
 }
 template <bool SHARED>
 __device__ __forceinline__ int64_t head_length(const ChunkParams& p, const Seq<SHARED>& s) {
   const int64_t R = row_blocks(p, s.n);
   if (R == 0) return 0;
-  if (!is_causal(p, s)) return R * (s.len + kCkUnitCost);
-  return unit_start(p, s, R - 1) + max(s.len - s.n, 0) + s.n + kCkUnitCost;
+  if (!is_causal(p, s)) return R * (s.len + unit_cost<SHARED>());
+  return unit_start(p, s, R - 1) + max(s.len - s.n, 0) + s.n + unit_cost<SHARED>();
 }
 // n / page_size for 0 <= n < 2^31.
 __device__ __forceinline__ int page_of(const ChunkParams& p, int n) {
@@ -213,15 +231,39 @@ __device__ __forceinline__ const int32_t* page_ids(const ChunkParams& p, const U
   return u.prefix ? p.prefix_indices : p.indices;
 }
 
-// Where the state (m, l, exact l, whether a prefix's state goes with it) and the sums of P.V of
-// a row go that attends in two parts: row (token, query head) of the own keys' or the prefixes'.
+// Where a part of a unit leaves a row's state (m, l, exact l, tag) and its sums of P.V: a unit
+// that is one part in the row's place (at: token, query head) among the own keys' or the prefixes'
+// rows, a part of a cut one in its range's slot; the first part then leaves the ranges of the
+// unit's first and last part and the row's place in their slots instead.
+struct StateRow {
+  float4_t* ml;
+  float* o;
+  float tag;
+};
 __device__ __forceinline__ float4_t* state_ml(const ChunkParams& p, const Unit<true>& u) {
   return reinterpret_cast<float4_t*>(p.states) + (u.prefix ? (int64_t)p.total_q * p.Hq : 0);
 }
 template <int D>
-__device__ __forceinline__ float* state_o(const ChunkParams& p, const Unit<true>& u) {
-  const int64_t rows = (int64_t)p.total_q * p.Hq;
-  return reinterpret_cast<float*>(p.states + rows * 32) + (u.prefix ? rows * D : 0);
+__device__ __forceinline__ StateRow state_row(const ChunkParams& p, const Unit<true>& u, int64_t at,
+                                              bool whole, bool first, int range, int64_t start,
+                                              int64_t Lw, int block, bool many, int slot_rows,
+                                              int row) {
+  const int tag = u.more ? kStateMore : 0;
+  if (whole) {
+    const int64_t rows = (int64_t)p.total_q * p.Hq;
+    return StateRow{state_ml(p, u) + at,
+                    reinterpret_cast<float*>(p.states + rows * 32) + ((u.prefix ? rows : 0) + at) * D,
+                    __int_as_float(tag)};
+  }
+  const int last = (u.kend - 1) / block * block;
+  const int wf = div_range(start + block - 1, Lw), wl = div_range(start + last + block - 1, Lw);
+  if (first)
+    state_ml(p, u)[at] = float4_t{__int_as_float(wf), __int_as_float(wl), __int_as_float(row),
+                                  __int_as_float(tag | kStateCut | (many ? kStateMany : 0))};
+  char* const slot =
+      p.partials + (many ? p.many_partial : 0) + (2 * (int64_t)range + (range == wf ? 1 : 0)) * slot_rows * state_bytes(D);
+  return StateRow{reinterpret_cast<float4_t*>(slot) + row,
+                  reinterpret_cast<float*>(slot + slot_rows * 16) + (int64_t)row * D, 0.f};
 }
 
 // Scores of the keys that a row does not see become -inf: of the step's 32 those past its
@@ -311,7 +353,8 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit<
 // The units of the ranges of workgroup `block` of W, on the axis of the sequences of few tokens
 // (SPLIT) or of many.  lds: the workgroup's tile buffers.
 template <int D, bool BF16, bool GRP, bool LSE, bool SHARED, bool SPLIT>
-__device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int block, int W) {
+__device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, const int4* table,
+                                            int block, int W) {
   constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
@@ -347,7 +390,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   auto mine = [&](const Seq<SHARED>& s) { return s.n > 0 && (s.n <= p.split_tokens) == SPLIT; };
   auto seq_length = [&](int b) -> int64_t {
     if (b >= num_seqs<SHARED>(p)) return 0;
-    const Seq<SHARED> s = load_seq<SHARED>(p, b);
+    const Seq<SHARED> s = load_seq<SHARED>(p, b, table);
     return mine(s) ? head_length(p, s) * p.Hkv : 0;
   };
   auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
@@ -727,6 +770,21 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       add_not_finite<D, BF16, SHARED>(p, u, k0 + max(u.first + 1 - k0, 0) / kBN * kBN, k1, g, lim, oacc);
     float l_row = xor32_sum(l_part);
     float x_row = LSE ? xor32_sum(x_part) : 0.f;
+    if constexpr (SHARED) {
+      if (lrow >= rows) return;
+      const int64_t at = (int64_t)(u.q0 + ltok) * p.Hq + u.kvh * p.G + (lrow - ltok * p.G);
+      const StateRow to = state_row<D>(p, u, at, whole, k0 == 0, wg, Ustart, Lw, kCkBlock,
+                                       true, 32 * WAVES, lrow);
+      if (g == 0) *to.ml = float4_t{m_run, l_row, x_row, to.tag};
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          st16(to.o + 32 * n + 8 * k + 4 * g,
+               as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
+                                  oacc[n][4 * k + 3]}));
+      return;
+    }
     if (!whole) {
       constexpr int64_t kWaveB = chunk_wave_bytes(D), kSlotB = WAVES * kWaveB;
       const int kb_last = (u.kend - 1) / kCkBlock * kCkBlock;
@@ -786,22 +844,6 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
             for (int j = 0; j < 4; ++j) oacc[i / 4][4 * (i % 4) + j] += f * ov[k][i][j];
         }
       }
-    }
-    if constexpr (SHARED) {
-      if (lrow < rows) {
-        const int64_t at =
-            (int64_t)(u.q0 + ltok) * p.Hq + u.kvh * p.G + (lrow - ltok * p.G);
-        if (g == 0) state_ml(p, u)[at] = float4_t{m_run, l_row, x_row, (float)u.more};
-        float* const so = state_o<D>(p, u) + at * D + 4 * g;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            st16(so + 32 * n + 8 * k,
-                 as_uint4f(float4_t{oacc[n][4 * k], oacc[n][4 * k + 1], oacc[n][4 * k + 2],
-                                    oacc[n][4 * k + 3]}));
-      }
-      return;
     }
     // Output rows through LDS, so that every lane stores 16 contiguous bytes.
     const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
@@ -1099,17 +1141,8 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
         }
       }
     }
-    const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
-    if constexpr (SHARED) {
-      if (row < rows) {
-        if (kg == 0 && g == 0) state_ml(p, u)[at] = float4_t{m_run, l_row, x_row, (float)u.more};
-#pragma unroll
-        for (int i = 0; i < NQ; ++i)
-          st16(state_o<D>(p, u) + at * D + 8 * (NQ * kg + i) + 4 * g, as_uint4f(acc[i]));
-      }
-      return;
-    }
     const float inv = l_row == 0.f ? 0.f : __builtin_amdgcn_rcpf(l_row);
+    const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
     if (LSE && kg == 0 && g == 0 && row < rows)
       p.lse[at] = l_row == 0.f ? AKT_C_NEG_INF : (m_run + __log2f(x_row)) * kLn2;
     // The lane halves hold 8-byte halves of a row's 16-byte chunks: half 0 takes chunk i
@@ -1175,7 +1208,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       len = seq_length(jb + lane0);
       inc = scan64(len);
     }
-    Seq<SHARED> s = load_seq_uniform<SHARED>(p, b);
+    Seq<SHARED> s = load_seq_uniform<SHARED>(p, b, table);
     int64_t hlen = uniform64(head_length(p, s));
     int kvh = div_range(x - U, hlen);
     int64_t hs = uniform64(U + kvh * hlen);  // the head's start
@@ -1202,8 +1235,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       u.ip0 = uniform(s.ip0);
       if constexpr (SHARED) {
         u.prefix = uniform(s.prefix);
-        u.more = uniform(!s.prefix && p.groups > 0 && b >= p.group_indptr[0] &&
-                         b < p.group_indptr[p.groups]);
+        u.more = uniform(s.more);
       }
       const int64_t us = uniform64(hs + unit_start(p, s, r));
       // Blocks from the first at or past x - us - (kCkBlock - 1) on are those of the ranges
@@ -1224,7 +1256,9 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
             const int tok = (int)((uint32_t)row * p.g_magic >> 16);
             const int64_t at = (int64_t)(u.q0 + tok) * p.Hq + u.kvh * p.G + (row - tok * p.G);
             if constexpr (SHARED) {
-              if (idx % CPR == 0) state_ml(p, u)[at] = float4_t{AKT_C_NEG_INF, 0.f, 0.f, (float)u.more};
+              if (idx % CPR == 0)
+                state_ml(p, u)[at] = float4_t{AKT_C_NEG_INF, 0.f, 0.f,
+                                              __int_as_float(u.more ? kStateMore : 0)};
               continue;
             }
             st16(p.o + at * D + idx % CPR * 8, uint4_t{0, 0, 0, 0});
@@ -1251,7 +1285,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
       kvh = 0;
       do {
         if (++b == num_seqs<SHARED>(p)) return;
-        s = load_seq_uniform<SHARED>(p, b);
+        s = load_seq_uniform<SHARED>(p, b, table);
       } while (!mine(s));
       R = uniform(row_blocks(p, s.n));
       hlen = uniform64(head_length(p, s));
@@ -1259,20 +1293,30 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, int
   }
 }
 
+#ifdef AKT_CHUNK_SHARED
+#include "paged_shared_few.hpp"
+#else
+template <int D, bool BF16>
+__device__ __forceinline__ void shared_few(const ChunkParams&, char*, const int4*, int, int) {}
+#endif
+
 // Workgroups (of all W, a multiple of 8) for the sequences of few tokens, where a launch may hold
 // both kinds: in proportion to the lengths of the two axes, a key of the other weighing 1 for a
 // unit of hardly any rows up to chunk_tile_cost for one of all rows.
 template <int D, bool SHARED>
-__device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
+__device__ __forceinline__ int split_share(const ChunkParams& p, const int4* table, int W) {
   constexpr int kRows = 32 * chunk_waves(D);
+  constexpr double kLow = SHARED ? kSharedTileCostLow : 1;
+  constexpr double kHigh = SHARED ? kSharedTileCost : chunk_tile_cost(D);
   const int lane = threadIdx.x & 63;
   double few = 0, many = 0;
   for (int b = lane; b < num_seqs<SHARED>(p); b += 64) {
-    const Seq<SHARED> s = load_seq<SHARED>(p, b);
-    const double len = (double)head_length(p, s);
+    const Seq<SHARED> s = load_seq<SHARED>(p, b, table);
+    const double len = (double)(SHARED && s.n <= p.split_tokens ? (s.n > 0 ? s.len + kWaveUnitCost : 0)
+                                                                : head_length(p, s));
     if (s.n <= p.split_tokens) few += len;
     else
-      many += len * (1 + (chunk_tile_cost(D) - 1) / kRows * min((double)s.n * p.G, (double)kRows));
+      many += len * (kLow + (kHigh - kLow) / kRows * min((double)s.n * p.G, (double)kRows));
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -1292,17 +1336,35 @@ void paged_chunk_kernel(ChunkParams p) {
   __shared__ __attribute__((aligned(16)))
   char lds[kCkNBuf * 2 * ck_tile_keys(D) * D * 2];
   const int block = blockIdx.x, W = gridDim.x;
+  const int4* table = nullptr;
+  if constexpr (SHARED) {
+    __shared__ int4 sm_table[kCkTable];
+    if (in_table(p)) {
+      for (int b = threadIdx.x; b < num_seqs<true>(p); b += 64 * chunk_waves(D)) {
+        const Seq<true> s = load_seq<true>(p, b);
+        sm_table[b] = int4{s.q0, s.n | s.more << 30, s.ip0, s.len};  // (n < 2^30)
+      }
+      __syncthreads();
+      table = sm_table;
+    }
+  }
   // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
   // of them in what follows.
   __shared__ int sm_share;
-  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D, SHARED>(p, W) : p.kinds == kCkFew ? W : 0;
+  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D, SHARED>(p, table, W) : p.kinds == kCkFew ? W : 0;
   if (threadIdx.x == 0) sm_share = share;
   __syncthreads();
   const int S = uniform(sm_share);
-  if (block < S)
-    chunk_range<D, BF16, GRP, LSE, SHARED, true>(p, lds, block, S);
+  if constexpr (SHARED) {
+    if (block < S) {
+      shared_few<D, BF16>(p, lds, table, block, S);
+      return;
+    }
+  }
+  if (!SHARED && block < S)
+    chunk_range<D, BF16, GRP, LSE, SHARED, true>(p, lds, table, block, S);
   else
-    chunk_range<D, BF16, GRP, LSE, SHARED, false>(p, lds, block - S, W - S);
+    chunk_range<D, BF16, GRP, LSE, SHARED, false>(p, lds, table, block - S, W - S);
 }
 
 // The instances of this translation unit: with or without shared prefixes.
@@ -1391,7 +1453,7 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   ChunkPlan c = {};
   // Sequences of up to chunk_split_rows rows to a kv head share out their keys.  How many tokens a
   // sequence has is known on the device alone, unless there is one, or all are few.
-  c.split_tokens = (int)(chunk_split_rows((int)D) / G);
+  c.split_tokens = (int)((shared ? 32 : chunk_split_rows((int)D)) / G);
   const bool few = total_q <= c.split_tokens;
   if (!few && batch == 1) c.split_tokens = 0;
   if (c.split_tokens > 0) c.kinds |= kCkFew;
@@ -1404,16 +1466,14 @@ ChunkPlan chunk_plan(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int
   // Two partial slots to a range, whichever kind a workgroup serves.
   if (c.kinds & kCkFew) {
     c.many_counter = c.wgs * waves;
-    c.many_partial = 2 * c.wgs * waves * chunk_split_wave_bytes((int)D);
+    c.many_partial = 2 * c.wgs * waves *
+                     (shared ? 32 * state_bytes((int)D) : chunk_split_wave_bytes((int)D));
   }
   c.counters = c.many_counter + (c.kinds & kCkMany ? c.wgs * waves : 0);
   c.partial_bytes =
       c.many_partial + (c.kinds & kCkMany ? 2 * c.wgs * waves * chunk_wave_bytes((int)D) : 0);
   return c;
 }
-
-// Bytes of the states of rows that attend in two parts.
-int64_t state_bytes(int64_t total_q, int64_t Hq, int64_t D) { return total_q * Hq * (32 + 8 * D); }
 
 bool sizes_served(int64_t Hq, int64_t Hkv, int64_t D) {
   return Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kCkRows &&
@@ -1481,7 +1541,7 @@ int chunk_call(const void* q, const int32_t* q_indptr, const void* kv_cache,
       chunk_plan(batch, total_q, num_kv_heads, G, head_dim, page_size, total_pages,
                  shared ? shared->groups : -1, shared ? shared->prefix_pages : 0);
   const size_t need =
-      workspace_bytes_of(plan, shared ? state_bytes(total_q, num_q_heads, head_dim) : 0);
+      workspace_bytes_of(plan, shared ? 2 * total_q * num_q_heads * state_bytes((int)head_dim) : 0);
   if (!workspace || workspace_bytes < need)
     return set_error(AKT_ERR_WORKSPACE, "chunk attention needs a workspace of %zu bytes, got %zu",
                      need, workspace ? workspace_bytes : (size_t)0);
@@ -1589,7 +1649,7 @@ extern "C" size_t akt_shared_prefix_paged_workspace_size(int64_t batch, int64_t 
     return 0;
   return workspace_bytes_of(chunk_plan(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads,
                                        head_dim, page_size, total_pages, groups, prefix_pages),
-                            state_bytes(total_q, num_q_heads, head_dim));
+                            2 * total_q * num_q_heads * state_bytes((int)head_dim));
 }
 
 extern "C" int akt_shared_prefix_paged_fwd(

@@ -19,10 +19,22 @@ constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
 // of 64 rows over 30000 takes 88 / 117, 16 over 500 to 4000 67 / 65.
 __host__ __device__ constexpr int chunk_split_rows(int D) { return D <= 128 ? 32 : 64; }
 constexpr int kCkFew = 1, kCkMany = 2;
+// With shared prefixes a wave serves a range of few rows alone: the grain of its cuts, the cost of
+// a unit's start and end in keys, and the fewest keys (with costs) of a range.
+constexpr int kCkWaveBlock = 64, kWaveUnitCost = 64, kCkWaveKeys = 192;
+constexpr int kSharedUnitCost = 320;  // and of a unit of many rows
 // A key of a unit of many rows costs a workgroup as much as so many of a unit of few (us at 1.4,
 // 2 and 3, 777 new tokens beside 15 single ones: D = 128 73.9 / 69.4 / 72.4, D = 256 77.6 / 83.6
 // / 97.8, D = 64 75.2 / 69.8 / 67.9; 2000 beside 7 after 3000 to 9000, D = 128 327 / 334 / 592).
 __host__ __device__ constexpr double chunk_tile_cost(int D) { return D <= 128 ? 2.0 : 1.4; }
+
+// The same with shared prefixes, by rows from hardly any to all.
+constexpr double kSharedTileCostLow = 1.5, kSharedTileCost = 2.0;
+// Bytes of a row's state: (m, l, exact l, tag) and fp32 sums of P.V.
+__host__ __device__ constexpr int64_t state_bytes(int D) { return 16 + 4 * D; }
+// Tags of a row's state: its sequence has a prefix; the state lies in the slots of several ranges,
+// which are of the second kind.
+constexpr int kStateMore = 1, kStateCut = 2, kStateMany = 4;
 
 struct ChunkParams {
   const half_t* q;     // [total_q, Hq, D] rows (strides q_st, q_sh)
@@ -60,7 +72,7 @@ struct ChunkParams {
   const int32_t* prefix_indices;
   const int32_t* prefix_last;
   int groups, prefix_pages;
-  // States of the rows, (m, l, exact l, -) and the sums of P.V, fp32: [2][total_q * Hq] rows of
+  // States of the rows, (m, l, exact l, tag) and the sums of P.V, fp32: [2][total_q * Hq] rows of
   // 16 bytes, then [2][total_q * Hq] of 4 D, own keys' first.
   char* states;
 };
