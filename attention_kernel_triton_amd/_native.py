@@ -80,8 +80,10 @@ _SIGNATURES = {
     "akt_shared_prefix_paged_fwd": (C.c_int, [_p] * 12 + [_i64] * 10 +
                                     [_i64x, _i64x, C.c_float, C.c_int, C.c_int, _p, C.c_size_t,
                                      _p]),
+    "akt_attention_weights_paged_workspace_size": (C.c_size_t, [_i64] * 7),
     "akt_attention_weights_paged": (C.c_int, [_p] * 9 + [_i64] * 10 +
-                                    [_i64x, _i64x, _i64x, C.c_float, C.c_int, _i64, C.c_int, _p]),
+                                    [_i64x, _i64x, _i64x, C.c_float, C.c_int, _i64, C.c_int, _p,
+                                     C.c_size_t, _p]),
     "akt_paged_keep": (C.c_int, [_p] * 9 + [_i64] * 9 + [_i64x, _i64x, _p]),
     "akt_kept_index_heaviest": (C.c_int, [_p] * 5 + [_i64] * 4 + [_i64x, _i64, _i64, _i64, _p]),
     "akt_kept_index_from_mask": (C.c_int, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, C.c_int, _p]),

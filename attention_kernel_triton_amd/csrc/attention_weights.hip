@@ -4,15 +4,27 @@
 // q, lse and the page table are those of an attention call (paged decode, chunk or shared
 // prefix); sequence b's token i sits at position len_b - n_b + i, as there.
 //
-// A workgroup owns 256 keys of one (sequence, kv head), wave w keys 64 w .. 64 w + 63 of them, and
-// reads them into registers once; the rows (token, query head of the group; token major) go by in
-// blocks of 32, staged in LDS once for the four waves.  S = Q K^T is computed with rows along the
-// registers and keys along the lanes (two v_mfma_f32_32x32x16 columns), so a lane sums its
-// key's weights in registers and every sum has one owner and one order: no atomics, and results do
-// not depend on the run.  A block's 16 terms are summed before they join the total.
+// S = Q K^T is computed with rows (token, query head of the group; token major) along the registers
+// and keys along the lanes (v_mfma_f32_32x32x16), so a lane sums its key's weights in registers, and
+// every sum has one owner and one order: no atomics on the sums, and results do not depend on the run.
+// The two kinds of sequences are served by workgroups of their own, in one launch (share_of):
 //
-// What bounds it: HBM (K once) for few rows; for many the three VALU instructions to a score (fma,
-// exp2, add) beside 1/1024 of an MFMA k-step each.
+// Few rows (at most 32 to a kv head).  HBM-bound: K is read once.  The keys of a (sequence, kv head)
+// are cut into steps of 32 (64 at D = 64), which stand on an axis; a wave serves a range of it as one
+// stream, with the keys of the next step and the page ids of the one after it on their way while a step
+// is computed.  Waves do not meet.
+//
+// Many rows.  Bound by the three VALU instructions to a score (fma, exp2, add) and the MFMAs, which
+// mostly add up.  A tile is 256 keys of one (sequence, kv head), wave w's the keys 64 w .. 64 w + 63 of
+// them, which it reads into registers once; the rows that see the tile go by in blocks of 32, staged
+// in LDS two blocks at a time for the four waves, the scores of one block computed beside the weights of the
+// one before.  A block's 16 terms are summed before they join the total.  The tiles stand on an axis,
+// each as long as its blocks plus kWTileCost, which is cut into equal ranges, one to a workgroup.  A tile
+// of many blocks may be cut: its parts leave their sums in slots (two to a range, as in
+// paged_chunk.hip) and count themselves; the last one adds them up in the order of the ranges.
+//
+// The workgroups stay for the whole launch and find their ranges from the page table (no plan on the
+// host).
 #include <math.h>
 
 #include <cmath>
@@ -27,6 +39,10 @@ constexpr int kWWaves = 4;
 constexpr int kWThreads = 64 * kWWaves;
 constexpr int kWKeys = 64;                   // keys of a wave
 constexpr int kWTile = kWKeys * kWWaves;  // and of a workgroup
+constexpr int kWTileCost = 6;                // cost of a tile's start and end, in blocks of rows
+constexpr int kWDiagCost = 2;                // cost of a tile with keys that not every row sees, in G
+constexpr int kWTable = 1024;                // sequences whose places a workgroup keeps in LDS
+constexpr int kWFew = 32;                    // rows of a sequence and kv head that are few
 
 struct WeightParams {
   const half_t* q;
@@ -41,7 +57,8 @@ struct WeightParams {
   int64_t q_st, q_sh;
   int64_t sp, sh, ss;  // page, head and slot strides of the pool
   int64_t w_sn, w_sh;
-  int64_t N, L;
+  int N;
+  int64_t L;
   int total_q, total_pages, num_pool_pages;
   int B, Hq, Hkv, G;
   int page_size;
@@ -50,6 +67,8 @@ struct WeightParams {
   int causal;
   int window;  // only the last so many of a sequence's tokens count
   float scale;  // softmax_scale * log2(e)
+  int* arrive;      // a counter to a range (zero between launches)
+  float* partials;  // two slots of kWTile sums to a range
 };
 
 // n / d for 0 <= n < 2^31, given magic = min(2^32 - 1, floor(2^32 / d)).
@@ -59,8 +78,9 @@ __device__ __forceinline__ int div_magic(int n, int d, uint32_t magic) {
 }
 
 struct WSeq {
-  int q0, n, first;  // first row of q that counts, rows that count, position of the first
+  int q0, n;  // first token of q that counts, tokens that count
   int ip0, len;
+  int row;    // of the sums; -1: none
 };
 // Table entries outside their ranges are taken clamped, so nothing outside the arrays is touched.
 __device__ __forceinline__ WSeq load_wseq(const WeightParams& p, int b) {
@@ -72,195 +92,814 @@ __device__ __forceinline__ WSeq load_wseq(const WeightParams& p, int b) {
   s.len = np > 0 ? (np - 1) * p.page_size + min(max(p.last_len[b], 0), p.page_size) : 0;
   s.n = min(n, p.window);
   s.q0 = q0 + n - s.n;
-  s.first = s.len - s.n;
+  s.row = p.rows ? p.rows[b] : b;
+  if ((uint32_t)s.row >= (uint32_t)p.N) s.row = -1;
   return s;
 }
 
-template <int D, bool BF16>
-__global__ __launch_bounds__(kWThreads) __attribute__((amdgpu_waves_per_eu(2)))
-void attention_weights_kernel(WeightParams p) {
-  typedef Elt<BF16> E;
-  typedef typename E::v8 v8;
-  constexpr int KS = D / 16;
-  constexpr int CPR = D / 8;
-  constexpr int ROWB = D * 2;
-  constexpr int PER_T = 32 * CPR / kWThreads;  // chunks of a block of rows to a thread
-  __shared__ __attribute__((aligned(16))) char lds_q[2][32 * ROWB];
-  __shared__ float4_t lds_nl[2][8];  // -lse log2(e) of each row
-  __shared__ int lds_lim[2][32];     // last key that the row sees, -1: none
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int l32 = lane & 31, g = lane >> 5;
-
-  // ---- this workgroup's tile: sequence by sequence, kv head by kv head.
-  int b = 0, item = 0;
-  {
-    const int x = blockIdx.x;
-    int before = 0;
-    for (int jb = 0;; jb += 64) {
-      if (jb >= p.B) return;
-      int tiles = 0;
-      if (jb + lane < p.B) {
-        const WSeq s = load_wseq(p, jb + lane);
-        if (s.n > 0) tiles = (s.len + kWTile - 1) / kWTile * p.Hkv;
-      }
-      int inc = tiles;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(inc, d, 64);
-        if (lane >= d) inc += u;
-      }
-      const uint64_t m = __ballot(before + inc > x);
-      if (m) {
-        const int l = __builtin_ctzll(m);
-        b = uniform(jb + l);
-        item = uniform(x - before - __shfl(inc - tiles, l, 64));
-        break;
-      }
-      before += uniform(__shfl(inc, 63, 64));
-    }
-  }
-  const WSeq sq = load_wseq(p, b);
-  const int q0 = uniform(sq.q0), n = uniform(sq.n), first = uniform(sq.first);
-  const int ip0 = uniform(sq.ip0), len = uniform(sq.len);
-  const int64_t wrow = p.rows ? (int64_t)p.rows[b] : b;
-  if (wrow < 0 || wrow >= p.N) return;
-  const int tiles = (len + kWTile - 1) / kWTile;
-  // (A malformed table may count more tiles than the scan's sums hold.)
-  if (tiles <= 0 || item < 0 || item >= tiles * p.Hkv) return;
-  const int kvh = item / tiles, key0 = (item - kvh * tiles) * kWTile;
-  const int rows = n * p.G;
-
-  // ---- K: lane (l32, g) holds chunks 2 k + g of keys l32 and 32 + l32 of the wave's.
-  const int wkey = key0 + kWKeys * wave;
-  v8 kf[2][KS];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int key = wkey + 32 * c + l32;
-    const int kk = min(key, len - 1);
-    const int lp = div_magic(kk, p.page_size, p.page_magic);
-    const int id = p.indices[ip0 + lp];
-    const bool ok = key < len && (uint32_t)id < (uint32_t)p.num_pool_pages;
-    const half_t* src = p.pool + id * p.sp + kvh * p.sh + (int64_t)(kk - lp * p.page_size) * p.ss + 8 * g;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      uint4_t v = {0, 0, 0, 0};
-      if (ok) v = ld16(src + 16 * k);
-      kf[c][k] = E::as8(v);
-    }
-  }
-
-  // ---- blocks of rows, from the first that holds a row which sees the tile's first key.
-  uint4_t st[PER_T];
-  float nl_st = 0.f;
-  int lim_st = -1;
-  auto load_block = [&](int r0) {
-#pragma unroll
-    for (int i = 0; i < PER_T; ++i) {
-      const int ch = tid + i * kWThreads;
-      const int row = r0 + ch / CPR;
-      st[i] = uint4_t{0, 0, 0, 0};
-      if (row < rows) {
-        const int tok = div_magic(row, p.G, p.g_magic);
-        st[i] = ld16(p.q + (int64_t)(q0 + tok) * p.q_st +
-                     (int64_t)(kvh * p.G + row - tok * p.G) * p.q_sh + ch % CPR * 8);
-      }
-    }
-    if (tid < 32) {
-      const int row = r0 + tid;
-      lim_st = -1;
-      nl_st = 0.f;
-      if (row < rows) {
-        const int tok = div_magic(row, p.G, p.g_magic);
-        const float l = p.lse[(int64_t)(q0 + tok) * p.Hq + kvh * p.G + row - tok * p.G];
-        nl_st = -l * kLog2e;
-        // A row that saw no key (lse -inf) drew on none.
-        if (l != -__builtin_inff()) lim_st = p.causal ? first + tok : len - 1;
-      }
-    }
-  };
-  auto store_block = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < PER_T; ++i) {
-      const int ch = tid + i * kWThreads;
-      const int row = ch / CPR, cc = ch % CPR;
-      *reinterpret_cast<uint4_t*>(lds_q[buf] + row * ROWB + ((cc ^ tswz<D>(row)) * 16)) = st[i];
-    }
-    if (tid < 32) {
-      reinterpret_cast<float*>(lds_nl[buf])[tid] = nl_st;
-      lds_lim[buf][tid] = lim_st;
-    }
-  };
-  float w[2] = {0.f, 0.f};
-  int r0 = 0;
-  if (p.causal && key0 > first) r0 = (int)((int64_t)(key0 - first) * p.G / 32 * 32);
-  load_block(r0);
-  store_block(0);
-  __syncthreads();
-  const float c = p.scale;
-#pragma clang loop unroll(disable)
-  for (int buf = 0; r0 < rows; r0 += 32, buf ^= 1) {
-    const bool more = r0 + 32 < rows;
-    if (more) load_block(r0 + 32);
-    if (wkey < len) {
-      float16_t s[2];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const v8 a = E::as8(*reinterpret_cast<const uint4_t*>(
-            lds_q[buf] + l32 * ROWB + (((2 * k + g) ^ tswz<D>(l32)) * 16)));
-        s[0] = E::mfma(a, kf[0][k], s[0]);
-        s[1] = E::mfma(a, kf[1][k], s[1]);
-      }
-      // Register 4 j + i of half g is row 8 j + 4 g + i.
-      if (__ballot(lds_lim[buf][l32] >= wkey + kWKeys - 1) == ~0ull) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4_t nl = lds_nl[buf][2 * j + g];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += fast_exp2(__builtin_fmaf(s[t][4 * j + i], c, nl[i]));
-          }
-          w[t] += sum;
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int key = wkey + 32 * t + l32;
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4_t nl = lds_nl[buf][2 * j + g];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float e = fast_exp2(__builtin_fmaf(s[t][4 * j + i], c, nl[i]));
-              sum += lds_lim[buf][8 * j + 4 * g + i] >= key ? e : 0.f;
-            }
-          }
-          w[t] += sum;
-        }
-      }
-    }
-    if (more) store_block(buf ^ 1);
-    __syncthreads();
-  }
-
-  // ---- half g writes keys 32 g + l32.
-  const float w0 = xor32_sum(w[0]), w1 = xor32_sum(w[1]);
-  const int key = wkey + lane;
-  const int id = p.indices[ip0 + div_magic(min(key, len - 1), p.page_size, p.page_magic)];
-  if (key < len && key < p.L && (uint32_t)id < (uint32_t)p.num_pool_pages) {
-    float* dst = p.w + wrow * p.w_sn + kvh * p.w_sh + key;
-    *dst += g ? w1 : w0;
-  }
+// The tiles of one (sequence, kv head) on the axis.  A tile's blocks of rows are those from `skip`
+// on: the first t0 tiles hold keys that every row sees (all blocks), tile t0 + i skips f0 + 8 G i.
+struct WHead {
+  int64_t full;  // blocks and cost of a tile that skips none
+  int tiles, t0, f0, step, diag;
+};
+__device__ __forceinline__ WHead head_of(const WeightParams& p, const WSeq& s) {
+  WHead h;
+  h.full = (int64_t)(((int64_t)s.n * p.G + 31) / 32) + kWTileCost;
+  h.tiles = s.n > 0 ? (s.len + kWTile - 1) / kWTile : 0;
+  const int first = s.len - s.n;  // position of the first row
+  h.t0 = !p.causal ? h.tiles : first < 0 ? 0 : min(first / kWTile + 1, h.tiles);
+  h.f0 = (int)((int64_t)max(h.t0 * kWTile - first, 0) * p.G / 32);
+  h.step = kWTile / 32 * p.G;
+  h.diag = kWDiagCost * p.G;
+  return h;
+}
+__device__ __forceinline__ int64_t skipped(const WHead& h, int t) {
+  return t < h.t0 ? 0 : h.f0 + (int64_t)(t - h.t0) * h.step;
+}
+// Start of tile t (t = tiles: the length of all).
+__device__ __forceinline__ int64_t tile_start(const WHead& h, int t) {
+  const int64_t i = max(t - h.t0, 0);
+  return t * h.full - i * h.f0 - i * (i - 1) / 2 * h.step + i * h.diag;
+}
+__device__ __forceinline__ int64_t w_uniform64(int64_t v) {
+  const uint32_t lo = (uint32_t)uniform((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)uniform((int)(uint32_t)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t w_shfl64(int64_t v, int src) {
+  return (int64_t)(((uint64_t)shfl_u((uint32_t)(v >> 32), src) << 32) | shfl_u((uint32_t)v, src));
+}
+// floor(a / b) for 0 <= a < 2^50, b >= 1 (see div_range in paged_chunk.hip).
+__device__ __forceinline__ int64_t w_div(int64_t a, int64_t b) {
+  return w_uniform64((int64_t)((double)a / (double)b));
 }
 
 template <int D>
-int launch_weights(const WeightParams& p, bool bf16, int64_t blocks, hipStream_t st) {
+__host__ __device__ constexpr int weight_waves() {
+  return D <= 128 ? 2 : 1;  // waves to a SIMD
+}
+
+// Sequences' places: in LDS, unless there are too many.
+struct WTable {
+  const int4* seq;  // null: load_wseq
+  const int* row;
+};
+__device__ __forceinline__ WSeq seq_of(const WeightParams& p, const WTable& t, int b) {
+  if (!t.seq) return load_wseq(p, b);
+  const int4 s = t.seq[b];
+  return WSeq{s.x, s.y, s.z, s.w, t.row[b]};
+}
+// The kinds; a sequence that has no row of sums is of neither.
+__device__ __forceinline__ bool is_few(const WeightParams& p, const WSeq& s) {
+  return s.n > 0 && s.row >= 0 && s.n * p.G <= kWFew;
+}
+__device__ __forceinline__ bool is_many(const WeightParams& p, const WSeq& s) {
+  return s.row >= 0 && s.n * p.G > kWFew;
+}
+__device__ __forceinline__ int64_t w_scan64(int64_t v, int lane) {  // inclusive sum over the lanes
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t u = w_shfl64(v, lane - d < 0 ? 0 : lane - d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// Keys of a step of few rows, and what a unit's start costs a wave, in steps.
+__host__ __device__ constexpr int few_keys(int D) { return D <= 64 ? 64 : 32; }
+constexpr int kFewCost = 1;
+__device__ __forceinline__ int few_length(const WSeq& s, int keys) {
+  return s.len > 0 ? (s.len + keys - 1) / keys + kFewCost : 0;
+}
+
+// A step of few rows.
+struct FewWStep {
+  int b, kvh;      // b = -1: the range is done
+  int64_t start;   // of the unit on the axis
+  int q0, n, ip0, len, row;
+  int j, j1;       // the step, and the first that is not the wave's
+};
+
+template <int D, bool BF16>
+__device__ __forceinline__ void few_weights(const WeightParams& p, const WTable& tab, int block,
+                                            int W) {
+  typedef Elt<BF16> E;
+  constexpr int KS = D / 16;
+  constexpr int KEYS = few_keys(D), NC = KEYS / 32;  // columns of 32 keys
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int l32 = lane & 31, g = lane >> 5;
+  // ---- this wave's range: consecutive ones go to one XCD (workgroup i runs on XCD i % 8).
+  const int range = ((block % 8) * (W / 8) + block / 8) * kWWaves + wave;
+  auto seq_length = [&](int b) -> int64_t {
+    if (b >= p.B) return 0;
+    const WSeq s = seq_of(p, tab, b);
+    return is_few(p, s) ? (int64_t)few_length(s, KEYS) * p.Hkv : 0;
+  };
+  int64_t length = seq_length(lane), inc = w_scan64(length, lane);
+  int64_t total = w_uniform64(w_shfl64(inc, 63));
+  for (int jb = 64; jb < p.B; jb += 64)
+    total += w_uniform64(w_shfl64(w_scan64(seq_length(jb + lane), lane), 63));
+  const int64_t Lw = w_uniform64((total + W * kWWaves - 1) / (W * kWWaves));
+  const int64_t x0 = range * Lw;
+  if (x0 >= total) return;
+  const int64_t x1 = x0 + Lw < total ? x0 + Lw : total;
+
+  auto take_seq = [&](FewWStep& s) -> bool {
+    const WSeq q = seq_of(p, tab, s.b);
+    s.q0 = uniform(q.q0);
+    s.n = uniform(q.n);
+    s.ip0 = uniform(q.ip0);
+    s.len = uniform(q.len);
+    s.row = uniform(q.row);
+    return uniform(is_few(p, q) && q.len > 0);
+  };
+  // The first step of the unit that s names, or of the next one with steps in the range.
+  auto enter = [&](FewWStep& s) {
+    for (;;) {
+      if (s.start >= x1) {
+        s.b = -1;
+        return;
+      }
+      const int steps = (s.len + KEYS - 1) / KEYS;
+      s.j = uniform((int)min(max(x0 - s.start, (int64_t)0), (int64_t)steps));
+      s.j1 = uniform((int)min(x1 - s.start, (int64_t)steps));
+      if (s.j < s.j1) return;
+      s.start = w_uniform64(s.start + steps + kFewCost);
+      if (++s.kvh < p.Hkv) continue;
+      s.kvh = 0;
+      do {
+        if (++s.b >= p.B) {
+          s.b = -1;
+          return;
+        }
+      } while (!take_seq(s));
+    }
+  };
+  auto advance = [&](FewWStep& s) {
+    if (++s.j < s.j1) return;
+    s.start = w_uniform64(s.start + (s.len + KEYS - 1) / KEYS + kFewCost);
+    if (++s.kvh == p.Hkv) {
+      s.kvh = 0;
+      do {
+        if (++s.b >= p.B) {
+          s.b = -1;
+          return;
+        }
+      } while (!take_seq(s));
+    }
+    enter(s);
+  };
+  FewWStep cur;
+  {
+    int64_t at = 0;
+    for (int jb = 0;;) {
+      const uint64_t m = __ballot(at + inc > x0);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        cur.b = uniform(jb + l);
+        at += w_uniform64(w_shfl64(inc - length, l));
+        break;
+      }
+      at += w_uniform64(w_shfl64(inc, 63));
+      jb += 64;
+      if (jb >= p.B) return;
+      length = seq_length(jb + lane);
+      inc = w_scan64(length, lane);
+    }
+    take_seq(cur);
+    const int unit = (cur.len + KEYS - 1) / KEYS + kFewCost;
+    cur.kvh = uniform((int)w_div(x0 - at, unit));
+    cur.start = w_uniform64(at + (int64_t)cur.kvh * unit);
+    enter(cur);
+  }
+  if (cur.b < 0) return;
+
+  // ---- loads.  Lane (l32, g) takes chunks 2 k + g of keys l32 (and 32 + l32) of a step.
+  int id[NC], slot[NC];
+  auto load_ids = [&](const FewWStep& s) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int key = min(s.j * KEYS + 32 * i + l32, s.len - 1);
+      const int lp = div_magic(key, p.page_size, p.page_magic);
+      slot[i] = key - lp * p.page_size;
+      id[i] = p.indices[s.ip0 + lp];
+    }
+  };
+  // Loads come back in the order in which they are asked for: a step's page ids are asked for before
+  // the keys of the step before it, so that waiting for them does not wait for those.
+  auto load_k = [&](const FewWStep& s, const FewWStep& after, uint4_t (&kf)[NC][KS], bool (&ok)[NC]) {
+    const half_t* src[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      ok[i] = s.j * KEYS + 32 * i + l32 < s.len && (uint32_t)id[i] < (uint32_t)p.num_pool_pages;
+      // A key that cannot be read takes a row of q: its sum is not written.
+      src[i] = (ok[i] ? p.pool + id[i] * p.sp + s.kvh * p.sh + (int64_t)slot[i] * p.ss : p.q) + 8 * g;
+    }
+    if (after.b >= 0) load_ids(after);
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kf[i][k] = ld16(src[i] + 16 * k);
+  };
+  // Rows: fragments of row l32 (the last one's again behind it), and -lse log2(e) of the rows of
+  // the lane's registers: register 4 j + i of half g is row 8 j + 4 g + i.
+  uint4_t qf[KS];
+  float nl[16];
+  uint32_t gone = 0;  // bit r: register r's row is not there, or drew on none (lse -inf)
+  auto load_rows = [&](const FewWStep& s) {
+    const int rows = s.n * p.G;
+    {
+      const int row = min(l32, rows - 1), tok = div_magic(row, p.G, p.g_magic);
+      const half_t* src = p.q + (int64_t)(s.q0 + tok) * p.q_st +
+                          (int64_t)(s.kvh * p.G + row - tok * p.G) * p.q_sh + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) qf[k] = ld16(src + 16 * k);
+    }
+    gone = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 8 * (r / 4) + 4 * g + r % 4;
+      nl[r] = -__builtin_inff();
+      if (8 * (r / 4) < rows) {  // wave-uniform
+        const int rr = min(row, rows - 1), tok = div_magic(rr, p.G, p.g_magic);
+        const float l = p.lse[(int64_t)(s.q0 + tok) * p.Hq + s.kvh * p.G + rr - tok * p.G];
+        const bool none = row >= rows || l == -__builtin_inff();
+        if (!none) nl[r] = -l * kLog2e;
+        gone |= none ? 1u << r : 0u;
+      }
+    }
+  };
+  const float c = p.scale;
+  // Weights of a step's keys, added to their sums by half g for keys 32 g + l32 (one column: half 0).
+  auto serve = [&](const FewWStep& s, const uint4_t (&kf)[NC][KS], const bool (&ok)[NC], float old) {
+    const int rows = s.n * p.G, first = s.len - s.n, key = s.j * KEYS + l32;
+    float16_t sc[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[i][r] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) sc[i] = E::mfma(E::as8(qf[k]), E::as8(kf[i][k]), sc[i]);
+    }
+    float sum[NC] = {};
+    bool odd = p.causal && s.j * KEYS + KEYS - 1 > first;  // keys that not every row sees
+    if (!odd) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (8 * j < rows)  // wave-uniform
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              sum[i] += fast_exp2(__builtin_fmaf(sc[i][4 * j + r], c, nl[4 * j + r]));
+      // A score that is not finite makes NaN of a row that is not there or drew on none.
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) nan |= sum[i] != sum[i];
+      odd = __any(nan);
+    }
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) sum[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (8 * j < rows)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = 8 * j + 4 * g + r;
+            const int last = (gone >> (4 * j + r)) & 1 ? -1
+                             : p.causal               ? first + div_magic(row, p.G, p.g_magic)
+                                                      : s.len - 1;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+              const float e = fast_exp2(__builtin_fmaf(sc[i][4 * j + r], c, nl[4 * j + r]));
+              sum[i] += last >= key + 32 * i ? e : 0.f;
+            }
+          }
+    }
+    float out = xor32_sum(sum[0]);
+    bool mine = ok[0] && g == 0;
+    if constexpr (NC == 2) {
+      const float out1 = xor32_sum(sum[1]);
+      if (g) {
+        out = out1;
+        mine = ok[1];
+      }
+    }
+    const int at = s.j * KEYS + (NC == 2 ? lane : l32);
+    if (mine && at < p.L) p.w[s.row * p.w_sn + s.kvh * p.w_sh + at] = old + out;
+  };
+  auto load_old = [&](const FewWStep& s) -> float {
+    const int at = min(s.j * KEYS + (NC == 2 ? lane : l32), s.len - 1);
+    return at < p.L ? p.w[s.row * p.w_sn + s.kvh * p.w_sh + at] : 0.f;
+  };
+
+  // ---- the stream.
+  uint4_t kA[NC][KS], kB[NC][KS];
+  bool okA[NC], okB[NC];
+  load_rows(cur);
+  load_ids(cur);
+  FewWStep next = cur;
+  advance(next);
+  load_k(cur, next, kA, okA);
+  auto step = [&](uint4_t (&k0)[NC][KS], bool (&ok0)[NC], uint4_t (&k1)[NC][KS], bool (&ok1)[NC]) -> bool {
+    FewWStep after = next;
+    if (next.b >= 0) advance(after);
+    const float old = load_old(cur);
+    if (next.b >= 0) load_k(next, after, k1, ok1);
+    serve(cur, k0, ok0, old);
+    if (next.b < 0) return false;
+    if (next.b != cur.b || next.kvh != cur.kvh) load_rows(next);
+    cur = next;
+    next = after;
+    return true;
+  };
+#pragma clang loop unroll(disable)
+  for (;;) {
+    if (!step(kA, okA, kB, okB)) return;
+    if (!step(kB, okB, kA, okA)) return;
+  }
+}
+
+// A tile and the part of its blocks that a workgroup serves.
+struct WTile {
+  int b, kvh, t;
+  int64_t start;   // on the axis
+  int q0, n, ip0, len;
+  int row;             // of the sums; -1: none
+  int blocks, j0, j1;  // its blocks of rows, and those of the part
+  int r0;              // row of block j0
+};
+
+// LDS of a workgroup of many rows.
+template <int D>
+struct ManyLds {
+  static constexpr int kStage = 64;  // rows to a stage: two blocks
+  char q[2][kStage * D * 2];
+  // A wave may still add the weights of a stage's second block while another stores the stage after
+  // the next, so rows' numbers are kept for longer than the rows.
+  float4_t nl[4][kStage / 4];  // -lse log2(e) of each row
+  int4 lim[4][kStage / 4];     // last key that each row sees, -1: none
+  int last;
+};
+
+template <int D, bool BF16>
+__device__ __forceinline__ void many_weights(const WeightParams& p, const WTable& tab,
+                                             ManyLds<D>& lds, int block, int W) {
+  typedef Elt<BF16> E;
+  constexpr int KS = D / 16;
+  constexpr int CPR = D / 8;
+  constexpr int ROWB = D * 2;
+  constexpr int kStage = ManyLds<D>::kStage;
+  constexpr int PER_T = kStage * CPR / kWThreads;  // chunks of a stage to a thread
+  constexpr int kPass = kWThreads / CPR;           // rows between a thread's chunks
+  constexpr int kFirst = 32;  // VALU instructions of a step before its first MFMA, while rows arrive
+  auto& lds_q = lds.q;
+  auto& lds_nl = lds.nl;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l32 = lane & 31, g = lane >> 5;
+
+  // ---- this workgroup's range.  Workgroup i runs on XCD i % 8: consecutive ranges go to one XCD.
+  const int wg = (block % 8) * (W / 8) + block / 8;
+  auto seq_length = [&](int b) -> int64_t {
+    if (b >= p.B) return 0;
+    const WSeq s = seq_of(p, tab, b);
+    if (!is_many(p, s)) return 0;
+    const WHead h = head_of(p, s);
+    return tile_start(h, h.tiles) * p.Hkv;
+  };
+  int64_t length = seq_length(lane), inc = w_scan64(length, lane);
+  int64_t total = w_uniform64(w_shfl64(inc, 63));
+  for (int jb = 64; jb < p.B; jb += 64)
+    total += w_uniform64(w_shfl64(w_scan64(seq_length(jb + lane), lane), 63));
+  const int64_t Lw = w_uniform64(max((total + W - 1) / W, (int64_t)(kWTileCost + 1)));
+  const int64_t x0 = wg * Lw;
+  if (x0 >= total) return;
+  const int64_t x1 = x0 + Lw < total ? x0 + Lw : total;
+
+  // ---- the tiles of the range, from the one that holds x0 on.  `head` is of the tile entered last.
+  WHead head;
+  auto take_seq = [&](WTile& a) {
+    const WSeq s = seq_of(p, tab, a.b);
+    a.q0 = uniform(s.q0);
+    a.n = uniform(s.n);
+    a.ip0 = uniform(s.ip0);
+    a.len = uniform(s.len);
+    a.row = uniform(s.row);
+    head = head_of(p, WSeq{a.q0, a.n, a.ip0, a.len, a.row});
+    if (!is_many(p, WSeq{a.q0, a.n, a.ip0, a.len, a.row})) head.tiles = 0;
+  };
+  // The part of the tile that a names; one without blocks is passed over.
+  auto enter = [&](WTile& a) {
+    for (;;) {
+      if (a.start >= x1) {
+        a.b = -1;
+        return;
+      }
+      const int64_t skip = skipped(head, a.t);
+      a.blocks = uniform((int)(head.full - kWTileCost - skip));
+      a.j0 = uniform((int)min(max(x0 - a.start, (int64_t)0), (int64_t)a.blocks));
+      a.j1 = uniform((int)min(x1 - a.start, (int64_t)a.blocks));
+      a.r0 = uniform((int)(32 * (skip + a.j0)));
+      if (a.j0 < a.j1) return;
+      a.start = w_uniform64(a.start + a.blocks + kWTileCost + (a.t >= head.t0 ? head.diag : 0));
+      if (++a.t < head.tiles) continue;
+      a.t = 0;
+      if (++a.kvh < p.Hkv) continue;
+      a.kvh = 0;
+      do {
+        if (++a.b >= p.B) {
+          a.b = -1;
+          return;
+        }
+        take_seq(a);
+      } while (head.tiles == 0);
+    }
+  };
+  auto advance = [&](WTile& a) {
+    a.start = w_uniform64(a.start + a.blocks + kWTileCost + (a.t >= head.t0 ? head.diag : 0));
+    if (++a.t == head.tiles) {
+      a.t = 0;
+      if (++a.kvh == p.Hkv) {
+        a.kvh = 0;
+        do {
+          if (++a.b >= p.B) {
+            a.b = -1;
+            return;
+          }
+          take_seq(a);
+        } while (head.tiles == 0);
+      }
+    }
+    enter(a);
+  };
+  WTile cur;
+  {
+    int64_t at = 0;
+    for (int jb = 0;;) {
+      const uint64_t m = __ballot(at + inc > x0);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        cur.b = uniform(jb + l);
+        at += w_uniform64(w_shfl64(inc - length, l));
+        break;
+      }
+      at += w_uniform64(w_shfl64(inc, 63));
+      jb += 64;
+      if (jb >= p.B) return;
+      length = seq_length(jb + lane);
+      inc = w_scan64(length, lane);
+    }
+    take_seq(cur);
+    const int64_t per = tile_start(head, head.tiles);
+    cur.kvh = (int)w_div(x0 - at, per);
+    at += cur.kvh * per;
+    cur.t = 0;
+    for (int lo = 1, hi = head.tiles; lo < hi;) {  // last t whose start is at or before x0
+      const int mid = (lo + hi) / 2;
+      if (at + tile_start(head, mid) <= x0) {
+        cur.t = mid;
+        lo = mid + 1;
+      } else {
+        hi = mid;
+      }
+    }
+    cur.t = uniform(cur.t);
+    cur.start = w_uniform64(at + tile_start(head, cur.t));
+    enter(cur);
+  }
+  if (cur.b < 0) return;
+
+  // ---- K: lane (l32, g) holds chunks 2 k + g of keys l32 and 32 + l32 of the wave's.
+  uint4_t kf[2][KS];
+  bool ok[2];
+  auto load_k = [&](const WTile& a) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = a.t * kWTile + kWKeys * wave + 32 * i + l32;
+      const int kk = min(key, a.len - 1), lp = div_magic(kk, p.page_size, p.page_magic);
+      const int id = p.indices[a.ip0 + lp];
+      ok[i] = key < a.len && (uint32_t)id < (uint32_t)p.num_pool_pages;
+      // A key that cannot be read takes a row of q: its sum is not written.
+      const half_t* src = (ok[i] ? p.pool + id * p.sp + a.kvh * p.sh +
+                                       (int64_t)(kk - lp * p.page_size) * p.ss
+                                 : p.q) + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kf[i][k] = ld16(src + 16 * k);
+    }
+  };
+
+  // ---- rows, a stage at a time: global memory -> registers -> LDS.  A thread's chunks are those of
+  // column tid % CPR of rows tid / CPR + kPass i.
+  uint4_t st[PER_T];
+  float nl_st = 0.f;
+  int lim_st = -1;
+  // Of the next stage to load: the thread's chunks (address and head of each row), and the row whose
+  // numbers it looks up (threads 0 .. kStage - 1).
+  const half_t* qsrc[PER_T];
+  int hd[PER_T], row0;
+  const float* lsrc;
+  int tokr, hdr;
+  // From a row to the one kStage behind it: heads and tokens on, and back by G heads for one more
+  // token where that is past the last.
+  const int adv_t = kStage / p.G, adv_h = kStage - adv_t * p.G;
+  const int64_t q_adv = adv_t * p.q_st + adv_h * p.q_sh, q_wrap = p.q_st - p.G * p.q_sh;
+  auto start_rows = [&](const WTile& a) {
+    row0 = a.r0 + tid / CPR;
+#pragma unroll
+    for (int i = 0; i < PER_T; ++i) {
+      const int row = row0 + kPass * i, tok = div_magic(row, p.G, p.g_magic);
+      hd[i] = row - tok * p.G;
+      qsrc[i] = p.q + (int64_t)(a.q0 + tok) * p.q_st + (int64_t)(a.kvh * p.G + hd[i]) * p.q_sh +
+                tid % CPR * 8;
+    }
+    tokr = div_magic(a.r0 + tid, p.G, p.g_magic);
+    hdr = a.r0 + tid - tokr * p.G;
+    lsrc = p.lse + (int64_t)(a.q0 + tokr) * p.Hq + a.kvh * p.G + hdr;
+  };
+  auto load_stage = [&](const WTile& a) {
+    const int rows = a.n * p.G;
+#pragma unroll
+    for (int i = 0; i < PER_T; ++i) {
+      // (A row past the last takes any: no key is seen by it.)
+      st[i] = ld16(row0 + kPass * i < rows ? qsrc[i] : p.q);
+      qsrc[i] += q_adv;
+    }
+    row0 += kStage;
+    if (adv_h) {
+#pragma unroll
+      for (int i = 0; i < PER_T; ++i) {
+        hd[i] += adv_h;
+        if (hd[i] >= p.G) {
+          hd[i] -= p.G;
+          qsrc[i] += q_wrap;
+        }
+      }
+    }
+    if (wave * 64 < kStage) {
+      const bool in = tokr < a.n;
+      const float l = *(in ? lsrc : p.lse);
+      // A row that saw no key (lse -inf) drew on none.
+      const bool none = l == -__builtin_inff();
+      nl_st = none ? l : -l * kLog2e;
+      lim_st = in && !none ? (p.causal ? a.len - a.n + tokr : a.len - 1) : -1;
+      lsrc += adv_t * p.Hq + adv_h;
+      tokr += adv_t;
+      hdr += adv_h;
+      if (hdr >= p.G) {
+        hdr -= p.G;
+        lsrc += p.Hq - p.G;
+        ++tokr;
+      }
+    }
+  };
+  auto store_stage = [&](int stage) {
+    const int buf = stage & 1;
+#pragma unroll
+    for (int i = 0; i < PER_T; ++i) {
+      const int row = tid / CPR + kPass * i, cc = tid % CPR;
+      *reinterpret_cast<uint4_t*>(lds_q[buf] + row * ROWB + ((cc ^ tswz<D>(row)) * 16)) = st[i];
+    }
+    if (wave * 64 < kStage) {
+      reinterpret_cast<float*>(lds_nl[stage & 3])[tid] = nl_st;
+      reinterpret_cast<int*>(lds.lim[stage & 3])[tid] = lim_st;
+    }
+  };
+
+  const float c = p.scale;
+  float w[2];
+  // A block's rows, as fragments: chunk 2 k + g of row l32 lies at ((2 k) ^ g ^ tswz) = k's bits over
+  // the rest of the address.
+  const int frag0 = l32 * ROWB + ((g ^ tswz<D>(l32)) * 16);
+  auto load_frags = [&](int stage, int half, uint4_t (&a)[KS]) {
+    const char* const base = lds_q[stage & 1] + 32 * half * ROWB;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) a[k] = *reinterpret_cast<const uint4_t*>(base + (frag0 ^ (32 * k)));
+  };
+  // Scores of a block.
+  auto scores = [&](const uint4_t (&a)[KS], float16_t (&sc)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[0][i] = sc[1][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      sc[0] = E::mfma(E::as8(a[k]), E::as8(kf[0][k]), sc[0]);
+      sc[1] = E::mfma(E::as8(a[k]), E::as8(kf[1][k]), sc[1]);
+    }
+  };
+  // A block's weights: register 4 j + i of half g is row 8 j + 4 g + i.
+  auto add_seen = [&](int stage, int half, const float16_t (&sc)[2], int key) {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4_t nl = lds_nl[stage & 3][8 * half + 2 * j + g];
+      const int4 lim = lds.lim[stage & 3][8 * half + 2 * j + g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int l = i == 0 ? lim.x : i == 1 ? lim.y : i == 2 ? lim.z : lim.w;
+        const float e0 = fast_exp2(__builtin_fmaf(sc[0][4 * j + i], c, nl[i]));
+        const float e1 = fast_exp2(__builtin_fmaf(sc[1][4 * j + i], c, nl[i]));
+        sum[0] += l >= key ? e0 : 0.f;
+        sum[1] += l >= key + 32 ? e1 : 0.f;
+      }
+    }
+    w[0] += sum[0];
+    w[1] += sum[1];
+  };
+
+  for (;;) {
+    load_k(cur);
+    const int wkey = cur.t * kWTile + kWKeys * wave;  // the wave's first key
+    const bool live = wkey < cur.len;
+    const int nb = cur.j1 - cur.j0;
+    start_rows(cur);
+    load_stage(cur);
+    // Half g adds to the sums of keys 32 g + l32.
+    const int key = wkey + lane;
+    const bool mine = (g ? ok[1] : ok[0]) && key < p.L;
+    float* const dst = p.w + cur.row * p.w_sn + cur.kvh * p.w_sh + key;
+    const bool whole = nb == cur.blocks;
+    float old = 0.f;
+    if (whole && mine) old = *dst;
+    __syncthreads();  // the last tile's LDS reads are done
+    store_stage(0);
+    if (nb > 2) load_stage(cur);
+    __syncthreads();
+
+    w[0] = w[1] = 0.f;
+    float16_t sA[2], sB[2];
+    uint4_t fr[KS];
+    if (live) {
+      load_frags(0, 0, fr);
+      scores(fr, sA);
+    }
+    // Scores of block i + 1 beside the weights of block i; a stage is published while its
+    // predecessor's second block goes by.
+    // The blocks whose rows are all there and see all of the wave's keys begin from row rfull on; in
+    // them nothing is masked.  (A row that drew on none has a weight of 0 there, or NaN where a
+    // score is not finite: then the block is summed again with its rows' limits.)
+    const int rows = cur.n * p.G;
+    const int rfull = p.causal ? max(wkey + kWKeys - 1 - (cur.len - cur.n), 0) * p.G
+                               : (wkey + kWKeys <= cur.len ? 0 : rows);
+    auto step = [&](int stage, int half, float16_t (&sc)[2], float16_t (&sn)[2]) {
+      const int r = cur.r0 + kStage * stage + 32 * half;
+      if (r >= rfull && r + 32 <= rows) {
+        float4_t nl[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) nl[j] = lds_nl[stage & 3][8 * half + 2 * j + g];
+        load_frags(stage + half, half ^ 1, fr);
+        __builtin_amdgcn_sched_barrier(0);  // all of the block's reads are asked for first
+        scores(fr, sn);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sum[0] += fast_exp2(__builtin_fmaf(sc[0][4 * j + i], c, nl[j][i]));
+            sum[1] += fast_exp2(__builtin_fmaf(sc[1][4 * j + i], c, nl[j][i]));
+          }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x402, kFirst, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x402, (96 - kFirst) / (2 * KS), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (__any(sum[0] != sum[0] || sum[1] != sum[1])) {
+          add_seen(stage, half, sc, wkey + l32);
+        } else {
+          w[0] += sum[0];
+          w[1] += sum[1];
+        }
+      } else {
+        load_frags(stage + half, half ^ 1, fr);
+        add_seen(stage, half, sc, wkey + l32);
+        scores(fr, sn);
+      }
+    };
+    int i = 0, stage = 0;
+#pragma clang loop unroll(disable)
+    for (;;) {
+      if (i + 1 == nb) break;
+      if (live) step(stage, 0, sA, sB);
+      if (++i + 1 == nb) {
+        sA[0] = sB[0];
+        sA[1] = sB[1];
+        break;
+      }
+      store_stage(stage + 1);
+      if (i + 3 < nb) load_stage(cur);
+      __syncthreads();
+      if (live) step(stage, 1, sB, sA);
+      ++i;
+      ++stage;
+    }
+    if (live) add_seen(stage, i & 1, sA, wkey + l32);
+    const float w0 = xor32_sum(w[0]), w1 = xor32_sum(w[1]);
+    const float sum = g ? w1 : w0;
+    if (whole) {
+      if (mine) *dst = old + sum;
+    } else {
+      // ---- a part: its sums to the slot, and the last one of the tile adds them all.
+      const int wf = (int)w_div(cur.start, Lw), wl = (int)w_div(cur.start + cur.blocks - 1, Lw);
+      auto slot_of = [&](int x) -> float* {
+        return p.partials + (2 * (int64_t)x + (x == wf ? 1 : 0)) * kWTile + tid;
+      };
+      __hip_atomic_store(slot_of(wg), sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // Every wave's store (device scope) is complete before the count.
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (tid == 0) {
+        const int prev = atomicAdd(&p.arrive[wf], 1);
+        if (prev == wl - wf) atomicExch(&p.arrive[wf], 0);
+        lds.last = prev == wl - wf;
+      }
+      __syncthreads();
+      if (lds.last) {
+        float all = 0.f;
+        for (int x = wf; x <= wl; ++x)
+          all += __hip_atomic_load(slot_of(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (mine) *dst += all;
+      }
+    }
+    advance(cur);
+    if (cur.b < 0) return;
+  }
+}
+
+// Workgroups (of all W, a multiple of 8) for the sequences of few rows, by the lengths of the two
+// axes: a step of few rows takes a workgroup's wave about as long as a block of many the workgroup.
+template <int D>
+__device__ __forceinline__ int share_of(const WeightParams& p, const WTable& tab, int W) {
+  const int lane = threadIdx.x & 63;
+  double few = 0, many = 0;
+  for (int b = lane; b < p.B; b += 64) {
+    const WSeq s = seq_of(p, tab, b);
+    if (is_few(p, s)) few += few_length(s, few_keys(D));
+    if (is_many(p, s)) {
+      const WHead h = head_of(p, s);
+      many += (double)tile_start(h, h.tiles);
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    few += __shfl_xor(few, d, 64);
+    many += __shfl_xor(many, d, 64);
+  }
+  if (many == 0) return W;
+  if (few == 0) return 0;
+  const int s = 8 * (int)(W / 8 * (few / (few + many)) + 0.5);
+  return uniform(min(max(s, 8), W - 8));
+}
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(kWThreads) __attribute__((amdgpu_waves_per_eu(weight_waves<D>(), weight_waves<D>())))
+void attention_weights_kernel(WeightParams p) {
+  __shared__ __attribute__((aligned(16))) ManyLds<D> lds;
+  __shared__ int4 lds_seq[kWTable];
+  __shared__ int lds_row[kWTable];
+  WTable tab = {nullptr, nullptr};
+  if (p.B <= kWTable) {
+    for (int b = threadIdx.x; b < p.B; b += kWThreads) {
+      const WSeq s = load_wseq(p, b);
+      lds_seq[b] = int4{s.q0, s.n, s.ip0, s.len};
+      lds_row[b] = s.row;
+    }
+    __syncthreads();
+    tab = WTable{lds_seq, lds_row};
+  }
+  const int W = gridDim.x, S = share_of<D>(p, tab, W);
+  if ((int)blockIdx.x < S) few_weights<D, BF16>(p, tab, blockIdx.x, S);
+  else many_weights<D, BF16>(p, tab, lds, blockIdx.x - S, W - S);
+}
+
+// Workgroups: as many as are resident, fewer where there are fewer tiles and blocks than that
+// (bounded from above by what the host knows).
+template <int D>
+int64_t weight_wgs(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t tokens) {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus <= 0 || cus > 1024)
+    cus = 256;  // no device: what an MI355X has
+  const int64_t resident = round_up((int64_t)cus * weight_waves<D>(), 8);
+  const double tiles = (double)(tokens / kWTile + batch) * Hkv;
+  const double blocks = tiles * (double)(total_q * G / 32 + 1 + kWTileCost + kWDiagCost * G);
+  const double wgs = ceil(blocks / (kWTileCost + 1)) + 16;  // eight of each kind at least
+  return wgs < (double)resident ? round_up((int64_t)wgs, 8) : resident;
+}
+int64_t weight_wgs(int64_t batch, int64_t total_q, int64_t Hkv, int64_t G, int64_t D,
+                   int64_t tokens) {
+  return D == 64    ? weight_wgs<64>(batch, total_q, Hkv, G, tokens)
+         : D == 256 ? weight_wgs<256>(batch, total_q, Hkv, G, tokens)
+                    : weight_wgs<128>(batch, total_q, Hkv, G, tokens);
+}
+
+template <int D>
+int launch_weights(const WeightParams& p, bool bf16, int64_t wgs, hipStream_t st) {
   KernelTimer timer;
-  const dim3 grid((unsigned)blocks), block(kWThreads);
+  const dim3 grid((unsigned)wgs), block(kWThreads);
   if (bf16) timer.launch(attention_weights_kernel<D, true>, grid, block, 0, st, p);
   else timer.launch(attention_weights_kernel<D, false>, grid, block, 0, st, p);
   return check_launch("attention_weights_kernel");
@@ -271,6 +910,18 @@ int launch_weights(const WeightParams& p, bool bf16, int64_t blocks, hipStream_t
 
 using namespace akt;
 
+extern "C" size_t akt_attention_weights_paged_workspace_size(
+    int64_t batch, int64_t total_q, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+    int64_t page_size, int64_t total_pages) {
+  if (batch <= 0 || total_q <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || page_size <= 0 ||
+      total_pages < 0 || num_q_heads % num_kv_heads ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return 0;
+  const int64_t wgs = weight_wgs(batch, total_q, num_kv_heads, num_q_heads / num_kv_heads, head_dim,
+                                 page_size * total_pages);
+  return (size_t)(round_up(AKT_WORKSPACE_ZERO_BYTES, 256) + 2 * wgs * kWTile * 4);
+}
+
 extern "C" int akt_attention_weights_paged(
     const void* q, const int32_t* q_indptr, const float* lse, const void* kv_cache,
     const int32_t* kv_page_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len,
@@ -278,7 +929,7 @@ extern "C" int akt_attention_weights_paged(
     int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t total_pages,
     int64_t num_pool_pages, int64_t num_rows, int64_t row_len, const int64_t q_stride[3],
     const int64_t kv_stride[5], const int64_t weight_stride[2], float softmax_scale, int causal,
-    int64_t window, int dtype, void* stream) {
+    int64_t window, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   AKT_CHECK(dtype == AKT_DTYPE_F16 || dtype == AKT_DTYPE_BF16,
             "dtype must be AKT_DTYPE_F16 or AKT_DTYPE_BF16, got %d", dtype);
@@ -309,9 +960,19 @@ extern "C" int akt_attention_weights_paged(
   AKT_CHECK(rows_aligned16(q, q_stride, 2) && rows_aligned16(kv_cache, kv_stride, 4) &&
                 aligned4(lse) && aligned4(weights),
             "tensors must have 16-byte aligned rows");
-  // Tiles that there can be at most.
-  const int64_t tiles = (total_pages * page_size / kWTile + batch) * num_kv_heads;
-  AKT_CHECK(tiles < (1ll << 31) && grid_fits(tiles, kWThreads), "problem too large");
+  // The axis stays below 2^50 (w_div).
+  AKT_CHECK((double)(total_pages * page_size / kWTile + batch) * num_kv_heads *
+                    (double)(total_q * G / 32 + 1 + kWTileCost + kWDiagCost * G) < 1e15,
+            "problem too large");
+  const int64_t wgs =
+      weight_wgs(batch, total_q, num_kv_heads, G, head_dim, page_size * total_pages);
+  const size_t need = akt_attention_weights_paged_workspace_size(
+      batch, total_q, num_q_heads, num_kv_heads, head_dim, page_size, total_pages);
+  if (!workspace || workspace_bytes < need)
+    return set_error(AKT_ERR_WORKSPACE, "attention weights need a workspace of %zu bytes, got %zu",
+                     need, workspace ? workspace_bytes : (size_t)0);
+  AKT_CHECK(aligned16(workspace), "the workspace must be 16-byte aligned");
+  AKT_CHECK(wgs <= (int64_t)(AKT_WORKSPACE_ZERO_BYTES - 256) / 4, "too many workgroups");
   WeightParams p = {};
   p.q = (const half_t*)q;
   p.pool = (const half_t*)kv_cache;
@@ -329,7 +990,7 @@ extern "C" int akt_attention_weights_paged(
   p.ss = kv_stride[3];
   p.w_sn = weight_stride[0];
   p.w_sh = weight_stride[1];
-  p.N = num_rows;
+  p.N = (int)(num_rows < (1ll << 31) ? num_rows : (1ll << 31) - 1);
   p.L = row_len;
   p.total_q = (int)total_q;
   p.total_pages = (int)total_pages;
@@ -348,9 +1009,11 @@ extern "C" int akt_attention_weights_paged(
   p.causal = causal ? 1 : 0;
   p.window = (int)(window < (1ll << 30) ? window : (1ll << 30));
   p.scale = softmax_scale * kLog2e;
+  p.arrive = (int*)((char*)workspace + 256);
+  p.partials = (float*)((char*)workspace + round_up(AKT_WORKSPACE_ZERO_BYTES, 256));
   hipStream_t st = (hipStream_t)stream;
   const bool bf16 = dtype == AKT_DTYPE_BF16;
-  if (head_dim == 64) return launch_weights<64>(p, bf16, tiles, st);
-  if (head_dim == 256) return launch_weights<256>(p, bf16, tiles, st);
-  return launch_weights<128>(p, bf16, tiles, st);
+  if (head_dim == 64) return launch_weights<64>(p, bf16, wgs, st);
+  if (head_dim == 256) return launch_weights<256>(p, bf16, wgs, st);
+  return launch_weights<128>(p, bf16, wgs, st);
 }

@@ -688,6 +688,10 @@ void attention_weights_paged(const at::Tensor& weights, const at::Tensor& q_,
   const float scale = softmax_scale.has_value() ? (float)*softmax_scale
                                                 : (float)(1.0 / std::sqrt((double)D));
   const DeviceGuard guard(dev);
+  hipStream_t st = stream_of(q);
+  const size_t ws_n =
+      akt_attention_weights_paged_workspace_size(B, T, Hq, Hkv, D, page, indices.numel());
+  at::Tensor ws = capture_workspace(ws_n, dev, st);
   const Strides qs = strides_of(q), ps = strides_of(pool);
   check_rc(akt_attention_weights_paged(
                ptr(q), (const int32_t*)ptr(q_indptr), (const float*)ptr(lse), ptr(pool),
@@ -695,7 +699,7 @@ void attention_weights_paged(const at::Tensor& weights, const at::Tensor& q_,
                (const int32_t*)ptr(last), (float*)ptr(weights), (const int32_t*)ptr(wr.rows), B, T,
                Hq, Hkv, D, page, indices.numel(), P, weights.size(0), weights.size(2), qs.v, ps.v,
                wr.stride, scale, causal ? 1 : 0, window.has_value() ? *window : INT64_MAX, dtype,
-               stream_of(q)),
+               ptr(ws), ws_n, st),
            "akt_attention_weights_paged");
 }
 

@@ -503,8 +503,13 @@ int akt_shared_prefix_paged_fwd(
  *   sequence whose row is outside [0, num_rows) is left out.
  *   window: only the last `window` tokens of each sequence count.
  * Keys on pages outside the pool are skipped.  head_dim: 64, 128 or 256; dtype AKT_DTYPE_F16 or
- * AKT_DTYPE_BF16 (q and the cache).
+ * AKT_DTYPE_BF16 (q and the cache).  The workspace is a decode workspace: its first
+ * AKT_WORKSPACE_ZERO_BYTES are zero before the first call and after every call.
  */
+size_t akt_attention_weights_paged_workspace_size(int64_t batch, int64_t total_q,
+                                                  int64_t num_q_heads, int64_t num_kv_heads,
+                                                  int64_t head_dim, int64_t page_size,
+                                                  int64_t total_pages);
 int akt_attention_weights_paged(
     const void* q, const int32_t* q_indptr, const float* lse, const void* kv_cache,
     const int32_t* kv_page_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len,
@@ -512,7 +517,7 @@ int akt_attention_weights_paged(
     int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t total_pages,
     int64_t num_pool_pages, int64_t num_rows, int64_t row_len, const int64_t q_stride[3],
     const int64_t kv_stride[5], const int64_t weight_stride[2], float softmax_scale, int causal,
-    int64_t window, int dtype, void* stream);
+    int64_t window, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Kept tokens close up within a cache, in place.  For each (sequence b, kv head h) and j <

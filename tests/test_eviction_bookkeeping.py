@@ -230,19 +230,24 @@ def test_shared_prefix_refuses_before_any_launch():
 
 def test_attention_weights_refuse_before_any_launch():
     lib = N.load()
+    size = lib.akt_attention_weights_paged_workspace_size
+    need = size(4, 4, 8, 2, 128, 16, 40)
+    assert need > N.WORKSPACE_ZERO_BYTES
+    assert size(0, 4, 8, 2, 128, 16, 40) == size(4, 4, 8, 3, 128, 16, 40) == size(4, 4, 8, 2, 96, 16, 40) == 0
 
     def call(B=4, T=4, Hq=8, Hkv=2, D=128, page=16, total=40, P=60, rows=4, L=100, scale=0.1, dtype=0,
-             window=1 << 40, q=P16, lse=P16, w=P16, which=P16, ks=(8192, 4096, 2048, 128, 1)):
+             window=1 << 40, q=P16, lse=P16, w=P16, which=P16, ks=(8192, 4096, 2048, 128, 1), ws=P16,
+             n=need):
         return lib.akt_attention_weights_paged(
             q, P16, lse, P16, P16, P16, P16, w, which, B, T, Hq, Hkv, D, page, total, P, rows, L,
-            _i64(1024, 128, 1), _i64(*ks), _i64(200, 100), scale, 1, window, dtype, None)
+            _i64(1024, 128, 1), _i64(*ks), _i64(200, 100), scale, 1, window, dtype, ws, n, None)
 
     for rc, kw in ((1, {"dtype": 1}), (1, {"rows": -1}), (1, {"window": -1}), (1, {"Hkv": 3}),
                    (2, {"D": 192}), (1, {"page": 0}), (1, {"lse": None}), (1, {"w": None}),
                    (1, {"which": None, "rows": 3}), (1, {"q": C.c_void_p(8)}),
                    (1, {"ks": (8192, 4096, 2048, 128, 2)}), (1, {"ks": (8192, 4096, 2048, 100, 1)}),
                    (1, {"scale": float("inf")}), (1, {"w": C.c_void_p(18)}),
-                   (1, {"total": 1 << 28}), (1, {"T": 1 << 29})):
+                   (1, {"total": 1 << 28}), (1, {"T": 1 << 29}), (3, {"n": need - 1}), (3, {"ws": None})):
         assert call(**kw) == rc, (kw, lib.akt_last_error())
     assert all(call(**kw) == 0 for kw in ({"B": 0}, {"T": 0}, {"rows": 0}, {"L": 0}, {"window": 0}))
 
