@@ -128,6 +128,21 @@ __device__ __forceinline__ float rows_sum(float v) {
   return xor32_sum(a + b);
 }
 
+// Inclusive prefix sum over the wave's lanes (two 16-bit halves at once: no
+// carry, a wave's counts stay below 2^16).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_inclusive_scan(uint32_t v) {
+  v = add_dpp<0x111, 0xf>(v);     // row_shr 1, 2, 4, 8: within 16 lanes
+  v = add_dpp<0x112, 0xf>(v);
+  v = add_dpp<0x114, 0xf>(v);
+  v = add_dpp<0x118, 0xf>(v);
+  v = add_dpp<0x142, 0xa>(v);     // lane 15 of rows 0 and 2 to rows 1 and 3
+  return add_dpp<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+}
+
 // ---------------------------------------------------------------------------
 // Arithmetic helpers.
 // ---------------------------------------------------------------------------

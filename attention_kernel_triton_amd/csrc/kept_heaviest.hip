@@ -3,27 +3,32 @@
 // index list (-1 padded) and a count, the form of the sparse decodes.  Equal sums go to the lower
 // index; a NaN counts as heavier than any number; -0 equals 0.
 //
-// One 1024-thread workgroup to a row.  The sums become 32-bit keys of the same order, and the key
-// of the lightest token that is still kept is found digit by digit (11, 11 and 10 bits): a
-// histogram in LDS of the keys that share the digits found so far, then a sum from the top that stops
-// at the bin where the count is reached.  The last pass walks the row in order and ranks what is
-// kept: heavier keys, and equal ones while any are wanted.  Lanes count in eight copies of a histogram
-// (lane mod 8), since sums of probabilities crowd into few binades.
+// One workgroup to a row.  The sums become 32-bit keys of the same order, and the key of the lightest
+// entry that is still kept is found digit by digit (11, 11 and 10 bits): a histogram in LDS of the
+// candidates that share the digits found so far, then a sum from the top that stops at the bin where
+// the count is reached, or at all digits that matter: where the bin's candidates are just those still
+// wanted, lower digits decide nothing (with hardly any equal sums the third is never looked at).  Then
+// what is kept is ranked in the row's order: heavier candidates, and equal ones while any are wanted.
+// Lanes count in four or eight copies of a histogram (lane mod that), since sums of probabilities crowd into few
+// binades.
 //
-// What bounds it: the passes of one workgroup over its row (L2 after the first), their LDS counts
-// and barriers; HBM reads a row once.
+// Rows of up to 64 k entries are read once and stay in registers (a wave's entries are consecutive,
+// so that ranks need the other waves once); longer ones are read again for each pass.
+//
+// What bounds it: with few rows, the round trips, LDS counts and barriers of one workgroup.
+#include <type_traits>
+
 #include "akt_common.hpp"
 #include "akt_host.hpp"
 
 namespace akt {
 namespace {
 
-constexpr int kHThreads = 1024;
+constexpr int kHThreads = 1024;  // of the kernel for long rows
 constexpr int kHWaves = kHThreads / kWave;
 constexpr int kHRun = 4;                       // consecutive entries to a lane
 constexpr int kHStep = kHThreads * kHRun;  // entries to a step
 constexpr int kHBins = 2048;
-constexpr int kHCopies = 8;
 
 struct HeavyParams {
   const float* w;  // [N, H, L]
@@ -42,91 +47,246 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return x != x ? 0xffffffffu : k;
 }
 
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ uint32_t wave_sum_scan(uint32_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t u = (uint32_t)__shfl_up((int)v, d, 64);
-    if (lane >= d) v += u;
+// What a workgroup's row asks for; false: all of it is kept, and written.
+struct HeavyRow {
+  const float* w;
+  int len, lo, hi;  // entries, and the candidates among them: lo .. hi - 1
+};
+template <int NT>
+__device__ __forceinline__ bool heavy_row(const HeavyParams& p, HeavyRow& r) {
+  const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
+  const int64_t row = p.rows ? (int64_t)p.rows[b] : b;
+  r.len = row < 0 || row >= p.N ? 0 : min(max(p.lengths[b], 0), p.L);
+  if (r.len <= p.keep) {
+    int32_t* const out = p.ind + (int64_t)blockIdx.x * p.keep;
+    for (int i = threadIdx.x; i < p.keep; i += NT) out[i] = i < r.len ? i : -1;
+    if (threadIdx.x == 0) p.nnz[blockIdx.x] = r.len;
+    return false;
   }
-  return v;
+  r.w = p.w + row * p.w_sn + h * p.w_sh;
+  r.lo = p.first;
+  r.hi = r.len - p.recent;
+  return true;
 }
 
-__global__ __launch_bounds__(kHThreads) void kept_heaviest_kernel(HeavyParams p) {
-  __shared__ __attribute__((aligned(16))) uint32_t hist[kHBins * kHCopies];
-  __shared__ uint32_t wave_tot[2][kHWaves];
-  __shared__ uint32_t found[2];  // digit, and how many are wanted of its keys
+// The digits found so far of the lightest kept candidate's key: those in `mask` are `key`, and of the
+// candidates that share them `want` are kept.
+struct HeavyKey {
+  uint32_t key, mask, want;
+};
+// LDS of the search: NC copies of a histogram, wave sums, and what a digit's search found.
+template <int NT, int NC>
+struct HeavyLds {
+  uint4_t hist[kHBins * NC / 4];
+  uint32_t tot[2][NT / kWave];
+  uint32_t digit, want, count;
+};
+// Finds the digits.  count(f): calls f(k) for the key k of each of the thread's candidates, and may
+// call it for 0, which is no number's key and the last in order.
+template <int NT, int NC, typename F>
+__device__ __forceinline__ HeavyKey find_key(HeavyLds<NT, NC>& lds, uint32_t want, F count) {
+  constexpr int BPT = kHBins / NT;  // bins to a thread
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
-  int32_t* const out = p.ind + (int64_t)blockIdx.x * p.keep;
-  const int64_t row = p.rows ? (int64_t)p.rows[b] : b;
-  const int len = row < 0 || row >= p.N ? 0 : min(max(p.lengths[b], 0), p.L);
-  if (len <= p.keep) {
-    for (int i = tid; i < p.keep; i += kHThreads) out[i] = i < len ? i : -1;
-    if (tid == 0) p.nnz[blockIdx.x] = len;
-    return;
+  uint32_t* const hist = reinterpret_cast<uint32_t*>(lds.hist) + (lane & (NC - 1));
+  HeavyKey r = {0, 0, want};
+  // One digit; whether the next ones matter.
+  auto digit = [&](auto pass_c) -> bool {
+    constexpr int kPass = decltype(pass_c)::value;
+    constexpr int kShift = kPass == 0 ? 21 : kPass == 1 ? 10 : 0;
+    constexpr uint32_t kDigits = kPass == 2 ? 1023u : 2047u;
+#pragma unroll
+    for (int i = 0; i < kHBins * NC / 4 / NT; ++i) lds.hist[i * NT + tid] = uint4_t{0, 0, 0, 0};
+    __syncthreads();
+    count([&](uint32_t k) {
+      if (kPass == 0 || (k & r.mask) == r.key)
+        atomicAdd(&hist[((k >> kShift) & kDigits) * NC], 1u);
+    });
+    __syncthreads();
+    // Thread t sums bins from the top: those from kHBins - 1 - BPT t down.
+    uint32_t c[BPT], mine = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      const uint4_t* v = lds.hist + (kHBins - 1 - BPT * tid - i) * NC / 4;
+      c[i] = 0;
+#pragma unroll
+      for (int j = 0; j < NC / 4; ++j) c[i] += v[j][0] + v[j][1] + v[j][2] + v[j][3];
+      mine += c[i];
+    }
+    const uint32_t incl = wave_inclusive_scan(mine);
+    if (lane == 63) lds.tot[0][wave] = incl;
+    __syncthreads();
+    uint32_t before = incl - mine;
+#pragma unroll
+    for (int i = 0; i < NT / kWave; ++i) {
+      const uint32_t t = lds.tot[0][i];
+      before += i < wave ? t : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      if (before < r.want && before + c[i] >= r.want) {
+        lds.digit = (uint32_t)(kHBins - 1 - BPT * tid - i);
+        lds.want = r.want - before;
+        lds.count = c[i];
+      }
+      before += c[i];
+    }
+    __syncthreads();
+    r.key |= (uint32_t)uniform((int)lds.digit) << kShift;
+    r.mask |= kDigits << kShift;
+    r.want = (uint32_t)uniform((int)lds.want);
+    return r.want != (uint32_t)uniform((int)lds.count);
+  };
+  if (want > 0 && digit(std::integral_constant<int, 0>{}) &&
+      digit(std::integral_constant<int, 1>{}))
+    digit(std::integral_constant<int, 2>{});
+  return r;
+}
+
+// Rows in registers.  Wave w has as many consecutive entries as the others, a multiple of 256; lane l
+// of its 64-entry chunk c has entry 64 c + l, so that a ballot has a chunk's bits in order.
+template <int NT, int PER>
+__global__ __launch_bounds__(NT) void kept_heaviest_kernel(HeavyParams p) {
+  constexpr int NC = NT == 1024 ? 8 : 4, NW = NT / kWave;
+  __shared__ HeavyLds<NT, NC> lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  HeavyRow r;
+  if (!heavy_row<NT>(p, r)) return;
+  const int len = uniform(r.len), lo = r.lo, hi = uniform(r.hi);
+  const int groups = (len + 256 * NW - 1) / (256 * NW);  // of four chunks, to a wave
+  const int e0 = wave * groups * 256;
+  // (Loads past the row's end read 0.)
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)r.w, 0, len * 4, kBufferWord3);
+  uint32_t key[PER];  // 0: not a candidate (no number's key)
+#pragma unroll
+  for (int c = 0; c < PER; c += 4)
+    if (c / 4 < groups)
+#pragma unroll
+      for (int i = c; i < c + 4; ++i)
+        key[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, (e0 + 64 * i + lane) * 4, 0, 0);
+#pragma unroll
+  for (int c = 0; c < PER; c += 4)
+    if (c / 4 < groups) {
+#pragma unroll
+      for (int i = c; i < c + 4; ++i) key[i] = order_key(__uint_as_float(key[i]));
+      const int e = e0 + 64 * c;
+      if (e < lo || e + 256 > hi)  // wave-uniform
+#pragma unroll
+        for (int i = c; i < c + 4; ++i) {
+          const int at = e0 + 64 * i + lane;
+          key[i] = at >= lo && at < hi ? key[i] : 0;
+        }
+    }
+  const HeavyKey f = find_key<NT, NC>(lds, (uint32_t)(p.keep - p.first - p.recent), [&](auto add) {
+#pragma unroll
+    for (int c = 0; c < PER; c += 4)
+      if (c / 4 < groups)
+#pragma unroll
+        for (int i = c; i < c + 4; ++i) add(key[i]);
+  });
+  // Bits of the entries kept for sure (heavier candidates, and those that are no candidates), and of
+  // the equal ones, of which the first f.want are kept; where no candidate is, nothing is heavier or
+  // equal.  Chunk i's go to LDS by lane i, and then thread t takes chunk t of the row.
+  const uint32_t mask = f.mask, least = f.mask ? f.key : 1u;
+  uint32_t sl = 0, sh = 0, ql = 0, qh = 0;
+#pragma unroll
+  for (int c = 0; c < PER; c += 4)
+    if (c / 4 < groups)
+#pragma unroll
+      for (int i = c; i < c + 4; ++i) {
+        const uint32_t k = key[i] & mask;
+        uint64_t s = __ballot(k > least);
+        const uint64_t q = __ballot(k == least);
+        const int e = e0 + 64 * i;
+        if (e < lo || e + 64 > hi) s |= __ballot(e + lane < lo || (e + lane >= hi && e + lane < len));
+        sl = lane == i ? (uint32_t)s : sl;
+        sh = lane == i ? (uint32_t)(s >> 32) : sh;
+        ql = lane == i ? (uint32_t)q : ql;
+        qh = lane == i ? (uint32_t)(q >> 32) : qh;
+      }
+  uint4_t* const bits = lds.hist;  // (its last reads are behind find_key's last barrier)
+  if (lane < 4 * groups) bits[wave * 4 * groups + lane] = uint4_t{sl, sh, ql, qh};
+  __syncthreads();
+  const int chunks = 4 * groups * NW;  // of the row: at most one to a thread
+  const uint4_t m = tid < chunks ? bits[tid] : uint4_t{0, 0, 0, 0};
+  uint64_t keep = (uint64_t)m[1] << 32 | m[0], equal = (uint64_t)m[3] << 32 | m[2];
+  const uint32_t s0 = (uint32_t)__builtin_popcountll(keep), q0 = (uint32_t)__builtin_popcountll(equal);
+  const uint32_t si = wave_inclusive_scan(s0), qi = wave_inclusive_scan(q0);
+  if (lane == 63) {
+    lds.tot[0][wave] = si;
+    lds.tot[1][wave] = qi;
   }
-  const float* const w = p.w + row * p.w_sn + h * p.w_sh;
-  const int lo = p.first, hi = len - p.recent;
+  __syncthreads();
+  int slot = (int)(si - s0), before = (int)(qi - q0);  // kept for sure, and equal, before the chunk
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int s = (int)lds.tot[0][i], q = (int)lds.tot[1][i];
+    slot += i < wave ? s : 0;
+    before += i < wave ? q : 0;
+  }
+  const int wanted = (int)f.want;
+  slot += min(before, wanted);
+  for (int n = wanted - before; equal && n > 0; --n) {
+    keep |= equal & -equal;
+    equal &= equal - 1;
+  }
+  // Every wave writes its chunks: lane l the entry of bit l, behind those of the bits below.
+  if (tid < chunks) bits[tid] = uint4_t{(uint32_t)keep, (uint32_t)(keep >> 32), (uint32_t)slot, 0};
+  __syncthreads();
+  int32_t* const out = p.ind + (int64_t)blockIdx.x * p.keep;
+#pragma unroll
+  for (int c = 0; c < PER; c += 4)
+    if (c / 4 < groups) {
+      uint4_t b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = bits[wave * 4 * groups + c + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (int)(b[i][2] + __builtin_amdgcn_mbcnt_hi(
+                                           b[i][1], __builtin_amdgcn_mbcnt_lo(b[i][0], 0)));
+        const bool is = ((lane < 32 ? b[i][0] : b[i][1]) >> (lane & 31)) & 1;
+        if (is && at < p.keep) out[at] = e0 + 64 * (c + i) + lane;
+      }
+    }
+  if (tid == 0) p.nnz[blockIdx.x] = p.keep;
+}
+
+// Rows of any length, read again for each pass.
+__global__ __launch_bounds__(kHThreads) void kept_heaviest_long_kernel(HeavyParams p) {
+  constexpr int NC = 8;
+  __shared__ HeavyLds<kHThreads, NC> lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  HeavyRow r;
+  if (!heavy_row<kHThreads>(p, r)) return;
+  const int len = r.len, lo = r.lo, hi = r.hi;
+  int32_t* const out = p.ind + (int64_t)blockIdx.x * p.keep;
   // The entries from e on that this lane looks at (entries past the row's end read as 0).
-  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)w, 0, len * 4, kBufferWord3);
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)r.w, 0, len * 4, kBufferWord3);
   auto load = [&](int e) {
     return as_float4u(
         __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, e * 4, 0, 0)));
   };
-
-  // ---- the key of the lightest kept entry: digits found so far, their mask, entries wanted.
-  uint32_t key = 0, mask = 0;
-  uint32_t want = (uint32_t)(p.keep - p.first - p.recent);
-  if (want > 0) {
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const uint32_t digits = pass == 2 ? 1023u : 2047u;
-      for (int i = tid; i < kHBins * kHCopies; i += kHThreads) hist[i] = 0;
-      __syncthreads();
-      for (int e = lo / kHRun * kHRun + tid * kHRun; e < hi; e += kHStep) {
-        const float4_t x = load(e);
+  const HeavyKey f =
+      find_key<kHThreads, NC>(lds, (uint32_t)(p.keep - p.first - p.recent), [&](auto add) {
+        constexpr int kAhead = 4;  // steps in flight
+        for (int e = lo / kHRun * kHRun + tid * kHRun; e < hi; e += kAhead * kHStep) {
+          float4_t x[kAhead];
 #pragma unroll
-        for (int i = 0; i < kHRun; ++i) {
-          const uint32_t k = order_key(x[i]);
-          if (e + i >= lo && e + i < hi && (k & mask) == key)
-            atomicAdd(&hist[((k >> shift) & digits) * kHCopies + (lane & (kHCopies - 1))], 1u);
+          for (int s = 0; s < kAhead; ++s) x[s] = load(e + s * kHStep);
+#pragma unroll
+          for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+            for (int i = 0; i < kHRun; ++i) {
+              const int at = e + s * kHStep + i;
+              if (at >= lo && at < hi) add(order_key(x[s][i]));
+            }
         }
-      }
-      __syncthreads();
-      // Thread t sums bins from the top: 2047 - 2 t and the one below it.
-      uint32_t c[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4_t* v = reinterpret_cast<const uint4_t*>(hist + (kHBins - 1 - 2 * tid - i) * kHCopies);
-#pragma unroll
-        for (int j = 0; j < kHCopies / 4; ++j) c[i] += v[j][0] + v[j][1] + v[j][2] + v[j][3];
-      }
-      const uint32_t incl = wave_sum_scan(c[0] + c[1], lane);
-      if (lane == 63) wave_tot[0][wave] = incl;
-      __syncthreads();
-      uint32_t before = incl - c[0] - c[1];
-      for (int i = 0; i < wave; ++i) before += wave_tot[0][i];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (before < want && before + c[i] >= want) {
-          found[0] = (uint32_t)(kHBins - 1 - 2 * tid - i);
-          found[1] = want - before;
-        }
-        before += c[i];
-      }
-      __syncthreads();
-      key |= found[0] << shift;
-      mask |= digits << shift;
-      want = found[1];
-    }
-  }
+      });
+  const uint32_t key = f.key, mask = f.mask;
 
   // ---- the kept entries in order: heavier than the key, or equal while any are wanted.
-  const bool none = p.keep == p.first + p.recent;
+  const bool none = mask == 0;  // no candidate is kept
   int kept = 0, equal = 0;  // before this step
-  const int wanted = (int)want;
+  const int wanted = (int)f.want;
   int buf = 0;
   float4_t nxt = load(tid * kHRun);
   for (int e0 = 0; e0 < len; e0 += kHStep, buf ^= 1) {
@@ -137,7 +297,7 @@ __global__ __launch_bounds__(kHThreads) void kept_heaviest_kernel(HeavyParams p)
     uint32_t sure = 0, same = 0;
 #pragma unroll
     for (int i = 0; i < kHRun; ++i) {
-      const uint32_t k = order_key(x[i]);
+      const uint32_t k = order_key(x[i]) & mask;
       const bool in = e + i >= lo && e + i < hi;
       const bool s = e + i < len && (!in || (!none && k > key));
       const bool q = in && !none && k == key;
@@ -145,13 +305,13 @@ __global__ __launch_bounds__(kHThreads) void kept_heaviest_kernel(HeavyParams p)
       same |= (q ? 1u : 0u) << i;
     }
     cnt = (uint32_t)__builtin_popcount(sure) | (uint32_t)__builtin_popcount(same) << 16;
-    const uint32_t incl = wave_sum_scan(cnt, lane);
-    if (lane == 63) wave_tot[buf][wave] = incl;
+    const uint32_t incl = wave_inclusive_scan(cnt);
+    if (lane == 63) lds.tot[buf][wave] = incl;
     __syncthreads();
     uint32_t before = incl - cnt, total = 0;
 #pragma unroll
     for (int i = 0; i < kHWaves; ++i) {
-      const uint32_t t = wave_tot[buf][i];
+      const uint32_t t = lds.tot[buf][i];
       if (i < wave) before += t;
       total += t;
     }
@@ -212,8 +372,19 @@ extern "C" int akt_kept_index_heaviest(const float* weights, const int32_t* leng
   p.keep = (int)keep;
   p.first = (int)first;
   p.recent = (int)recent;
+  // The smallest workgroup whose registers hold a row: fewer threads to a short row have fewer bins
+  // and waves to meet.
   KernelTimer timer;
-  timer.launch(kept_heaviest_kernel, dim3((unsigned)(batch * num_heads)), dim3(kHThreads), 0,
-               (hipStream_t)stream, p);
+  const dim3 grid((unsigned)(batch * num_heads));
+  hipStream_t st = (hipStream_t)stream;
+  auto small = [&](auto kernel) { timer.launch(kernel, grid, dim3(256), 0, st, p); };
+  auto large = [&](auto kernel) { timer.launch(kernel, grid, dim3(1024), 0, st, p); };
+  if (row_len <= 1024) small(kept_heaviest_kernel<256, 4>);
+  else if (row_len <= 2048) small(kept_heaviest_kernel<256, 8>);
+  else if (row_len <= 4096) small(kept_heaviest_kernel<256, 16>);
+  else if (row_len <= 16384) large(kept_heaviest_kernel<1024, 16>);
+  else if (row_len <= 32768) large(kept_heaviest_kernel<1024, 32>);
+  else if (row_len <= 65536) large(kept_heaviest_kernel<1024, 64>);
+  else timer.launch(kept_heaviest_long_kernel, grid, dim3(kHThreads), 0, st, p);
   return check_launch("kept_heaviest_kernel");
 }

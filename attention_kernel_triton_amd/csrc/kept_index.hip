@@ -39,21 +39,6 @@ constexpr int kStep = kKThreads * kPer;       // elements per step
 // 4-byte aligned (16 to a load), or mask bytes at any address (byte loads).
 enum : int { kUniform = 0, kMaskWords = 1, kMaskBytes = 2 };
 
-// Inclusive prefix sum over the wave's lanes (two 16-bit halves at once: no
-// carry, a wave's counts stay below 2^16).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_inclusive_scan(uint32_t v) {
-  v = add_dpp<0x111, 0xf>(v);     // row_shr 1, 2, 4, 8: within 16 lanes
-  v = add_dpp<0x112, 0xf>(v);
-  v = add_dpp<0x114, 0xf>(v);
-  v = add_dpp<0x118, 0xf>(v);
-  v = add_dpp<0x142, 0xa>(v);     // lane 15 of rows 0 and 2 to rows 1 and 3
-  return add_dpp<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
-}
-
 template <int SRC>
 __global__ __launch_bounds__(kKThreads) void kept_index_kernel(
     const uint8_t* __restrict__ mask, const float* __restrict__ draws, float ratio, int64_t n,

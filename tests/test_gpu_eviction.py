@@ -246,7 +246,7 @@ def check_select(dev, w, lengths, keep, first=0, recent=0, rows=None):
         assert g.dtype == torch.int32 and torch.equal(g.cpu(), x)
 
 
-@pytest.mark.parametrize("L", [1, 2, 63, 64, 65, 1000, 1024, 4095, 4096, 4097, 9000])
+@pytest.mark.parametrize("L", [1, 2, 63, 64, 65, 1000, 1024, 1025, 2049, 4095, 4096, 4097, 9000, 17000, 33000])
 @pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 0.97])
 def test_selections(dev, L, share):
     g = torch.Generator().manual_seed(L)
@@ -305,10 +305,9 @@ def test_selection_of_long_rows(dev):
     g = torch.Generator().manual_seed(3)
     w = torch.exp(2 * torch.randn(2, 1, 120001, generator=g))
     w[1] = torch.round(w[1] * 4) / 4
-    lengths = [120001, 100000]
-    ind, nnz = select_heaviest(w.to(dev), i32(lengths, dev), 12345, first=4, recent=77)
-    want = serving.heaviest(w, lengths, 12345, 4, 77)
-    assert torch.equal(ind.cpu(), want[0]) and torch.equal(nnz.cpu(), want[1])
+    for L, lengths in ((120001, [120001, 100000]), (65536, [65536, 65535]), (65537, [65537, 40000])):
+        for first, recent in ((4, 77), (0, 12345), (12000, 300)):
+            check_select(dev, w[:, :, :L].contiguous(), lengths, 12345, first, recent)
 
 
 def test_selection_replays(dev):
