@@ -9,7 +9,15 @@
 // and takes the entries in order; columns do not touch each other.  A page that a sequence shares can
 // be replaced: the slots of dst_indices, where they differ from the table's, take the rows instead.
 //
-// HBM-bound: 8 D bytes read and written a kept token and kv head.
+// Bound by memory: 4 D bytes read and 4 D written a kept token and kv head.  What it measured at 8
+// kv heads and D = 128, after steps (16 sequences of 1,025 to 1,088 tokens, 1,024 kept: 136 MB) and
+// after prompts (8 of 4,000 to 9,000 tokens, 2,500 kept, bf16: 167 MB): 25.6 and 44.4 us, or 5.3 and
+// 3.8 TB/s; without the look-ahead 26.1 and 56.2.  The prompts' case is 256 columns, one to a compute
+// unit, so what bounds it is how many rows of its column a workgroup has in flight.
+//   Columns of 64 bytes would be twice as many, and every line of 128 bytes would be touched by two
+// workgroups: 35.6 and 47.9 us (one sequence of 8,000 tokens to 4,000: 15.3 instead of 24.6).
+//   Batches of 128, 256 and 512 rows: 24.9, 25.6 and 29.0 us (step), 47.8, 44.4 and 44.3 (prompt);
+// more rows than that spill.
 #include "akt_common.hpp"
 #include "akt_host.hpp"
 
@@ -17,9 +25,9 @@ namespace akt {
 namespace {
 
 constexpr int kEThreads = 1024;
-constexpr int kELanes = 8;                         // 16-byte chunks of a column
+constexpr int kELanes = 8;                   // 16-byte chunks of a column
 constexpr int kERows = kEThreads / kELanes;  // rows at a time
-constexpr int kEPer = 4;                           // and times to a batch
+constexpr int kEPer = 2;                     // and times to a batch
 constexpr int kEBatch = kERows * kEPer;
 
 struct KeepParams {
@@ -41,6 +49,12 @@ struct KeepParams {
 __device__ __forceinline__ int keep_page(const KeepParams& p, int n) {
   const int q = (int)__umulhi((uint32_t)n, p.page_magic);
   return n - q * p.page_size >= p.page_size ? q + 1 : q;
+}
+
+// Waits for a value that was loaded: what reads a register waits for it, a barrier alone does not.
+template <typename T>
+__device__ __forceinline__ void arrived(const T& x) {
+  asm volatile("" ::"v"(x));
 }
 
 __global__ __launch_bounds__(kEThreads) void paged_keep_kernel(KeepParams p) {
@@ -69,6 +83,9 @@ __global__ __launch_bounds__(kEThreads) void paged_keep_kernel(KeepParams p) {
         ok[k] = j < nnz && t >= j && t < len && j < p.L;
         x[k] = ok[k] && t < p.L ? w[t] : 0.f;
       }
+      // Every wave's sums are here (not merely asked for) before any is overwritten.
+#pragma unroll
+      for (int k = 0; k < kEPer; ++k) arrived(x[k]);
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < kEPer; ++k)
@@ -84,30 +101,77 @@ __global__ __launch_bounds__(kEThreads) void paged_keep_kernel(KeepParams p) {
   const int chunk = (part - v * p.columns) * kELanes + tid % kELanes;
   half_t* const base = p.pool + v * p.skv + h * p.sh + 8 * chunk;
   const bool mine = chunk < p.cpr;
-  for (int j0 = 0; j0 < nnz; j0 += kEBatch) {
+  // A batch's entries, the pages of their rows, and the rows are looked up one batch after another:
+  // while a batch is written, the rows of the next one, the pages of the one after it and the entries of
+  // the third are on their way.  Loads come back in the order in which they are asked for, so the
+  // rows go last: the next batch's looking up does not wait for them.
+  struct Pages {
+    int t[kEPer], sid[kEPer], did[kEPer];  // t: token, -1: none
+  };
+  struct Rows {
     uint4_t x[kEPer];
-    half_t* to[kEPer];
+    half_t* to[kEPer];  // null: not moved
+  };
+  const int32_t* const dst = p.dst ? p.dst : p.indices;
+  auto slot = [&](int i, int k) -> int { return i * kEBatch + k * kERows + tid / kELanes; };
+  int e[kEPer];
+  Pages g;
+  auto load_entries = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < kEPer; ++k) e[k] = ind[min(slot(i, k), nnz - 1)];
+  };
+  auto load_pages = [&](int i) {
 #pragma unroll
     for (int k = 0; k < kEPer; ++k) {
-      const int j = j0 + k * kERows + tid / kELanes;
-      to[k] = nullptr;
-      const int t = mine && j < nnz ? ind[j] : -1;
-      if (t >= j && t < len) {
-        const int sl = keep_page(p, t), dl = keep_page(p, j);
-        const int sid = p.indices[ip0 + sl], did = (p.dst ? p.dst : p.indices)[ip0 + dl];
-        if ((uint32_t)sid < (uint32_t)p.num_pool_pages &&
-            (uint32_t)did < (uint32_t)p.num_pool_pages && (t != j || sid != did)) {
-          x[k] = ld16(base + sid * p.sp + (t - sl * p.page_size) * p.ss);
-          to[k] = base + did * p.sp + (j - dl * p.page_size) * p.ss;
-        }
-      }
+      const int j = slot(i, k);
+      g.t[k] = j < nnz && e[k] >= j && e[k] < len ? e[k] : -1;
+      g.sid[k] = p.indices[ip0 + keep_page(p, max(g.t[k], 0))];
+      g.did[k] = dst[ip0 + keep_page(p, min(j, nnz - 1))];
     }
+  };
+  const half_t* src[kEPer];
+  auto find_rows = [&](int i, Rows& r) {
+#pragma unroll
+    for (int k = 0; k < kEPer; ++k) {
+      const int j = slot(i, k), t = g.t[k];
+      const bool move = mine && t >= 0 && (uint32_t)g.sid[k] < (uint32_t)p.num_pool_pages &&
+                        (uint32_t)g.did[k] < (uint32_t)p.num_pool_pages &&
+                        (t != j || g.sid[k] != g.did[k]);
+      src[k] = base + g.sid[k] * p.sp + (t - keep_page(p, max(t, 0)) * p.page_size) * p.ss;
+      r.to[k] = move ? base + g.did[k] * p.sp + (j - keep_page(p, j) * p.page_size) * p.ss : nullptr;
+    }
+  };
+  auto load_rows = [&](Rows& r) {
+#pragma unroll
+    for (int k = 0; k < kEPer; ++k)
+      if (r.to[k]) r.x[k] = ld16(src[k]);
+  };
+  if (nnz == 0) return;
+  Rows ra, rb;
+  load_entries(0);
+  load_pages(0);
+  load_entries(1);
+  find_rows(0, ra);
+  load_pages(1);
+  load_entries(2);
+  load_rows(ra);
+  auto batch = [&](int i, Rows& r, Rows& next) {
+    find_rows(i + 1, next);
+    load_pages(i + 2);
+    load_entries(i + 3);
+    load_rows(next);
     // Every wave's rows are here (not merely asked for) before any is overwritten.
-    __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll
+    for (int k = 0; k < kEPer; ++k) arrived(r.x[k]);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEPer; ++k)
-      if (to[k]) st16(to[k], x[k]);
+      if (r.to[k]) st16(r.to[k], r.x[k]);
+  };
+  for (int i = 0; i * kEBatch < nnz; i += 2) {
+    batch(i, ra, rb);
+    if ((i + 1) * kEBatch >= nnz) break;
+    batch(i + 1, rb, ra);
   }
 }
 
