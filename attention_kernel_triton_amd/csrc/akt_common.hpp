@@ -142,6 +142,40 @@ __device__ __forceinline__ uint32_t wave_inclusive_scan(uint32_t v) {
   v = add_dpp<0x142, 0xa>(v);     // lane 15 of rows 0 and 2 to rows 1 and 3
   return add_dpp<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
 }
+// The same of 64-bit numbers, and the sum of floats over the wave (the same in every lane and run).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t add_dpp64(int64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+__device__ __forceinline__ int64_t wave_inclusive_scan64(int64_t v) {
+  v = add_dpp64<0x111, 0xf>(v);
+  v = add_dpp64<0x112, 0xf>(v);
+  v = add_dpp64<0x114, 0xf>(v);
+  v = add_dpp64<0x118, 0xf>(v);
+  v = add_dpp64<0x142, 0xa>(v);
+  return add_dpp64<0x143, 0xc>(v);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_dppf(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = add_dppf<0x111, 0xf>(v);
+  v = add_dppf<0x112, 0xf>(v);
+  v = add_dppf<0x114, 0xf>(v);
+  v = add_dppf<0x118, 0xf>(v);
+  v = add_dppf<0x142, 0xa>(v);
+  v = add_dppf<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+// Lane `lane` (wave-uniform) of a 64-bit number.
+__device__ __forceinline__ int64_t read_lane64(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
 
 // ---------------------------------------------------------------------------
 // Arithmetic helpers.

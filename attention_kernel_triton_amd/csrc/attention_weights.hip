@@ -127,9 +127,6 @@ __device__ __forceinline__ int64_t w_uniform64(int64_t v) {
   const uint32_t hi = (uint32_t)uniform((int)(uint32_t)(v >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ int64_t w_shfl64(int64_t v, int src) {
-  return (int64_t)(((uint64_t)shfl_u((uint32_t)(v >> 32), src) << 32) | shfl_u((uint32_t)v, src));
-}
 // floor(a / b) for 0 <= a < 2^50, b >= 1 (see div_range in paged_chunk.hip).
 __device__ __forceinline__ int64_t w_div(int64_t a, int64_t b) {
   return w_uniform64((int64_t)((double)a / (double)b));
@@ -156,14 +153,6 @@ __device__ __forceinline__ bool is_few(const WeightParams& p, const WSeq& s) {
 }
 __device__ __forceinline__ bool is_many(const WeightParams& p, const WSeq& s) {
   return s.row >= 0 && s.n * p.G > kWFew;
-}
-__device__ __forceinline__ int64_t w_scan64(int64_t v, int lane) {  // inclusive sum over the lanes
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t u = w_shfl64(v, lane - d < 0 ? 0 : lane - d);
-    if (lane >= d) v += u;
-  }
-  return v;
 }
 
 // Keys of a step of few rows, and what a unit's start costs a wave, in steps.
@@ -196,11 +185,11 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
     const WSeq s = seq_of(p, tab, b);
     return is_few(p, s) ? (int64_t)few_length(s, KEYS) * p.Hkv : 0;
   };
-  int64_t length = seq_length(lane), inc = w_scan64(length, lane);
-  int64_t total = w_uniform64(w_shfl64(inc, 63));
+  int64_t length = seq_length(lane), inc = wave_inclusive_scan64(length);
+  int64_t total = read_lane64(inc, 63);
   for (int jb = 64; jb < p.B; jb += 64)
-    total += w_uniform64(w_shfl64(w_scan64(seq_length(jb + lane), lane), 63));
-  const int64_t Lw = w_uniform64((total + W * kWWaves - 1) / (W * kWWaves));
+    total += read_lane64(wave_inclusive_scan64(seq_length(jb + lane)), 63);
+  const int64_t Lw = w_div(total + W * kWWaves - 1, W * kWWaves);
   const int64_t x0 = range * Lw;
   if (x0 >= total) return;
   const int64_t x1 = x0 + Lw < total ? x0 + Lw : total;
@@ -258,14 +247,14 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
       if (m) {
         const int l = __builtin_ctzll(m);
         cur.b = uniform(jb + l);
-        at += w_uniform64(w_shfl64(inc - length, l));
+        at += read_lane64(inc - length, l);
         break;
       }
-      at += w_uniform64(w_shfl64(inc, 63));
+      at += read_lane64(inc, 63);
       jb += 64;
       if (jb >= p.B) return;
       length = seq_length(jb + lane);
-      inc = w_scan64(length, lane);
+      inc = wave_inclusive_scan64(length);
     }
     take_seq(cur);
     const int unit = (cur.len + KEYS - 1) / KEYS + kFewCost;
@@ -469,11 +458,11 @@ __device__ __forceinline__ void many_weights(const WeightParams& p, const WTable
     const WHead h = head_of(p, s);
     return tile_start(h, h.tiles) * p.Hkv;
   };
-  int64_t length = seq_length(lane), inc = w_scan64(length, lane);
-  int64_t total = w_uniform64(w_shfl64(inc, 63));
+  int64_t length = seq_length(lane), inc = wave_inclusive_scan64(length);
+  int64_t total = read_lane64(inc, 63);
   for (int jb = 64; jb < p.B; jb += 64)
-    total += w_uniform64(w_shfl64(w_scan64(seq_length(jb + lane), lane), 63));
-  const int64_t Lw = w_uniform64(max((total + W - 1) / W, (int64_t)(kWTileCost + 1)));
+    total += read_lane64(wave_inclusive_scan64(seq_length(jb + lane)), 63);
+  const int64_t Lw = max(w_div(total + W - 1, W), (int64_t)(kWTileCost + 1));
   const int64_t x0 = wg * Lw;
   if (x0 >= total) return;
   const int64_t x1 = x0 + Lw < total ? x0 + Lw : total;
@@ -542,14 +531,14 @@ __device__ __forceinline__ void many_weights(const WeightParams& p, const WTable
       if (m) {
         const int l = __builtin_ctzll(m);
         cur.b = uniform(jb + l);
-        at += w_uniform64(w_shfl64(inc - length, l));
+        at += read_lane64(inc - length, l);
         break;
       }
-      at += w_uniform64(w_shfl64(inc, 63));
+      at += read_lane64(inc, 63);
       jb += 64;
       if (jb >= p.B) return;
       length = seq_length(jb + lane);
-      inc = w_scan64(length, lane);
+      inc = wave_inclusive_scan64(length);
     }
     take_seq(cur);
     const int64_t per = tile_start(head, head.tiles);
@@ -833,23 +822,20 @@ __device__ __forceinline__ void many_weights(const WeightParams& p, const WTable
 template <int D>
 __device__ __forceinline__ int share_of(const WeightParams& p, const WTable& tab, int W) {
   const int lane = threadIdx.x & 63;
-  double few = 0, many = 0;
+  float few = 0, many = 0;
   for (int b = lane; b < p.B; b += 64) {
     const WSeq s = seq_of(p, tab, b);
-    if (is_few(p, s)) few += few_length(s, few_keys(D));
+    if (is_few(p, s)) few += (float)few_length(s, few_keys(D));
     if (is_many(p, s)) {
       const WHead h = head_of(p, s);
-      many += (double)tile_start(h, h.tiles);
+      many += (float)tile_start(h, h.tiles);
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    few += __shfl_xor(few, d, 64);
-    many += __shfl_xor(many, d, 64);
-  }
+  few = wave_sum(few);
+  many = wave_sum(many);
   if (many == 0) return W;
   if (few == 0) return 0;
-  const int s = 8 * (int)(W / 8 * (few / (few + many)) + 0.5);
+  const int s = 8 * (int)((float)(W / 8) * (few / (few + many)) + 0.5f);
   return uniform(min(max(s, 8), W - 8));
 }
 

@@ -100,6 +100,9 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int src) {
 }
 // floor(a / b) for 0 <= a < 2^50, b >= 1: doubles hold both, and the quotient's distance
 // to the next integer (at least 1 / b) is more than its rounding.
+__device__ __forceinline__ int64_t div_range64(int64_t a, int64_t b) {
+  return uniform64((int64_t)((double)a / (double)b));
+}
 __device__ __forceinline__ int div_range(int64_t a, int64_t b) {
   return uniform((int)((double)a / (double)b));
 }
@@ -394,6 +397,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
     return mine(s) ? head_length(p, s) * p.Hkv : 0;
   };
   auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
+    if constexpr (SHARED) return wave_inclusive_scan64(v);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int64_t u = shfl64(v, lane0 - d < 0 ? 0 : lane0 - d);
@@ -1184,7 +1188,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
       // 30000 54.5 / 42.8, two of those 71.5 / 62.0, four after 10000 49.8 / 45.9; eight after
       // 10000, past the limit, 76 either way).
       const int used = SPLIT && seqs * p.Hkv <= W / 8 ? W : ranges;
-      Lw = (total + used - 1) / used;
+      Lw = SHARED ? div_range64(total + used - 1, used) : (total + used - 1) / used;
       if (Lw < p.min_keys) Lw = p.min_keys;
       Lw = uniform64(Lw);
       x0 = wg * Lw;
@@ -1306,26 +1310,32 @@ __device__ __forceinline__ void shared_few(const ChunkParams&, char*, const int4
 template <int D, bool SHARED>
 __device__ __forceinline__ int split_share(const ChunkParams& p, const int4* table, int W) {
   constexpr int kRows = 32 * chunk_waves(D);
-  constexpr double kLow = SHARED ? kSharedTileCostLow : 1;
-  constexpr double kHigh = SHARED ? kSharedTileCost : chunk_tile_cost(D);
+  typedef std::conditional_t<SHARED, float, double> Sum;
+  constexpr Sum kLow = SHARED ? kSharedTileCostLow : 1;
+  constexpr Sum kHigh = SHARED ? kSharedTileCost : chunk_tile_cost(D);
   const int lane = threadIdx.x & 63;
-  double few = 0, many = 0;
+  Sum few = 0, many = 0;
   for (int b = lane; b < num_seqs<SHARED>(p); b += 64) {
     const Seq<SHARED> s = load_seq<SHARED>(p, b, table);
-    const double len = (double)(SHARED && s.n <= p.split_tokens ? (s.n > 0 ? s.len + kWaveUnitCost : 0)
+    const Sum len = (Sum)(SHARED && s.n <= p.split_tokens ? (s.n > 0 ? s.len + kWaveUnitCost : 0)
                                                                 : head_length(p, s));
     if (s.n <= p.split_tokens) few += len;
     else
-      many += len * (kLow + (kHigh - kLow) / kRows * min((double)s.n * p.G, (double)kRows));
+      many += len * (kLow + (kHigh - kLow) / kRows * min((Sum)s.n * p.G, (Sum)kRows));
   }
+  if constexpr (SHARED) {
+    few = wave_sum(few);
+    many = wave_sum(many);
+  } else {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    few += __shfl_xor(few, d, 64);
-    many += __shfl_xor(many, d, 64);
+    for (int d = 1; d < 64; d *= 2) {
+      few += __shfl_xor(few, d, 64);
+      many += __shfl_xor(many, d, 64);
+    }
   }
   if (many == 0) return W;
   if (few == 0) return 0;
-  const int s = 8 * (int)(W / 8 * (few / (few + many)) + 0.5);
+  const int s = 8 * (int)((Sum)(W / 8) * (few / (few + many)) + (Sum)0.5);
   return uniform(min(max(s, 8), W - 8));
 }
 

@@ -42,21 +42,11 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
   auto seq_length = [&](int b) -> int64_t {
     return b < ns ? (int64_t)cost(load_seq<true>(p, b, table)) * p.Hkv : 0;
   };
-  auto scan64 = [&](int64_t v) -> int64_t {  // inclusive sum over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int64_t u = shfl64(v, lane - d < 0 ? 0 : lane - d);
-      if (lane >= d) v += u;
-    }
-    return v;
-  };
-  int64_t len = seq_length(lane), inc = scan64(len);
-  int64_t total = uniform64(shfl64(inc, 63));
+  int64_t len = seq_length(lane), inc = wave_inclusive_scan64(len);
+  int64_t total = read_lane64(inc, 63);
   for (int jb = 64; jb < ns; jb += 64)
-    total += uniform64(shfl64(scan64(seq_length(jb + lane)), 63));
-  int64_t Lw = (total + W * WAVES - 1) / (W * WAVES);
-  if (Lw < kCkWaveKeys) Lw = kCkWaveKeys;
-  Lw = uniform64(Lw);
+    total += read_lane64(wave_inclusive_scan64(seq_length(jb + lane)), 63);
+  const int64_t Lw = max(div_range64(total + W * WAVES - 1, W * WAVES), (int64_t)kCkWaveKeys);
   const int64_t x0 = range * Lw;
   if (x0 >= total) return;
   const int64_t x1 = x0 + Lw < total ? x0 + Lw : total;
@@ -131,13 +121,13 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
       if (m) {
         const int l = __builtin_ctzll(m);
         lead.b = uniform(jb + l);
-        at += uniform64(shfl64(inc - len, l));
+        at += read_lane64(inc - len, l);
         break;
       }
-      at += uniform64(shfl64(inc, 63));
+      at += read_lane64(inc, 63);
       jb += 64;
       len = seq_length(jb + lane);
-      inc = scan64(len);
+      inc = wave_inclusive_scan64(len);
     }
     ns_seq = load_seq_uniform<true>(p, lead.b, table);
     const int unit = cost(ns_seq);

@@ -4,11 +4,13 @@ Tolerances as for chunk attention (tests/test_gpu_chunk.py): the two parts' prob
 rounded to the type in numerator and normaliser, their sums are joined in 32 bits (the factors
 2^(m - M) of two maxima are as exact as the probabilities' own exponents), and O is rounded once.
 """
+import ctypes as C
 import math
 
 import pytest
 import torch
 
+from attention_kernel_triton_amd import _native as N
 from attention_kernel_triton_amd.chunk_flash_attention_paged import flash_attention_chunk_paged
 from attention_kernel_triton_amd.shared_prefix_flash_attention_paged import (
     flash_attention_shared_prefix_paged)
@@ -193,6 +195,45 @@ def test_strided_tensors_and_rows_of_no_sequence(dev):
     o, lse = flash_attention_shared_prefix_paged(*a, return_lse=True)
     o2, lse2 = flash_attention_shared_prefix_paged(*c.args(dev), return_lse=True)
     assert torch.equal(o[:4], o2[:4]) and torch.equal(lse[:4], lse2[:4])
+
+
+@pytest.mark.parametrize("word", [-1, 0x7fffffff, 6, 0])
+@pytest.mark.parametrize("D,n", [(64, 1), (128, 9), (256, 2)])
+def test_a_workspace_may_hold_anything_behind_its_counters(dev, D, n, word):
+    """Rows of no sequence, and rows that no part writes because q_indptr is not in order, name no
+    slots: whatever the workspace holds, they lead nowhere, and rows of no sequence stay."""
+    c = Case([(3, 700)], [4, 300, 9], [n, 2, n], 4, 2, D, 16, slack=5)
+    a = c.args(dev)
+    T, Hq = c.q.shape[:2]
+    lib = N.load()
+    sizes = (3, T, Hq, 2, D, 16, a[4].numel())
+    size = lib.akt_shared_prefix_paged_workspace_size(*sizes, 1, a[8].numel())
+    i64 = lambda x: (C.c_int64 * len(x))(*x)  # noqa: E731
+    ptr = lambda x: C.c_void_p(x.data_ptr())  # noqa: E731
+
+    def call(q_indptr, group_indptr):
+        ws = torch.full((-(-size // 4),), word, dtype=torch.int32, device=dev)
+        ws[:N.WORKSPACE_ZERO_BYTES // 4] = 0
+        o = torch.full((T, Hq, D), 7.0, dtype=F16, device=dev)
+        lse = torch.full((T, Hq), 7.0, device=dev)
+        t = dict(zip(c.names, a), q_indptr=q_indptr, group_indptr=group_indptr)
+        rc = lib.akt_shared_prefix_paged_fwd(
+            *(ptr(t[k]) for k in ("q", "q_indptr", "pool", "indptr", "indices", "last", "group_indptr",
+                                  "prefix_indptr", "prefix_indices", "prefix_last")), ptr(o), ptr(lse),
+            *sizes, 1, a[8].numel(), c.pool.shape[0], i64(a[0].stride()), i64(a[2].stride()), D ** -0.5, 1,
+            0, ptr(ws), size, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0
+        torch.cuda.synchronize()
+        return o, lse
+
+    o, lse = call(a[1], a[6])
+    o2, lse2 = flash_attention_shared_prefix_paged(*a, return_lse=True)
+    end = int(c.q_indptr[-1])
+    assert torch.equal(o[:end], o2[:end]) and torch.equal(lse[:end], lse2[:end])
+    assert bool((o[end:] == 7).all()) and bool((lse[end:] == 7).all())
+    i32 = dict(dtype=torch.int32, device=dev)
+    o, lse = call(torch.tensor([0, T - 1, 2, T - 2], **i32), torch.tensor([1, 3], **i32))
+    assert bool((o[T - 1:] == 7).all()) and bool((lse[T - 1:] == 7).all())
 
 
 def test_results_do_not_depend_on_the_run_or_the_stream(dev):
