@@ -1300,7 +1300,7 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
 #ifdef AKT_CHUNK_SHARED
 #include "paged_shared_few.hpp"
 #else
-template <int D, bool BF16>
+template <int D, bool BF16, bool LSE>
 __device__ __forceinline__ void shared_few(const ChunkParams&, char*, const int4*, int, int) {}
 #endif
 
@@ -1367,7 +1367,7 @@ void paged_chunk_kernel(ChunkParams p) {
   const int S = uniform(sm_share);
   if constexpr (SHARED) {
     if (block < S) {
-      shared_few<D, BF16>(p, lds, table, block, S);
+      shared_few<D, BF16, LSE>(p, lds, table, block, S);
       return;
     }
   }
@@ -1388,10 +1388,8 @@ template <int D, bool BF16, bool GRP>
 int launch_lse(const ChunkParams& p, hipStream_t st) {
   KernelTimer timer;
   const dim3 grid(p.wgs), block(64 * chunk_waves(D));
-  if constexpr (kShared)
-    timer.launch(paged_chunk_kernel<D, BF16, GRP, true, true>, grid, block, 0, st, p);
-  else if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true, false>, grid, block, 0, st, p);
-  else timer.launch(paged_chunk_kernel<D, BF16, GRP, false, false>, grid, block, 0, st, p);
+  if (p.lse) timer.launch(paged_chunk_kernel<D, BF16, GRP, true, kShared>, grid, block, 0, st, p);
+  else timer.launch(paged_chunk_kernel<D, BF16, GRP, false, kShared>, grid, block, 0, st, p);
   return check_launch("paged_chunk_kernel");
 }
 

@@ -19,7 +19,7 @@ struct FewStep {
   int k0, k1, k;   // the part that the wave serves, and the step's first key
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool LSE>
 __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, const int4* table,
                                            int block, int W) {
   constexpr int WAVES = chunk_waves(D);
@@ -279,7 +279,7 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
       const float p0 = fast_exp2(__builtin_fmaf(sv[i], c, -m_run));
       const float p1 = fast_exp2(__builtin_fmaf(sv[i + 1], c, -m_run));
       pk[i >> 1] = E::pack2(p0, p1);
-      x_part += p0 + p1;
+      if constexpr (LSE) x_part += p0 + p1;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) l_part = E::dot2(pk[i], E::kOnes, l_part);
