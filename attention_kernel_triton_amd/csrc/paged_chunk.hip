@@ -354,10 +354,11 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Unit<
 }
 
 // The units of the ranges of workgroup `block` of W, on the axis of the sequences of few tokens
-// (SPLIT) or of many.  lds: the workgroup's tile buffers.
+// (SPLIT) or of many.  lds: the workgroup's tile buffers.  total: the axis's length, where prefixes
+// are shared.
 template <int D, bool BF16, bool GRP, bool LSE, bool SHARED, bool SPLIT>
 __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, const int4* table,
-                                            int block, int W) {
+                                            int block, int W, int64_t total = 0) {
   constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
@@ -1174,14 +1175,21 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
   int last_b = -1, last_kvh = 0, last_r = 0;
 #pragma clang loop unroll(disable)
   for (int pass = 0; pass < 2; ++pass) {
-    int64_t len = seq_length(lane0), inc = scan64(len);
+    int64_t len = 0, inc = 0;
+    if constexpr (!SHARED) {
+      len = seq_length(lane0);
+      inc = scan64(len);
+    }
     if (pass == 0) {
-      int64_t total = uniform64(shfl64(inc, 63));
-      int seqs = __builtin_popcountll(__ballot(len > 0));
-      for (int jb = 64; jb < num_seqs<SHARED>(p); jb += 64) {
-        const int64_t more = seq_length(jb + lane0);
-        total += uniform64(shfl64(scan64(more), 63));
-        seqs += __builtin_popcountll(__ballot(more > 0));
+      int seqs = 0;
+      if constexpr (!SHARED) {
+        total = uniform64(shfl64(inc, 63));
+        seqs = __builtin_popcountll(__ballot(len > 0));
+        for (int jb = 64; jb < p.B; jb += 64) {
+          const int64_t more = seq_length(jb + lane0);
+          total += uniform64(shfl64(scan64(more), 63));
+          seqs += __builtin_popcountll(__ballot(more > 0));
+        }
       }
       // Where few units share the axis, one range to a workgroup, not one to a team: half the
       // partials to a unit (us, D = 128 over 8 kv heads, a team / a workgroup: one token after
@@ -1200,17 +1208,23 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
     int b = 0;
     int64_t U = 0;  // the sequence's start
     for (int jb = 0;;) {
+      if constexpr (SHARED) {  // (here and nowhere else: every copy is fetched cold)
+        len = seq_length(jb + lane0);
+        inc = scan64(len);
+      }
       const uint64_t m = __ballot(U + inc > x);
       if (m) {
         const int l = __builtin_ctzll(m);
         b = uniform(jb + l);
-        U += uniform64(shfl64(inc - len, l));
+        U += SHARED ? read_lane64(inc - len, l) : uniform64(shfl64(inc - len, l));
         break;
       }
-      U += uniform64(shfl64(inc, 63));
+      U += SHARED ? read_lane64(inc, 63) : uniform64(shfl64(inc, 63));
       jb += 64;
-      len = seq_length(jb + lane0);
-      inc = scan64(len);
+      if constexpr (!SHARED) {
+        len = seq_length(jb + lane0);
+        inc = scan64(len);
+      }
     }
     Seq<SHARED> s = load_seq_uniform<SHARED>(p, b, table);
     int64_t hlen = uniform64(head_length(p, s));
@@ -1301,42 +1315,63 @@ __device__ __forceinline__ void chunk_range(const ChunkParams& p, char* lds, con
 #include "paged_shared_few.hpp"
 #else
 template <int D, bool BF16, bool LSE>
-__device__ __forceinline__ void shared_few(const ChunkParams&, char*, const int4*, int, int) {}
+__device__ __forceinline__ void shared_few(const ChunkParams&, char*, const int4*, int, int, int64_t) {}
 #endif
 
 // Workgroups (of all W, a multiple of 8) for the sequences of few tokens, where a launch may hold
 // both kinds: in proportion to the lengths of the two axes, a key of the other weighing 1 for a
 // unit of hardly any rows up to chunk_tile_cost for one of all rows.
-template <int D, bool SHARED>
-__device__ __forceinline__ int split_share(const ChunkParams& p, const int4* table, int W) {
+template <int D>
+__device__ __forceinline__ int split_share(const ChunkParams& p, int W) {
   constexpr int kRows = 32 * chunk_waves(D);
-  typedef std::conditional_t<SHARED, float, double> Sum;
-  constexpr Sum kLow = SHARED ? kSharedTileCostLow : 1;
-  constexpr Sum kHigh = SHARED ? kSharedTileCost : chunk_tile_cost(D);
   const int lane = threadIdx.x & 63;
-  Sum few = 0, many = 0;
-  for (int b = lane; b < num_seqs<SHARED>(p); b += 64) {
-    const Seq<SHARED> s = load_seq<SHARED>(p, b, table);
-    const Sum len = (Sum)(SHARED && s.n <= p.split_tokens ? (s.n > 0 ? s.len + kWaveUnitCost : 0)
-                                                                : head_length(p, s));
+  double few = 0, many = 0;
+  for (int b = lane; b < p.B; b += 64) {
+    const Seq<false> s = load_seq<false>(p, b);
+    const double len = (double)head_length(p, s);
     if (s.n <= p.split_tokens) few += len;
     else
-      many += len * (kLow + (kHigh - kLow) / kRows * min((Sum)s.n * p.G, (Sum)kRows));
+      many += len * (1 + (chunk_tile_cost(D) - 1) / kRows * min((double)s.n * p.G, (double)kRows));
   }
-  if constexpr (SHARED) {
-    few = wave_sum(few);
-    many = wave_sum(many);
-  } else {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      few += __shfl_xor(few, d, 64);
-      many += __shfl_xor(many, d, 64);
-    }
+  for (int d = 1; d < 64; d *= 2) {
+    few += __shfl_xor(few, d, 64);
+    many += __shfl_xor(many, d, 64);
   }
   if (many == 0) return W;
   if (few == 0) return 0;
-  const int s = 8 * (int)((Sum)(W / 8) * (few / (few + many)) + (Sum)0.5);
+  const int s = 8 * (int)(W / 8 * (few / (few + many)) + 0.5);
   return uniform(min(max(s, 8), W - 8));
+}
+// The same where prefixes are shared (a key weighs kSharedTileCostLow to kSharedTileCost), and the
+// lengths of the two axes.
+struct Shares {
+  int64_t few, many;
+  int wgs;
+};
+template <int D>
+__device__ __forceinline__ Shares shared_shares(const ChunkParams& p, const int4* table, int W) {
+  constexpr float kRows = 32 * chunk_waves(D);
+  constexpr float kLow = kSharedTileCostLow, kSlope = (kSharedTileCost - kSharedTileCostLow) / kRows;
+  const int lane = threadIdx.x & 63;
+  int64_t few = 0, many = 0;
+  float cost = 0;
+  for (int b = lane; b < num_seqs<true>(p); b += 64) {
+    const Seq<true> s = load_seq<true>(p, b, table);
+    if (s.n <= p.split_tokens) {
+      if (s.n > 0) few += s.len + kWaveUnitCost;
+    } else {
+      const int64_t len = head_length(p, s);
+      many += len;
+      cost += (float)len * (kLow + kSlope * min((float)s.n * p.G, kRows));
+    }
+  }
+  few = read_lane64(wave_inclusive_scan64(few), 63);
+  many = read_lane64(wave_inclusive_scan64(many), 63);
+  cost = wave_sum(cost);
+  const int s = 8 * (int)((float)(W / 8) * ((float)few / ((float)few + cost)) + 0.5f);
+  const int wgs = many == 0 ? W : few == 0 ? 0 : min(max(s, 8), W - 8);
+  return Shares{few * p.Hkv, many * p.Hkv, wgs};
 }
 
 template <int D, bool BF16, bool GRP, bool LSE, bool SHARED>
@@ -1361,23 +1396,33 @@ void paged_chunk_kernel(ChunkParams p) {
   // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
   // of them in what follows.
   __shared__ int sm_share;
-  const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D, SHARED>(p, table, W) : p.kinds == kCkFew ? W : 0;
-  if (threadIdx.x == 0) sm_share = share;
-  __syncthreads();
-  const int S = uniform(sm_share);
   if constexpr (SHARED) {
-    if (block < S) {
-      shared_few<D, BF16, LSE>(p, lds, table, block, S);
-      return;
+    __shared__ int64_t sm_total[2];
+    if (threadIdx.x < 64) {
+      const Shares c = shared_shares<D>(p, table, W);
+      if (threadIdx.x == 0) {
+        sm_share = c.wgs;
+        sm_total[0] = c.few;
+        sm_total[1] = c.many;
+      }
     }
+    __syncthreads();
+    const int S = uniform(sm_share);
+    if (block < S) shared_few<D, BF16, LSE>(p, lds, table, block, S, uniform64(sm_total[0]));
+    else
+      chunk_range<D, BF16, GRP, LSE, true, false>(p, lds, table, block - S, W - S,
+                                                  uniform64(sm_total[1]));
+  } else {
+    const int share = p.kinds == (kCkFew | kCkMany) ? split_share<D>(p, W) : p.kinds == kCkFew ? W : 0;
+    if (threadIdx.x == 0) sm_share = share;
+    __syncthreads();
+    const int S = uniform(sm_share);
+    if (block < S) chunk_range<D, BF16, GRP, LSE, false, true>(p, lds, table, block, S);
+    else
+      chunk_range<D, BF16, GRP, LSE, false, false>(p, lds, table, block - S, W - S);
   }
-  if (!SHARED && block < S)
-    chunk_range<D, BF16, GRP, LSE, SHARED, true>(p, lds, table, block, S);
-  else
-    chunk_range<D, BF16, GRP, LSE, SHARED, false>(p, lds, table, block - S, W - S);
 }
 
-// The instances of this translation unit: with or without shared prefixes.
 #ifdef AKT_CHUNK_SHARED
 constexpr bool kShared = true;
 #else

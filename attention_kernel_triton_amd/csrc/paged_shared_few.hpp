@@ -21,7 +21,7 @@ struct FewStep {
 
 template <int D, bool BF16, bool LSE>
 __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, const int4* table,
-                                           int block, int W) {
+                                           int block, int W, int64_t total) {
   constexpr int WAVES = chunk_waves(D);
   typedef Elt<BF16> E;
   typedef typename E::v8 v8;
@@ -42,10 +42,6 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
   auto seq_length = [&](int b) -> int64_t {
     return b < ns ? (int64_t)cost(load_seq<true>(p, b, table)) * p.Hkv : 0;
   };
-  int64_t len = seq_length(lane), inc = wave_inclusive_scan64(len);
-  int64_t total = read_lane64(inc, 63);
-  for (int jb = 64; jb < ns; jb += 64)
-    total += read_lane64(wave_inclusive_scan64(seq_length(jb + lane)), 63);
   const int64_t Lw = max(div_range64(total + W * WAVES - 1, W * WAVES), (int64_t)kCkWaveKeys);
   const int64_t x0 = range * Lw;
   if (x0 >= total) return;
@@ -116,7 +112,8 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
   FewStep lead;  // the step whose page ids are asked for
   {
     int64_t at = 0;
-    for (int jb = 0;;) {
+    for (int jb = 0;; jb += 64) {
+      const int64_t len = seq_length(jb + lane), inc = wave_inclusive_scan64(len);
       const uint64_t m = __ballot(at + inc > x0);
       if (m) {
         const int l = __builtin_ctzll(m);
@@ -125,9 +122,6 @@ __device__ __forceinline__ void shared_few(const ChunkParams& p, char* lds, cons
         break;
       }
       at += read_lane64(inc, 63);
-      jb += 64;
-      len = seq_length(jb + lane);
-      inc = wave_inclusive_scan64(len);
     }
     ns_seq = load_seq_uniform<true>(p, lead.b, table);
     const int unit = cost(ns_seq);
