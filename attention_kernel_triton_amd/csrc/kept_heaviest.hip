@@ -15,7 +15,10 @@
 // Rows of up to 64 k entries are read once and stay in registers (a wave's entries are consecutive,
 // so that ranks need the other waves once); longer ones are read again for each pass.
 //
-// What bounds it: with few rows, the round trips, LDS counts and barriers of one workgroup.
+// What bounds it: with few rows, the round trips, LDS counts and barriers of one workgroup.  128 rows
+// of about 1,060, 1,024 kept: 7.4 to 7.8 us, of which a launch is 4; 64 rows of 20,000 to 40,000,
+// 4,000 kept: 25.7 us, of which the loads take 2, a digit's counts 1.7 and its search 1, what is
+// written 3 to 6 (the entries as they are ranked, scattered over 64 lanes' slots).
 #include <type_traits>
 
 #include "akt_common.hpp"
@@ -372,16 +375,15 @@ extern "C" int akt_kept_index_heaviest(const float* weights, const int32_t* leng
   p.keep = (int)keep;
   p.first = (int)first;
   p.recent = (int)recent;
-  // The smallest workgroup whose registers hold a row: fewer threads to a short row have fewer bins
-  // and waves to meet.
+  // Few threads to a short row have few bins and waves to meet; the registers hold what a row
+  // needs (us, half of 32 rows of so many kept, 256 threads / 1024: 1,000 6.4 / 8.2, 2,000 7.3 /
+  // 8.1, 4,000 9.7 / 8.6, 8,000 13.7 / 10.7; 32,000 with 32 / 64 entries to a thread 21.1 / 21.9; read
+  // again for each pass 35.4, and of 65,000 65 against 36).
   KernelTimer timer;
   const dim3 grid((unsigned)(batch * num_heads));
   hipStream_t st = (hipStream_t)stream;
-  auto small = [&](auto kernel) { timer.launch(kernel, grid, dim3(256), 0, st, p); };
   auto large = [&](auto kernel) { timer.launch(kernel, grid, dim3(1024), 0, st, p); };
-  if (row_len <= 1024) small(kept_heaviest_kernel<256, 4>);
-  else if (row_len <= 2048) small(kept_heaviest_kernel<256, 8>);
-  else if (row_len <= 4096) small(kept_heaviest_kernel<256, 16>);
+  if (row_len <= 2048) timer.launch(kept_heaviest_kernel<256, 8>, grid, dim3(256), 0, st, p);
   else if (row_len <= 16384) large(kept_heaviest_kernel<1024, 16>);
   else if (row_len <= 32768) large(kept_heaviest_kernel<1024, 32>);
   else if (row_len <= 65536) large(kept_heaviest_kernel<1024, 64>);
