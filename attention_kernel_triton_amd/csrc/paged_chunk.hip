@@ -38,6 +38,10 @@
 // in the order of the ranges (not of arrival, so results do not depend on it) and
 // leaves the counter at zero.  Nothing waits for another workgroup.
 //
+// Shared prefixes (SHARED).  A group's tokens together are one more sequence behind the others, whose
+// keys are the prefix, seen whole by every row.  Every part leaves a state (state_row), a second
+// kernel joins them (paged_shared.hip), and units of few rows are served by paged_shared_few.hpp.
+//
 // Tiles (many).  As in the dense prefill kernel: K and V tiles go global -> registers -> one
 // of four LDS buffers, three tiles ahead; both products run transposed so that a lane owns
 // a row; the running max is raised only when a step's sum says so.  The page ids of a tile

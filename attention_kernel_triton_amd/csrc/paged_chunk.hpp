@@ -20,15 +20,20 @@ constexpr int kCkUnitCost = 128;  // cost of a unit's start and end, in keys
 __host__ __device__ constexpr int chunk_split_rows(int D) { return D <= 128 ? 32 : 64; }
 constexpr int kCkFew = 1, kCkMany = 2;
 // With shared prefixes a wave serves a range of few rows alone: the grain of its cuts, the cost of
-// a unit's start and end in keys, and the fewest keys (with costs) of a range.
+// a unit's start and end in keys, and the fewest keys (with costs) of a range; and the cost of a unit
+// of many rows, whose 32-bit states are written.  Measured (us; a decode step of 32 sequences behind
+// 4,096 tokens / 64 samples behind 20,001 / eight prompts behind 8,000; as they are 29.3 / 81.4 / 335):
+// costs of few 128 29.6 / 82.5 / 339; fewest keys 128 29.5 / 82.2 / 336, 384 32.5 / 81.8 / 336; costs of
+// many 160 29.2 / 87.0 / 426, 640 30.2 / 81.7 / 345.
 constexpr int kCkWaveBlock = 64, kWaveUnitCost = 64, kCkWaveKeys = 192;
-constexpr int kSharedUnitCost = 320;  // and of a unit of many rows
+constexpr int kSharedUnitCost = 320;
 // A key of a unit of many rows costs a workgroup as much as so many of a unit of few (us at 1.4,
 // 2 and 3, 777 new tokens beside 15 single ones: D = 128 73.9 / 69.4 / 72.4, D = 256 77.6 / 83.6
 // / 97.8, D = 64 75.2 / 69.8 / 67.9; 2000 beside 7 after 3000 to 9000, D = 128 327 / 334 / 592).
 __host__ __device__ constexpr double chunk_tile_cost(int D) { return D <= 128 ? 2.0 : 1.4; }
 
-// The same with shared prefixes, by rows from hardly any to all.
+// The same with shared prefixes, by rows from hardly any to all (the same three at 1 to 1.5: 30.6 /
+// 82.3 / 336, at 2 to 3: 31.6 / 85.0 / 335).
 constexpr double kSharedTileCostLow = 1.5, kSharedTileCost = 2.0;
 // Bytes of a row's state: (m, l, exact l, tag) and fp32 sums of P.V.
 __host__ __device__ constexpr int64_t state_bytes(int D) { return 16 + 4 * D; }
