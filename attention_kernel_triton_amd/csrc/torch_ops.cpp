@@ -626,7 +626,7 @@ struct WeightRows {
   at::Tensor rows;
 };
 WeightRows weight_rows(const at::Tensor& weights, const c10::optional<at::Tensor>& rows_,
-                       const at::Device& dev, int64_t B, int64_t H) {
+                       const at::Device& dev, int64_t B, int64_t H, bool written) {
   need_gpu("weights", weights);
   same_device("weights", weights, dev);
   if (weights.scalar_type() != at::kFloat)
@@ -636,6 +636,10 @@ WeightRows weight_rows(const at::Tensor& weights, const c10::optional<at::Tensor
     throw py::value_error("weights must be [N, Hkv, L], got " + c10::str(weights.sizes()));
   if (weights.size(2) > 1 && weights.stride(2) != 1)
     throw py::value_error("weights need a unit last stride");
+  if (written && weights.numel() > 0 &&
+      ((weights.size(0) > 1 && weights.stride(0) == 0) ||
+       (weights.size(1) > 1 && weights.stride(1) == 0)))
+    throw py::value_error("weights are written: their rows must not be one and the same memory");
   WeightRows r{{weights.stride(0), weights.stride(1)}, at::Tensor()};
   if (rows_.has_value() && rows_->defined()) {
     r.rows = int32_on("rows", *rows_, dev).contiguous();
@@ -683,7 +687,7 @@ void attention_weights_paged(const at::Tensor& weights, const at::Tensor& q_,
   if (lse_.dim() != 2 || lse_.size(0) != T || lse_.size(1) != Hq)
     throw py::value_error("lse must be [" + std::to_string(T) + ", " + std::to_string(Hq) + "]");
   at::Tensor lse = lse_.contiguous();
-  const WeightRows wr = weight_rows(weights, rows, dev, B, Hkv);
+  const WeightRows wr = weight_rows(weights, rows, dev, B, Hkv, true);
   if (window.has_value() && *window < 0) throw py::value_error("window must be non-negative");
   const float scale = softmax_scale.has_value() ? (float)*softmax_scale
                                                 : (float)(1.0 / std::sqrt((double)D));
@@ -711,7 +715,7 @@ py::tuple kept_heaviest(const at::Tensor& weights, const at::Tensor& lengths_, i
   at::Tensor lengths = int32_on("lengths", lengths_, dev).contiguous();
   if (lengths.dim() != 1) throw py::value_error("lengths must be [B]");
   const int64_t B = lengths.numel();
-  const WeightRows wr = weight_rows(weights, rows, dev, B, -1);
+  const WeightRows wr = weight_rows(weights, rows, dev, B, -1, false);
   if (keep < 0 || first < 0 || recent < 0 || first > keep || recent > keep - first)
     throw py::value_error("keep must be at least first + recent, and none negative");
   const DeviceGuard guard(dev);
@@ -898,7 +902,7 @@ void keep_tokens(const at::Tensor& pool, const at::Tensor& indptr_, const at::Te
   }
   const bool sums = weights.has_value() && weights->defined();
   WeightRows wr{{0, 0}, at::Tensor()};
-  if (sums) wr = weight_rows(*weights, rows, dev, B, Hkv);
+  if (sums) wr = weight_rows(*weights, rows, dev, B, Hkv, true);
   const DeviceGuard guard(dev);
   const Strides ps = strides_of(pool);
   check_rc(akt_paged_keep(ptr(pool), (const int32_t*)ptr(indptr), (const int32_t*)ptr(indices),

@@ -100,10 +100,11 @@ def test_sums_of_a_prompt_in_many_blocks(dev):
     Step([100], [900], 4, 1, 256, 16).check(dev)
 
 
-@pytest.mark.parametrize("B", [64, 65, 200])
+@pytest.mark.parametrize("B", [64, 65, 200, 1030])
 def test_sums_of_many_sequences(dev, B):
     g = torch.Generator().manual_seed(B)
     n = torch.randint(0, 4, (B,), generator=g).tolist()
+    n[B - 3] = 30
     ctx = torch.randint(0, 90, (B,), generator=g).tolist()
     n[B // 2:B // 2 + 20] = [0] * 20
     Step(ctx, n, 4, 2, 64, 16).check(dev)
@@ -227,6 +228,8 @@ def test_sums_refusals(dev):
     call()
     for err, over in ((TypeError, {"w": a["w"].half()}), (ValueError, {"w": a["w"].cpu()}),
                       (ValueError, {"w": a["w"][:, :1]}), (ValueError, {"w": a["w"][..., ::2]}),
+                      (ValueError, {"w": a["w"][:1].expand_as(a["w"])}),
+                      (ValueError, {"w": a["w"][:, :1].expand_as(a["w"])}),
                       (ValueError, {"w": a["w"][:1], "rows": None}), (TypeError, {"lse": a["lse"].half()}),
                       (ValueError, {"lse": a["lse"][:1]}), (ValueError, {"lse": a["lse"].cpu()}),
                       (TypeError, {"q": a["q"].float()}), (TypeError, {"pool": a["pool"].bfloat16()}),
@@ -473,6 +476,7 @@ def test_move_refusals(dev):
                     (ValueError, {"nnz": a["nnz"][:1]}), (ValueError, {"dst": a["indices"][:-1]}),
                     (ValueError, {"weights": w[:1]}), (TypeError, {"weights": w.double()}),
                     (ValueError, {"weights": w, "rows": i32([1], dev)}),
+                    (ValueError, {"weights": w[:, :1].expand_as(w)}),
                     (ValueError, {"indptr": a["indptr"][:2]}), (ValueError, {"pool": a["pool"][..., ::2]})):
         with pytest.raises(err):
             call(**kw)

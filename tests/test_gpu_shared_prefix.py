@@ -123,6 +123,15 @@ def test_more_sequences_and_groups_than_lanes(dev):
     Case([(2, i % 50) for i in range(70)], ctx, n, 4, 2, 64, 16, before=3).check(dev)
 
 
+def test_more_sequences_than_the_kernel_keeps_places_of(dev):
+    g = torch.Generator().manual_seed(1)
+    B = 1000
+    n = torch.randint(0, 3, (B,), generator=g).tolist()
+    n[400], n[990] = 40, 70
+    ctx = torch.randint(0, 20, (B,), generator=g).tolist()
+    Case([(9, i % 40) for i in range(100)], ctx, n, 2, 1, 64, 16, before=5).check(dev)
+
+
 def test_own_keys_or_prefix_may_be_missing(dev):
     """No own token beyond the contract (a table without pages), empty prefixes, no groups at all."""
     c = Case([(2, 100), (1, 0)], [0, 5, 0], [1, 1, 1], 8, 2, 64, 16)
