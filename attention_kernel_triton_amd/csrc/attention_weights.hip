@@ -31,12 +31,12 @@
 // Keys that a row does not see are left out by a select, rows that saw none (lse -inf) count nothing.
 //
 // What it measured (us; bf16 or fp16, 32 query heads over 8, D = 128): one token each of 32 sequences over
-// 256 to 8,192 keys 46 (201 MB, 4.4 TB/s; 63.7 with a tile of 256 keys to a workgroup and no
+// 256 to 8,192 keys 43.6 (201 MB, 4.6 TB/s; 63.7 with a tile of 256 keys to a workgroup and no
 // look-ahead), 2,048 tokens after 6,000 142 (118 GFLOP, 830 TFLOP/s; 312 with one block of rows staged
 // at a time and whole tiles: 256 keys of each of 8 heads are 256 tiles of unlike lengths).  There a
 // block of 32 rows by 256 keys takes a wave about 142 VALU instructions beside its 16 MFMAs; the matrix
 // pipe is busy 38% of the time, and two workgroups to a processor take 1.07 us a block each where one
-// alone takes 0.85: the two kinds of instructions hardly overlap.  Five tokens after twelve: 6.1,
+// alone takes 0.85: the two kinds of instructions hardly overlap.  Five tokens after twelve: 5.7,
 // of which a launch is 4; the rest is the sequences' table, the page ids, K and q, one after another.
 #include <math.h>
 
@@ -307,33 +307,33 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
 #pragma unroll
       for (int k = 0; k < KS; ++k) kf[i][k] = ld16(src[i] + 16 * k);
   };
-  // Rows: fragments of row l32 (the last one's again behind it), and -lse log2(e) of the rows of
-  // the lane's registers: register 4 j + i of half g is row 8 j + 4 g + i.
+  // Rows: fragments of row l32 (the last one's again behind it) and its lse, which is looked at when the
+  // unit's first step is served (its keys, asked for before, then need not be waited for here).
   uint4_t qf[KS];
-  float nl[16];
-  uint32_t gone = 0;  // bit r: register r's row is not there, or drew on none (lse -inf)
+  float lse_row;
+  bool fresh = true;
   auto load_rows = [&](const FewWStep& s) {
+    const int row = min(l32, s.n * p.G - 1), tok = div_magic(row, p.G, p.g_magic);
+    const int head = s.kvh * p.G + row - tok * p.G;
+    const half_t* src = p.q + (int64_t)(s.q0 + tok) * p.q_st + (int64_t)head * p.q_sh + 8 * g;
+    lse_row = p.lse[(int64_t)(s.q0 + tok) * p.Hq + head];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[k] = ld16(src + 16 * k);
+    fresh = true;
+  };
+  // -lse log2(e) of the rows of the lane's registers: register 4 j + i of half g is row 8 j + 4 g + i.
+  float nl[16];
+  uint32_t gone = 0;  // bit i: row i is not there, or drew on none (lse -inf)
+  auto take_rows = [&](const FewWStep& s) {
     const int rows = s.n * p.G;
-    {
-      const int row = min(l32, rows - 1), tok = div_magic(row, p.G, p.g_magic);
-      const half_t* src = p.q + (int64_t)(s.q0 + tok) * p.q_st +
-                          (int64_t)(s.kvh * p.G + row - tok * p.G) * p.q_sh + 8 * g;
+    const bool none = l32 >= rows || lse_row == -__builtin_inff();
+    const float n = none ? -__builtin_inff() : -lse_row * kLog2e;
+    gone = (uint32_t)__ballot(none);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) qf[k] = ld16(src + 16 * k);
-    }
-    gone = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = 8 * (r / 4) + 4 * g + r % 4;
-      nl[r] = -__builtin_inff();
-      if (8 * (r / 4) < rows) {  // wave-uniform
-        const int rr = min(row, rows - 1), tok = div_magic(rr, p.G, p.g_magic);
-        const float l = p.lse[(int64_t)(s.q0 + tok) * p.Hq + s.kvh * p.G + rr - tok * p.G];
-        const bool none = row >= rows || l == -__builtin_inff();
-        if (!none) nl[r] = -l * kLog2e;
-        gone |= none ? 1u << r : 0u;
-      }
-    }
+    for (int r = 0; r < 16; ++r)
+      if (8 * (r / 4) < rows)  // wave-uniform
+        nl[r] = __shfl(n, 8 * (r / 4) + 4 * g + r % 4, 64);
+    fresh = false;
   };
   const float c = p.scale;
   // Weights of a step's keys, added to their sums by half g for keys 32 g + l32 (one column: half 0).
@@ -373,7 +373,7 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row = 8 * j + 4 * g + r;
-            const int last = (gone >> (4 * j + r)) & 1 ? -1
+            const int last = (gone >> row) & 1 ? -1
                              : p.causal               ? first + div_magic(row, p.G, p.g_magic)
                                                       : s.len - 1;
 #pragma unroll
@@ -403,8 +403,8 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
   // ---- the stream.
   uint4_t kA[NC][KS], kB[NC][KS];
   bool okA[NC], okB[NC];
-  load_rows(cur);
   load_ids(cur);
+  load_rows(cur);
   FewWStep next = cur;
   advance(next);
   load_k(cur, next, kA, okA);
@@ -413,6 +413,7 @@ __device__ __forceinline__ void few_weights(const WeightParams& p, const WTable&
     if (next.b >= 0) advance(after);
     const float old = load_old(cur);
     if (next.b >= 0) load_k(next, after, k1, ok1);
+    if (fresh) take_rows(cur);
     serve(cur, k0, ok0, old);
     if (next.b < 0) return false;
     if (next.b != cur.b || next.kvh != cur.kvh) load_rows(next);
