@@ -32,11 +32,11 @@
 //
 // What it measured (us; bf16 or fp16, 32 query heads over 8, D = 128): one token each of 32 sequences over
 // 256 to 8,192 keys 43.6 (201 MB, 4.6 TB/s; 63.7 with a tile of 256 keys to a workgroup and no
-// look-ahead), 2,048 tokens after 6,000 142 (118 GFLOP, 830 TFLOP/s; 312 with one block of rows staged
+// look-ahead), 2,048 tokens after 6,000 139 (118 GFLOP, 850 TFLOP/s; 312 with one block of rows staged
 // at a time and whole tiles: 256 keys of each of 8 heads are 256 tiles of unlike lengths).  There a
 // block of 32 rows by 256 keys takes a wave about 142 VALU instructions beside its 16 MFMAs; the matrix
 // pipe is busy 38% of the time, and two workgroups to a processor take 1.07 us a block each where one
-// alone takes 0.85: the two kinds of instructions hardly overlap.  Five tokens after twelve: 5.7,
+// alone takes 0.85: the two kinds of instructions hardly overlap.  Five tokens after twelve: 5.3,
 // of which a launch is 4; the rest is the sequences' table, the page ids, K and q, one after another.
 #include <math.h>
 
