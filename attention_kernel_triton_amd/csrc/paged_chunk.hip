@@ -140,6 +140,18 @@ __device__ __forceinline__ bool in_table(const ChunkParams& p) {
 }
 // Table entries outside their ranges are taken clamped, so nothing outside the arrays is
 // touched.
+struct Prefix {
+  int b0, b1, ip0, len;  // sequences b0 .. b1 - 1, first page table entry, tokens
+};
+__device__ __forceinline__ Prefix load_prefix(const ChunkParams& p, int i) {
+  Prefix x;
+  x.b0 = min(max(p.group_indptr[i], 0), p.B);
+  x.b1 = min(max(p.group_indptr[i + 1], x.b0), p.B);
+  x.ip0 = min(max(p.prefix_indptr[i], 0), p.prefix_pages);
+  const int np = min(max(p.prefix_indptr[i + 1], x.ip0), p.prefix_pages) - x.ip0;
+  x.len = np > 0 ? (np - 1) * p.page_size + min(max(p.prefix_last[i], 0), p.page_size) : 0;
+  return x;
+}
 template <bool SHARED>
 __device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b,
                                                 const int4* table = nullptr) {
@@ -152,14 +164,11 @@ __device__ __forceinline__ Seq<SHARED> load_seq(const ChunkParams& p, int b,
     }
     s.more = !s.prefix && p.groups > 0 && b >= p.group_indptr[0] && b < p.group_indptr[p.groups];
     if (s.prefix) {
-      const int i = b - p.B;
-      const int b0 = min(max(p.group_indptr[i], 0), p.B);
-      const int b1 = min(max(p.group_indptr[i + 1], b0), p.B);
-      s.q0 = min(max(p.q_indptr[b0], 0), p.total_q);
-      s.n = b1 > b0 ? min(max(p.q_indptr[b1], s.q0), p.total_q) - s.q0 : 0;
-      s.ip0 = min(max(p.prefix_indptr[i], 0), p.prefix_pages);
-      const int np = min(max(p.prefix_indptr[i + 1], s.ip0), p.prefix_pages) - s.ip0;
-      s.len = np > 0 ? (np - 1) * p.page_size + min(max(p.prefix_last[i], 0), p.page_size) : 0;
+      const Prefix x = load_prefix(p, b - p.B);
+      s.q0 = min(max(p.q_indptr[x.b0], 0), p.total_q);
+      s.n = x.b1 > x.b0 ? min(max(p.q_indptr[x.b1], s.q0), p.total_q) - s.q0 : 0;
+      s.ip0 = x.ip0;
+      s.len = x.len;
       return s;
     }
   }
@@ -1388,13 +1397,27 @@ void paged_chunk_kernel(ChunkParams p) {
   const int4* table = nullptr;
   if constexpr (SHARED) {
     __shared__ int4 sm_table[kCkTable];
+    __shared__ int sm_end;  // end of the last sequence's tokens
     if (in_table(p)) {
       for (int b = threadIdx.x; b < num_seqs<true>(p); b += 64 * chunk_waves(D)) {
-        const Seq<true> s = load_seq<true>(p, b);
-        sm_table[b] = int4{s.q0, s.n | s.more << 30, s.ip0, s.len};  // (n < 2^30)
+        if (b < p.B) {
+          const Seq<true> s = load_seq<true>(p, b);
+          sm_table[b] = int4{s.q0, s.n | s.more << 30, s.ip0, s.len};  // (n < 2^30)
+          if (b == p.B - 1) sm_end = min(max(p.q_indptr[p.B], 0), p.total_q);
+        } else {  // its tokens from the sequences' places, below
+          const Prefix x = load_prefix(p, b - p.B);
+          sm_table[b] = int4{x.b0, x.b1, x.ip0, x.len};
+        }
       }
       __syncthreads();
       table = sm_table;
+      if (threadIdx.x < 64)
+        for (int b = p.B + threadIdx.x; b < num_seqs<true>(p); b += 64) {
+          const int4 t = sm_table[b];
+          const int q0 = t.x < p.B ? sm_table[t.x].x : sm_end;
+          const int q1 = t.y < p.B ? sm_table[t.y].x : sm_end;
+          sm_table[b] = int4{q0, t.y > t.x ? max(q1 - q0, 0) : 0, t.z, t.w};
+        }
     }
   }
   // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
