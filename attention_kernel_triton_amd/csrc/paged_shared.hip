@@ -38,6 +38,7 @@ template <int D, bool BF16, int PG>
 __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(ChunkParams p) {
   constexpr int LPR = D / 4;  // lanes to a row, 4 dims each
   constexpr int RPB = kJoinThreads / LPR / PG;  // rows to a workgroup
+  static_assert(RPB >= 1, "a row's threads are in one workgroup");
   const int rows = p.total_q * p.Hq;
   const int pg = PG == 1 ? 0 : (int)threadIdx.x / (LPR * RPB);
   const int in = (int)threadIdx.x % (LPR * RPB);
