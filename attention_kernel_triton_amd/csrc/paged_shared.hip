@@ -16,7 +16,7 @@
 // rows by the round trips to the places, the slots, and the slots' later batches.  Joining in
 // the kernel before by the last part to arrive cost more: the parts of a cut unit ended one by one,
 // and the wave that came last joined all rows alone (a decode step of 32 sequences behind 4,096
-// tokens: 50.6 us so, 29.3 now, 5 of them here; of 64 k rows in two or three parts 26 us of 325).
+// tokens: 50.6 us so, 28.3 now, 5 of them here; of 64 k rows in two or three parts 26 us of 325).
 #include <type_traits>
 
 #include "akt_common.hpp"

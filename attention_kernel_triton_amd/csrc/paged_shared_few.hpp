@@ -10,10 +10,10 @@
 // a unit are joined: see state_row.
 //
 // Bound by memory (K and V once) in long launches, by the start in short ones: the sequences'
-// places, the share, the wave's place on the axis, page ids, K and V stand one behind another, about 10 of the
-// 24 us of a decode step of 32 sequences with 100 to 1,000 own keys.  With teams of four waves to a
+// places, the share, the wave's place on the axis, page ids, K and V stand one behind another, about 9 of the
+// 23 us of a decode step of 32 sequences with 100 to 1,000 own keys.  With teams of four waves to a
 // range, as without shared prefixes, units this short spend their time on a team's start, merge and
-// barriers (that step: 50.6 us, 29.3 now; 33.7 with this stream and the join alone).
+// barriers (that step: 50.6 us, 28.3 now; 33.7 with this stream and the join alone).
 
 static_assert(kWaveUnitCost >= kCkWaveBlock, "a unit's last block lies before its end on the axis");
 
