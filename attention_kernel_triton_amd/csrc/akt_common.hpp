@@ -177,6 +177,13 @@ __device__ __forceinline__ int64_t read_lane64(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+// Orders what lanes of this wave stored in LDS before what other lanes of it load from there.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ---------------------------------------------------------------------------
 // Arithmetic helpers.
 // ---------------------------------------------------------------------------

@@ -1418,6 +1418,8 @@ void paged_chunk_kernel(ChunkParams p) {
           const int q1 = t.y < p.B ? sm_table[t.y].x : sm_end;
           sm_table[b] = int4{q0, t.y > t.x ? max(q1 - q0, 0) : 0, t.z, t.w};
         }
+      // Read by other lanes of the wave in shared_shares, by the other waves behind the barrier after it.
+      wave_lds_sync();
     }
   }
   // The share goes through LDS: passed on in a register, it made the compiler spill 96 more
