@@ -298,8 +298,11 @@ class PagedKVCache:
         Neighbours in seq_ids that share leading pages form groups; the last counts[i] tokens of each
         sequence (default: one) are its queries and stay out of the prefixes."""
         counts = [1] * len(seq_ids) if counts is None else counts
+        return self._split(seq_ids, self._groups(seq_ids, counts))
+
+    def _split(self, seq_ids, groups):
         group, prefixes, own = [0], [], []
-        for a, end, held in self._groups(seq_ids, counts):
+        for a, end, held in groups:
             group.append(end)
             prefixes.append((self._pages.get(seq_ids[a], [])[:held], held * self.page_size))
             for s in seq_ids[a:end]:
@@ -368,7 +371,7 @@ class PagedKVCache:
         flash_attention_chunk_paged returns for q over the grown cache.  A call that is refused
         leaves the sequences with the tokens they had.
         shared_prefix: leading pages that neighbours in seq_ids share (fork) are read once for all
-        of them (flash_attention_shared_prefix_paged).
+        of them (flash_attention_shared_prefix_paged); where none do, the step is as without it.
         observe: where the cache keeps sums of attention weight, the last `observe` of each
         sequence's new tokens add theirs (default: all; 0: none).  A whole prompt's cost is about half its
         attention again.
@@ -394,8 +397,11 @@ class PagedKVCache:
                 q = append_paged_kv_rotary(q, k_new, v_new, q_indptr, self.pool, *table, inv_freq,
                                            interleaved=interleaved, factor=factor, **at)
             kw = dict(causal=causal, softmax_scale=softmax_scale, return_lse=return_lse or watch)
-            if shared_prefix:
-                own = self.split_table(seq_ids, counts)
+            # With no page in common the shared call would only add states and their join (us, 16
+            # prompts of 300 tokens 119 against 43, 64 single tokens over 100 keys 20.9 against 19.5).
+            groups = self._groups(seq_ids, counts) if shared_prefix else []
+            if any(held for _, _, held in groups):
+                own = self._split(seq_ids, groups)
                 out = _ops.shared_prefix_paged(q, q_indptr, self.pool, *own, **kw)
             else:
                 out = _ops.chunk_paged(q, q_indptr, self.pool, *table, **kw)
