@@ -232,7 +232,7 @@ def workspace_buffers():
 
 
 class kernel_timer:
-    """Context manager: HIP-event time of each entry point's dominant kernel.
+    """Context manager: HIP-event time of each entry point's dominant kernel (shared prefixes: of both).
 
     >>> with kernel_timer() as t:
     ...     run()

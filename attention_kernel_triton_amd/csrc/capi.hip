@@ -28,8 +28,8 @@ int check_launch(const char* what) {
   return AKT_OK;
 }
 
-// Opt-in kernel timer: while enabled, every entry point's dominant kernel is
-// launched with an event pair stamped by the runtime at the dispatch's start
+// Opt-in kernel timer: while enabled, every entry point's dominant kernel (with shared prefixes,
+// both) is launched with an event pair stamped by the runtime at the dispatch's start
 // and end; akt_kernel_timer_read() waits for the recorded pairs and returns
 // their summed elapsed time.
 namespace {

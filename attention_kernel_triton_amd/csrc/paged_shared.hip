@@ -124,12 +124,13 @@ template <int D, bool BF16>
 int launch_join(const ChunkParams& p, hipStream_t st) {
   const int64_t lanes = (int64_t)p.total_q * p.Hq * (D / 4);
   const dim3 block(kJoinThreads);
+  KernelTimer timer;
   if (lanes <= kJoinPairLanes) {
     const dim3 grid((unsigned)ceil_div(lanes * 2, kJoinThreads));
-    hipLaunchKernelGGL((shared_join_kernel<D, BF16, 2>), grid, block, 0, st, p);
+    timer.launch(shared_join_kernel<D, BF16, 2>, grid, block, 0, st, p);
   } else {
     const dim3 grid((unsigned)ceil_div(lanes, kJoinThreads));
-    hipLaunchKernelGGL((shared_join_kernel<D, BF16, 1>), grid, block, 0, st, p);
+    timer.launch(shared_join_kernel<D, BF16, 1>, grid, block, 0, st, p);
   }
   return check_launch("shared_join_kernel");
 }

@@ -578,7 +578,8 @@ int akt_kept_index_from_uniform(const float* uniform, float kept_ratio, int64_t 
 /*
  * Kernel timer (diagnostics; no counterpart in the reference, which times
  * whole Python calls with triton.testing.do_bench).  While enabled, every
- * entry point above records a HIP event pair around its dominant kernel on
+ * entry point above records a HIP event pair around its dominant kernel
+ * (akt_shared_prefix_paged_fwd: around each of its two) on
  * the launch stream.  akt_kernel_timer_read() waits for the recorded events
  * and returns the summed elapsed milliseconds and the number of launches;
  * akt_kernel_timer_enable() discards what was recorded.

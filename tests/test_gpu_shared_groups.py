@@ -90,3 +90,15 @@ def test_prompts_alone_among_more_sequences_than_the_kernel_keeps_places_of(dev)
     n = [1] * 700
     n[5], n[333], n[699] = 50, 70, 33
     Case([(1, 0)] * 600, [i % 9 for i in range(700)], n, 2, 1, 64, 16, before=2).check(dev)
+
+
+@pytest.mark.parametrize("rows", [1, 700])
+def test_the_kernel_timer_counts_both_launches(dev, rows):
+    """One thread to a row's dims in the join, or two where rows are few: either is timed."""
+    c = Case([(2, 100)], [5, 9], [rows, 1], 32, 8, 64, 16)
+    a = c.args(dev)
+    flash_attention_shared_prefix_paged(*a)
+    torch.cuda.synchronize()
+    with N.kernel_timer() as t:
+        flash_attention_shared_prefix_paged(*a)
+    assert t.launches == 2 and t.total_ms > 0
