@@ -417,43 +417,50 @@ class PagedKVCache:
             self._restore(before)
             raise
 
-    def evict(self, seq_ids, keep: int, first: int = 0, recent: int = 0) -> int:
-        """Cut sequences of more than `keep` tokens down to so many; returns the tokens dropped.
+    def _eviction_steps(self, seqs, held):
+        """The sequences that give up tokens in one call each, as slices of seqs: all at once where the
+        free pages replace every shared page that is written, else one after another in an order in
+        which they suffice (found a sequence at a time, not among all orders): a page's last holder
+        keeps it, and what one gives up the next can take."""
+        free = len(self._free)
+        need = sum(self._refs[p] > 1 for s in seqs for p in self._pages[s][:held])
+        if need <= free:
+            return [slice(0, len(seqs))]
+        refs = {p: self._refs[p] for s in seqs for p in self._pages[s]}
+        steps, left = [], list(range(len(seqs)))
+        while left:
+            # Those that give up as many pages as they take first, then those that give up most, now or
+            # with the sequences that share their pages behind.
+            best = None
+            for i in left:
+                pages = self._pages[seqs[i]]
+                take = sum(refs[p] > 1 for p in pages[:held])
+                give = sum(refs[p] == 1 for p in pages[held:])
+                rank = (give >= take, give, sum(1 / refs[p] for p in pages[held:]))
+                if take <= free and (best is None or rank > best[0]):
+                    best = rank, i, give - take
+            if best is None:
+                raise MemoryError(f"page pool exhausted: need {need} pages, {len(self._free)} free")
+            _, i, more = best
+            for j, p in enumerate(self._pages[seqs[i]]):
+                if j >= held or refs[p] > 1:
+                    refs[p] -= 1
+            free += more
+            left.remove(i)
+            steps.append(slice(i, i + 1))
+        return steps
 
-        Each kv head keeps the first `first` tokens, the last `recent`, and of the others those that
-        drew most attention (select_heaviest over the cache's sums), in their order; K, V and sums
-        move to the front of the sequence's pages, and the pages behind return to the free list.
-        New tokens keep counting positions from the tokens there were (next_position).  Shared pages are
-        left to the other sequences: the kept tokens go into free ones.  A call that is refused
-        changes nothing.
-        """
-        if self.weights is None:
-            raise ValueError("the cache keeps no sums of attention weight (weight_rows)")
-        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
-            raise ValueError("keep must be positive and at least first + recent")
-        seqs = [s for s in dict.fromkeys(seq_ids) if self.seq_len(s) > keep]
-        if not seqs:
-            return 0
-        for s in seqs:
-            if self._len[s] > self.weights.shape[2]:
-                raise ValueError(f"sequence {s!r} has {self._len[s]} tokens, the sums hold "
-                                 f"{self.weights.shape[2]}")
-        held = -(-keep // self.page_size)  # pages of a sequence afterwards
+    def _close_up(self, seqs, keep, ind, nnz, rows) -> int:
+        """Cuts sequences down to the tokens listed; returns the tokens dropped."""
+        held = -(-keep // self.page_size)
         shared = [(s, i) for s in seqs for i in range(held) if self._refs[self._pages[s][i]] > 1]
-        if len(shared) > len(self._free):
-            raise MemoryError(f"page pool exhausted: need {len(shared)} pages, "
-                              f"{len(self._free)} free")
         fresh = dict(zip(shared, self._free[len(self._free) - len(shared):][::-1]))
-        rows = self._row_table(seqs)
-        table = self.page_table(seqs)
         dst = None
         if fresh:
             dst = self._ints([fresh.get((s, i), p) for s in seqs
                               for i, p in enumerate(self._pages[s])])
-        ind, nnz = select_heaviest(self.weights, self._ints([self._len[s] for s in seqs]), keep,
-                                   first=first, recent=recent, rows=rows)
-        keep_tokens(self.pool, *table, ind, nnz, dst_page_indices=dst, weights=self.weights,
-                    rows=rows)
+        keep_tokens(self.pool, *self.page_table(seqs), ind, nnz, dst_page_indices=dst,
+                    weights=self.weights, rows=rows)
         del self._free[len(self._free) - len(shared):]
         dropped = 0
         for s in seqs:
@@ -468,6 +475,38 @@ class PagedKVCache:
             dropped += self._len[s] - keep
             self._dropped[s] = self._dropped.get(s, 0) + self._len[s] - keep
             self._len[s] = keep
+        return dropped
+
+    def evict(self, seq_ids, keep: int, first: int = 0, recent: int = 0) -> int:
+        """Cut sequences of more than `keep` tokens down to so many; returns the tokens dropped.
+
+        Each kv head keeps the first `first` tokens, the last `recent`, and of the others those that
+        drew most attention (select_heaviest over the cache's sums), in their order; K, V and sums
+        move to the front of the sequence's pages, and the pages behind return to the free list.
+        New tokens keep counting positions from the tokens there were (next_position).  Shared pages are
+        left to the other sequences: the kept tokens go into free ones.  Where these do not suffice for
+        all sequences at once, the sequences are cut one after another, those first that give up most
+        pages, and the last holder of a shared page keeps it.  A call that is refused changes nothing.
+        """
+        if self.weights is None:
+            raise ValueError("the cache keeps no sums of attention weight (weight_rows)")
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise ValueError("keep must be positive and at least first + recent")
+        seqs = [s for s in dict.fromkeys(seq_ids) if self.seq_len(s) > keep]
+        if not seqs:
+            return 0
+        for s in seqs:
+            if self._len[s] > self.weights.shape[2]:
+                raise ValueError(f"sequence {s!r} has {self._len[s]} tokens, the sums hold "
+                                 f"{self.weights.shape[2]}")
+        held = -(-keep // self.page_size)  # pages of a sequence afterwards
+        steps = self._eviction_steps(seqs, held)
+        rows = self._row_table(seqs)
+        ind, nnz = select_heaviest(self.weights, self._ints([self._len[s] for s in seqs]), keep,
+                                   first=first, recent=recent, rows=rows)
+        dropped = 0
+        for at in steps:
+            dropped += self._close_up(seqs[at], keep, ind[at], nnz[at], rows[at])
         return dropped
 
 

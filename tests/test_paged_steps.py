@@ -1,10 +1,14 @@
-"""PagedKVCache's steps on the host: which attention call a step makes, with the kernels' work left out
-or done on the CPU."""
+"""PagedKVCache's steps on the host: which attention call a step makes, and evictions that the free pages
+serve in some orders only, with the kernels' work left out or done on the CPU."""
+import itertools
+
 import pytest
 import torch
 
 from attention_kernel_triton_amd import _ops, paged_kv
 from attention_kernel_triton_amd.paged_kv import PagedKVCache
+from oracle import serving
+from test_eviction_bookkeeping import host, rows_of  # noqa: F401
 
 
 @pytest.fixture
@@ -46,3 +50,142 @@ def test_a_step_without_a_shared_page_attends_as_without_shared_prefixes(calls):
     assert calls[-1] == ("chunk", 0)
     out, lse = step(["a", "c"], return_lse=True, shared_prefix=True)
     assert calls[-1] == ("shared", 1) and out.shape == (2, 1, 8) and lse.shape == (2, 1)
+
+
+# ---- evictions with few free pages.
+class Full:
+    """A cache with sums, and what each sequence should hold."""
+
+    def __init__(self, pages, page=4, rows=20, seed=0, device="cpu"):
+        self.g, self.device = torch.Generator().manual_seed(seed), device
+        self.cache = PagedKVCache(pages, 2, page, 8, device=device, weight_rows=rows, weight_len=200)
+
+    def append(self, s, n):
+        k, v = (torch.randn(n, 2, 8, generator=self.g).half().to(self.device) for _ in range(2))
+        self.cache.append([s], k, v, [n])
+        row = int(self.cache._row_table([s])[0])
+        self.cache.weights[row, :, :self.cache.seq_len(s)] = torch.rand(
+            2, self.cache.seq_len(s), generator=self.g).to(self.device)
+
+    def state(self):
+        c = self.cache
+        return ({s: (rows_of(c, s).cpu().clone(), c.weights[c._rows[s]].cpu().clone(), c.next_position(s))
+                 for s in c._pages}, list(c._free), {s: list(p) for s, p in c._pages.items()},
+                list(c._refs), dict(c._len))
+
+    def evict(self, seqs, keep, first=0, recent=0):
+        before, c = self.state()[0], self.cache
+        got = c.evict(seqs, keep, first, recent)
+        want = 0
+        for s, (kv, w, at) in before.items():
+            n = kv.shape[2]
+            assert c.next_position(s) == at
+            if s in seqs and n > keep:
+                ind = serving.heaviest(w[None, :, :n], [n], keep, first, recent)[0][0].long()
+                kv = torch.stack([kv[:, h, ind[h]] for h in range(2)], 1)
+                w = torch.nn.functional.pad(torch.stack([w[h, ind[h]] for h in range(2)]), (0, 200 - keep))
+                want += n - keep
+            assert torch.equal(rows_of(c, s).cpu(), kv) and torch.equal(c.weights[c._rows[s]].cpu(), w)
+        assert got == want
+        held = [p for pages in c._pages.values() for p in pages]
+        assert sorted(set(held) | set(c._free)) == list(range(c.pool.shape[0]))
+        assert len(c._free) == len(set(c._free)) and not set(held) & set(c._free)
+        assert all(c._refs[p] == held.count(p) for p in range(c.pool.shape[0]))
+        return got
+
+
+def last_holder(f):
+    f.append(0, 20)
+    f.cache.fork(0, 1)  # five pages of two sequences, three free ones
+    old = set(f.cache._pages[0])
+    assert f.evict([0, 1], 10, 1, 2) == 20
+    assert set(f.cache._pages[1]) <= old and not set(f.cache._pages[0]) & old
+    assert f.cache.free_pages == 2
+
+
+def test_the_last_holder_of_shared_pages_keeps_them(host):
+    last_holder(Full(8))
+
+
+@pytest.mark.gpu
+def test_sequences_cut_one_after_another_on_the_device(dev):
+    last_holder(Full(8, device=dev))
+    f = Full(13, device=dev)
+    f.append("a", 24)
+    f.cache.fork("a", "b")
+    f.append("x", 28)
+    assert f.evict(["a", "b", "x"], 12, 1, 3) == 12 + 12 + 16
+
+
+def test_pages_that_one_sequence_gives_up_serve_the_next(host):
+    f = Full(13)
+    f.append("a", 24)
+    f.cache.fork("a", "b")
+    f.append("x", 28)
+    assert f.cache.free_pages == 0
+    assert f.evict(["a", "b", "x"], 12) == 12 + 12 + 16  # x gives up four pages, a takes three
+    assert f.cache.free_pages == 13 - 9
+    f = Full(6)
+    f.append("a", 24)
+    f.cache.fork("a", "b")
+    before = f.state()
+    with pytest.raises(MemoryError, match="need 6 pages, 0 free"):
+        f.cache.evict(["a", "b"], 12)
+    after = f.state()
+    assert before[1:] == after[1:]
+    assert all(torch.equal(x, y) for s in before[0] for x, y in zip(before[0][s][:2], after[0][s][:2]))
+
+
+def _some_order_serves(cache, seqs, held):
+    for order in itertools.permutations(seqs):
+        refs, free, ok = list(cache._refs), len(cache._free), True
+        for s in order:
+            pages = cache._pages[s]
+            free -= sum(refs[p] > 1 for p in pages[:held])
+            if free < 0:
+                ok = False
+                break
+            for i, p in enumerate(pages):
+                if i < held and refs[p] == 1:
+                    continue
+                refs[p] -= 1
+                free += refs[p] == 0
+        if ok:
+            return True
+    return False
+
+
+def test_evictions_on_nearly_full_pools(host):
+    """Random forests of forks: what no order of the sequences serves is refused and changes nothing, and
+    so, rarely, is what some order would (the order is found a sequence at a time)."""
+    refused = ordered = missed = 0
+    for seed in range(400):
+        g = torch.Generator().manual_seed(seed)
+        r = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+        f = Full(10 + r(14), seed=seed)
+        c = f.cache
+        names = iter(range(100))
+        try:
+            for _ in range(9):
+                live = list(c._pages)
+                if live and r(2) and len(live) < 5:
+                    c.fork(live[r(len(live))], next(names))
+                else:
+                    f.append(live[r(len(live))] if live and r(2) else next(names), 1 + r(18))
+        except MemoryError:
+            pass
+        seqs = [s for s in c._pages if r(4)][:5]
+        keep = 1 + r(16)
+        held = -(-keep // 4)
+        long = [s for s in seqs if c.seq_len(s) > keep]
+        at_once = sum(c._refs[p] > 1 for s in long for p in c._pages[s][:held]) <= len(c._free)
+        some, before = _some_order_serves(c, long, held), f.state()[1:]
+        try:
+            f.evict(seqs, keep)
+            assert some
+            ordered += not at_once
+        except MemoryError:
+            assert before == f.state()[1:] and not at_once
+            refused += not some
+            missed += some
+    assert refused > 50 and ordered > 50 and missed <= ordered // 50
