@@ -502,7 +502,9 @@ class PagedKVCache:
         held = -(-keep // self.page_size)  # pages of a sequence afterwards
         steps = self._eviction_steps(seqs, held)
         rows = self._row_table(seqs)
-        ind, nnz = select_heaviest(self.weights, self._ints([self._len[s] for s in seqs]), keep,
+        lens = [self._len[s] for s in seqs]
+        # (Rows as wide as the longest sequence: the kernel is chosen by their width, not the cache's.)
+        ind, nnz = select_heaviest(self.weights[:, :, :max(lens)], self._ints(lens), keep,
                                    first=first, recent=recent, rows=rows)
         dropped = 0
         for at in steps:

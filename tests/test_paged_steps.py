@@ -189,3 +189,16 @@ def test_evictions_on_nearly_full_pools(host):
             refused += not some
             missed += some
     assert refused > 50 and ordered > 50 and missed <= ordered // 50
+
+
+def test_an_eviction_selects_from_rows_as_wide_as_its_longest_sequence(host, monkeypatch):
+    seen, select = [], paged_kv.select_heaviest
+    monkeypatch.setattr(paged_kv, "select_heaviest",
+                        lambda w, *a, **kw: seen.append(tuple(w.shape)) or select(w, *a, **kw))
+    f = Full(60)
+    f.append("a", 30)
+    f.append("b", 9)
+    f.append("c", 41)
+    f.append("d", 70)
+    f.evict(["a", "b", "c"], 8, 1, 2)
+    assert seen == [(20, 2, 41)]
