@@ -104,6 +104,8 @@ class PagedKVCache:
 
     With weight_rows, `weights` [weight_rows, Hkv, weight_len] keeps for as many sequences the
     attention that each token has drawn from the steps so far (extend), by which evict chooses.
+    Tokens from position weight_len on have no sums: a sequence that outgrows them is still served,
+    and can be evicted again once truncate has cut it to weight_len.
 
     A page table describes the cache as it is: append, extend, fork, truncate, evict,
     release and compact make the tables handed out before them stale.
@@ -111,6 +113,8 @@ class PagedKVCache:
 
     def __init__(self, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
                  device="cuda", dtype=torch.float16, weight_rows: int = 0, weight_len: int = 0):
+        if weight_rows > 0 and weight_len < 1:
+            raise ValueError("weight_rows need a weight_len: the most tokens whose sums a row holds")
         self.page_size = page_size
         self.pool = torch.zeros((num_pages, 2, num_kv_heads, page_size, head_dim), dtype=dtype,
                                 device=device)

@@ -64,8 +64,8 @@ class Full:
         k, v = (torch.randn(n, 2, 8, generator=self.g).half().to(self.device) for _ in range(2))
         self.cache.append([s], k, v, [n])
         row = int(self.cache._row_table([s])[0])
-        self.cache.weights[row, :, :self.cache.seq_len(s)] = torch.rand(
-            2, self.cache.seq_len(s), generator=self.g).to(self.device)
+        n = min(self.cache.seq_len(s), 200)
+        self.cache.weights[row, :, :n] = torch.rand(2, n, generator=self.g).to(self.device)
 
     def state(self):
         c = self.cache
@@ -202,3 +202,17 @@ def test_an_eviction_selects_from_rows_as_wide_as_its_longest_sequence(host, mon
     f.append("d", 70)
     f.evict(["a", "b", "c"], 8, 1, 2)
     assert seen == [(20, 2, 41)]
+
+
+def test_rows_of_sums_need_a_length(host):
+    with pytest.raises(ValueError, match="weight_len"):
+        PagedKVCache(4, 1, 4, 8, device="cpu", weight_rows=4)
+    with pytest.raises(ValueError, match="weight_len"):
+        PagedKVCache(4, 1, 4, 8, device="cpu", weight_rows=1, weight_len=-1)
+    assert PagedKVCache(4, 1, 4, 8, device="cpu", weight_len=9).weights is None
+    f = Full(60)  # of 200 entries to a row
+    f.append("a", 203)
+    with pytest.raises(ValueError, match="sums hold 200"):
+        f.cache.evict(["a"], 20)
+    f.cache.truncate("a", 200)
+    assert f.evict(["a"], 20) == 180
