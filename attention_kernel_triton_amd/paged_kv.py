@@ -390,7 +390,9 @@ class PagedKVCache:
         before, rows_before = {s: self._len.get(s) for s in seq_ids}, set(self._rows)
         self._grow(seq_ids, counts)
         try:
-            rows = self._row_table(seq_ids) if watch else None
+            if watch:  # a sequence without new tokens draws nothing and needs no row
+                self._row_table([s for s, n in zip(seq_ids, counts) if n])
+                rows = self._ints([self._rows.get(s, -1) for s in seq_ids])
             table = self.page_table(seq_ids)
             q_indptr = self._indptr(counts)
             if inv_freq is None:

@@ -216,3 +216,17 @@ def test_rows_of_sums_need_a_length(host):
         f.cache.evict(["a"], 20)
     f.cache.truncate("a", 200)
     assert f.evict(["a"], 20) == 180
+
+
+def test_a_sequence_without_new_tokens_takes_no_row_of_sums(calls, monkeypatch):
+    seen = []
+    monkeypatch.setattr(paged_kv, "accumulate_attention_weights_paged",
+                        lambda *a, rows, **kw: seen.append(rows.tolist()))
+    cache = PagedKVCache(40, 1, 4, 8, device="cpu", weight_rows=2, weight_len=50)
+    cache.extend(["a", None, "b", None], _z(6), _z(6), _z(6), [5, 0, 1, 0])
+    assert seen == [[0, -1, 1, -1]] and sorted(cache._rows) == ["a", "b"]
+    cache.extend(["b", "a"], _z(1), _z(1), _z(1), [1, 0])
+    assert seen[1] == [1, 0]
+    with pytest.raises(MemoryError, match="rows"):
+        cache.extend(["b", "c"], _z(2), _z(2), _z(2), [1, 1])
+    assert cache.seq_len("b") == 2 and not cache._free_rows and "c" not in cache._pages
