@@ -302,6 +302,10 @@ class PagedKVCache:
         Neighbours in seq_ids that share leading pages form groups; the last counts[i] tokens of each
         sequence (default: one) are its queries and stay out of the prefixes."""
         counts = [1] * len(seq_ids) if counts is None else counts
+        if len(counts) != len(seq_ids):
+            raise ValueError("one count per sequence")
+        if any(n < 0 for n in counts):
+            raise ValueError("counts must be non-negative")
         return self._split(seq_ids, self._groups(seq_ids, counts))
 
     def _split(self, seq_ids, groups):

@@ -230,3 +230,13 @@ def test_a_sequence_without_new_tokens_takes_no_row_of_sums(calls, monkeypatch):
     with pytest.raises(MemoryError, match="rows"):
         cache.extend(["b", "c"], _z(2), _z(2), _z(2), [1, 1])
     assert cache.seq_len("b") == 2 and not cache._free_rows and "c" not in cache._pages
+
+
+def test_split_tables_take_a_count_of_tokens_to_a_sequence(host):
+    cache = PagedKVCache(40, 1, 4, 8, device="cpu")
+    cache.append(["a"], _z(20), _z(20), [20])
+    cache.fork("a", "b")
+    for counts in ([1], [1, 1, 1], [-9, -9], [1, -1]):  # -9: a prefix of more pages than there are
+        with pytest.raises(ValueError):
+            cache.split_table(["a", "b"], counts)
+    assert cache.split_table(["a", "b"], [0, 0])[4].tolist() == [0, 5]
