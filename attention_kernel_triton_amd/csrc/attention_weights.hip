@@ -36,7 +36,8 @@
 // at a time and whole tiles: 256 keys of each of 8 heads are 256 tiles of unlike lengths).  There a
 // block of 32 rows by 256 keys takes a wave about 142 VALU instructions beside its 16 MFMAs; the matrix
 // pipe is busy 38% of the time, and two workgroups to a processor take 1.07 us a block each where one
-// alone takes 0.85: the two kinds of instructions hardly overlap.  Five tokens after twelve: 5.3,
+// alone takes 0.85: the two kinds of instructions hardly overlap.  (At D = 128 the kernel spills eight
+// vector registers, at the tiles' starts and ends, not in the walk over the blocks.)  Five tokens after twelve: 5.3,
 // of which a launch is 4; the rest is the sequences' table, the page ids, K and q, one after another.
 #include <math.h>
 

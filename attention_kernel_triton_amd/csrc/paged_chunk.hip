@@ -41,6 +41,8 @@
 // Shared prefixes (SHARED).  A group's tokens together are one more sequence behind the others, whose
 // keys are the prefix, seen whole by every row.  Every part leaves a state (state_row), a second
 // kernel joins them (paged_shared.hip), and units of few rows are served by paged_shared_few.hpp.
+// At D = 128 these instances spill 5 to 27 vector registers, outside the walks over keys but for
+// three reloads a block in the one with pages that are not whole 16-token groups and with the LSE.
 //
 // Tiles (many).  As in the dense prefill kernel: K and V tiles go global -> registers -> one
 // of four LDS buffers, three tiles ahead; both products run transposed so that a lane owns

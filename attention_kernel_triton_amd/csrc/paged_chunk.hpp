@@ -21,7 +21,8 @@ __host__ __device__ constexpr int chunk_split_rows(int D) { return D <= 128 ? 32
 constexpr int kCkFew = 1, kCkMany = 2;
 // With shared prefixes a wave serves a range of few rows alone: the grain of its cuts, the cost of
 // a unit's start and end in keys, and the fewest keys (with costs) of a range; and the cost of a unit
-// of many rows, whose 32-bit states are written.  Measured (us; a decode step of 32 sequences behind
+// of many rows, whose 32-bit states are written.  Measured at D = 128 only, and several are within noise
+// of what they are compared with (us; a decode step of 32 sequences behind
 // 4,096 tokens / 64 samples behind 20,001 / eight prompts behind 8,000; as they are 29.3 / 81.4 / 335):
 // costs of few 128 29.6 / 82.5 / 339; fewest keys 128 29.5 / 82.2 / 336, 384 32.5 / 81.8 / 336; costs of
 // many 160 29.2 / 87.0 / 426, 640 30.2 / 81.7 / 345.

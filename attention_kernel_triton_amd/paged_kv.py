@@ -157,7 +157,10 @@ class PagedKVCache:
             self._free_rows.append(self._rows.pop(seq_id))
 
     def truncate(self, seq_id, length: int) -> None:
-        """Forget a sequence's tokens from position `length` on (rejected drafts, say)."""
+        """Forget a sequence's tokens from position `length` on (rejected drafts, say).
+
+        Their own sums of attention weight are cleared; what their queries added to the sums of the
+        tokens that stay remains there (extend(observe=0) adds nothing)."""
         if not 0 <= length <= self.seq_len(seq_id):
             raise ValueError(f"length {length} is not in [0, {self.seq_len(seq_id)}]")
         if seq_id not in self._pages:
@@ -381,8 +384,9 @@ class PagedKVCache:
         shared_prefix: leading pages that neighbours in seq_ids share (fork) are read once for all
         of them (flash_attention_shared_prefix_paged); where none do, the step is as without it.
         observe: where the cache keeps sums of attention weight, the last `observe` of each
-        sequence's new tokens add theirs (default: all; 0: none).  A whole prompt's cost is about half its
-        attention again.
+        sequence's new tokens add theirs (default: all; 0: none), drafted tokens that truncate takes
+        away again among them.  A whole prompt's cost is about half its attention again.
+        The page tables are made on the host at each step, with shared_prefix two of them.
         """
         watch = self.weights is not None and observe != 0
         if observe is not None and observe < 0:

@@ -29,7 +29,15 @@ def flash_attention_shared_prefix_paged(q, q_indptr, paged_kv_cache, kv_page_ind
     them.  Every new token sees the whole prefix; of its sequence's own tokens it sees those up to itself
     (causal=True) or all.  fp16 or bf16; any page_size; D = 64, 128 or 256; up to 128 query heads
     per kv head.  Rows that see no key get zeros (lse -inf); rows of q that belong to no sequence
-    are left unwritten.  Probabilities are rounded to q's type, as there.
+    are left unwritten.  Probabilities are rounded to q's type, as there.  total_q * Hq must be below
+    2^25; the stream's workspace holds 2 (4 D + 16) bytes for each query row and head, besides
+    the parts of cut units (up to 139 MB).
+
+    It pays where prefixes are read by sequences of few new tokens (us, this call / the chunk call over
+    whole tables, the same inputs each time: 32 single tokens behind 4,096 28 / 84, 64 behind 20,001
+    76 / 569, 1 to 6 drafts of 24 sequences in four groups 35 / 43).  Prompts read a prefix once for each
+    256 rows either way (eight of 150 to 350 tokens behind 8,000 324 / 317), and a call of a few short
+    sequences is bound by its second launch (two behind 40 tokens 12.9 / 11.4).
     """
     return _ops.shared_prefix_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices,
                                     kv_last_page_len, group_indptr, prefix_page_indptr,

@@ -475,7 +475,9 @@ int akt_paged_copy(void* kv_cache, const int32_t* src, const int32_t* dst,
  * tokens).  Every query token sees the whole prefix; of the own keys query i of n_b, at own
  * position len_b - n_b + i, sees those up to its own position (causal) or all.
  * The rest is as in akt_chunk_paged_fwd; so is the workspace, and the first
- * AKT_WORKSPACE_ZERO_BYTES of it that every call leaves zero.  Two launches.
+ * AKT_WORKSPACE_ZERO_BYTES of it that every call leaves zero.  Besides the parts of cut units it holds
+ * two 32-bit states, 2 (4 head_dim + 16) bytes, for each query row and head.  total_q * num_q_heads
+ * must be below 2^25.  Two launches.
  */
 size_t akt_shared_prefix_paged_workspace_size(int64_t batch, int64_t total_q, int64_t num_q_heads,
                                               int64_t num_kv_heads, int64_t head_dim,

@@ -240,3 +240,12 @@ def test_split_tables_take_a_count_of_tokens_to_a_sequence(host):
         with pytest.raises(ValueError):
             cache.split_table(["a", "b"], counts)
     assert cache.split_table(["a", "b"], [0, 0])[4].tolist() == [0, 5]
+
+
+def test_what_removed_tokens_drew_goes_and_what_they_gave_stays(host):
+    f = Full(20)
+    f.append("a", 30)
+    row = f.cache.weights[f.cache._rows["a"]].clone()
+    f.cache.truncate("a", 21)
+    after = f.cache.weights[f.cache._rows["a"]]
+    assert torch.equal(after[:, :21], row[:, :21]) and not after[:, 21:].any()
