@@ -16,7 +16,8 @@ def accumulate_attention_weights_paged(weights, q, q_indptr, lse, paged_kv_cache
                                        softmax_scale=None, window=None) -> None:
     """Adds to weights[rows[b], h, j] the softmax weight that token j of sequence b draws in kv head h.
 
-    weights: float32 [N, Hkv, L] (unit last stride), written in place; tokens from L on are left out.
+    weights: float32 [N, Hkv, L] (unit last stride, no two rows with memory in common), written in
+    place; tokens from L on are left out.
     rows: int32 [B], each sequence's row of weights (default: its own number); no row twice, and a
     sequence whose row is not in [0, N) is left out.
     q [total_q, Hq, D] (fp16 or bf16, the cache's type), q_indptr, the cache and its page table,

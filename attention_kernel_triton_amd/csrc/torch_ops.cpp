@@ -625,6 +625,20 @@ struct WeightRows {
   int64_t stride[2];
   at::Tensor rows;
 };
+// Whether two of the rows of `len` elements at n sn + h sh (0 <= n < N, 0 <= h < H) have an element in
+// common: whether n sn + h sh is within len of 0 for some -N < n < N and 0 <= h < H, not both 0.
+bool rows_overlap(int64_t N, int64_t H, int64_t len, int64_t sn, int64_t sh) {
+  if (N > 1 && sn < len) return true;
+  for (int64_t h = 1; h < H; ++h) {
+    const int64_t at = h * sh;
+    if (at < len) return true;
+    if (N == 1) continue;
+    const int64_t n = at / sn;  // rows n and n + 1 of the others are the nearest before and behind
+    if (n < N && at - n * sn < len) return true;
+    if (n + 1 < N && (n + 1) * sn - at < len) return true;
+  }
+  return false;
+}
 WeightRows weight_rows(const at::Tensor& weights, const c10::optional<at::Tensor>& rows_,
                        const at::Device& dev, int64_t B, int64_t H, bool written) {
   need_gpu("weights", weights);
@@ -637,8 +651,8 @@ WeightRows weight_rows(const at::Tensor& weights, const c10::optional<at::Tensor
   if (weights.size(2) > 1 && weights.stride(2) != 1)
     throw py::value_error("weights need a unit last stride");
   if (written && weights.numel() > 0 &&
-      ((weights.size(0) > 1 && weights.stride(0) == 0) ||
-       (weights.size(1) > 1 && weights.stride(1) == 0)))
+      rows_overlap(weights.size(0), weights.size(1), weights.size(2), weights.stride(0),
+                   weights.stride(1)))
     throw py::value_error("weights are written: their rows must not be one and the same memory");
   WeightRows r{{weights.stride(0), weights.stride(1)}, at::Tensor()};
   if (rows_.has_value() && rows_->defined()) {

@@ -500,7 +500,8 @@ int akt_shared_prefix_paged_fwd(
  * for the keys j < min(len_b, row_len).  q [total_q, num_q_heads, head_dim], q_indptr, the page
  * table and causal are those of an attention call, lse (contiguous fp32 [total_q, num_q_heads]) what
  * it returned; rows of q with lse -inf count nothing.
- *   weights: fp32 [num_rows, num_kv_heads, row_len], strides weight_stride[0..1], unit in the last.
+ *   weights: fp32 [num_rows, num_kv_heads, row_len], strides weight_stride[0..1], unit in the last; no
+ *   two rows may overlap.
  *   rows: int32 [batch], the row of each sequence (NULL: b); no row may be named twice, and a
  *   sequence whose row is outside [0, num_rows) is left out.
  *   window: only the last `window` tokens of each sequence count.
